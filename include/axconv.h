@@ -332,6 +332,38 @@ int axc_fake_quant(const float *x, size_t count, const float *range2, float *out
 enum { AXC_COLUMN_SUM_ROWS = 296 };
 int axc_column_sums(const float *x, size_t rows, int cols, float *scratch, float *out, int device, void *stream);
 
+/* ---- training of the exact end of a network (no counterpart in the reference, whose models take these steps from the host
+ *      framework) -------------------------------------------------------------------------------------------------- */
+/* Types of matrices, parameters and gradients; sums and statistics are fp32 throughout. */
+enum { AXC_TYPE_FLOAT32 = 0, AXC_TYPE_BFLOAT16 = 1, AXC_TYPE_FLOAT16 = 2 };
+
+/* One step of AdamW over many tensors, in one launch per 800 of them:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  g = grad_scale * gradient
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in fp32; parameters and gradients have one type and are contiguous, at any alignment of their type.  A tensor without a
+ * gradient (NULL) keeps its values and its moments.
+ * The moments of the tensors lie one after the other in the caller's buffers, each tensor's at a multiple of AXC_ADAMW_BLOCK values
+ * (axc_adamw_state_blocks: how many blocks in all), zeros before the first step; 16-byte aligned.
+ * state_bits 32: fp32, exp_avg = m, exp_avg_sq = v.  state_bits 8: e4m3 codes, one byte each, with one fp32 scale per block;
+ * exp_avg_sq then holds the codes of sqrt(v).  step counts from 1.  Only the calls' own kernels are enqueued: capturable. */
+enum { AXC_ADAMW_BLOCK = 256 };
+typedef struct {
+    void *param;
+    const void *grad;
+    int64_t count;
+    double lr, weight_decay;
+} axc_adamw_tensor;
+typedef struct {
+    int32_t type, state_bits;
+    int64_t step;
+    double beta1, beta2, eps;
+    float grad_scale;
+    void *exp_avg, *exp_avg_sq;
+    float *exp_avg_scale, *exp_avg_sq_scale;   /* state_bits 8 only */
+} axc_adamw_desc;
+int axc_adamw_state_blocks(const int64_t *counts, int32_t tensors, int64_t *blocks);
+int axc_adamw_step(const axc_adamw_desc *desc, const axc_adamw_tensor *tensors, int32_t count, int device, void *stream);
+
 /* ---- quantisation parameters: Nudge + UpdateVarQuantProps
  *      (tf2/src/approx_ops_types.h:29-49, 135-152).  out3 = {scale, 1/scale, nudged_min}. */
 int axc_quant_props(float min_value, float max_value, float out3[3]);

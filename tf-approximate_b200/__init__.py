@@ -16,3 +16,4 @@ from .ops import (approx_conv2d_with_min_max_vars, approx_depthwise_conv2d_with_
                   ax_conv2d, approx_conv2d,
                   conv2d_output_shape, launch_count, measure_lookup_peak, Table)
 from .layers import FakeApproxConv2D, fake_quant_with_min_max_vars  # noqa: F401
+from .optimizers import AdamW  # noqa: F401

@@ -16,6 +16,7 @@ SYMBOLS = [
     "axc_quant_props", "axc_status_string", "axc_last_cuda_error", "axc_launch_count", "axc_measure_lookup_peak", "axc_debug_bounds_record", "axc_debug_wait_polls",
     "axc_add_residual", "axc_max_pool_same", "axc_conv2d_forward_fused", "axc_depthwise_conv2d_forward_fused", "axc_tensor_range", "axc_fake_quant", "axc_column_sums", "axc_conv2d_forward_sharded", "axc_gather_outputs",
     "axc_qconv2d_workspace_bytes", "axc_qconv2d_fast_workspace_bytes", "axc_qconv2d_route", "axc_qconv2d_forward", "axc_quantized_zero_point", "axc_quantized_output_range",
+    "axc_adamw_state_blocks", "axc_adamw_step",
 ]
 
 
@@ -36,6 +37,16 @@ class Epilogue(C.Structure):
 
 class DebugOut(C.Structure):
     _fields_ = [("qinput", C.c_void_p), ("qfilter", C.c_void_p), ("acc", C.c_void_p)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("count", C.c_int64), ("lr", C.c_double), ("weight_decay", C.c_double)]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("state_bits", C.c_int32), ("step", C.c_int64), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("grad_scale", C.c_float), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p)]
 
 
 _lib = None
@@ -99,6 +110,8 @@ def load():
     L.axc_fake_quant.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
     L.axc_column_sums.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
     L.axc_quant_props.argtypes = [C.c_float, C.c_float, C.POINTER(C.c_float)]
+    L.axc_adamw_state_blocks.argtypes = [C.POINTER(C.c_int64), C.c_int32, C.POINTER(C.c_int64)]
+    L.axc_adamw_step.argtypes = [C.POINTER(AdamwDesc), C.c_void_p, C.c_int32, C.c_int, C.c_void_p]
     L.axc_status_string.argtypes = [C.c_int]
     L.axc_status_string.restype = C.c_char_p
     L.axc_last_cuda_error.restype = C.c_int
