@@ -336,6 +336,51 @@ int axc_column_sums(const float *x, size_t rows, int cols, float *scratch, float
  *      framework) -------------------------------------------------------------------------------------------------- */
 /* Types of matrices, parameters and gradients; sums and statistics are fp32 throughout. */
 enum { AXC_TYPE_FLOAT32 = 0, AXC_TYPE_BFLOAT16 = 1, AXC_TYPE_FLOAT16 = 2 };
+enum { AXC_ACTIVATION_NONE = 0, AXC_ACTIVATION_RELU = 1, AXC_ACTIVATION_GELU = 2, AXC_ACTIVATION_SILU = 3 };
+
+/* The exact dense layer:  y = act(x kernel + bias + residual),  x [rows, inputs], kernel [inputs, units], any strides (elements);
+ * bias [units]; residual [rows, units] with unit stride along a row; y [rows, units] contiguous, all of one type but the bias.
+ * Sums and everything up to y's rounding are fp32; fp32 operands go through the tensor cores as three bf16 terms each, to about
+ * fp32's own precision (2^-22 of the largest products).
+ * pre (may be NULL): z = x kernel + bias + residual in y's type, which the gradient of gelu (the exact one, with erf) and silu needs.
+ * backward: dz = dy act'(kept) with kept = z, for relu y;  dx = dz kernel^T, dkernel = x^T dz ([units, inputs] in memory where
+ * kernel_gradient_transposed), dbias = column sums of dz, dresidual = dz; outputs contiguous, any may be NULL.  dy [rows, units]
+ * contiguous.
+ * Workspace: axc_dense_workspace_bytes for the tensors' addresses (NULL: enough for any), 256-byte aligned, nothing kept in it.  Calls only
+ * enqueue kernels (and a memset): capturable.  axc_matrix_status reads the workspace's status word after the stream is idle: 0, or 3
+ * where a wait inside a kernel ran out; the output is then not valid. */
+typedef struct {
+    int64_t rows, inputs, units;
+    int32_t type, bias_type, activation, kernel_gradient_transposed;
+    int64_t x_row_stride, x_column_stride, kernel_row_stride, kernel_column_stride, residual_row_stride;
+} axc_dense_desc;
+int axc_dense_workspace_bytes(const axc_dense_desc *desc, const void *x, const void *kernel, int device, size_t *forward, size_t *backward);
+int axc_dense_forward(const axc_dense_desc *desc, const void *x, const void *kernel, const void *bias, const void *residual, void *y, void *pre,
+                      void *workspace, size_t workspace_bytes, int device, void *stream);
+int axc_dense_backward(const axc_dense_desc *desc, const void *dy, const void *x, const void *kernel, const void *kept, void *dx, void *dkernel,
+                       void *dbias, void *dresidual, void *workspace, size_t workspace_bytes, int device, void *stream);
+int axc_matrix_status(const void *workspace, int32_t *status, int device, void *stream);
+
+/* Softmax cross entropy of a dense classifier with its gradients, without keeping the logits:
+ *   l = x kernel + bias;  row_loss_t = log sum_v exp(l_tv) - l_t,labels[t];  loss = sum or mean over the rows whose label is not
+ *   ignore_index (0 where there is none);  dl = grad_scale * d loss / d l;  dx = dl kernel^T, dkernel = x^T dl, dbias = column sums of dl.
+ * x [rows, inputs], kernel [inputs, classes], any strides; labels int64 [rows]; a label that is neither a class nor ignore_index
+ * makes its loss, and every gradient, NaN.  Classes whose bias is -inf take no part.  loss: one float; row_loss: [rows] or NULL;
+ * gradients contiguous (dkernel [classes, inputs] in memory where kernel_gradient_transposed), any may be NULL; all NULL: the loss alone.
+ * The exponentials are kept in the workspace where they fit into scratch_limit bytes (0: AXC_ENTROPY_SCRATCH), else the logits are
+ * computed a second time in pieces of the classes.  Workspace, status and streams as for the dense layer. */
+enum { AXC_REDUCE_MEAN = 0, AXC_REDUCE_SUM = 1 };
+#define AXC_ENTROPY_SCRATCH (4ll << 30)
+typedef struct {
+    int64_t rows, inputs, classes;
+    int32_t type, bias_type, reduction, kernel_gradient_transposed;
+    int64_t ignore_index, scratch_limit;
+    int64_t x_row_stride, x_column_stride, kernel_row_stride, kernel_column_stride;
+    float grad_scale;
+} axc_entropy_desc;
+int axc_entropy_workspace_bytes(const axc_entropy_desc *desc, const void *x, const void *kernel, int device, size_t *loss_only, size_t *gradients);
+int axc_entropy(const axc_entropy_desc *desc, const void *x, const void *kernel, const void *bias, const int64_t *labels, float *loss, float *row_loss,
+                void *dx, void *dkernel, void *dbias, void *workspace, size_t workspace_bytes, int device, void *stream);
 
 /* One step of AdamW over many tensors, in one launch per 800 of them:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  g = grad_scale * gradient

@@ -17,6 +17,7 @@ SYMBOLS = [
     "axc_add_residual", "axc_max_pool_same", "axc_conv2d_forward_fused", "axc_depthwise_conv2d_forward_fused", "axc_tensor_range", "axc_fake_quant", "axc_column_sums", "axc_conv2d_forward_sharded", "axc_gather_outputs",
     "axc_qconv2d_workspace_bytes", "axc_qconv2d_fast_workspace_bytes", "axc_qconv2d_route", "axc_qconv2d_forward", "axc_quantized_zero_point", "axc_quantized_output_range",
     "axc_adamw_state_blocks", "axc_adamw_step",
+    "axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes", "axc_entropy",
 ]
 
 
@@ -47,6 +48,19 @@ class AdamwDesc(C.Structure):
     _fields_ = [("type", C.c_int32), ("state_bits", C.c_int32), ("step", C.c_int64), ("beta1", C.c_double), ("beta2", C.c_double),
                 ("eps", C.c_double), ("grad_scale", C.c_float), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
                 ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p)]
+
+
+class DenseDesc(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "inputs", "units")] +
+                [(n, C.c_int32) for n in ("type", "bias_type", "activation", "kernel_gradient_transposed")] +
+                [(n, C.c_int64) for n in ("x_row_stride", "x_column_stride", "kernel_row_stride", "kernel_column_stride", "residual_row_stride")])
+
+
+class EntropyDesc(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "inputs", "classes")] +
+                [(n, C.c_int32) for n in ("type", "bias_type", "reduction", "kernel_gradient_transposed")] +
+                [(n, C.c_int64) for n in ("ignore_index", "scratch_limit", "x_row_stride", "x_column_stride", "kernel_row_stride", "kernel_column_stride")] +
+                [("grad_scale", C.c_float)])
 
 
 _lib = None
@@ -112,6 +126,12 @@ def load():
     L.axc_quant_props.argtypes = [C.c_float, C.c_float, C.POINTER(C.c_float)]
     L.axc_adamw_state_blocks.argtypes = [C.POINTER(C.c_int64), C.c_int32, C.POINTER(C.c_int64)]
     L.axc_adamw_step.argtypes = [C.POINTER(AdamwDesc), C.c_void_p, C.c_int32, C.c_int, C.c_void_p]
+    L.axc_dense_workspace_bytes.argtypes = [C.POINTER(DenseDesc), C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
+    L.axc_dense_forward.argtypes = [C.POINTER(DenseDesc)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_int, C.c_void_p]
+    L.axc_dense_backward.argtypes = [C.POINTER(DenseDesc)] + [C.c_void_p] * 9 + [C.c_size_t, C.c_int, C.c_void_p]
+    L.axc_matrix_status.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_void_p]
+    L.axc_entropy_workspace_bytes.argtypes = [C.POINTER(EntropyDesc), C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
+    L.axc_entropy.argtypes = [C.POINTER(EntropyDesc)] + [C.c_void_p] * 10 + [C.c_size_t, C.c_int, C.c_void_p]
     L.axc_status_string.argtypes = [C.c_int]
     L.axc_status_string.restype = C.c_char_p
     L.axc_last_cuda_error.restype = C.c_int

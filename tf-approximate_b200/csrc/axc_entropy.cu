@@ -1,0 +1,414 @@
+// Softmax cross entropy of a dense classifier with its gradients:
+//   l = x kernel + bias,  loss_t = log sum_v exp(l_tv) - l_t,label,  dl = w (softmax(l) - onehot),  dx = dl kernel^T,  dkernel = x^T dl
+// The logits never reach memory.  One pass of matrix tiles over the classes (axc_gemm.cu) leaves, for every row and segment of 64
+// classes, the largest logit and the sum of exponentials relative to it.  A pass over the rows joins them to the row's
+// log-sum-exp.  Then one of two forms gives the gradient of the logits, 16-bit values that are rounded once:
+//   kept     the exponentials, relative to their segment's largest logit, were kept in scratch, and the pass over the rows turns them
+//            into the gradient: 6 T D V operations, 2 bytes of scratch per logit (bf16; 6 for fp16, 10 for fp32)
+//   pieces   the logits of a piece of the classes are computed again, with the log-sum-exp at hand, and become the gradient in the
+//            tile's last step: 8 T D V operations, scratch for one piece
+// The kept exponentials are fp16 for bf16 operands (rounded to 2^-12, the gradient to 2^-9), fp32 for others.
+// For fp16 the stored gradient is (softmax - onehot) 2^14, whose smallest normal value is 3.7e-9; the products' factor takes it out.
+#include "axc_gemm.h"
+
+namespace axc {
+namespace {
+
+constexpr int kSegment = 64;
+constexpr float kHalfScale = 16384.0f;
+
+struct RowArgs {
+    long long rows, classes;
+    const long long *labels;
+    long long ignore;
+    const float2 *stats;
+    int segments;
+    float *label_logit, *lse, *row_scale, *row_loss;
+    float stored;                              // scale of the stored gradient
+    // kept form
+    void *keep;
+    long long line;
+    uint16_t *gradient;                        // planes of [rows][line]; may be `keep`
+    long long plane;
+};
+
+__device__ __forceinline__ float block_max(float v, float *shared)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float r = shared[0];
+    for (int i = 1; i < int(blockDim.x >> 5); ++i) r = fmaxf(r, shared[i]);
+    return r;
+}
+__device__ __forceinline__ float block_sum(float v, float *shared)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float r = 0.0f;
+    for (int i = 0; i < int(blockDim.x >> 5); ++i) r += shared[i];
+    return r;
+}
+
+// One block per row: its log-sum-exp and loss; FORM 0: no more, 1: fp16 exponentials in place to bf16 gradients, 2: fp32 to fp16,
+// 3: fp32 to three bf16 planes.  Bound by reading and writing the exponentials once.
+template <int FORM>
+__global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
+{
+    __shared__ float shared[8];
+    const long long row = blockIdx.x;
+    const float2 *stats = A.stats + row * A.segments;
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < A.segments; i += 256) top = fmaxf(top, stats[i].x);
+    top = block_max(top, shared);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < A.segments; i += 256) {
+        const float2 s = stats[i];
+        sum += s.x == -INFINITY ? s.y : s.y * __expf(s.x - base);
+    }
+    sum = block_sum(sum, shared);
+    const long long label = A.labels[row];
+    const bool counts = label != A.ignore, known = label >= 0 && label < A.classes;
+    const float lse = base + logf(sum);
+    // a label outside the classes shows in the loss and in every gradient
+    const float scale = !counts ? 0.0f : known ? A.stored : NAN;
+    if (threadIdx.x == 0) {
+        A.row_loss[row] = !counts ? 0.0f : known ? lse - A.label_logit[row] : NAN;
+        if (FORM == 0 && A.lse) {
+            A.lse[row] = lse;
+            A.row_scale[row] = scale;
+        }
+    }
+    if (FORM == 0) return;
+    const int groups = int(A.line / 8);
+    for (int i = threadIdx.x; i < groups; i += 256) {
+        const int c = i * 8;
+        const float first = stats[c / kSegment].x;
+        float factor = scale / sum;
+        if (first != -INFINITY) factor *= __expf(first - base);
+        if (!counts) factor = 0.0f;
+        float v[8];
+        if (FORM == 1) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(A.keep) + row * A.line + c);
+            const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 t = __half22float2(reinterpret_cast<const __half2 &>(u[j]));
+                v[2 * j] = t.x;
+                v[2 * j + 1] = t.y;
+            }
+        } else {
+            const float4 *from = reinterpret_cast<const float4 *>(static_cast<const float *>(A.keep) + row * A.line + c);
+            const float4 w0 = from[0], w1 = from[1];
+            v[0] = w0.x; v[1] = w0.y; v[2] = w0.z; v[3] = w0.w;
+            v[4] = w1.x; v[5] = w1.y; v[6] = w1.z; v[7] = w1.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = counts ? v[j] * factor : 0.0f;               // a row without a label stays out, whatever its logits are
+            if (c + j == label && counts) v[j] -= scale;
+        }
+        uint16_t *to = A.gradient + row * A.line + c;
+        for (int p = 0; p < (FORM == 3 ? 3 : 1); ++p, to += A.plane) {
+            unsigned u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = pack2(v[2 * j], v[2 * j + 1], FORM != 2);
+                if (FORM == 3) {
+                    const float2 t = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]));
+                    v[2 * j] -= t.x;
+                    v[2 * j + 1] -= t.y;
+                }
+            }
+            *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+}
+
+// The rows' losses added in a fixed order, and the factor of the gradients; one block.
+__global__ void __launch_bounds__(1024) loss_kernel(const float *__restrict__ row_loss, const long long *__restrict__ labels, long long rows, long long ignore,
+                                                    int mean, float grad_factor, float *loss, float *alpha)
+{
+    __shared__ float shared[32];
+    float sum = 0.0f, count = 0.0f, low = 0.0f;                 // compensated: a sum may run over a million rows
+    for (long long i = threadIdx.x; i < rows; i += 1024) {
+        if (labels[i] == ignore) continue;
+        const float y = row_loss[i] - low, t = sum + y;
+        low = isfinite(t) ? (t - sum) - y : 0.0f;
+        sum = t;
+        count += 1.0f;
+    }
+    sum = block_sum(sum, shared);
+    count = block_sum(count, shared);
+    if (threadIdx.x == 0) {
+        const float share = mean ? (count > 0.0f ? 1.0f / count : 0.0f) : 1.0f;
+        *loss = sum * share;
+        *alpha = grad_factor * share;
+    }
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+size_t largest(size_t a, size_t b) { return a > b ? a : b; }
+
+const void *const kUnknown = reinterpret_cast<const void *>(uintptr_t(2));
+
+Matrix x_of(const axc_entropy_desc &d, const void *x) { return {x, d.rows, d.inputs, d.x_row_stride, d.x_column_stride, d.type}; }
+Matrix kernel_of(const axc_entropy_desc &d, const void *k) { return {k, d.classes, d.inputs, d.kernel_column_stride, d.kernel_row_stride, d.type}; }
+
+// How a call runs: the exponentials kept, or so many classes at a time; and where the parts of its workspace lie.
+struct Layout {
+    bool gradients, kept;
+    long long piece, line;                     // classes at a time, and values from row to row of what is stored for them
+    int segments;
+    size_t x, kernel, stats, rows, keep, gradient, dx, part, scratch, total;
+};
+
+Layout layout_of(const axc_entropy_desc &d, bool gradients, const void *x, const void *kernel, const DeviceInfo &di)
+{
+    Layout l = {};
+    const int planes = d.type == kFloat32 ? 3 : 1;
+    const long long whole = (d.classes + kSegment - 1) / kSegment * kSegment;
+    const size_t keep_bytes = d.type == kBfloat16 ? 2 : 4, gradient_bytes = d.type == kFloat32 ? 6 : d.type == kFloat16 ? 2 : 0;
+    l.gradients = gradients;
+    l.segments = int(whole / kSegment);
+    const size_t limit = d.scratch_limit > 0 ? size_t(d.scratch_limit) : size_t(AXC_ENTROPY_SCRATCH);
+    l.kept = gradients && size_t(d.rows) * size_t(whole) * (keep_bytes + gradient_bytes) <= limit;
+    l.piece = whole;
+    if (gradients && !l.kept) {
+        // as few pieces as the limit allows, of equal size, at least 256 classes
+        const size_t each = size_t(d.rows) * 2 * planes, most = limit / (each ? each : 1) / 256 * 256;
+        const long long cap = most < 256 ? 256 : (long long)most < whole ? (long long)most : whole;
+        const long long pieces = (whole + cap - 1) / cap;
+        l.piece = ((whole + pieces - 1) / pieces + 255) / 256 * 256;
+    }
+    l.line = l.piece < whole ? l.piece : whole;
+    l.x = 256;
+    l.kernel = l.x + up(operand_bytes(x_of(d, x)));
+    l.stats = l.kernel + up(operand_bytes(kernel_of(d, kernel)));
+    l.rows = l.stats + up(size_t(d.rows) * l.segments * 8);
+    l.keep = l.rows + 4 * up(size_t(d.rows) * 4) + 256;
+    l.gradient = l.keep + (l.kept ? up(size_t(d.rows) * l.line * keep_bytes) : 0);
+    if (gradients && l.kept && d.type == kBfloat16) l.gradient = l.keep;
+    l.dx = l.keep;
+    if (gradients) l.dx = (l.kept && d.type == kBfloat16 ? l.keep + up(size_t(d.rows) * l.line * 2) : l.gradient + up(size_t(d.rows) * l.line * 2 * planes));
+    l.part = l.dx + (gradients && !l.kept ? up(size_t(d.rows) * size_t((d.inputs + 3) / 4 * 4) * 4) : 0);
+    l.scratch = l.part + (gradients ? up(slope_scratch(d.rows, l.line)) : 0);
+    size_t most = 0;
+    if (gradients) {
+        // pieces are equal but for the last
+        const long long sizes[2] = {l.kept ? d.classes : l.piece < d.classes ? l.piece : d.classes, l.kept ? d.classes : d.classes - (d.classes - 1) / l.piece * l.piece};
+        for (int i = 0; i < 2; ++i) {
+            most = largest(most, gemm_scratch(d.rows, d.inputs, sizes[i], planes, di));
+            most = largest(most, d.kernel_gradient_transposed ? gemm_scratch(sizes[i], d.inputs, d.rows, planes, di) : gemm_scratch(d.inputs, sizes[i], d.rows, planes, di));
+        }
+    }
+    l.total = l.scratch + up(most);
+    return l;
+}
+
+int check_desc(const axc_entropy_desc *d)
+{
+    if (!d || d->type < kFloat32 || d->type > kFloat16 || d->bias_type < kFloat32 || d->bias_type > kFloat16) return AXC_INVALID_ARGUMENT;
+    if (d->rows < 0 || d->inputs < 1 || d->classes < 1 || d->rows > 0x7fffff00ll || d->inputs > 0x7fffff00ll || d->classes > 0x7fffff00ll) return AXC_INVALID_ARGUMENT;
+    if (d->x_row_stride < 0 || d->x_column_stride < 0 || d->kernel_row_stride < 0 || d->kernel_column_stride < 0) return AXC_INVALID_ARGUMENT;
+    if (d->reduction != AXC_REDUCE_MEAN && d->reduction != AXC_REDUCE_SUM) return AXC_INVALID_ARGUMENT;
+    return AXC_OK;
+}
+
+int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const void *kernel, const void *bias, const long long *labels, float *loss, float *row_loss,
+            void *dx, void *dkernel, void *dbias, char *ws, const DeviceInfo &di, cudaStream_t stream)
+{
+    const int planes = d.type == kFloat32 ? 3 : 1;
+    const float stored = d.type == kFloat16 ? kHalfScale : 1.0f;
+    unsigned *status = reinterpret_cast<unsigned *>(ws);
+    const size_t per_row = up(size_t(d.rows) * 4);
+    float *label_logit = reinterpret_cast<float *>(ws + l.rows), *lse = reinterpret_cast<float *>(ws + l.rows + per_row);
+    float *row_scale = reinterpret_cast<float *>(ws + l.rows + 2 * per_row), *alpha = reinterpret_cast<float *>(ws + l.rows + 4 * per_row);
+    if (!row_loss) row_loss = reinterpret_cast<float *>(ws + l.rows + 3 * per_row);
+    Gemm g = {};
+    g.planes = planes;
+    g.bf16 = d.type != kFloat16;
+    Operand ox = {}, ok = {};
+    int rc = AXC_OK;
+    if (d.rows > 0) {
+        rc = make_operand(x_of(d, x), ws + l.x, &ox, di, stream);
+        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + l.kernel, &ok, di, stream);
+        if (rc) return rc;
+        g.m = d.rows;
+        g.n = d.classes;
+        g.k = d.inputs;
+        g.a = ox;
+        g.b = ok;
+        EntropyArgs e = {};
+        e.bias = bias;
+        e.bias_type = d.bias_type;
+        e.labels = labels;
+        e.keep = l.kept ? ws + l.keep : nullptr;
+        e.line = l.line;
+        e.keep_fp32 = d.type != kBfloat16;
+        e.stats = reinterpret_cast<float2 *>(ws + l.stats);
+        e.segments = l.segments;
+        e.label_logit = label_logit;
+        rc = gemm_entropy(g, e, false, status, true, di, stream);
+        if (rc) return rc;
+        RowArgs r = {};
+        r.rows = d.rows;
+        r.classes = d.classes;
+        r.labels = labels;
+        r.ignore = d.ignore_index;
+        r.stats = e.stats;
+        r.segments = l.segments;
+        r.label_logit = label_logit;
+        r.lse = l.gradients ? lse : nullptr;
+        r.row_scale = row_scale;
+        r.row_loss = row_loss;
+        r.stored = stored;
+        r.keep = e.keep;
+        r.line = l.line;
+        r.gradient = reinterpret_cast<uint16_t *>(ws + l.gradient);
+        r.plane = l.line * d.rows;
+        const unsigned grid = unsigned(d.rows);
+        if (!l.kept) row_kernel<0><<<grid, 256, 0, stream>>>(r);
+        else if (d.type == kBfloat16) row_kernel<1><<<grid, 256, 0, stream>>>(r);
+        else if (d.type == kFloat16) row_kernel<2><<<grid, 256, 0, stream>>>(r);
+        else row_kernel<3><<<grid, 256, 0, stream>>>(r);
+        count_launch();
+    } else AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), stream));
+    loss_kernel<<<1, 1024, 0, stream>>>(row_loss, labels, d.rows, d.ignore_index, d.reduction == AXC_REDUCE_MEAN, d.grad_scale / stored, loss, alpha);
+    count_launch();
+    if (!l.gradients) return AXC_OK;
+    const size_t size = type_size(d.type);
+    float *dx_sum = reinterpret_cast<float *>(ws + l.dx);
+    const long long dx_line = (d.inputs + 3) / 4 * 4;
+    for (long long c0 = 0; c0 < d.classes; c0 += l.kept ? d.classes : l.piece) {
+        const long long n = l.kept ? d.classes : d.classes - c0 < l.piece ? d.classes - c0 : l.piece;
+        Operand part = ok;                     // the kernel's rows from class c0 on
+        part.data = static_cast<const uint16_t *>(ok.data) + (ok.rows_contiguous ? c0 : c0 * ok.line);
+        if (!l.kept && d.rows > 0) {
+            Gemm again = g;
+            again.n = n;
+            again.b = part;
+            EntropyArgs e = {};
+            e.bias = bias;
+            e.bias_type = d.bias_type;
+            e.labels = labels;
+            e.keep = ws + l.gradient;
+            e.line = l.line;
+            e.plane = l.line * d.rows;
+            e.lse = lse;
+            e.row_scale = row_scale;
+            e.column0 = int(c0);
+            rc = gemm_entropy(again, e, true, status, false, di, stream);
+            if (rc) return rc;
+        }
+        const Operand dl = {ws + l.gradient, l.line, l.line * d.rows, false};
+        Gemm p = {};
+        p.planes = planes;
+        p.bf16 = g.bf16;
+        p.fin.alpha = 1.0f;
+        p.fin.alpha_dev = alpha;
+        if (dx) {
+            const bool last = c0 + n >= d.classes;
+            p.m = d.rows;
+            p.n = d.inputs;
+            p.k = n;
+            p.a = dl;
+            p.b = transposed(part);
+            p.fin.addend = c0 > 0 ? dx_sum : nullptr;
+            p.fin.addend_type = kFloat32;
+            p.fin.addend_line = dx_line;
+            p.fin.out = last ? dx : dx_sum;
+            p.fin.out_type = last ? d.type : kFloat32;
+            p.fin.out_line = last ? d.inputs : dx_line;
+            rc = gemm(p, ws + l.scratch, status, false, di, stream);
+            if (rc) return rc;
+            p.fin.addend = nullptr;
+        }
+        if (dkernel) {
+            p.k = d.rows;
+            p.fin.out_type = d.type;
+            if (d.kernel_gradient_transposed) {
+                p.m = n;
+                p.n = d.inputs;
+                p.a = transposed(dl);
+                p.b = transposed(ox);
+                p.fin.out = static_cast<char *>(dkernel) + size_t(c0) * size_t(d.inputs) * size;
+                p.fin.out_line = d.inputs;
+            } else {
+                p.m = d.inputs;
+                p.n = n;
+                p.a = transposed(ox);
+                p.b = transposed(dl);
+                p.fin.out = static_cast<char *>(dkernel) + size_t(c0) * size;
+                p.fin.out_line = d.classes;
+            }
+            rc = gemm(p, ws + l.scratch, status, false, di, stream);
+            if (rc) return rc;
+        }
+        if (dbias) {
+            Slope s = {};
+            s.dy = ws + l.gradient;
+            s.type = d.type == kFloat16 ? kFloat16 : kBfloat16;
+            s.dy_planes = planes;
+            s.plane = l.line * d.rows;
+            s.rows = d.rows;
+            s.columns = n;
+            s.dy_line = l.line;
+            s.sums = static_cast<char *>(dbias) + size_t(c0) * type_size(d.bias_type);
+            s.sums_type = d.bias_type;
+            s.scale = 1.0f;
+            s.scale_dev = alpha;
+            rc = slope(s, ws + l.part, di, stream);
+            if (rc) return rc;
+        }
+    }
+    return AXC_OK;
+}
+
+}  // namespace
+}  // namespace axc
+
+extern "C" int axc_entropy_workspace_bytes(const axc_entropy_desc *desc, const void *x, const void *kernel, int device, size_t *loss_only, size_t *gradients)
+{
+    using namespace axc;
+    int rc = check_desc(desc);
+    if (rc) return rc;
+    DeviceInfo di;
+    rc = device_info(device, &di);
+    if (rc) return rc;
+    if (!x) x = kUnknown;
+    if (!kernel) kernel = kUnknown;
+    if (loss_only) *loss_only = layout_of(*desc, false, x, kernel, di).total;
+    if (gradients) *gradients = layout_of(*desc, true, x, kernel, di).total;
+    return AXC_OK;
+}
+
+extern "C" int axc_entropy(const axc_entropy_desc *desc, const void *x, const void *kernel, const void *bias, const int64_t *labels, float *loss, float *row_loss,
+                           void *dx, void *dkernel, void *dbias, void *workspace, size_t workspace_bytes, int device, void *stream)
+{
+    using namespace axc;
+    int rc = check_desc(desc);
+    if (rc) return rc;
+    const axc_entropy_desc &d = *desc;
+    if (!loss || !kernel || (d.rows > 0 && (!x || !labels))) return AXC_INVALID_ARGUMENT;
+    DeviceInfo di;
+    rc = device_info(device, &di);
+    if (rc) return rc;
+    const bool gradients = dx || dkernel || dbias;
+    const Layout l = layout_of(d, gradients, x ? x : kUnknown, kernel, di);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < l.total) return AXC_INTERNAL;
+    int prev = 0;
+    AXC_CUDA(cudaGetDevice(&prev));
+    if (prev != device) AXC_CUDA(cudaSetDevice(device));
+    rc = entropy(d, l, x, kernel, bias, reinterpret_cast<const long long *>(labels), loss, row_loss, dx, dkernel, dbias, static_cast<char *>(workspace), di,
+                 cudaStream_t(stream));
+    const cudaError_t e = cudaGetLastError();
+    if (prev != device) cudaSetDevice(prev);
+    return rc != AXC_OK ? rc : e == cudaSuccess ? AXC_OK : cuda_failed(e);
+}

@@ -1,0 +1,786 @@
+// Matrix products on the 5th-generation tensor cores: out[m, n] = sum over k of a[m, k] b[n, k], either operand with k or with its
+// rows contiguous, so that a layer's forward product and both of its gradients read their operands where they lie.
+//
+// A CTA (or a pair of CTAs on two SMs that share one tile) is persistent and walks over tiles.  One thread keeps a ring of stages
+// of 64 k full with tiled bulk copies (128-byte swizzle), one thread issues the matrix instructions, whose sums stay in tensor
+// memory, and eight warps take finished sums out while the next tile's are being made in the other half of the tensor memory.
+//   pairs, 256 x 256 tiles    each SM loads 128 rows of a and half of b: 64 bytes of shared memory written and as many read per
+//                             clock, half of what a lone SM needs for 128 x 256
+//   lone CTAs, 128 x N tiles  for products with too few tiles to fill the GPU, and for few rows (then the weights are `a`)
+//
+// fp32 operands are split exactly into three bf16 terms, x = x0 + x1 + x2, each 2^-8 of the one before; six of the nine products
+// of terms are summed (x2 y0, x1 y1, x0 y2, x1 y0, x0 y1, x0 y0), the three left out are below 2^-24 of x y.
+//
+// Sums are fp32.  The tensor cores cut a sum off at 24 bits at every step of 16 k (measured: 2e-8 of it on average, always towards
+// zero), which 16-bit results do not show.  For fp32 the sums of every 64 k, the small products first, are taken out and added in
+// registers, with rounding: an error of 1e-7 instead of 2e-5 at k = 16384; the eight warps do that while the next 64 k run.
+//
+// Products whose tiles are too few have k split over CTAs; the partial sums are added in a fixed order by a second
+// kernel, which also applies what follows the product.
+#include <cudaTypedefs.h>
+
+#include "axc_gemm.h"
+#include "axc_mma.cuh"
+
+namespace axc {
+namespace {
+
+constexpr int kStageK = 64;                    // k of a stage: 128 bytes, a swizzled line
+constexpr int kThreads = 384;                  // warps: 0 loads, 1 multiplies, 2 holds the tensor memory, 4 to 11 take the sums out
+constexpr unsigned kHeader = 1024;             // barriers and such, before the stages
+constexpr unsigned kSmem = 227 * 1024;
+constexpr int kMaxStages = 12;
+constexpr int kSegment = 64;                   // columns whose exponentials share a largest logit
+
+enum { kStore = 0, kPartial = 1, kEntropy = 2, kGradient = 3 };
+
+struct GemmArgs {
+    CUtensorMap map_a, map_b;
+    int m, n;
+    int tiles_m, tiles_n, splits, k_steps;     // k_steps: stages of the whole k
+    int planes, stages;
+    unsigned a_bytes, b_bytes;                 // of one plane of a stage, per CTA
+    unsigned a_box_rows, b_box_rows;           // a box has that many rows (k contiguous), or 64 (rows contiguous)
+    bool a_rows, b_rows;
+    unsigned shape;
+    bool swapped;                              // m runs along the output's lines: out[n][m]
+    Finish fin;
+    EntropyArgs ent;
+    float *part;                               // [split][line][part_line]
+    long long part_line, part_stride;
+    unsigned *status;
+    bool first;                                // of a call: clears the status
+};
+
+struct Header {                                // in shared memory
+    uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2];
+    unsigned tmem;
+};
+
+__device__ __forceinline__ float activate(float z, int act)
+{
+    if (act == kActRelu) return max_keep_nan(z, 0.0f);
+    if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    if (act == kActSilu) return z / (1.0f + __expf(-z));
+    return z;
+}
+
+// One row of W sums (columns n0 ..), W a multiple of 16
+template <int W>
+__device__ __forceinline__ void finish_row(const GemmArgs &P, unsigned (&x)[W], int row, int n0, float alpha)
+{
+    const Finish &f = P.fin;
+    if (row >= P.m || n0 >= P.n) return;
+    const bool full = n0 + W <= P.n;
+    float v[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = alpha * __uint_as_float(x[i]);
+    if (P.swapped) {                           // neighbouring lanes write neighbouring values
+        const float bias = f.bias ? load_as_float(f.bias, row, f.bias_type) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if (n0 + i < P.n) {
+                float z = v[i] + bias;
+                if (f.addend) z += load_as_float(f.addend, (long long)(n0 + i) * f.addend_line + row, f.addend_type);
+                const long long at = (long long)(n0 + i) * f.out_line + row;
+                if (f.pre) store_from_float(f.pre, at, f.out_type, z);
+                store_from_float(f.out, at, f.out_type, activate(z, f.activation));
+            }
+        }
+        return;
+    }
+    if (f.bias) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (full || n0 + i < P.n) v[i] += load_as_float(f.bias, n0 + i, f.bias_type);
+    }
+    if (f.addend) {
+        const char *at = static_cast<const char *>(f.addend) + ((long long)row * f.addend_line + n0) * (f.addend_type == kFloat32 ? 4 : 2);
+        if (full && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+            if (f.addend_type == kFloat32) {
+#pragma unroll
+                for (int i = 0; i < W; i += 4) {
+                    const float4 w = *reinterpret_cast<const float4 *>(at + i * 4);
+                    v[i] += w.x; v[i + 1] += w.y; v[i + 2] += w.z; v[i + 3] += w.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; i += 8) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(at + i * 2);
+                    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 t = f.addend_type == kBfloat16 ? __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]))
+                                                                    : __half22float2(reinterpret_cast<const __half2 &>(u[j]));
+                        v[i + 2 * j] += t.x;
+                        v[i + 2 * j + 1] += t.y;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (full || n0 + i < P.n) v[i] += load_as_float(f.addend, (long long)row * f.addend_line + n0 + i, f.addend_type);
+        }
+    }
+#pragma unroll 1
+    for (int pass = f.pre ? 0 : 1; pass < 2; ++pass) {
+        void *base = pass == 0 ? f.pre : f.out;
+        if (pass == 1 && f.activation != kActNone) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = activate(v[i], f.activation);
+        }
+        char *at = static_cast<char *>(base) + ((long long)row * f.out_line + n0) * (f.out_type == kFloat32 ? 4 : 2);
+        if (full && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+            if (f.out_type == kFloat32) {
+#pragma unroll
+                for (int i = 0; i < W; i += 4) *reinterpret_cast<float4 *>(at + i * 4) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+                const bool bf16 = f.out_type == kBfloat16;
+#pragma unroll
+                for (int i = 0; i < W; i += 8)
+                    *reinterpret_cast<uint4 *>(at + i * 2) = make_uint4(pack2(v[i], v[i + 1], bf16), pack2(v[i + 2], v[i + 3], bf16),
+                                                                        pack2(v[i + 4], v[i + 5], bf16), pack2(v[i + 6], v[i + 7], bf16));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (full || n0 + i < P.n) store_from_float(base, (long long)row * f.out_line + n0 + i, f.out_type, v[i]);
+        }
+    }
+}
+
+// Partial sums in the order of the output's lines
+template <int W>
+__device__ __forceinline__ void store_part(const GemmArgs &P, unsigned (&x)[W], int row, int n0, int split)
+{
+    if (row >= P.m || n0 >= P.n) return;
+    float *part = P.part + (long long)split * P.part_stride;
+    if (P.swapped) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (n0 + i < P.n) part[(long long)(n0 + i) * P.part_line + row] = __uint_as_float(x[i]);
+        return;
+    }
+    float *at = part + (long long)row * P.part_line + n0;      // lines are padded to 4 values
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+        if (n0 + i < P.n)
+            *reinterpret_cast<float4 *>(at + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+}
+
+// One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
+// A segment of -inf has the exponentials 0 (relative to 0, not to itself).
+__device__ __forceinline__ void entropy_segment(const GemmArgs &P, unsigned (&x0)[32], unsigned (&x1)[32], int row, int n0)
+{
+    const EntropyArgs &e = P.ent;
+    if (row >= P.m || n0 >= P.n) return;
+    float top = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+        float l = __uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]);
+        if (n0 + i < P.n) {
+            if (e.bias) l += load_as_float(e.bias, n0 + i, e.bias_type);
+        } else l = -INFINITY;
+        if (i < 32) x0[i & 31] = __float_as_uint(l);
+        else x1[i & 31] = __float_as_uint(l);
+        top = fmaxf(top, l);
+        nan |= l != l;
+    }
+    const long long label = e.labels[row] - n0;
+    if (label >= 0 && label < kSegment && n0 + label < P.n) {
+        float mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            if (i == int(label)) mine = __uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]);
+        e.label_logit[row] = mine;
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+        const float p = __expf(__uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]) - base);
+        sum += p;
+        if (i < 32) x0[i & 31] = __float_as_uint(p);
+        else x1[i & 31] = __float_as_uint(p);
+    }
+    if (nan) sum = NAN;
+    e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, sum);
+    if (!e.keep) return;
+    if (e.keep_fp32) {
+        float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(e.keep) + (long long)row * e.line + n0);
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+            unsigned u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = i + j < 32 ? x0[(i + j) & 31] : x1[(i + j) & 31];
+            to[i / 4] = make_float4(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3]));
+        }
+    } else {
+        uint4 *to = reinterpret_cast<uint4 *>(static_cast<__half *>(e.keep) + (long long)row * e.line + n0);
+#pragma unroll
+        for (int i = 0; i < 64; i += 8) {
+            unsigned u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = i + 2 * j;
+                u[j] = pack2(__uint_as_float(c < 32 ? x0[c & 31] : x1[c & 31]), __uint_as_float(c < 32 ? x0[(c + 1) & 31] : x1[(c + 1) & 31]), false);
+            }
+            to[i / 8] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+}
+
+// 32 logits of a row and what the loss's gradient is there: row_scale * (exp(logit - lse) - [label])
+__device__ __forceinline__ void gradient_columns(const GemmArgs &P, unsigned (&x)[32], int row, int n0)
+{
+    const EntropyArgs &e = P.ent;
+    if (row >= P.m || n0 >= e.line) return;
+    const float lse = e.lse[row], scale = e.row_scale[row];
+    const long long label = e.labels[row] - e.column0 - n0;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        v[i] = 0.0f;
+        if (n0 + i < P.n && scale != 0.0f) {
+            float l = __uint_as_float(x[i]);
+            if (e.bias) l += load_as_float(e.bias, e.column0 + n0 + i, e.bias_type);
+            v[i] = scale * (__expf(l - lse) - (label == i ? 1.0f : 0.0f));
+        }
+    }
+    uint16_t *keep = static_cast<uint16_t *>(e.keep) + (long long)row * e.line + n0;
+    const bool bf16 = P.shape >> 7 & 1;
+    for (int plane = 0; plane < P.planes; ++plane) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            unsigned u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = pack2(v[i + 2 * j], v[i + 2 * j + 1], bf16);
+                if (P.planes == 3) {
+                    const float2 t = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]));
+                    v[i + 2 * j] -= t.x;
+                    v[i + 2 * j + 1] -= t.y;
+                }
+            }
+            *reinterpret_cast<uint4 *>(keep + i) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        keep += e.plane;
+    }
+}
+
+// tile index -> place: groups of 8 rows of tiles, so that the tiles in flight share lines of both operands
+__device__ __forceinline__ void place_of(const GemmArgs &P, int tile, int &tm, int &tn)
+{
+    const int per = 8 * P.tiles_n, group = tile / per, first = group * 8, rows = min(8, P.tiles_m - first);
+    tm = first + (tile - group * per) % rows;
+    tn = (tile - group * per) / rows;
+}
+
+// CG: CTAs per tile.  BN: columns of a tile.  MODE: what becomes of the sums.  PLANES: terms of an operand.
+template <int CG, int BN, int MODE, int PLANES>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs P)
+{
+    constexpr int TM = 128 * CG;
+    constexpr unsigned kColumns = BN < 32 ? 32 : BN;           // tensor memory of one tile's sums
+    constexpr int kBuffers = 2;
+    extern __shared__ char raw[];
+    const unsigned base = (mma::smem_address(raw) + 1023u) & ~1023u;
+    Header *head = reinterpret_cast<Header *>(raw + (base - mma::smem_address(raw)));
+    const unsigned ring = base + kHeader, stage_bytes = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
+    const unsigned full = mma::smem_address(head->full), empty = mma::smem_address(head->empty);
+    const unsigned sums_full = mma::smem_address(head->sums_full), sums_empty = mma::smem_address(head->sums_empty);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = CG == 2 ? mma::cluster_rank() : 0u;
+    const int worker = int(blockIdx.x) / CG, workers = int(gridDim.x) / CG;
+    const int units = P.tiles_m * P.tiles_n * P.splits;
+
+    if (threadIdx.x == 0) {
+        if (P.first && blockIdx.x == 0) *P.status = 0u;        // a wait runs out after a second, not before this
+        for (int i = 0; i < P.stages; ++i) {
+            mma::barrier_init(full + 8 * i, 1);
+            mma::barrier_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < kBuffers; ++i) {
+            mma::barrier_init(sums_full + 8 * i, 1);
+            mma::barrier_init(sums_empty + 8 * i, 8 * CG);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mma::prefetch_map(&P.map_a);
+        mma::prefetch_map(&P.map_b);
+    }
+    if (warp == 2) mma::tmem_alloc<CG>(mma::smem_address(&head->tmem), kColumns * kBuffers);
+    mma::fence_before();
+    if (CG == 2) mma::cluster_sync();
+    else __syncthreads();
+    mma::fence_after();
+    const unsigned tmem = head->tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // operands may come from the kernel before
+    bool ok = true;
+
+    if (warp == 0 && lane == 0) {
+        const unsigned signal = CG == 2 ? mma::in_cta(full, 0) : full;
+        int s = 0;
+        unsigned phase = 1;
+        for (int u = worker; u < units && ok; u += workers) {
+            int tm, tn;
+            place_of(P, u / P.splits, tm, tn);
+            const int split = u % P.splits;
+            const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
+            const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
+            for (int k = k0; k < k1; ++k) {
+                if (!(ok = mma::barrier_wait(empty + 8 * s, phase))) break;
+                if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
+                unsigned at = ring + unsigned(s) * stage_bytes;
+                for (int p = 0; p < PLANES; ++p) {
+                    if (P.a_rows) {
+                        for (int r = 0; r < 128; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_a, signal + 8 * s, row_a + r, k * kStageK, p);
+                    } else mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kStageK, row_a, p);
+                    at += P.a_bytes;
+                    if (P.b_rows) {
+                        for (int r = 0; r < BN / CG; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_b, signal + 8 * s, row_b + r, k * kStageK, p);
+                    } else mma::load_box<CG>(at, &P.map_b, signal + 8 * s, k * kStageK, row_b, p);
+                    at += P.b_bytes;
+                }
+                if (++s == P.stages) s = 0, phase ^= 1u;
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        int s = 0, buffer = 0;
+        unsigned phase = 0, sums_phase = 1;
+        // the products of the three terms, smallest first: the terms of a and of b
+        const unsigned of_a = PLANES == 3 ? 0x001012u : 0u, of_b = PLANES == 3 ? 0x010210u : 0u;
+        constexpr int kProducts = PLANES == 3 ? 6 : 1;
+        const unsigned chunk_a = P.a_rows ? 8192u : 0u, chunk_b = P.b_rows ? 8192u : 0u;
+        const unsigned step_a = P.a_rows ? 2048u : 32u, step_b = P.b_rows ? 2048u : 32u;
+        for (int u = worker; u < units && ok; u += workers) {
+            const int split = u % P.splits;
+            const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
+            unsigned d = 0;
+            for (int k = k0; k < k1; ++k) {
+                if (PLANES == 3 || k == k0) {
+                    if (!(ok = mma::barrier_wait(sums_empty + 8 * buffer, sums_phase))) break;
+                    d = tmem + unsigned(buffer) * kColumns;
+                }
+                if (!(ok = mma::barrier_wait(full + 8 * s, phase))) break;
+                mma::fence_after();
+                const unsigned at = ring + unsigned(s) * stage_bytes;
+#pragma unroll
+                for (int q = 0; q < kProducts; ++q) {
+                    const unsigned a = at + (of_a >> (4 * q) & 15u) * (P.a_bytes + P.b_bytes);
+                    const unsigned b = at + (of_b >> (4 * q) & 15u) * (P.a_bytes + P.b_bytes) + P.a_bytes;
+#pragma unroll
+                    for (int j = 0; j < kStageK / 16; ++j)
+                        mma::multiply<CG>(d, mma::operand(a + j * step_a, chunk_a), mma::operand(b + j * step_b, chunk_b), P.shape,
+                                          (PLANES == 1 && k > k0) || q > 0 || j > 0);
+                }
+                mma::commit<CG>(empty + 8 * s);
+                if (++s == P.stages) s = 0, phase ^= 1u;
+                if (PLANES == 3 || k + 1 == k1) {
+                    mma::commit<CG>(sums_full + 8 * buffer);
+                    if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // warps 4 to 7 take the first half of the columns, 8 to 11 the second; a warp reaches the 32 lanes of its place in four
+        constexpr int kHalves = BN >= 128 ? 2 : 1;
+        const int half = (warp - 4) >> 2, quarter = warp & 3;
+        const float alpha = MODE == kStore ? P.fin.alpha * (P.fin.alpha_dev ? *P.fin.alpha_dev : 1.0f) : 1.0f;
+        int buffer = 0;
+        unsigned phase = 0;
+        constexpr int kMine = BN / kHalves, W = kMine < 32 ? 16 : 32;
+        for (int u = worker; u < units && ok; u += workers) {
+            int tm, tn;
+            place_of(P, u / P.splits, tm, tn);
+            const int split = u % P.splits;
+            const int row = tm * TM + int(rank) * 128 + quarter * 32 + lane, n0 = tn * BN + half * kMine;
+            // sums of columns c .. c + W (entropy: both halves of a segment)
+            auto take = [&](unsigned (&x)[W], int c) {
+                if constexpr (MODE == kStore) finish_row<W>(P, x, row, n0 + c, alpha);
+                else if constexpr (MODE == kPartial) store_part<W>(P, x, row, n0 + c, split);
+                else if constexpr (MODE == kGradient) gradient_columns(P, x, row, n0 + c);
+            };
+            const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
+            if constexpr (PLANES == 3) {
+                const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
+                unsigned sum[kMine / W][W];
+#pragma unroll
+                for (int c = 0; c < kMine / W; ++c)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) sum[c][i] = 0u;
+                for (int k = k0; k < k1; ++k) {
+                    if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
+                    mma::fence_after();
+                    __syncwarp();
+                    if (half < kHalves) {
+#pragma unroll
+                        for (int c = 0; c < kMine / W; ++c) {
+                            unsigned x[W];
+                            mma::load_columns(mine + unsigned(buffer) * kColumns + c * W, x);
+                            mma::load_wait(x);
+#pragma unroll
+                            for (int i = 0; i < W; ++i) sum[c][i] = __float_as_uint(__uint_as_float(sum[c][i]) + __uint_as_float(x[i]));
+                        }
+                    }
+                    mma::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mma::barrier_arrive_cluster(mma::in_cta(sums_empty + 8 * buffer, 0));
+                    if (++buffer == kBuffers) buffer = 0, phase ^= 1u;
+                }
+                if (!ok) break;
+                if (half < kHalves) {
+                    if constexpr (MODE == kEntropy) entropy_segment(P, sum[0], sum[1], row, n0);
+                    else {
+#pragma unroll
+                        for (int c = 0; c < kMine / W; ++c) take(sum[c], c * W);
+                    }
+                }
+            } else {
+                if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
+                mma::fence_after();
+                __syncwarp();
+                if (half < kHalves) {
+                    const unsigned at = mine + unsigned(buffer) * kColumns;
+                    constexpr int kStep = MODE == kEntropy ? kSegment : W;
+#pragma unroll 1
+                    for (int c = 0; c < kMine; c += kStep) {
+                        unsigned x[W];
+                        mma::load_columns(at + c, x);
+                        if constexpr (MODE == kEntropy) {
+                            unsigned y[W];
+                            mma::load_columns(at + c + 32, y);
+                            mma::load_wait(x);
+                            mma::load_wait(y);
+                            entropy_segment(P, x, y, row, n0 + c);
+                        } else {
+                            mma::load_wait(x);
+                            take(x, c);
+                        }
+                    }
+                }
+                mma::fence_before();
+                __syncwarp();
+                if (lane == 0) mma::barrier_arrive_cluster(mma::in_cta(sums_empty + 8 * buffer, 0));
+                if (++buffer == kBuffers) buffer = 0, phase ^= 1u;
+            }
+        }
+    }
+    if (!ok) {
+        // A wait ran out: no further copy is started; those in flight end within microseconds, this waits for milliseconds.
+        atomicMax(P.status, 3u);
+        for (int i = 0; i < 64; ++i) __nanosleep(200000);
+    }
+    __syncwarp();
+    mma::fence_before();
+    if (CG == 2) mma::cluster_sync();
+    else __syncthreads();
+    if (warp == 2) {
+        mma::fence_after();
+        mma::tmem_free<CG>(tmem, kColumns * kBuffers);
+    }
+}
+
+// The partial sums of a split product, added in the order of the splits, and what follows the product
+__global__ void __launch_bounds__(256) finish_kernel(const float *__restrict__ part, long long stride, long long part_line, int splits, int lines,
+                                                     int columns, const Finish f)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int quads = (columns + 3) / 4;
+    const long long total = (long long)lines * quads;
+    const float alpha = f.alpha * (f.alpha_dev ? *f.alpha_dev : 1.0f);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long line = i / quads;
+        const int c = int(i - line * quads) * 4;
+        const float *at = part + line * part_line + c;
+        float4 s = splits > 0 ? *reinterpret_cast<const float4 *>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 1; k < splits; ++k) {
+            const float4 t = *reinterpret_cast<const float4 *>(at + k * stride);
+            s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+        }
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j < columns) {
+                float z = alpha * v[j];
+                if (f.bias) z += load_as_float(f.bias, c + j, f.bias_type);
+                if (f.addend) z += load_as_float(f.addend, line * f.addend_line + c + j, f.addend_type);
+                if (f.pre) store_from_float(f.pre, line * f.out_line + c + j, f.out_type, z);
+                store_from_float(f.out, line * f.out_line + c + j, f.out_type, activate(z, f.activation));
+            }
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 encoder()
+{
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// Boxes of 64 k x `box` rows (k contiguous), or 64 rows x 64 k; what lies outside the matrix arrives as zeros.
+bool make_map(const Operand &o, long long rows, long long k, int planes, bool bf16, unsigned box, CUtensorMap *map)
+{
+    PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+    if (!encode) return false;
+    const cuuint64_t inner = cuuint64_t(o.rows_contiguous ? rows : k), outer = cuuint64_t(o.rows_contiguous ? k : rows);
+    const cuuint64_t dims[3] = {inner, outer, cuuint64_t(planes)};
+    const cuuint64_t line = cuuint64_t(o.line) * 2, strides[2] = {line, planes > 1 ? cuuint64_t(o.plane) * 2 : line};
+    const cuuint32_t boxes[3] = {64, o.rows_contiguous ? 64u : box, 1}, unit[3] = {1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(o.data), dims, strides,
+                  boxes, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a product is cut up: CTAs per tile, columns of a tile, splits of k; and whether the operands change places, so that the longer
+// of m and n runs over the 128 lanes.
+struct Plan {
+    int cg, bn, splits;
+    bool swapped;
+};
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, bool may_swap, int sms)
+{
+    Plan best = {1, 128, 1, false};
+    double least = 1e300;
+    const long long steps = ceil_div(k > 0 ? k : 1, kStageK);
+    for (int swapped = 0; swapped < (may_swap ? 2 : 1); ++swapped) {
+        const long long tall = swapped ? n : m, wide = swapped ? m : n;
+        for (int c = 0; c < 6; ++c) {
+            static const int kCg[6] = {2, 1, 1, 1, 1, 1}, kBn[6] = {256, 256, 128, 64, 32, 16};
+            // clocks of a stage: the matrix instructions, or the copies that feed a narrow tile
+            static const double kClocks[6] = {540, 620, 330, 220, 190, 180};
+            const int cg = kCg[c], bn = planes == 3 && cg == 2 ? 128 : kBn[c];
+            if (!may_swap && bn < 64) continue;                 // segments of 64 columns
+            if (planes == 3 && bn == 256) continue;             // its sums do not fit into registers
+            const long long tiles = ceil_div(tall, 128 * cg) * ceil_div(wide, bn);
+            const int workers = sms / cg;
+            for (int splits = 1; splits <= (may_split ? 16 : 1); splits *= 2) {
+                if (splits > 1 && steps / splits < 4) break;
+                const double waves = double(ceil_div(tiles * splits, workers));
+                double clocks = waves * (double(ceil_div(steps, splits)) * (planes == 3 ? (cg == 2 ? 270 : kClocks[c]) * 6 : kClocks[c]) + 600) + 4000;
+                if (splits > 1) clocks += 4500 + double(m) * n * splits * 8 / 3000;
+                if (clocks < least * 0.97) {
+                    least = clocks;
+                    best = {cg, bn, splits, swapped != 0};
+                }
+            }
+        }
+    }
+    return best;
+}
+
+template <int CG, int BN, int MODE, int PLANES>
+int launch(GemmArgs &P, long long units, const DeviceInfo &di, cudaStream_t stream)
+{
+    const unsigned stage = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
+    P.stages = int((kSmem - kHeader - 1024) / stage);
+    if (P.stages > kMaxStages) P.stages = kMaxStages;
+    const unsigned smem = kHeader + 1024 + unsigned(P.stages) * stage;
+    AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+    const long long workers = di.sm_count / CG;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned((units < workers ? units : workers) * CG));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AXC_CUDA(cudaLaunchKernelEx(&cfg, gemm_kernel<CG, BN, MODE, PLANES>, P));
+    count_launch();
+    return AXC_OK;
+}
+
+template <int MODE, int PLANES>
+int launch_tiles(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, cudaStream_t stream)
+{
+    if constexpr (PLANES == 1) {
+        if (plan.bn == 256) return plan.cg == 2 ? launch<2, 256, MODE, 1>(P, units, di, stream) : launch<1, 256, MODE, 1>(P, units, di, stream);
+    } else {
+        if (plan.cg == 2) return launch<2, 128, MODE, 3>(P, units, di, stream);
+    }
+    if (plan.bn == 128) return launch<1, 128, MODE, PLANES>(P, units, di, stream);
+    if (plan.bn == 64) return launch<1, 64, MODE, PLANES>(P, units, di, stream);
+    if constexpr (MODE == kStore || MODE == kPartial) {
+        if (plan.bn == 32) return launch<1, 32, MODE, PLANES>(P, units, di, stream);
+        return launch<1, 16, MODE, PLANES>(P, units, di, stream);
+    }
+    return AXC_INTERNAL;
+}
+
+template <int MODE>
+int launch_plan(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, cudaStream_t stream)
+{
+    return P.planes == 3 ? launch_tiles<MODE, 3>(P, plan, units, di, stream) : launch_tiles<MODE, 1>(P, plan, units, di, stream);
+}
+
+int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, GemmArgs *P)
+{
+    const Operand &a = plan.swapped ? g.b : g.a, &b = plan.swapped ? g.a : g.b;
+    const long long tall = plan.swapped ? g.n : g.m, wide = plan.swapped ? g.m : g.n;
+    if (tall > 0x7fffff00ll || wide > 0x7fffff00ll || g.k > 0x7fffff00ll) return AXC_INVALID_ARGUMENT;
+    const unsigned b_rows_per_cta = unsigned(plan.bn / plan.cg);
+    P->m = int(tall);
+    P->n = int(wide);
+    P->tiles_m = int(ceil_div(tall, 128 * plan.cg));
+    P->tiles_n = int(ceil_div(wide, plan.bn));
+    P->splits = plan.splits;
+    P->k_steps = int(ceil_div(g.k, kStageK));
+    P->planes = g.planes;
+    P->a_rows = a.rows_contiguous;
+    P->b_rows = b.rows_contiguous;
+    P->a_bytes = 128 * 128;
+    P->b_bytes = (b.rows_contiguous && b_rows_per_cta < 64 ? 64u : b_rows_per_cta) * 128u;
+    P->shape = mma::instruction_shape(128 * plan.cg, plan.bn, g.bf16, a.rows_contiguous, b.rows_contiguous);
+    P->swapped = plan.swapped;
+    P->fin = g.fin;
+    P->status = status;
+    P->first = first;
+    if (!make_map(a, tall, g.k, g.planes, g.bf16, 128, &P->map_a) || !make_map(b, wide, g.k, g.planes, g.bf16, b_rows_per_cta, &P->map_b))
+        return AXC_INTERNAL;
+    return AXC_OK;
+}
+
+int launch_finish(const float *part, long long stride, long long line, int splits, const Gemm &g, const DeviceInfo &di, cudaStream_t stream)
+{
+    const long long work = ceil_div(g.m * ceil_div(g.n, 4), 256), most = (long long)di.sm_count * 8;
+    finish_kernel<<<unsigned(work < most ? work : most), 256, 0, stream>>>(part, stride, line, splits, int(g.m), int(g.n), g.fin);
+    count_launch();
+    return AXC_OK;
+}
+
+}  // namespace
+
+size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di)
+{
+    if (m == 0 || n == 0 || k == 0) return 0;
+    const Plan plan = choose_plan(m, n, k, planes, true, true, di.sm_count);
+    return plan.splits > 1 ? size_t(plan.splits) * size_t(m) * size_t((n + 3) / 4 * 4) * 4 : 0;
+}
+
+int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream)
+{
+    if (g.m == 0 || g.n == 0) return AXC_OK;
+    if (g.k == 0) {                                             // sums of nothing
+        if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), stream));
+        return launch_finish(nullptr, 0, 0, 0, g, di, stream);
+    }
+    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, true, di.sm_count);
+    GemmArgs P = {};
+    int rc = fill_args(g, plan, status, first, &P);
+    if (rc) return rc;
+    const long long units = (long long)P.tiles_m * P.tiles_n * plan.splits;
+    if (units > 0x7fffffffll) return AXC_INVALID_ARGUMENT;
+    if (plan.splits == 1) return launch_plan<kStore>(P, plan, units, di, stream);
+    P.part = static_cast<float *>(scratch);
+    P.part_line = (g.n + 3) / 4 * 4;
+    P.part_stride = P.part_line * g.m;
+    rc = launch_plan<kPartial>(P, plan, units, di, stream);
+    if (rc) return rc;
+    return launch_finish(P.part, P.part_stride, P.part_line, plan.splits, g, di, stream);
+}
+
+int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream)
+{
+    if (g.m == 0 || g.n == 0) return AXC_OK;
+    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, false, false, di.sm_count);
+    GemmArgs P = {};
+    int rc = fill_args(g, plan, status, first, &P);
+    if (rc) return rc;
+    const long long units = (long long)P.tiles_m * P.tiles_n;
+    if (units > 0x7fffffffll) return AXC_INVALID_ARGUMENT;
+    P.ent = e;
+    return gradient ? launch_plan<kGradient>(P, plan, units, di, stream) : launch_plan<kEntropy>(P, plan, units, di, stream);
+}
+
+// ---- operands -----------------------------------------------------------------------------------------------------------
+namespace {
+
+// Copies a matrix into lines of a multiple of 8 values, 16-bit types as they are, fp32 as three bf16 planes: the value rounded to
+// bf16, the rest rounded again, and what is left then, which bf16 holds exactly.  A value beyond bf16's range keeps its largest
+// finite term, and infinities and NaNs are whole in the first plane.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) lay_out_kernel(const void *__restrict__ src, int type, long long outer, long long inner, long long outer_stride,
+                                                      long long inner_stride, uint16_t *__restrict__ dst, long long line, long long plane)
+{
+    const long long groups = line / 8, total = outer * groups;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long o = i / groups, c = (i - o * groups) * 8;
+        union { uint16_t h[8]; uint4 w; } out[SPLIT ? 3 : 1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long long at = o * outer_stride + (c + j) * inner_stride;
+            if (SPLIT) {
+                float x = c + j < inner ? __ldg(static_cast<const float *>(src) + at) : 0.0f;
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    __nv_bfloat16 h = __float2bfloat16_rn(x);
+                    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __float2bfloat16_rz(x);
+                    out[p].h[j] = __bfloat16_as_ushort(h);
+                    x = isfinite(x) ? x - __bfloat162float(h) : 0.0f;
+                }
+            } else out[0].h[j] = c + j < inner ? __ldg(static_cast<const uint16_t *>(src) + at) : uint16_t(0);
+        }
+#pragma unroll
+        for (int p = 0; p < (SPLIT ? 3 : 1); ++p) *reinterpret_cast<uint4 *>(dst + p * plane + o * line + c) = out[p].w;
+    }
+}
+
+// rows or columns contiguous: which of the two is the inner dimension of the copy
+bool columns_inner(const Matrix &x) { return x.column_stride == 1 || x.columns == 1 || x.row_stride != 1; }
+
+}  // namespace
+
+bool readable_in_place(const Matrix &x)
+{
+    if (x.type == kFloat32 || (reinterpret_cast<uintptr_t>(x.data) & 15u)) return false;
+    const bool by_columns = x.column_stride == 1 && x.row_stride % 8 == 0 && x.row_stride >= x.columns;
+    const bool by_rows = x.row_stride == 1 && x.column_stride % 8 == 0 && x.column_stride >= x.rows;
+    return by_columns || by_rows;
+}
+
+size_t operand_bytes(const Matrix &x)
+{
+    if (x.rows == 0 || x.columns == 0 || readable_in_place(x)) return 0;
+    const bool in = columns_inner(x);
+    const size_t inner = size_t(in ? x.columns : x.rows), outer = size_t(in ? x.rows : x.columns);
+    return (outer * ((inner + 7) / 8 * 8) * 2 * (x.type == kFloat32 ? 3 : 1) + 255) / 256 * 256;
+}
+
+int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, cudaStream_t stream)
+{
+    if (readable_in_place(x)) {
+        const bool by_columns = x.column_stride == 1 && x.row_stride % 8 == 0 && x.row_stride >= x.columns;
+        *out = {x.data, by_columns ? x.row_stride : x.column_stride, 0, !by_columns};
+        return AXC_OK;
+    }
+    const bool in = columns_inner(x);
+    const long long inner = in ? x.columns : x.rows, outer = in ? x.rows : x.columns, line = (inner + 7) / 8 * 8;
+    *out = {scratch, line, outer * line, !in};
+    const long long work = ceil_div(outer * (line / 8), 256);
+    const unsigned grid = unsigned(work < di.sm_count * 16 ? work : di.sm_count * 16);
+    if (x.type == kFloat32)
+        lay_out_kernel<true><<<grid, 256, 0, stream>>>(x.data, x.type, outer, inner, in ? x.row_stride : x.column_stride, in ? x.column_stride : x.row_stride,
+                                                       static_cast<uint16_t *>(scratch), line, outer * line);
+    else
+        lay_out_kernel<false><<<grid, 256, 0, stream>>>(x.data, x.type, outer, inner, in ? x.row_stride : x.column_stride, in ? x.column_stride : x.row_stride,
+                                                        static_cast<uint16_t *>(scratch), line, outer * line);
+    count_launch();
+    return AXC_OK;
+}
+
+}  // namespace axc

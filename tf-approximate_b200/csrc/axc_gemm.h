@@ -1,0 +1,144 @@
+// Matrix products on the tensor cores, shared by the dense layer and the dense cross entropy.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "axc_internal.h"
+
+namespace axc {
+
+enum { kFloat32 = AXC_TYPE_FLOAT32, kBfloat16 = AXC_TYPE_BFLOAT16, kFloat16 = AXC_TYPE_FLOAT16 };
+inline size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
+
+template <typename T> __device__ __forceinline__ float widen(T x);
+template <> __device__ __forceinline__ float widen<float>(float x) { return x; }
+template <> __device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float widen<__half>(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T narrow(float x);
+template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
+
+// element i of an array of `type`
+__device__ __forceinline__ float load_as_float(const void *p, long long i, int type)
+{
+    if (type == kFloat32) return __ldg(static_cast<const float *>(p) + i);
+    if (type == kBfloat16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(p) + i));
+    return __half2float(__ldg(static_cast<const __half *>(p) + i));
+}
+__device__ __forceinline__ void store_from_float(void *p, long long i, int type, float x)
+{
+    if (type == kFloat32) static_cast<float *>(p)[i] = x;
+    else if (type == kBfloat16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half *>(p)[i] = __float2half_rn(x);
+}
+// two values of a 16-bit type, the first in the low half
+__device__ __forceinline__ unsigned pack2(float a, float b, bool bf16)
+{
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return reinterpret_cast<const unsigned &>(h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<const unsigned &>(h);
+}
+
+// A matrix of `rows` x `k` as the tensor cores read it: 16-bit values (bf16, or fp16), either k or the rows contiguous, 16-byte
+// aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_planes).
+struct Operand {
+    const void *data;
+    long long line;             // values from one line to the next
+    long long plane;            // values from one plane to the next
+    bool rows_contiguous;
+};
+
+enum { kActNone = AXC_ACTIVATION_NONE, kActRelu = AXC_ACTIVATION_RELU, kActGelu = AXC_ACTIVATION_GELU, kActSilu = AXC_ACTIVATION_SILU };
+
+// What becomes of a sum: out = act(alpha * sum + bias[column] + addend), columns of the output.
+struct Finish {
+    float alpha;
+    const float *alpha_dev;     // NULL, or a factor in device memory
+    const void *bias;
+    int bias_type;
+    const void *addend;
+    int addend_type;
+    long long addend_line;
+    int activation;
+    void *out;
+    int out_type;
+    long long out_line;
+    void *pre;                  // NULL, or where the activation's argument goes (out_type, out_line)
+};
+
+// What the cross entropy makes of a tile of logits; see axc_entropy.cu.
+struct EntropyArgs {
+    const void *bias;
+    int bias_type;
+    const long long *labels;
+    void *keep;                 // exponentials relative to their segment's largest logit, or (gradient) the logits' gradient
+    long long line, plane;
+    int keep_fp32;              // exponentials as fp32 instead of fp16
+    float2 *stats;              // [rows][segments] {largest logit, sum of exponentials relative to it}
+    int segments;
+    float *label_logit;
+    const float *lse;           // gradient only
+    const float *row_scale;     // gradient only: 0 for rows without a label, else the scale of the stored gradient
+    int column0;                // gradient only: first class of this piece
+};
+
+struct Gemm {
+    long long m, n, k;          // out[m, n] = sum over k of a[m, k] b[n, k]
+    Operand a, b;
+    int planes;                 // 1, or 3 for fp32 operands
+    bool bf16;
+    Finish fin;
+};
+
+// Scratch for the partial sums of a product whose k is split; 0 where it is not.
+size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di);
+// `first`: of the products of a call; it clears the status word.
+int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream);
+// Tiles of logits, never split; `gradient`: the second pass of the piecewise form.
+int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream);
+
+// Gradient of an activation and the sums of its columns, in one pass over dy [rows, columns]:
+//   dz = dy * act'(kept);  to `same` (dy's type and layout) and / or to the 16-bit planes of an operand, where given;
+//   sums[column] = scale * sum of dz, as bias_type, where given.
+// `kept`: the activation's argument, for relu its value; NULL without an activation.
+struct Slope {
+    const void *dy, *kept;
+    int type;
+    long long rows, columns, dy_line;
+    int activation;
+    void *same;
+    uint16_t *planes;
+    long long line, plane;
+    int plane_count;
+    int dy_planes;              // 1, or 3: dy is bf16 and the sum of three planes `plane` apart
+    void *sums;
+    int sums_type;
+    float scale;
+    const float *scale_dev;
+};
+size_t slope_scratch(long long rows, long long columns);       // partial sums
+int slope(const Slope &s, void *scratch, const DeviceInfo &di, cudaStream_t stream);
+
+// ---- operands -----------------------------------------------------------------------------------------------------------
+// A matrix in the caller's memory: element (r, c) at data[r * row_stride + c * column_stride]
+struct Matrix {
+    const void *data;
+    long long rows, columns, row_stride, column_stride;
+    int type;
+};
+// Whether the tensor cores can read it where it is (16-bit, one unit stride, lines of a multiple of 16 bytes, aligned).
+bool readable_in_place(const Matrix &x);
+size_t operand_bytes(const Matrix &x);          // scratch that operand() fills, 0 where it reads in place
+// The matrix as an operand whose rows are x's rows (or, transposed, x's columns); copies and splits into `scratch` as needed.
+int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, cudaStream_t stream);
+inline Operand transposed(Operand o)
+{
+    o.rows_contiguous = !o.rows_contiguous;
+    return o;
+}
+
+}  // namespace axc

@@ -4,7 +4,7 @@ input and kernel, the table convolution, then bias and activation; the backward 
 convolution's (the reference registers `conv2d_backprop_input/filter` as the gradient, :264-302)."""
 import torch
 
-from . import ops
+from . import dense_ops, ops
 from .ops import approx_conv2d_with_min_max_vars
 
 
@@ -206,3 +206,25 @@ class FakeApproxConv2D(torch.nn.Module):
         if self.activation is not None:
             y = self.activation(y)
         return y
+
+
+class Dense(torch.nn.Module):
+    """The exact dense layer at the end of a network of table convolutions: activation(inputs kernel + bias), in the manner of the
+    Keras layer that the reference's models end with.  The kernel is [in_features, units]; inputs are cast to its type."""
+
+    def __init__(self, in_features, units, activation=None, use_bias=True, dtype=torch.float32):
+        super().__init__()
+        dense_ops._activation(activation)                       # refuses an unknown name here, not at the first call
+        limit = (6.0 / (in_features + units)) ** 0.5
+        self.activation = activation
+        self.kernel = torch.nn.Parameter(torch.empty(in_features, units).uniform_(-limit, limit).to(dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(units, dtype=dtype)) if use_bias else None
+
+    def forward(self, inputs, residual=None):
+        return dense_ops.dense(inputs.to(self.kernel.dtype), self.kernel, self.bias, residual, self.activation)
+
+    def cross_entropy(self, inputs, labels, ignore_index=-100, reduction="mean"):
+        """The softmax cross entropy of this layer's outputs as logits, without computing them as a tensor."""
+        if self.activation not in (None, "none", "linear"):
+            raise ops.InvalidArgumentError("the logits of a cross entropy have no activation")
+        return dense_ops.dense_cross_entropy(inputs.to(self.kernel.dtype), self.kernel, labels, self.bias, ignore_index, reduction)
