@@ -12,11 +12,12 @@ namespace {
 // ------------------------------------------------------------------------------------------------
 constexpr int kShares = 64;                    // blocks that share the rows, at most
 
+template <bool EXACT>
 __device__ __forceinline__ float slope_of(float kept, int act)
 {
     if (act == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
-    if (act == kActGelu) return 0.5f * (1.0f + erff(kept * 0.70710678f)) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
-    const float s = 1.0f / (1.0f + __expf(-kept));
+    if (act == kActGelu) return 0.5f * (1.0f + (EXACT ? erff(kept * 0.70710678f) : erf_16bit(kept * 0.70710678f))) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
+    const float s = __fdividef(1.0f, 1.0f + __expf(-kept));
     return s * (1.0f + kept * (1.0f - s));
 }
 
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const Slope S, float *part, 
                 float k[V];
                 load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, k);
 #pragma unroll
-                for (int i = 0; i < V; ++i) d[i] *= slope_of(k[i], S.activation);
+                for (int i = 0; i < V; ++i) d[i] *= slope_of<sizeof(T) == 4>(k[i], S.activation);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] += d[i];

@@ -57,25 +57,149 @@ struct Header {                                // in shared memory
     unsigned tmem;
 };
 
-__device__ __forceinline__ float activate(float z, int act)
+// `exact`: for fp32 results
+__device__ __forceinline__ float activate(float z, int act, bool exact)
 {
     if (act == kActRelu) return max_keep_nan(z, 0.0f);
-    if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-    if (act == kActSilu) return z / (1.0f + __expf(-z));
+    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f)));
+    if (act == kActSilu) return __fdividef(z, 1.0f + __expf(-z));
     return z;
 }
 
-// One row of W sums (columns n0 ..), W a multiple of 16
-template <int W>
-__device__ __forceinline__ void finish_row(const GemmArgs &P, unsigned (&x)[W], int row, int n0, float alpha)
+// ---- lines of 32 rows between a warp's registers and memory --------------------------------------------------------------
+// A lane has a row of the sums, memory wants neighbouring lanes to have neighbouring values: 16 bytes stored by every lane to its own
+// row took 11 300 clocks for a tile of 128 x 256, three times what 512 k of the matrix instructions take.  So the warp turns the
+// rows over in shared memory, 16-byte units exchanged by row so that neither side has bank conflicts, and moves N units of a row
+// (128 bytes, or 32 where the stages leave no more room) at a time.
+struct Lines {
+    unsigned stage;                            // the warp's shared memory
+    int lane, rows;                            // rows of the 32 that exist
+};
+
+template <int N>
+__device__ __forceinline__ unsigned unit_at(unsigned stage, int row, int unit) { return stage + unsigned(row * N + (unit ^ (row & (N - 1)))) * 16u; }
+
+// `bytes`: how many of a row exist; aligned: all rows start on 16 bytes
+template <int M, int N>
+__device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M], char *out, long long line, int bytes, int size, bool aligned)
+{
+#pragma unroll
+    for (int part = 0; part < M; part += N) {
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, L.lane, u)), "r"(q[part + u].x), "r"(q[part + u].y),
+                         "r"(q[part + u].z), "r"(q[part + u].w) : "memory");
+        __syncwarp();
+        char *to = out + part * 16;
+        const int left = bytes - part * 16;
+        if (aligned && left >= N * 16) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = (i * 32 + L.lane) / N, u = L.lane % N;
+                uint4 w;
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(unit_at<N>(L.stage, r, u)));
+                if (r < L.rows) *reinterpret_cast<uint4 *>(to + r * line + u * 16) = w;
+            }
+        } else {
+            // single values, neighbouring lanes neighbouring ones
+            const int in_row = left < N * 16 ? left : N * 16;
+            for (int r = 0; r < L.rows; ++r)
+                for (int b = L.lane * size; b < in_row; b += 32 * size) {
+                    const unsigned from = unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15);
+                    if (size == 2) {
+                        unsigned short h;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from));
+                        *reinterpret_cast<unsigned short *>(to + r * line + b) = h;
+                    } else {
+                        unsigned w;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from));
+                        *reinterpret_cast<unsigned *>(to + r * line + b) = w;
+                    }
+                }
+        }
+    }
+}
+
+// The other way: M units of the lane's row, zeros where there is nothing.
+template <int M, int N>
+__device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const char *in, long long line, int bytes, int size, bool aligned)
+{
+#pragma unroll
+    for (int part = 0; part < M; part += N) {
+        __syncwarp();
+        const char *from = in + part * 16;
+        const int left = bytes - part * 16;
+        if (aligned && left >= N * 16) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = (i * 32 + L.lane) / N, u = L.lane % N;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (r < L.rows) w = *reinterpret_cast<const uint4 *>(from + r * line + u * 16);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, r, u)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+            }
+        } else {
+            for (int r = 0; r < 32; ++r)
+                for (int b = L.lane * size; b < N * 16; b += 32 * size) {
+                    const unsigned to = unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15);
+                    const bool there = r < L.rows && b < left;
+                    if (size == 2) {
+                        const unsigned short h = there ? *reinterpret_cast<const unsigned short *>(from + r * line + b) : (unsigned short)0;
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(h) : "memory");
+                    } else {
+                        const unsigned w = there ? *reinterpret_cast<const unsigned *>(from + r * line + b) : 0u;
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(w) : "memory");
+                    }
+                }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[part + u].x), "=r"(q[part + u].y), "=r"(q[part + u].z), "=r"(q[part + u].w)
+                         : "r"(unit_at<N>(L.stage, L.lane, u)));
+    }
+}
+
+__device__ __forceinline__ bool lines_aligned(const void *base, long long line_bytes) { return ((reinterpret_cast<uintptr_t>(base) | uintptr_t(line_bytes)) & 15u) == 0; }
+
+// W fp32 values of every lane's row, as `type`; columns n0 .. of n
+template <int W, int N>
+__device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], void *base, int type, long long line, int row0, int n0, int n)
+{
+    const int size = type == kFloat32 ? 4 : 2, left = n - n0;
+    char *out = static_cast<char *>(base) + (row0 * line + n0) * size;
+    const bool aligned = lines_aligned(base, line * size);
+    const int bytes = (left < W ? left : W) * size;
+    if (type == kFloat32) {
+        uint4 q[W / 4];
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i)
+            q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+        store_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, out, line * 4, bytes, 4, aligned);
+    } else {
+        const bool bf16 = type == kBfloat16;
+        uint4 q[W / 8];
+#pragma unroll
+        for (int i = 0; i < W / 8; ++i)
+            q[i] = make_uint4(pack2(v[8 * i], v[8 * i + 1], bf16), pack2(v[8 * i + 2], v[8 * i + 3], bf16), pack2(v[8 * i + 4], v[8 * i + 5], bf16),
+                              pack2(v[8 * i + 6], v[8 * i + 7], bf16));
+        store_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, out, line * 2, bytes, 2, aligned);
+    }
+}
+
+// One row of W sums (columns n0 ..), W a multiple of 16; all lanes of the warp, whether their row exists or not
+template <int W, int N>
+__device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0, float alpha)
 {
     const Finish &f = P.fin;
-    if (row >= P.m || n0 >= P.n) return;
-    const bool full = n0 + W <= P.n;
+    if (n0 >= P.n) return;
+    const bool full = n0 + W <= P.n, exact = f.out_type == kFloat32;
+    const int row = row0 + L.lane;
     float v[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = alpha * __uint_as_float(x[i]);
-    if (P.swapped) {                           // neighbouring lanes write neighbouring values
+    if (P.swapped) {                           // neighbouring lanes have neighbouring values
+        if (row >= P.m) return;
         const float bias = f.bias ? load_as_float(f.bias, row, f.bias_type) : 0.0f;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -84,7 +208,7 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, unsigned (&x)[W], 
                 if (f.addend) z += load_as_float(f.addend, (long long)(n0 + i) * f.addend_line + row, f.addend_type);
                 const long long at = (long long)(n0 + i) * f.out_line + row;
                 if (f.pre) store_from_float(f.pre, at, f.out_type, z);
-                store_from_float(f.out, at, f.out_type, activate(z, f.activation));
+                store_from_float(f.out, at, f.out_type, activate(z, f.activation, exact));
             }
         }
         return;
@@ -95,86 +219,82 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, unsigned (&x)[W], 
             if (full || n0 + i < P.n) v[i] += load_as_float(f.bias, n0 + i, f.bias_type);
     }
     if (f.addend) {
-        const char *at = static_cast<const char *>(f.addend) + ((long long)row * f.addend_line + n0) * (f.addend_type == kFloat32 ? 4 : 2);
-        if (full && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
-            if (f.addend_type == kFloat32) {
+        const int size = f.addend_type == kFloat32 ? 4 : 2, left = P.n - n0, bytes = (left < W ? left : W) * size;
+        const char *in = static_cast<const char *>(f.addend) + ((long long)row0 * f.addend_line + n0) * size;
+        const bool aligned = lines_aligned(f.addend, f.addend_line * size);
+        if (size == 4) {
+            uint4 q[W / 4];
+            load_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, in, f.addend_line * 4, bytes, 4, aligned);
 #pragma unroll
-                for (int i = 0; i < W; i += 4) {
-                    const float4 w = *reinterpret_cast<const float4 *>(at + i * 4);
-                    v[i] += w.x; v[i + 1] += w.y; v[i + 2] += w.z; v[i + 3] += w.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; i += 8) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(at + i * 2);
-                    const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 t = f.addend_type == kBfloat16 ? __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]))
-                                                                    : __half22float2(reinterpret_cast<const __half2 &>(u[j]));
-                        v[i + 2 * j] += t.x;
-                        v[i + 2 * j + 1] += t.y;
-                    }
-                }
+            for (int i = 0; i < W / 4; ++i) {
+                v[4 * i] += __uint_as_float(q[i].x);
+                v[4 * i + 1] += __uint_as_float(q[i].y);
+                v[4 * i + 2] += __uint_as_float(q[i].z);
+                v[4 * i + 3] += __uint_as_float(q[i].w);
             }
         } else {
+            uint4 q[W / 8];
+            load_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, in, f.addend_line * 2, bytes, 2, aligned);
 #pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (full || n0 + i < P.n) v[i] += load_as_float(f.addend, (long long)row * f.addend_line + n0 + i, f.addend_type);
+            for (int i = 0; i < W / 8; ++i) {
+                const unsigned u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 t = f.addend_type == kBfloat16 ? __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]))
+                                                                : __half22float2(reinterpret_cast<const __half2 &>(u[j]));
+                    v[8 * i + 2 * j] += t.x;
+                    v[8 * i + 2 * j + 1] += t.y;
+                }
+            }
         }
     }
-#pragma unroll 1
-    for (int pass = f.pre ? 0 : 1; pass < 2; ++pass) {
-        void *base = pass == 0 ? f.pre : f.out;
-        if (pass == 1 && f.activation != kActNone) {
+    if (f.pre) store_row<W, N>(L, v, f.pre, f.out_type, f.out_line, row0, n0, P.n);
+    if (f.activation == kActRelu) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = activate(v[i], f.activation);
-        }
-        char *at = static_cast<char *>(base) + ((long long)row * f.out_line + n0) * (f.out_type == kFloat32 ? 4 : 2);
-        if (full && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
-            if (f.out_type == kFloat32) {
+        for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActRelu, exact);
+    } else if (f.activation == kActGelu) {
+        if (exact) {
 #pragma unroll
-                for (int i = 0; i < W; i += 4) *reinterpret_cast<float4 *>(at + i * 4) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            } else {
-                const bool bf16 = f.out_type == kBfloat16;
-#pragma unroll
-                for (int i = 0; i < W; i += 8)
-                    *reinterpret_cast<uint4 *>(at + i * 2) = make_uint4(pack2(v[i], v[i + 1], bf16), pack2(v[i + 2], v[i + 3], bf16),
-                                                                        pack2(v[i + 4], v[i + 5], bf16), pack2(v[i + 6], v[i + 7], bf16));
-            }
+            for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActGelu, true);
         } else {
 #pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (full || n0 + i < P.n) store_from_float(base, (long long)row * f.out_line + n0 + i, f.out_type, v[i]);
+            for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActGelu, false);
         }
+    } else if (f.activation == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActSilu, exact);
     }
+    store_row<W, N>(L, v, f.out, f.out_type, f.out_line, row0, n0, P.n);
 }
 
 // Partial sums in the order of the output's lines
-template <int W>
-__device__ __forceinline__ void store_part(const GemmArgs &P, unsigned (&x)[W], int row, int n0, int split)
+template <int W, int N>
+__device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0, int split)
 {
-    if (row >= P.m || n0 >= P.n) return;
+    if (n0 >= P.n) return;
     float *part = P.part + (long long)split * P.part_stride;
     if (P.swapped) {
+        if (row0 + L.lane >= P.m) return;
 #pragma unroll
         for (int i = 0; i < W; ++i)
-            if (n0 + i < P.n) part[(long long)(n0 + i) * P.part_line + row] = __uint_as_float(x[i]);
+            if (n0 + i < P.n) part[(long long)(n0 + i) * P.part_line + row0 + L.lane] = __uint_as_float(x[i]);
         return;
     }
-    float *at = part + (long long)row * P.part_line + n0;      // lines are padded to 4 values
+    float v[W];
 #pragma unroll
-    for (int i = 0; i < W; i += 4)
-        if (n0 + i < P.n)
-            *reinterpret_cast<float4 *>(at + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+    for (int i = 0; i < W; ++i) v[i] = __uint_as_float(x[i]);
+    store_row<W, N>(L, v, part, kFloat32, P.part_line, row0, n0, P.n);
 }
 
 // One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
 // A segment of -inf has the exponentials 0 (relative to 0, not to itself).
-__device__ __forceinline__ void entropy_segment(const GemmArgs &P, unsigned (&x0)[32], unsigned (&x1)[32], int row, int n0)
+template <int N>
+__device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &L, unsigned (&x0)[32], unsigned (&x1)[32], int row0, int n0)
 {
     const EntropyArgs &e = P.ent;
-    if (row >= P.m || n0 >= P.n) return;
+    if (n0 >= P.n) return;
+    const int row = row0 + L.lane;
+    float v[2][32];
     float top = -INFINITY;
     bool nan = false;
 #pragma unroll
@@ -183,60 +303,41 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, unsigned (&x0
         if (n0 + i < P.n) {
             if (e.bias) l += load_as_float(e.bias, n0 + i, e.bias_type);
         } else l = -INFINITY;
-        if (i < 32) x0[i & 31] = __float_as_uint(l);
-        else x1[i & 31] = __float_as_uint(l);
+        v[i / 32][i & 31] = l;
         top = fmaxf(top, l);
         nan |= l != l;
     }
-    const long long label = e.labels[row] - n0;
-    if (label >= 0 && label < kSegment && n0 + label < P.n) {
-        float mine = 0.0f;
+    if (row < P.m) {
+        const long long label = e.labels[row] - n0;
+        if (label >= 0 && label < kSegment && n0 + label < P.n) {
+            float mine = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-            if (i == int(label)) mine = __uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]);
-        e.label_logit[row] = mine;
+            for (int i = 0; i < 64; ++i) mine = fmaxf(mine, i == int(label) ? v[i / 32][i & 31] : -INFINITY);
+            e.label_logit[row] = mine;
+        }
     }
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 64; ++i) {
-        const float p = __expf(__uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]) - base);
-        sum += p;
-        if (i < 32) x0[i & 31] = __float_as_uint(p);
-        else x1[i & 31] = __float_as_uint(p);
+        v[i / 32][i & 31] = __expf(v[i / 32][i & 31] - base);
+        sum += v[i / 32][i & 31];
     }
     if (nan) sum = NAN;
-    e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, sum);
+    if (row < P.m) e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, sum);
     if (!e.keep) return;
-    if (e.keep_fp32) {
-        float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(e.keep) + (long long)row * e.line + n0);
+    const int type = e.keep_fp32 ? kFloat32 : kFloat16;
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-            unsigned u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) u[j] = i + j < 32 ? x0[(i + j) & 31] : x1[(i + j) & 31];
-            to[i / 4] = make_float4(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]), __uint_as_float(u[3]));
-        }
-    } else {
-        uint4 *to = reinterpret_cast<uint4 *>(static_cast<__half *>(e.keep) + (long long)row * e.line + n0);
-#pragma unroll
-        for (int i = 0; i < 64; i += 8) {
-            unsigned u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = i + 2 * j;
-                u[j] = pack2(__uint_as_float(c < 32 ? x0[c & 31] : x1[c & 31]), __uint_as_float(c < 32 ? x0[(c + 1) & 31] : x1[(c + 1) & 31]), false);
-            }
-            to[i / 8] = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-    }
+    for (int i = 0; i < 2; ++i) store_row<32, N>(L, v[i], e.keep, type, e.line, row0, n0 + 32 * i, int(e.line));
 }
 
 // 32 logits of a row and what the loss's gradient is there: row_scale * (exp(logit - lse) - [label])
-__device__ __forceinline__ void gradient_columns(const GemmArgs &P, unsigned (&x)[32], int row, int n0)
+template <int N>
+__device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines &L, unsigned (&x)[32], int row0, int n0)
 {
     const EntropyArgs &e = P.ent;
-    if (row >= P.m || n0 >= e.line) return;
+    if (n0 >= e.line) return;
+    const int row = row0 + L.lane < P.m ? row0 + L.lane : P.m - 1;
     const float lse = e.lse[row], scale = e.row_scale[row];
     const long long label = e.labels[row] - e.column0 - n0;
     float v[32];
@@ -249,22 +350,13 @@ __device__ __forceinline__ void gradient_columns(const GemmArgs &P, unsigned (&x
             v[i] = scale * (__expf(l - lse) - (label == i ? 1.0f : 0.0f));
         }
     }
-    uint16_t *keep = static_cast<uint16_t *>(e.keep) + (long long)row * e.line + n0;
-    const bool bf16 = P.shape >> 7 & 1;
+    uint16_t *keep = static_cast<uint16_t *>(e.keep);
+    const int type = (P.shape >> 7 & 1) ? kBfloat16 : kFloat16;
     for (int plane = 0; plane < P.planes; ++plane) {
+        store_row<32, N>(L, v, keep, type, e.line, row0, n0, int(e.line));
+        if (P.planes == 3) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            unsigned u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] = pack2(v[i + 2 * j], v[i + 2 * j + 1], bf16);
-                if (P.planes == 3) {
-                    const float2 t = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]));
-                    v[i + 2 * j] -= t.x;
-                    v[i + 2 * j + 1] -= t.y;
-                }
-            }
-            *reinterpret_cast<uint4 *>(keep + i) = make_uint4(u[0], u[1], u[2], u[3]);
+            for (int i = 0; i < 32; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
         }
         keep += e.plane;
     }
@@ -284,11 +376,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 {
     constexpr int TM = 128 * CG;
     constexpr unsigned kColumns = BN < 32 ? 32 : BN;           // tensor memory of one tile's sums
-    constexpr int kBuffers = 2;
+    constexpr int kBuffers = 2, kUnits = PLANES == 3 ? 2 : 8;
     extern __shared__ char raw[];
     const unsigned base = (mma::smem_address(raw) + 1023u) & ~1023u;
     Header *head = reinterpret_cast<Header *>(raw + (base - mma::smem_address(raw)));
-    const unsigned ring = base + kHeader, stage_bytes = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
+    const unsigned lines = base + kHeader, ring = lines + 8u * kUnits * 512u, stage_bytes = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
     const unsigned full = mma::smem_address(head->full), empty = mma::smem_address(head->empty);
     const unsigned sums_full = mma::smem_address(head->sums_full), sums_empty = mma::smem_address(head->sums_empty);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -395,12 +487,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             int tm, tn;
             place_of(P, u / P.splits, tm, tn);
             const int split = u % P.splits;
-            const int row = tm * TM + int(rank) * 128 + quarter * 32 + lane, n0 = tn * BN + half * kMine;
+            const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + half * kMine;
+            const Lines L = {lines + unsigned(warp - 4) * kUnits * 512u, lane, min(32, P.m - row0)};
             // sums of columns c .. c + W (entropy: both halves of a segment)
             auto take = [&](unsigned (&x)[W], int c) {
-                if constexpr (MODE == kStore) finish_row<W>(P, x, row, n0 + c, alpha);
-                else if constexpr (MODE == kPartial) store_part<W>(P, x, row, n0 + c, split);
-                else if constexpr (MODE == kGradient) gradient_columns(P, x, row, n0 + c);
+                if constexpr (MODE == kStore) finish_row<W, kUnits>(P, L, x, row0, n0 + c, alpha);
+                else if constexpr (MODE == kPartial) store_part<W, kUnits>(P, L, x, row0, n0 + c, split);
+                else if constexpr (MODE == kGradient) gradient_columns<kUnits>(P, L, x, row0, n0 + c);
             };
             const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
             if constexpr (PLANES == 3) {
@@ -431,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 }
                 if (!ok) break;
                 if (half < kHalves) {
-                    if constexpr (MODE == kEntropy) entropy_segment(P, sum[0], sum[1], row, n0);
+                    if constexpr (MODE == kEntropy) entropy_segment<kUnits>(P, L, sum[0], sum[1], row0, n0);
                     else {
 #pragma unroll
                         for (int c = 0; c < kMine / W; ++c) take(sum[c], c * W);
@@ -453,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                             mma::load_columns(at + c + 32, y);
                             mma::load_wait(x);
                             mma::load_wait(y);
-                            entropy_segment(P, x, y, row, n0 + c);
+                            entropy_segment<kUnits>(P, L, x, y, row0, n0 + c);
                         } else {
                             mma::load_wait(x);
                             take(x, c);
@@ -508,7 +601,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float *__restrict__ p
                 if (f.bias) z += load_as_float(f.bias, c + j, f.bias_type);
                 if (f.addend) z += load_as_float(f.addend, line * f.addend_line + c + j, f.addend_type);
                 if (f.pre) store_from_float(f.pre, line * f.out_line + c + j, f.out_type, z);
-                store_from_float(f.out, line * f.out_line + c + j, f.out_type, activate(z, f.activation));
+                store_from_float(f.out, line * f.out_line + c + j, f.out_type, activate(z, f.activation, true));
             }
         }
     }
@@ -584,9 +677,10 @@ template <int CG, int BN, int MODE, int PLANES>
 int launch(GemmArgs &P, long long units, const DeviceInfo &di, cudaStream_t stream)
 {
     const unsigned stage = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
-    P.stages = int((kSmem - kHeader - 1024) / stage);
+    const unsigned lines = PLANES == 3 ? 8 * 1024 : 8 * 4096;
+    P.stages = int((kSmem - kHeader - 1024 - lines) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
-    const unsigned smem = kHeader + 1024 + unsigned(P.stages) * stage;
+    const unsigned smem = kHeader + 1024 + lines + unsigned(P.stages) * stage;
     AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
     const long long workers = di.sm_count / CG;
     cudaLaunchAttribute attr[2] = {};
