@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     const unsigned lines = base + kHeader, ring = lines + 8u * kUnits * 512u, stage_bytes = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
     const unsigned full = mma::smem_address(head->full), empty = mma::smem_address(head->empty);
     const unsigned sums_full = mma::smem_address(head->sums_full), sums_empty = mma::smem_address(head->sums_empty);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const unsigned rank = CG == 2 ? mma::cluster_rank() : 0u;
     const int worker = int(blockIdx.x) / CG, workers = int(gridDim.x) / CG;
     const int units = P.tiles_m * P.tiles_n * P.splits;
@@ -411,7 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     asm volatile("griddepcontrol.wait;" ::: "memory");          // operands may come from the kernel before
     bool ok = true;
 
-    if (warp == 0 && lane == 0) {
+    // The loading and the multiplying warp run as a whole and one of their threads acts, so that what it hands over is computed once for
+    // the warp: with a branch around the loop the 4 matrix instructions of a stage took 660 clocks instead of 512, the issuing thread's own.
+    if (warp == 0) {
+        const bool leader = mma::elect();
         const unsigned signal = CG == 2 ? mma::in_cta(full, 0) : full;
         int s = 0;
         unsigned phase = 1;
@@ -423,29 +426,33 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
             for (int k = k0; k < k1; ++k) {
                 if (!(ok = mma::barrier_wait(empty + 8 * s, phase))) break;
-                if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
-                unsigned at = ring + unsigned(s) * stage_bytes;
-                for (int p = 0; p < PLANES; ++p) {
-                    if (P.a_rows) {
-                        for (int r = 0; r < 128; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_a, signal + 8 * s, row_a + r, k * kStageK, p);
-                    } else mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kStageK, row_a, p);
-                    at += P.a_bytes;
-                    if (P.b_rows) {
-                        for (int r = 0; r < BN / CG; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_b, signal + 8 * s, row_b + r, k * kStageK, p);
-                    } else mma::load_box<CG>(at, &P.map_b, signal + 8 * s, k * kStageK, row_b, p);
-                    at += P.b_bytes;
+                if (leader) {
+                    if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
+                    unsigned at = ring + unsigned(s) * stage_bytes;
+                    for (int p = 0; p < PLANES; ++p) {
+                        if (P.a_rows) {
+                            for (int r = 0; r < 128; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_a, signal + 8 * s, row_a + r, k * kStageK, p);
+                        } else mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kStageK, row_a, p);
+                        at += P.a_bytes;
+                        if (P.b_rows) {
+                            for (int r = 0; r < BN / CG; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_b, signal + 8 * s, row_b + r, k * kStageK, p);
+                        } else mma::load_box<CG>(at, &P.map_b, signal + 8 * s, k * kStageK, row_b, p);
+                        at += P.b_bytes;
+                    }
                 }
+                __syncwarp();
                 if (++s == P.stages) s = 0, phase ^= 1u;
             }
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+        const bool leader = mma::elect();
         int s = 0, buffer = 0;
         unsigned phase = 0, sums_phase = 1;
         // the products of the three terms, smallest first: the terms of a and of b
         const unsigned of_a = PLANES == 3 ? 0x001012u : 0u, of_b = PLANES == 3 ? 0x010210u : 0u;
         constexpr int kProducts = PLANES == 3 ? 6 : 1;
         const unsigned chunk_a = P.a_rows ? 8192u : 0u, chunk_b = P.b_rows ? 8192u : 0u;
-        const unsigned step_a = P.a_rows ? 2048u : 32u, step_b = P.b_rows ? 2048u : 32u;
+        const unsigned step_a = (P.a_rows ? 2048u : 32u) >> 4, step_b = (P.b_rows ? 2048u : 32u) >> 4;
         for (int u = worker; u < units && ok; u += workers) {
             const int split = u % P.splits;
             const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
@@ -457,20 +464,22 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 }
                 if (!(ok = mma::barrier_wait(full + 8 * s, phase))) break;
                 mma::fence_after();
-                const unsigned at = ring + unsigned(s) * stage_bytes;
+                const unsigned at = (ring + unsigned(s) * stage_bytes) >> 4, plane = (P.a_bytes + P.b_bytes) >> 4;
+                if (leader) {
 #pragma unroll
-                for (int q = 0; q < kProducts; ++q) {
-                    const unsigned a = at + (of_a >> (4 * q) & 15u) * (P.a_bytes + P.b_bytes);
-                    const unsigned b = at + (of_b >> (4 * q) & 15u) * (P.a_bytes + P.b_bytes) + P.a_bytes;
+                    for (int q = 0; q < kProducts; ++q) {
+                        const unsigned a = at + (of_a >> (4 * q) & 15u) * plane, b = at + (of_b >> (4 * q) & 15u) * plane + (P.a_bytes >> 4);
 #pragma unroll
-                    for (int j = 0; j < kStageK / 16; ++j)
-                        mma::multiply<CG>(d, mma::operand(a + j * step_a, chunk_a), mma::operand(b + j * step_b, chunk_b), P.shape,
-                                          (PLANES == 1 && k > k0) || q > 0 || j > 0);
+                        for (int j = 0; j < kStageK / 16; ++j)
+                            mma::multiply<CG>(d, mma::operand(a + j * step_a, chunk_a), mma::operand(b + j * step_b, chunk_b), P.shape,
+                                              (PLANES == 1 && k > k0) || q > 0 || j > 0);
+                    }
+                    mma::commit<CG>(empty + 8 * s);
+                    if (PLANES == 3 || k + 1 == k1) mma::commit<CG>(sums_full + 8 * buffer);
                 }
-                mma::commit<CG>(empty + 8 * s);
+                __syncwarp();
                 if (++s == P.stages) s = 0, phase ^= 1u;
                 if (PLANES == 3 || k + 1 == k1) {
-                    mma::commit<CG>(sums_full + 8 * buffer);
                     if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
                 }
             }

@@ -29,6 +29,14 @@ __device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank)
     return r;
 }
 
+// true in one thread of the warp, the same one every time
+__device__ __forceinline__ bool elect()
+{
+    unsigned yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
 __device__ __forceinline__ void barrier_init(unsigned bar, unsigned count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -42,14 +50,14 @@ __device__ __forceinline__ void barrier_arrive_cluster(unsigned bar)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Waits for the phase `parity`; false when it did not come within the limit.
+// The whole warp waits for the phase `parity`; false, in all its threads, when it did not come within the limit.
 __device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity)
 {
     for (int it = 0; it < kWaitPolls; ++it) {
         unsigned done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
+        if (__all_sync(0xffffffffu, done != 0)) return true;
     }
     return false;
 }
@@ -150,10 +158,10 @@ __device__ __forceinline__ void load_wait(unsigned (&x)[16])
 
 // Descriptor of an operand in shared memory, 128-byte swizzle.  K contiguous: rows of 64 values, 8 rows make a group of 1024 bytes
 // (stride 1024 from group to group).  Rows contiguous: 64 of them side by side, one line for each k; groups of 8 k are 1024 bytes
-// apart, the next 64 rows `chunk` bytes on.
-__device__ __forceinline__ uint64_t operand(unsigned addr, unsigned chunk)
+// apart, the next 64 rows `chunk` bytes on.  `unit`: the address in units of 16 bytes.
+__device__ __forceinline__ uint64_t operand(unsigned unit, unsigned chunk)
 {
-    return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(chunk >> 4) << 16) | (uint64_t(1024u >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+    return uint64_t(unit & 0x3fffu) | (uint64_t(chunk >> 4) << 16) | (uint64_t(1024u >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 // Shape of the instruction: fp32 sums of bf16 or fp16 products, M x N, operands with K or with rows contiguous
 __host__ __device__ inline unsigned instruction_shape(int m, int n, bool bf16, bool a_rows, bool b_rows)
