@@ -6,11 +6,12 @@ namespace axc {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
-// dz = dy act'(kept), column sums on the way.  A block takes 32 groups of V neighbouring columns and a share of the rows, 8 rows at
-// a time; the sums of its 8 rows are added in shared memory, those of the blocks by a second kernel, in a fixed order.  Bound by
-// reading dy and kept and writing dz once.
+// dz = dy act'(kept), column sums on the way.  A block takes 32 groups of V neighbouring columns and a share of the rows, four times 8
+// rows at a time; the sums of its 8 rows are added in shared memory, those of the blocks by a second kernel, in a fixed order.  Bound
+// by reading dy and kept and writing dz once.
 // ------------------------------------------------------------------------------------------------
 constexpr int kShares = 64;                    // blocks that share the rows, at most
+constexpr int kRows = 4;                       // of a thread, whose loads are in flight together
 
 template <bool EXACT>
 __device__ __forceinline__ float slope_of(float kept, int act)
@@ -49,58 +50,67 @@ __global__ void __launch_bounds__(256) slope_kernel(const Slope S, float *part, 
     const int group = threadIdx.x & 31, r0 = threadIdx.x >> 5;
     const long long c = ((long long)blockIdx.x * 32 + group) * V, left = S.columns - c;
     const long long begin = S.rows * blockIdx.y / gridDim.y, end = S.rows * (blockIdx.y + 1) / gridDim.y;
-    const bool full = vec && left >= V;
+    const bool full = vec && (left >= V || S.padded);
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     if (left > 0) {
-        for (long long r = begin + r0; r < end; r += 8) {
-            float d[V];
-            load_group(static_cast<const T *>(S.dy) + r * S.dy_line + c, full, left, d);
-            for (int p = 1; p < S.dy_planes; ++p) {
-                float more[V];
-                load_group(static_cast<const T *>(S.dy) + p * S.plane + r * S.dy_line + c, full, left, more);
+        for (long long first = begin + r0; first < end; first += 8 * kRows) {
+            float dy[kRows][V], kept[kRows][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) d[i] += more[i];
-            }
-            if (S.kept) {
-                float k[V];
-                load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, k);
-#pragma unroll
-                for (int i = 0; i < V; ++i) d[i] *= slope_of<sizeof(T) == 4>(k[i], S.activation);
+            for (int q = 0; q < kRows; ++q) {
+                const long long r = first + 8 * q < end ? first + 8 * q : first;
+                load_group(static_cast<const T *>(S.dy) + r * S.dy_line + c, full, left, dy[q]);
+                if (S.kept) load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, kept[q]);
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] += d[i];
-            if (S.same) {
-                T *to = static_cast<T *>(S.same) + r * S.columns + c;
-                if (full) {
-                    union { uint4 w; T t[V]; } u;
+            for (int q = 0; q < kRows; ++q) {
+                const long long r = first + 8 * q;
+                if (r >= end) break;
+                float (&d)[V] = dy[q];
+                for (int p = 1; p < S.dy_planes; ++p) {
+                    float more[V];
+                    load_group(static_cast<const T *>(S.dy) + p * S.plane + r * S.dy_line + c, full, left, more);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(d[i]);
-                    *reinterpret_cast<uint4 *>(to) = u.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (i < left) to[i] = narrow<T>(d[i]);
+                    for (int i = 0; i < V; ++i) d[i] += more[i];
                 }
-            }
-            if (S.planes) {                    // lines of a multiple of 8 values, zeros behind the last column
-                uint16_t *to = S.planes + r * S.line + c;
-                if (sizeof(T) == 2) {
-                    union { uint4 w; T t[V]; } u;
+                if (S.kept) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(i < left ? d[i] : 0.0f);
-                    *reinterpret_cast<uint4 *>(to) = u.w;
-                } else {
-                    for (int p = 0; p < 3; ++p) {
-                        union { uint2 w; __nv_bfloat16 h[4]; } u;
+                    for (int i = 0; i < V; ++i) d[i] *= slope_of<sizeof(T) == 4>(kept[q][i], S.activation);
+                }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            u.h[i] = narrow<__nv_bfloat16>(i < left ? d[i] : 0.0f);
-                            const float h = __bfloat162float(u.h[i]);
-                            d[i] = isfinite(h) ? d[i] - h : 0.0f;
+                for (int i = 0; i < V; ++i) sum[i] += d[i];
+                if (S.same) {
+                    T *to = static_cast<T *>(S.same) + r * S.columns + c;
+                    if (full) {
+                        union { uint4 w; T t[V]; } u;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(d[i]);
+                        *reinterpret_cast<uint4 *>(to) = u.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (i < left) to[i] = narrow<T>(d[i]);
+                    }
+                }
+                if (S.planes) {                // lines of a multiple of 8 values, zeros behind the last column
+                    uint16_t *to = S.planes + r * S.line + c;
+                    if (sizeof(T) == 2) {
+                        union { uint4 w; T t[V]; } u;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(i < left ? d[i] : 0.0f);
+                        *reinterpret_cast<uint4 *>(to) = u.w;
+                    } else {
+                        for (int p = 0; p < 3; ++p) {
+                            union { uint2 w; __nv_bfloat16 h[4]; } u;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                u.h[i] = narrow<__nv_bfloat16>(i < left ? d[i] : 0.0f);
+                                const float h = __bfloat162float(u.h[i]);
+                                d[i] = isfinite(h) ? d[i] - h : 0.0f;
+                            }
+                            *reinterpret_cast<uint2 *>(to + p * S.plane) = u.w;
                         }
-                        *reinterpret_cast<uint2 *>(to + p * S.plane) = u.w;
                     }
                 }
             }
@@ -131,9 +141,9 @@ __global__ void __launch_bounds__(256) slope_sums_kernel(const float *__restrict
 
 int shares_of(long long rows, long long columns)
 {
-    // enough blocks for every SM a few times, at least 64 rows each
-    long long shares = (rows + 63) / 64;
-    const long long across = columns / 128 + 1, most = across >= 600 ? 1 : 600 / across + 1;
+    // about six blocks for every SM, of at least one round of rows each
+    long long shares = (rows + 8 * kRows - 1) / (8 * kRows);
+    const long long across = columns / 256 + 1, most = 888 / across + 1;
     if (shares > most) shares = most;
     if (shares > kShares) shares = kShares;
     return int(shares < 1 ? 1 : shares);
@@ -287,7 +297,6 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
             s.planes = reinterpret_cast<uint16_t *>(ws + parts.dz);
             s.line = line;
             s.plane = line * d.rows;
-            s.plane_count = planes;
             dz = {s.planes, line, s.plane, false};
         }
     }

@@ -356,6 +356,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             s.dy = ws + l.gradient;
             s.type = d.type == kFloat16 ? kFloat16 : kBfloat16;
             s.dy_planes = planes;
+            s.padded = true;
             s.plane = l.line * d.rows;
             s.rows = d.rows;
             s.columns = n;

@@ -187,13 +187,28 @@ __device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], v
     }
 }
 
+// bias[n0 + i] of W columns, W / 32 in each lane; column() hands one to all lanes
+template <int W>
+struct ColumnValues {
+    float mine[W < 32 ? 1 : W / 32];
+    __device__ __forceinline__ ColumnValues(const void *values, int type, int n0, int n, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < (W < 32 ? 1 : W / 32); ++i) {
+            const int c = n0 + 32 * i + lane;
+            mine[i] = values && c < n ? load_as_float(values, c, type) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ float column(int i) const { return __shfl_sync(0xffffffffu, mine[i / 32], i & 31); }
+};
+
 // One row of W sums (columns n0 ..), W a multiple of 16; all lanes of the warp, whether their row exists or not
 template <int W, int N>
 __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0, float alpha)
 {
     const Finish &f = P.fin;
     if (n0 >= P.n) return;
-    const bool full = n0 + W <= P.n, exact = f.out_type == kFloat32;
+    const bool exact = f.out_type == kFloat32;
     const int row = row0 + L.lane;
     float v[W];
 #pragma unroll
@@ -214,9 +229,9 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
         return;
     }
     if (f.bias) {
+        const ColumnValues<W> bias(f.bias, f.bias_type, n0, P.n, L.lane);
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (full || n0 + i < P.n) v[i] += load_as_float(f.bias, n0 + i, f.bias_type);
+        for (int i = 0; i < W; ++i) v[i] += bias.column(i);
     }
     if (f.addend) {
         const int size = f.addend_type == kFloat32 ? 4 : 2, left = P.n - n0, bytes = (left < W ? left : W) * size;
@@ -287,76 +302,77 @@ __device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, un
 }
 
 // One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
-// A segment of -inf has the exponentials 0 (relative to 0, not to itself).
+// A segment of -inf has the exponentials 0 (relative to 0, not to itself); one with a NaN has nothing else.  `label`: the row's.
 template <int N>
-__device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &L, unsigned (&x0)[32], unsigned (&x1)[32], int row0, int n0)
+__device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &L, unsigned (&x)[64], int row0, int n0, long long label)
 {
     const EntropyArgs &e = P.ent;
     if (n0 >= P.n) return;
     const int row = row0 + L.lane;
-    float v[2][32];
-    float top = -INFINITY;
-    bool nan = false;
+    float v[64];
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-        float l = __uint_as_float(i < 32 ? x0[i & 31] : x1[i & 31]);
-        if (n0 + i < P.n) {
-            if (e.bias) l += load_as_float(e.bias, n0 + i, e.bias_type);
-        } else l = -INFINITY;
-        v[i / 32][i & 31] = l;
-        top = fmaxf(top, l);
-        nan |= l != l;
-    }
-    if (row < P.m) {
-        const long long label = e.labels[row] - n0;
-        if (label >= 0 && label < kSegment && n0 + label < P.n) {
-            float mine = -INFINITY;
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(x[i]);
+    if (e.bias || n0 + 64 > P.n) {             // classes that are not there count as -inf
+        const ColumnValues<64> bias(e.bias, e.bias_type, n0, P.n, L.lane);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) mine = fmaxf(mine, i == int(label) ? v[i / 32][i & 31] : -INFINITY);
-            e.label_logit[row] = mine;
+        for (int i = 0; i < 64; ++i) {
+            const float b = bias.column(i);
+            v[i] = n0 + i < P.n ? v[i] + b : -INFINITY;
         }
     }
+    float top4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < 64; ++i) top4[i & 3] = max_keep_nan(top4[i & 3], v[i]);
+    const float top = max_keep_nan(max_keep_nan(top4[0], top4[1]), max_keep_nan(top4[2], top4[3]));
+    label -= n0;
+    if (row < P.m && label >= 0 && label < kSegment && n0 + label < P.n) {
+        float mine = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mine = fmaxf(mine, i == int(label) ? v[i] : -INFINITY);
+        e.label_logit[row] = mine;
+    }
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 64; ++i) {
-        v[i / 32][i & 31] = __expf(v[i / 32][i & 31] - base);
-        sum += v[i / 32][i & 31];
+        v[i] = __expf(v[i] - base);
+        sum4[i & 3] += v[i];
     }
-    if (nan) sum = NAN;
-    if (row < P.m) e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, sum);
-    if (!e.keep) return;
-    const int type = e.keep_fp32 ? kFloat32 : kFloat16;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) store_row<32, N>(L, v[i], e.keep, type, e.line, row0, n0 + 32 * i, int(e.line));
+    if (row < P.m) e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+    if (e.keep) store_row<64, N>(L, v, e.keep, e.keep_fp32 ? kFloat32 : kFloat16, e.line, row0, n0, int(e.line));
 }
 
-// 32 logits of a row and what the loss's gradient is there: row_scale * (exp(logit - lse) - [label])
-template <int N>
-__device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines &L, unsigned (&x)[32], int row0, int n0)
+// W logits of a row and what the loss's gradient is there: row_scale * (exp(logit - lse) - [label])
+template <int W, int N>
+__device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0)
 {
     const EntropyArgs &e = P.ent;
     if (n0 >= e.line) return;
     const int row = row0 + L.lane < P.m ? row0 + L.lane : P.m - 1;
     const float lse = e.lse[row], scale = e.row_scale[row];
     const long long label = e.labels[row] - e.column0 - n0;
-    float v[32];
+    float v[W];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[i] = 0.0f;
-        if (n0 + i < P.n && scale != 0.0f) {
-            float l = __uint_as_float(x[i]);
-            if (e.bias) l += load_as_float(e.bias, e.column0 + n0 + i, e.bias_type);
-            v[i] = scale * (__expf(l - lse) - (label == i ? 1.0f : 0.0f));
+    for (int i = 0; i < W; ++i) v[i] = __uint_as_float(x[i]);
+    if (e.bias || n0 + W > P.n) {
+        const ColumnValues<W> bias(e.bias ? static_cast<const char *>(e.bias) + (long long)e.column0 * (e.bias_type == kFloat32 ? 4 : 2) : nullptr, e.bias_type, n0,
+                                   P.n, L.lane);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float b = bias.column(i);
+            v[i] = n0 + i < P.n ? v[i] + b : -INFINITY;
         }
     }
+    // a row without a label stays out, whatever its logits are
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = scale != 0.0f ? scale * (__expf(v[i] - lse) - (label == i ? 1.0f : 0.0f)) : 0.0f;
     uint16_t *keep = static_cast<uint16_t *>(e.keep);
     const int type = (P.shape >> 7 & 1) ? kBfloat16 : kFloat16;
     for (int plane = 0; plane < P.planes; ++plane) {
-        store_row<32, N>(L, v, keep, type, e.line, row0, n0, int(e.line));
+        store_row<W, N>(L, v, keep, type, e.line, row0, n0, int(e.line));
         if (P.planes == 3) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
+            for (int i = 0; i < W; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
         }
         keep += e.plane;
     }
@@ -491,18 +507,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         const float alpha = MODE == kStore ? P.fin.alpha * (P.fin.alpha_dev ? *P.fin.alpha_dev : 1.0f) : 1.0f;
         int buffer = 0;
         unsigned phase = 0;
-        constexpr int kMine = BN / kHalves, W = kMine < 32 ? 16 : 32;
+        constexpr int kMine = BN / kHalves, W = kMine < 32 ? 16 : kMine < 64 || (PLANES == 3 && MODE != kEntropy) ? 32 : 64;
         for (int u = worker; u < units && ok; u += workers) {
             int tm, tn;
             place_of(P, u / P.splits, tm, tn);
             const int split = u % P.splits;
             const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + half * kMine;
             const Lines L = {lines + unsigned(warp - 4) * kUnits * 512u, lane, min(32, P.m - row0)};
-            // sums of columns c .. c + W (entropy: both halves of a segment)
+            const int of_lane = row0 + lane < P.m ? row0 + lane : P.m - 1;
+            const long long label = MODE == kEntropy ? P.ent.labels[of_lane] : 0;
             auto take = [&](unsigned (&x)[W], int c) {
                 if constexpr (MODE == kStore) finish_row<W, kUnits>(P, L, x, row0, n0 + c, alpha);
                 else if constexpr (MODE == kPartial) store_part<W, kUnits>(P, L, x, row0, n0 + c, split);
-                else if constexpr (MODE == kGradient) gradient_columns<kUnits>(P, L, x, row0, n0 + c);
+                else if constexpr (MODE == kGradient) gradient_columns<W, kUnits>(P, L, x, row0, n0 + c);
+                else entropy_segment<kUnits>(P, L, x, row0, n0 + c, label);
             };
             const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
             if constexpr (PLANES == 3) {
@@ -518,12 +536,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                     __syncwarp();
                     if (half < kHalves) {
 #pragma unroll
-                        for (int c = 0; c < kMine / W; ++c) {
-                            unsigned x[W];
-                            mma::load_columns(mine + unsigned(buffer) * kColumns + c * W, x);
+                        for (int c = 0; c < kMine; c += (W < 32 ? W : 32)) {
+                            unsigned x[W < 32 ? W : 32];
+                            mma::load_columns(mine + unsigned(buffer) * kColumns + c, x);
                             mma::load_wait(x);
 #pragma unroll
-                            for (int i = 0; i < W; ++i) sum[c][i] = __float_as_uint(__uint_as_float(sum[c][i]) + __uint_as_float(x[i]));
+                            for (int i = 0; i < (W < 32 ? W : 32); ++i)
+                                sum[c / W][c % W + i] = __float_as_uint(__uint_as_float(sum[c / W][c % W + i]) + __uint_as_float(x[i]));
                         }
                     }
                     mma::fence_before();
@@ -533,11 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 }
                 if (!ok) break;
                 if (half < kHalves) {
-                    if constexpr (MODE == kEntropy) entropy_segment<kUnits>(P, L, sum[0], sum[1], row0, n0);
-                    else {
 #pragma unroll
-                        for (int c = 0; c < kMine / W; ++c) take(sum[c], c * W);
-                    }
+                    for (int c = 0; c < kMine / W; ++c) take(sum[c], c * W);
                 }
             } else {
                 if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
@@ -545,21 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 __syncwarp();
                 if (half < kHalves) {
                     const unsigned at = mine + unsigned(buffer) * kColumns;
-                    constexpr int kStep = MODE == kEntropy ? kSegment : W;
 #pragma unroll 1
-                    for (int c = 0; c < kMine; c += kStep) {
+                    for (int c = 0; c < kMine; c += W) {
                         unsigned x[W];
                         mma::load_columns(at + c, x);
-                        if constexpr (MODE == kEntropy) {
-                            unsigned y[W];
-                            mma::load_columns(at + c + 32, y);
-                            mma::load_wait(x);
-                            mma::load_wait(y);
-                            entropy_segment<kUnits>(P, L, x, y, row0, n0 + c);
-                        } else {
-                            mma::load_wait(x);
-                            take(x, c);
-                        }
+                        mma::load_wait(x);
+                        take(x, c);
                     }
                 }
                 mma::fence_before();

@@ -121,8 +121,8 @@ struct Slope {
     void *same;
     uint16_t *planes;
     long long line, plane;
-    int plane_count;
     int dy_planes;              // 1, or 3: dy is bf16 and the sum of three planes `plane` apart
+    bool padded;                // dy's lines have values that do not matter up to a multiple of 16 bytes
     void *sums;
     int sums_type;
     float scale;

@@ -156,6 +156,18 @@ __device__ __forceinline__ void load_wait(unsigned (&x)[16])
                  :: "memory");
 }
 
+// the same for 64 columns
+__device__ __forceinline__ void load_columns(unsigned at, unsigned (&x)[64])
+{
+    load_columns(at, reinterpret_cast<unsigned(&)[32]>(x[0]));
+    load_columns(at + 32, reinterpret_cast<unsigned(&)[32]>(x[32]));
+}
+__device__ __forceinline__ void load_wait(unsigned (&x)[64])
+{
+    load_wait(reinterpret_cast<unsigned(&)[32]>(x[0]));
+    load_wait(reinterpret_cast<unsigned(&)[32]>(x[32]));
+}
+
 // Descriptor of an operand in shared memory, 128-byte swizzle.  K contiguous: rows of 64 values, 8 rows make a group of 1024 bytes
 // (stride 1024 from group to group).  Rows contiguous: 64 of them side by side, one line for each k; groups of 8 k are 1024 bytes
 // apart, the next 64 rows `chunk` bytes on.  `unit`: the address in units of 16 bytes.
