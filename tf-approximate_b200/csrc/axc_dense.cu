@@ -13,37 +13,36 @@ namespace {
 constexpr int kShares = 64;                    // blocks that share the rows, at most
 constexpr int kRows = 4;                       // of a thread, whose loads are in flight together
 
-template <bool EXACT>
-__device__ __forceinline__ float slope_of(float kept, int act)
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float slope_of(float kept)
 {
-    if (act == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
-    if (act == kActGelu) return 0.5f * (1.0f + (EXACT ? erff(kept * 0.70710678f) : erf_16bit(kept * 0.70710678f))) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
+    if (ACT == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
+    if (ACT == kActGelu) return 0.5f * (1.0f + (EXACT ? erff(kept * 0.70710678f) : erf_16bit(kept * 0.70710678f))) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
     const float s = __fdividef(1.0f, 1.0f + __expf(-kept));
     return s * (1.0f + kept * (1.0f - s));
 }
 
-template <typename T> struct Group;            // values of 16 bytes
-template <> struct Group<float> { static constexpr int V = 4; };
-template <> struct Group<__nv_bfloat16> { static constexpr int V = 8; };
-template <> struct Group<__half> { static constexpr int V = 8; };
+template <typename T>
+union Group {                                  // 16 bytes of values
+    static constexpr int V = 16 / sizeof(T);
+    uint4 w;
+    T t[V];
+    __device__ Group() {}
+};
 
 template <typename T>
-__device__ __forceinline__ void load_group(const T *at, bool vec, long long left, float (&x)[Group<T>::V])
+__device__ __forceinline__ void load_group(const T *at, bool vec, long long left, Group<T> &g)
 {
-    constexpr int V = Group<T>::V;
-    union { uint4 w; T t[V]; } u;
-    if (vec) {
-        u.w = __ldg(reinterpret_cast<const uint4 *>(at));
+    if (vec) g.w = __ldcs(reinterpret_cast<const uint4 *>(at));
+    else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = widen(u.t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = i < left ? widen(at[i]) : 0.0f;
+        for (int i = 0; i < Group<T>::V; ++i) g.t[i] = i < left ? at[i] : narrow<T>(0.0f);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(const Slope S, float *part, bool vec)
+// What is loaded stays packed until it is needed: 8 loads of a thread in flight and three blocks on an SM.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part, bool vec)
 {
     constexpr int V = Group<T>::V;
     __shared__ float sums[8][32 * V];
@@ -56,61 +55,55 @@ __global__ void __launch_bounds__(256) slope_kernel(const Slope S, float *part, 
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     if (left > 0) {
         for (long long first = begin + r0; first < end; first += 8 * kRows) {
-            float dy[kRows][V], kept[kRows][V];
+            Group<T> dy[kRows], kept[ACT != kActNone ? kRows : 1];
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
                 const long long r = first + 8 * q < end ? first + 8 * q : first;
                 load_group(static_cast<const T *>(S.dy) + r * S.dy_line + c, full, left, dy[q]);
-                if (S.kept) load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, kept[q]);
+                if constexpr (ACT != kActNone) load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, kept[q]);
             }
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
                 const long long r = first + 8 * q;
-                if (r >= end) break;
-                float (&d)[V] = dy[q];
+                if (r >= end) continue;
+                float d[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[i] = widen(dy[q].t[i]);
                 for (int p = 1; p < S.dy_planes; ++p) {
-                    float more[V];
+                    Group<T> more;
                     load_group(static_cast<const T *>(S.dy) + p * S.plane + r * S.dy_line + c, full, left, more);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] += more[i];
+                    for (int i = 0; i < V; ++i) d[i] += widen(more.t[i]);
                 }
-                if (S.kept) {
+                if constexpr (ACT != kActNone) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] *= slope_of<sizeof(T) == 4>(kept[q][i], S.activation);
+                    for (int i = 0; i < V; ++i) d[i] *= slope_of<ACT, sizeof(T) == 4>(widen(kept[q].t[i]));
                 }
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += d[i];
-                if (S.same) {
-                    T *to = static_cast<T *>(S.same) + r * S.columns + c;
-                    if (full) {
-                        union { uint4 w; T t[V]; } u;
+                if (S.same || (S.planes && sizeof(T) == 2)) {
+                    Group<T> u;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(d[i]);
-                        *reinterpret_cast<uint4 *>(to) = u.w;
-                    } else {
+                    for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(i < left ? d[i] : 0.0f);
+                    if (S.same) {
+                        T *to = static_cast<T *>(S.same) + r * S.columns + c;
+                        if (full) *reinterpret_cast<uint4 *>(to) = u.w;
+                        else {
 #pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (i < left) to[i] = narrow<T>(d[i]);
-                    }
-                }
-                if (S.planes) {                // lines of a multiple of 8 values, zeros behind the last column
-                    uint16_t *to = S.planes + r * S.line + c;
-                    if (sizeof(T) == 2) {
-                        union { uint4 w; T t[V]; } u;
-#pragma unroll
-                        for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(i < left ? d[i] : 0.0f);
-                        *reinterpret_cast<uint4 *>(to) = u.w;
-                    } else {
-                        for (int p = 0; p < 3; ++p) {
-                            union { uint2 w; __nv_bfloat16 h[4]; } u;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                u.h[i] = narrow<__nv_bfloat16>(i < left ? d[i] : 0.0f);
-                                const float h = __bfloat162float(u.h[i]);
-                                d[i] = isfinite(h) ? d[i] - h : 0.0f;
-                            }
-                            *reinterpret_cast<uint2 *>(to + p * S.plane) = u.w;
+                            for (int i = 0; i < V; ++i)
+                                if (i < left) to[i] = u.t[i];
                         }
+                    }
+                    // lines of a multiple of 8 values, zeros behind the last column
+                    if (S.planes && sizeof(T) == 2) *reinterpret_cast<uint4 *>(S.planes + r * S.line + c) = u.w;
+                }
+                if (S.planes && sizeof(T) == 4) {
+                    uint16_t *to = S.planes + r * S.line + c;
+                    for (int p = 0; p < 3; ++p) {
+                        union { uint2 w; uint16_t h[4]; } u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(i < left ? d[i] : 0.0f, d[i]);
+                        *reinterpret_cast<uint2 *>(to + p * S.plane) = u.w;
                     }
                 }
             }
@@ -141,9 +134,9 @@ __global__ void __launch_bounds__(256) slope_sums_kernel(const float *__restrict
 
 int shares_of(long long rows, long long columns)
 {
-    // about six blocks for every SM, of at least one round of rows each
+    // about eight blocks for every SM, of at least one round of rows each
     long long shares = (rows + 8 * kRows - 1) / (8 * kRows);
-    const long long across = columns / 256 + 1, most = 888 / across + 1;
+    const long long across = columns / 256 + 1, most = 1184 / across + 1;
     if (shares > most) shares = most;
     if (shares > kShares) shares = kShares;
     return int(shares < 1 ? 1 : shares);
@@ -152,8 +145,11 @@ int shares_of(long long rows, long long columns)
 template <typename T>
 void launch_slope(const Slope &s, float *part, int shares, bool vec, cudaStream_t stream)
 {
-    const unsigned across = unsigned((s.columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V));
-    slope_kernel<T><<<dim3(across, unsigned(shares)), 256, 0, stream>>>(s, part, vec);
+    const dim3 grid(unsigned((s.columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
+    if (!s.kept) slope_kernel<T, kActNone><<<grid, 256, 0, stream>>>(s, part, vec);
+    else if (s.activation == kActRelu) slope_kernel<T, kActRelu><<<grid, 256, 0, stream>>>(s, part, vec);
+    else if (s.activation == kActGelu) slope_kernel<T, kActGelu><<<grid, 256, 0, stream>>>(s, part, vec);
+    else slope_kernel<T, kActSilu><<<grid, 256, 0, stream>>>(s, part, vec);
     count_launch();
 }
 

@@ -79,6 +79,18 @@ struct Lines {
 template <int N>
 __device__ __forceinline__ unsigned unit_at(unsigned stage, int row, int unit) { return stage + unsigned(row * N + (unit ^ (row & (N - 1)))) * 16u; }
 
+// Lines that do not start on 16 bytes: value by value, neighbouring lanes neighbouring ones, several on their way at a time.
+template <int N, typename Pointer, typename Move>
+__device__ __forceinline__ void single_values(const Lines &L, Pointer lines, long long line, int left, int size, Move move)
+{
+    const int in_row = N * 16 / size;          // a power of two, 8 to 64
+#pragma unroll 8
+    for (int i = 0; i < in_row; ++i) {
+        const int at = i * 32 + L.lane, r = at / in_row, b = (at & (in_row - 1)) * size;
+        if (r < L.rows && b < left) move(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), lines + r * line + b, size);
+    }
+}
+
 // `bytes`: how many of a row exist; aligned: all rows start on 16 bytes
 template <int M, int N>
 __device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M], char *out, long long line, int bytes, int size, bool aligned)
@@ -102,21 +114,17 @@ __device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M],
                 if (r < L.rows) *reinterpret_cast<uint4 *>(to + r * line + u * 16) = w;
             }
         } else {
-            // single values, neighbouring lanes neighbouring ones
-            const int in_row = left < N * 16 ? left : N * 16;
-            for (int r = 0; r < L.rows; ++r)
-                for (int b = L.lane * size; b < in_row; b += 32 * size) {
-                    const unsigned from = unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15);
-                    if (size == 2) {
-                        unsigned short h;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from));
-                        *reinterpret_cast<unsigned short *>(to + r * line + b) = h;
-                    } else {
-                        unsigned w;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from));
-                        *reinterpret_cast<unsigned *>(to + r * line + b) = w;
-                    }
+            single_values<N>(L, to, line, left, size, [](unsigned from, char *at, int size) {
+                if (size == 2) {
+                    unsigned short h;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from));
+                    *reinterpret_cast<unsigned short *>(at) = h;
+                } else {
+                    unsigned w;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from));
+                    *reinterpret_cast<unsigned *>(at) = w;
                 }
+            });
         }
     }
 }
@@ -139,18 +147,10 @@ __device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const 
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, r, u)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
             }
         } else {
-            for (int r = 0; r < 32; ++r)
-                for (int b = L.lane * size; b < N * 16; b += 32 * size) {
-                    const unsigned to = unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15);
-                    const bool there = r < L.rows && b < left;
-                    if (size == 2) {
-                        const unsigned short h = there ? *reinterpret_cast<const unsigned short *>(from + r * line + b) : (unsigned short)0;
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(h) : "memory");
-                    } else {
-                        const unsigned w = there ? *reinterpret_cast<const unsigned *>(from + r * line + b) : 0u;
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(w) : "memory");
-                    }
-                }
+            single_values<N>(L, from, line, left, size, [](unsigned to, const char *at, int size) {
+                if (size == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(*reinterpret_cast<const unsigned short *>(at)) : "memory");
+                else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<const unsigned *>(at)) : "memory");
+            });
         }
         __syncwarp();
 #pragma unroll
@@ -821,8 +821,7 @@ int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *s
 namespace {
 
 // Copies a matrix into lines of a multiple of 8 values, 16-bit types as they are, fp32 as three bf16 planes: the value rounded to
-// bf16, the rest rounded again, and what is left then, which bf16 holds exactly.  A value beyond bf16's range keeps its largest
-// finite term, and infinities and NaNs are whole in the first plane.
+// bf16, the rest rounded again, and what is left then, which bf16 holds exactly.
 template <bool SPLIT>
 __global__ void __launch_bounds__(256) lay_out_kernel(const void *__restrict__ src, int type, long long outer, long long inner, long long outer_stride,
                                                       long long inner_stride, uint16_t *__restrict__ dst, long long line, long long plane)
@@ -837,12 +836,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const void *__restrict__ s
             if (SPLIT) {
                 float x = c + j < inner ? __ldg(static_cast<const float *>(src) + at) : 0.0f;
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    __nv_bfloat16 h = __float2bfloat16_rn(x);
-                    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __float2bfloat16_rz(x);
-                    out[p].h[j] = __bfloat16_as_ushort(h);
-                    x = isfinite(x) ? x - __bfloat162float(h) : 0.0f;
-                }
+                for (int p = 0; p < 3; ++p) out[p].h[j] = split_term(x, x);
             } else out[0].h[j] = c + j < inner ? __ldg(static_cast<const uint16_t *>(src) + at) : uint16_t(0);
         }
 #pragma unroll

@@ -51,6 +51,16 @@ __device__ __forceinline__ float erf_16bit(float x)
     return copysignf(1.0f - poly * __expf(-a * a), x);
 }
 
+// The next bf16 term of x, and in `rest` what it leaves.  A value beyond bf16's range keeps its largest finite term; infinities and
+// NaNs are whole in their first term.
+__device__ __forceinline__ uint16_t split_term(float x, float &rest)
+{
+    __nv_bfloat16 h = __float2bfloat16_rn(x);
+    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __float2bfloat16_rz(x);
+    rest = isfinite(x) ? x - __bfloat162float(h) : 0.0f;
+    return __bfloat16_as_ushort(h);
+}
+
 // A matrix of `rows` x `k` as the tensor cores read it: 16-bit values (bf16, or fp16), either k or the rows contiguous, 16-byte
 // aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_planes).
 struct Operand {
