@@ -6,20 +6,25 @@ namespace axc {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
-// dz = dy act'(kept), column sums on the way.  A block takes 32 groups of V neighbouring columns and a share of the rows, four times 8
-// rows at a time; the sums of its 8 rows are added in shared memory, those of the blocks by a second kernel, in a fixed order.  Bound
-// by reading dy and kept and writing dz once.
+// dz = dy act'(kept), column sums on the way.  A block takes 32 groups of V columns (16 bytes) and a share of the rows; a thread has
+// the V columns of a group, 2 to 8 rows in flight, packed until they are needed.  Lines that do not start on 16 bytes are read value by
+// value, the V values of a thread 32 apart, so that neighbouring lanes still read neighbouring ones.  The sums of the block's 8 rows are
+// added in shared memory, those of the blocks by a second kernel, in a fixed order.  Bound by reading dy and kept and writing dz once.
 // ------------------------------------------------------------------------------------------------
 constexpr int kShares = 64;                    // blocks that share the rows, at most
-constexpr int kRows = 4;                       // of a thread, whose loads are in flight together
 
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float slope_of(float kept)
 {
     if (ACT == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
-    if (ACT == kActGelu) return 0.5f * (1.0f + (EXACT ? erff(kept * 0.70710678f) : erf_16bit(kept * 0.70710678f))) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
-    const float s = __fdividef(1.0f, 1.0f + __expf(-kept));
-    return s * (1.0f + kept * (1.0f - s));
+    if (ACT == kActGelu) {
+        if (EXACT) return 0.5f * (1.0f + erff(kept * 0.70710678f)) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
+        float bell;
+        const float e = erf_16bit(kept * 0.70710678f, bell);
+        return fmaf(0.5f, e, fmaf(kept * bell, 0.39894228f, 0.5f));
+    }
+    const float s = reciprocal(1.0f + __expf(-kept));
+    return s * fmaf(kept, 1.0f - s, 1.0f);
 }
 
 template <typename T>
@@ -30,80 +35,94 @@ union Group {                                  // 16 bytes of values
     __device__ Group() {}
 };
 
-template <typename T>
-__device__ __forceinline__ void load_group(const T *at, bool vec, long long left, Group<T> &g)
+// V columns of a row: neighbours at `at`, or 32 apart, those below `left`
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_group(const T *at, long long left, Group<T> &g)
 {
-    if (vec) g.w = __ldcs(reinterpret_cast<const uint4 *>(at));
+    if (VEC) g.w = __ldcs(reinterpret_cast<const uint4 *>(at));
     else {
 #pragma unroll
-        for (int i = 0; i < Group<T>::V; ++i) g.t[i] = i < left ? at[i] : narrow<T>(0.0f);
+        for (int i = 0; i < Group<T>::V; ++i) g.t[i] = 32 * i < left ? at[32 * i] : narrow<T>(0.0f);
     }
 }
 
-// What is loaded stays packed until it is needed: 8 loads of a thread in flight and three blocks on an SM.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part, bool vec)
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part)
 {
-    constexpr int V = Group<T>::V;
+    constexpr int V = Group<T>::V, kRows = (ACT == kActNone ? 8 : 4) / (VEC ? 1 : 2), kApart = VEC ? 1 : 32;
     __shared__ float sums[8][32 * V];
-    const int group = threadIdx.x & 31, r0 = threadIdx.x >> 5;
-    const long long c = ((long long)blockIdx.x * 32 + group) * V, left = S.columns - c;
+    const int group = threadIdx.x & 31, r0 = threadIdx.x >> 5, first_column = VEC ? group * V : group;
+    const long long c = (long long)blockIdx.x * 32 * V + first_column, left = S.columns - c;
     const long long begin = S.rows * blockIdx.y / gridDim.y, end = S.rows * (blockIdx.y + 1) / gridDim.y;
-    const bool full = vec && (left >= V || S.padded);
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
-    if (left > 0) {
-        for (long long first = begin + r0; first < end; first += 8 * kRows) {
-            Group<T> dy[kRows], kept[ACT != kActNone ? kRows : 1];
+    // operand lines are a multiple of 8 values: zeros behind the last column
+    const long long mine = S.planes ? S.line - c : left;
+    if (mine > 0) {
+        const T *dy = static_cast<const T *>(S.dy) + (begin + r0) * S.dy_line + c, *kept = static_cast<const T *>(S.kept) + (begin + r0) * S.columns + c;
+        for (long long r = begin + r0; r < end; r += 8 * kRows, dy += 8 * kRows * S.dy_line, kept += 8 * kRows * S.columns) {
+            Group<T> g[kRows], k[ACT != kActNone ? kRows : 1];
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
-                const long long r = first + 8 * q < end ? first + 8 * q : first;
-                load_group(static_cast<const T *>(S.dy) + r * S.dy_line + c, full, left, dy[q]);
-                if constexpr (ACT != kActNone) load_group(static_cast<const T *>(S.kept) + r * S.columns + c, full, left, kept[q]);
+                const int step = r + 8 * q < end ? 8 * q : 0;      // behind the last row: the first one again, not used
+                load_group<VEC>(dy + step * S.dy_line, left, g[q]);
+                if constexpr (ACT != kActNone) load_group<VEC>(kept + step * S.columns, left, k[q]);
             }
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
-                const long long r = first + 8 * q;
-                if (r >= end) continue;
+                const long long row = r + 8 * q;
+                if (row >= end) continue;
                 float d[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) d[i] = widen(dy[q].t[i]);
+                for (int i = 0; i < V; ++i) d[i] = widen(g[q].t[i]);
                 for (int p = 1; p < S.dy_planes; ++p) {
                     Group<T> more;
-                    load_group(static_cast<const T *>(S.dy) + p * S.plane + r * S.dy_line + c, full, left, more);
+                    load_group<VEC>(dy + 8 * q * S.dy_line + p * S.plane, left, more);
 #pragma unroll
                     for (int i = 0; i < V; ++i) d[i] += widen(more.t[i]);
                 }
                 if constexpr (ACT != kActNone) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] *= slope_of<ACT, sizeof(T) == 4>(widen(kept[q].t[i]));
+                    for (int i = 0; i < V; ++i) d[i] *= slope_of<ACT, sizeof(T) == 4>(widen(k[q].t[i]));
                 }
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += d[i];
                 if (S.same || (S.planes && sizeof(T) == 2)) {
                     Group<T> u;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(i < left ? d[i] : 0.0f);
+                    for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(d[i]);
+                    T *to = static_cast<T *>(S.same) + row * S.columns + c;
                     if (S.same) {
-                        T *to = static_cast<T *>(S.same) + r * S.columns + c;
-                        if (full) *reinterpret_cast<uint4 *>(to) = u.w;
+                        if (VEC) *reinterpret_cast<uint4 *>(to) = u.w;
                         else {
 #pragma unroll
                             for (int i = 0; i < V; ++i)
-                                if (i < left) to[i] = u.t[i];
+                                if (32 * i < left) to[32 * i] = u.t[i];
                         }
                     }
-                    // lines of a multiple of 8 values, zeros behind the last column
-                    if (S.planes && sizeof(T) == 2) *reinterpret_cast<uint4 *>(S.planes + r * S.line + c) = u.w;
+                    T *operand = reinterpret_cast<T *>(S.planes) + row * S.line + c;
+                    if (S.planes && sizeof(T) == 2) {
+                        if (VEC) *reinterpret_cast<uint4 *>(operand) = u.w;
+                        else {
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                if (32 * i < mine) operand[32 * i] = u.t[i];
+                        }
+                    }
                 }
                 if (S.planes && sizeof(T) == 4) {
-                    uint16_t *to = S.planes + r * S.line + c;
-                    for (int p = 0; p < 3; ++p) {
+                    uint16_t *to = S.planes + row * S.line + c;
+                    for (int p = 0; p < 3; ++p, to += S.plane) {
                         union { uint2 w; uint16_t h[4]; } u;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(i < left ? d[i] : 0.0f, d[i]);
-                        *reinterpret_cast<uint2 *>(to + p * S.plane) = u.w;
+                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(d[i], d[i]);
+                        if (VEC) *reinterpret_cast<uint2 *>(to) = u.w;
+                        else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (32 * i < mine) to[32 * i] = u.h[i];
+                        }
                     }
                 }
             }
@@ -111,7 +130,7 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
     }
     if (!part) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[r0][group * V + i] = sum[i];
+    for (int i = 0; i < V; ++i) sums[r0][first_column + kApart * i] = sum[i];
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * V; i += 256) {
         float s = sums[0][i];
@@ -134,22 +153,23 @@ __global__ void __launch_bounds__(256) slope_sums_kernel(const float *__restrict
 
 int shares_of(long long rows, long long columns)
 {
-    // about eight blocks for every SM, of at least one round of rows each
-    long long shares = (rows + 8 * kRows - 1) / (8 * kRows);
+    // about eight blocks for every SM, of at least 32 rows each
+    long long shares = (rows + 31) / 32;
     const long long across = columns / 256 + 1, most = 1184 / across + 1;
     if (shares > most) shares = most;
     if (shares > kShares) shares = kShares;
     return int(shares < 1 ? 1 : shares);
 }
 
-template <typename T>
-void launch_slope(const Slope &s, float *part, int shares, bool vec, cudaStream_t stream)
+template <typename T, bool VEC>
+void launch_slope(const Slope &s, float *part, int shares, cudaStream_t stream)
 {
-    const dim3 grid(unsigned((s.columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
-    if (!s.kept) slope_kernel<T, kActNone><<<grid, 256, 0, stream>>>(s, part, vec);
-    else if (s.activation == kActRelu) slope_kernel<T, kActRelu><<<grid, 256, 0, stream>>>(s, part, vec);
-    else if (s.activation == kActGelu) slope_kernel<T, kActGelu><<<grid, 256, 0, stream>>>(s, part, vec);
-    else slope_kernel<T, kActSilu><<<grid, 256, 0, stream>>>(s, part, vec);
+    const long long columns = s.planes && s.line > s.columns ? s.line : s.columns;
+    const dim3 grid(unsigned((columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
+    if (!s.kept) slope_kernel<T, kActNone, VEC><<<grid, 256, 0, stream>>>(s, part);
+    else if (s.activation == kActRelu) slope_kernel<T, kActRelu, VEC><<<grid, 256, 0, stream>>>(s, part);
+    else if (s.activation == kActGelu) slope_kernel<T, kActGelu, VEC><<<grid, 256, 0, stream>>>(s, part);
+    else slope_kernel<T, kActSilu, VEC><<<grid, 256, 0, stream>>>(s, part);
     count_launch();
 }
 
@@ -163,12 +183,13 @@ int slope(const Slope &s, void *scratch, const DeviceInfo &di, cudaStream_t stre
     if (s.columns == 0 || (s.rows == 0 && !s.sums)) return AXC_OK;
     const int shares = shares_of(s.rows, s.columns);
     float *part = s.sums ? static_cast<float *>(scratch) : nullptr;
+    // whole groups of 16 bytes, in every line of every tensor
     const uintptr_t all = reinterpret_cast<uintptr_t>(s.dy) | reinterpret_cast<uintptr_t>(s.kept) | reinterpret_cast<uintptr_t>(s.same);
     const long long size = s.type == kFloat32 ? 4 : 2;
-    const bool vec = (all & 15u) == 0 && s.dy_line * size % 16 == 0 && ((!s.kept && !s.same) || s.columns * size % 16 == 0) && s.plane * size % 16 == 0;
-    if (s.type == kFloat32) launch_slope<float>(s, part, shares, vec, stream);
-    else if (s.type == kBfloat16) launch_slope<__nv_bfloat16>(s, part, shares, vec, stream);
-    else launch_slope<__half>(s, part, shares, vec, stream);
+    const bool vec = (all & 15u) == 0 && s.dy_line * size % 16 == 0 && (s.padded || s.columns * size % 16 == 0) && s.plane * size % 16 == 0;
+    if (s.type == kFloat32) vec ? launch_slope<float, true>(s, part, shares, stream) : launch_slope<float, false>(s, part, shares, stream);
+    else if (s.type == kBfloat16) vec ? launch_slope<__nv_bfloat16, true>(s, part, shares, stream) : launch_slope<__nv_bfloat16, false>(s, part, shares, stream);
+    else vec ? launch_slope<__half, true>(s, part, shares, stream) : launch_slope<__half, false>(s, part, shares, stream);
     if (s.sums) {
         slope_sums_kernel<<<unsigned((s.columns + 255) / 256), 256, 0, stream>>>(part, s.columns, shares, s.scale, s.scale_dev, s.sums, s.sums_type);
         count_launch();

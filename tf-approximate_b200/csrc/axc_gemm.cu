@@ -61,8 +61,9 @@ struct Header {                                // in shared memory
 __device__ __forceinline__ float activate(float z, int act, bool exact)
 {
     if (act == kActRelu) return max_keep_nan(z, 0.0f);
-    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f)));
-    if (act == kActSilu) return __fdividef(z, 1.0f + __expf(-z));
+    float bell;
+    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f, bell)));
+    if (act == kActSilu) return z * reciprocal(1.0f + __expf(-z));
     return z;
 }
 
