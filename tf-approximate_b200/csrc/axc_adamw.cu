@@ -9,13 +9,15 @@
 // (1/16 at most), and its range within a block, 2^17.8, is that of the first moment: held as v, the codes would reach gradients
 // down to 1/470 of the block's largest only.  A root above zero keeps the smallest code, or a first moment that still has a code
 // would be divided by eps.  The step itself uses the moments before they are rounded.
-// The square root and the quotient are the 2^-22 approximations: their error is below a hundredth of an ulp of a fp32 parameter for
-// steps up to a hundredth of its size, and the exact ones would make the 8-bit kernel bound by arithmetic.
+// The reciprocals and roots are the approximations to 2^-22: their error is below a hundredth of an ulp of a fp32 parameter for steps up
+// to a hundredth of its size, and the exact ones would make the 8-bit kernel bound by arithmetic.
 //
 // Bound by memory: 28 bytes per fp32 value with fp32 moments, 16.03 with 8-bit ones, 10.03 for a 16-bit value with those.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "axc_internal.h"
 
@@ -39,7 +41,7 @@ static_assert(sizeof(AdamwEntry) == 40, "table entries are packed");
 // the large form holds what 32 KiB of parameters can.
 template <int CAP>
 struct AdamwTable {
-    int count, per_cta;                        // tensors; blocks per CTA
+    int count;                                 // tensors
     unsigned base, blocks;                     // blocks of this launch: [base, base + blocks)
     float c1, c2, inv_root, eps, grad_scale;   // 1 - beta1, 1 - beta2, 1 / sqrt(1 - beta2^t)
     void *m, *v;
@@ -48,11 +50,43 @@ struct AdamwTable {
 };
 constexpr int kSmallTable = 96, kLargeTable = 800;
 
-__device__ __forceinline__ float approx_sqrt(float x)
+__device__ __forceinline__ float reciprocal(float x)
 {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+__device__ __forceinline__ float reciprocal_root(float x)
+{
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Two fp32 values that one instruction computes with
+struct Two {
+    unsigned long long v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+    __device__ __forceinline__ float2 both() const
+    {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
+{
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b)
+{
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
 }
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -68,47 +102,42 @@ template <> struct Word<4> { typedef unsigned type; };
 template <> struct Word<8> { typedef uint2 type; };
 template <> struct Word<16> { typedef uint4 type; };
 
-// V values at `at`, as one load or store where `vec`, else those below `left`
+// V values as they lie in memory
 template <typename T, int V>
-__device__ __forceinline__ void load_values(const T *at, bool vec, long long left, float (&x)[V])
+union Packed {
+    typename Word<V * sizeof(T)>::type w;
+    T t[V];
+    __device__ Packed() {}
+};
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T *at, bool vec, long long left, Packed<T, V> &x)
 {
-    typedef typename Word<V * sizeof(T)>::type word;
-    if (vec) {
-        union { word w; T t[V]; } u;
-        u.w = __ldcs(reinterpret_cast<const word *>(at));
+    if (vec) x.w = __ldcs(reinterpret_cast<const typename Word<V * sizeof(T)>::type *>(at));
+    else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = to_float(u.t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = i < left ? to_float(at[i]) : 0.0f;
+        for (int i = 0; i < V; ++i) x.t[i] = i < left ? at[i] : T(0);
     }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_values(T *at, bool vec, long long left, const float (&x)[V])
 {
-    typedef typename Word<V * sizeof(T)>::type word;
-    if (vec) {
-        union { word w; T t[V]; } u;
+    Packed<T, V> u;
 #pragma unroll
-        for (int i = 0; i < V; ++i) u.t[i] = from_float<T>(x[i]);
-        __stcs(reinterpret_cast<word *>(at), u.w);
-    } else {
+    for (int i = 0; i < V; ++i) u.t[i] = from_float<T>(x[i]);
+    if (vec) __stcs(reinterpret_cast<typename Word<V * sizeof(T)>::type *>(at), u.w);
+    else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i < left) at[i] = from_float<T>(x[i]);
+            if (i < left) at[i] = u.t[i];
     }
 }
+// codes 2 i and 2 i + 1, times `scale`
 template <int V>
-__device__ __forceinline__ void load_codes(const uint8_t *at, float scale, float (&x)[V])
+__device__ __forceinline__ Two decode(const Packed<uint8_t, V> &codes, int i, Two scale)
 {
-    union { typename Word<V>::type w; __nv_fp8x2_storage_t c[V / 2]; } u;
-    u.w = __ldcs(reinterpret_cast<const typename Word<V>::type *>(at));
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(u.c[i], __NV_E4M3)));
-        x[2 * i] = f.x * scale;
-        x[2 * i + 1] = f.y * scale;
-    }
+    const __nv_fp8x2_storage_t two = __nv_fp8x2_storage_t(codes.t[2 * i] | codes.t[2 * i + 1] << 8);
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    return mul2(Two(f.x, f.y), scale);
 }
 template <int V>
 __device__ __forceinline__ void store_codes(uint8_t *at, const float (&x)[V])
@@ -125,116 +154,161 @@ __device__ __forceinline__ float warp_max(float x)
     return x;
 }
 
-// A warp takes 256 values at a time: 16-bit parameters with 8-bit moments 8 neighbours per lane (16-byte and 8-byte accesses), all
-// else 4 neighbours twice.
-template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ AdamwTable<CAP> tab)
-{
-    constexpr int V = sizeof(T) == 2 && BITS == 8 ? 8 : 4, N = kBlock / 32 / V;
-    const int lane = threadIdx.x & 31;
-    unsigned b = tab.base + blockIdx.x * unsigned(tab.per_cta) + (threadIdx.x >> 5);
-    const unsigned end = min(tab.base + blockIdx.x * unsigned(tab.per_cta) + unsigned(tab.per_cta), tab.base + tab.blocks);
-    int lo = 0, hi = tab.count;                 // the last tensor that starts at b or before
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tab.entry[mid].first <= b) lo = mid;
-        else hi = mid;
-    }
-    for (; b < end; b += kWarps) {
-        while (lo + 1 < tab.count && tab.entry[lo + 1].first <= b) ++lo;
-        const AdamwEntry &e = tab.entry[lo];
-        const long long at = (long long)(b - e.first) * kBlock, left = e.count - at;
-        if (left <= 0) continue;               // blocks of a tensor without a gradient
-        T *param = static_cast<T *>(e.param) + at;
-        const T *grad = static_cast<const T *>(e.grad) + at;
-        const bool vec = left >= kBlock && ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & (V * sizeof(T) - 1)) == 0;
-        const size_t state = size_t(b) * kBlock;
-        float p[N][V], g[N][V], m[N][V], v[N][V];
+// What a lane has of a block of 256 values: V neighbours, N times
+template <typename T, int BITS>
+struct Part {
+    // 16-bit parameters with 8-bit moments: 8 neighbours (16-byte and 8-byte accesses), all else 4 neighbours twice
+    static constexpr int V = sizeof(T) == 2 && BITS == 8 ? 8 : 4, N = kBlock / 32 / V;
+    typedef typename std::conditional<BITS == 32, float, uint8_t>::type State;
+    Packed<T, V> p[N], g[N];
+    Packed<State, V> m[N], v[N];
+    float m_scale = 0.0f, v_scale = 0.0f, decay, step_size;
+    T *param;
+    long long left;                            // values of the tensor from the block's first on; 0: a tensor without a gradient
+    bool vec;
+
+    template <int CAP>
+    __device__ __forceinline__ void load(const AdamwTable<CAP> &tab, int at, unsigned b, int lane)
+    {
+        const AdamwEntry &e = tab.entry[at];
+        const long long first = (long long)(b - e.first) * kBlock;
+        left = e.count - first;
+        param = static_cast<T *>(e.param) + first;
+        const T *grad = static_cast<const T *>(e.grad) + first;
+        decay = e.decay;
+        step_size = e.step_size;
+        vec = left >= kBlock && ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & (V * sizeof(T) - 1)) == 0;
+        if (left <= 0) return;
+        const State *ms = static_cast<const State *>(tab.m) + size_t(b) * kBlock, *vs = static_cast<const State *>(tab.v) + size_t(b) * kBlock;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = (n * 32 + lane) * V;
             load_values<T, V>(grad + i, vec, left - i, g[n]);
             load_values<T, V>(param + i, vec, left - i, p[n]);
-            if constexpr (BITS == 32) {
-                load_values<float, V>(static_cast<const float *>(tab.m) + state + i, true, 0, m[n]);
-                load_values<float, V>(static_cast<const float *>(tab.v) + state + i, true, 0, v[n]);
-            } else {
-                load_codes<V>(static_cast<const uint8_t *>(tab.m) + state + i, tab.m_scale[b], m[n]);
-                load_codes<V>(static_cast<const uint8_t *>(tab.v) + state + i, tab.v_scale[b], v[n]);
-            }
-        }
-        float m_top = 0.0f, r_top = 0.0f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float gi = g[n][i] * tab.grad_scale;
-                const float old = BITS == 32 ? v[n][i] : v[n][i] * v[n][i];
-                m[n][i] = fmaf(tab.c1, gi - m[n][i], m[n][i]);
-                const float second = fmaf(tab.c2, fmaf(gi, gi, -old), old);
-                const float root = approx_sqrt(second);
-                p[n][i] = p[n][i] * e.decay - e.step_size * __fdividef(m[n][i], fmaf(root, tab.inv_root, tab.eps));
-                v[n][i] = BITS == 32 ? second : root;
-                m_top = fmaxf(m_top, fabsf(m[n][i]));
-                r_top = fmaxf(r_top, root);
-            }
-            const int i = (n * 32 + lane) * V;
-            store_values<T, V>(param + i, vec, left - i, p[n]);
+            load_values<State, V>(ms + i, true, 0, m[n]);
+            load_values<State, V>(vs + i, true, 0, v[n]);
         }
         if constexpr (BITS == 8) {
-            // a scale below the smallest normal number has no reciprocal: the block's moments are then zeros
-            float ms = warp_max(m_top) * (1.0f / 448.0f), rs = warp_max(r_top) * (1.0f / 448.0f);
-            if (ms < 1.17549435e-38f) ms = 0.0f;
-            if (rs < 1.17549435e-38f) rs = 0.0f;
-            const float mi = ms > 0.0f ? __fdividef(1.0f, ms) : 0.0f, ri = rs > 0.0f ? __fdividef(1.0f, rs) : 0.0f;
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    m[n][i] *= mi;
-                    const float r = v[n][i] * ri;
-                    v[n][i] = r > 0.0f ? fmaxf(r, 0.001953125f) : r;
-                }
-            if (lane == 0) {
-                tab.m_scale[b] = ms;
-                tab.v_scale[b] = rs;
-            }
+            m_scale = tab.m_scale[b];
+            v_scale = tab.v_scale[b];
         }
+    }
+
+    template <int CAP>
+    __device__ __forceinline__ void step(const AdamwTable<CAP> &tab, unsigned b, int lane) const
+    {
+        if (left <= 0) return;
+        State *ms = static_cast<State *>(tab.m) + size_t(b) * kBlock, *vs = static_cast<State *>(tab.v) + size_t(b) * kBlock;
+        float first[N][V], second[N][V], m_top = 0.0f, r_top = 0.0f;
+        const Two minus(-1.0f), c1(tab.c1), c2(tab.c2), grad_scale(tab.grad_scale), inv_root(tab.inv_root), eps(tab.eps), keep(decay), move(-step_size);
+        const Two ms2(m_scale), vs2(v_scale);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const size_t i = state + (n * 32 + lane) * V;
-            if constexpr (BITS == 32) {
-                store_values<float, V>(static_cast<float *>(tab.m) + i, true, 0, m[n]);
-                store_values<float, V>(static_cast<float *>(tab.v) + i, true, 0, v[n]);
-            } else {
-                store_codes<V>(static_cast<uint8_t *>(tab.m) + i, m[n]);
-                store_codes<V>(static_cast<uint8_t *>(tab.v) + i, v[n]);
+            float x[V];
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const Two gi = mul2(Two(to_float(g[n].t[i]), to_float(g[n].t[i + 1])), grad_scale);
+                Two m0, v0;
+                if constexpr (BITS == 32) {
+                    m0 = Two(m[n].t[i], m[n].t[i + 1]);
+                    v0 = Two(v[n].t[i], v[n].t[i + 1]);
+                } else {
+                    m0 = decode<V>(m[n], i / 2, ms2);
+                    v0 = decode<V>(v[n], i / 2, vs2);
+                    v0 = mul2(v0, v0);
+                }
+                const Two m1 = fma2(c1, fma2(m0, minus, gi), m0), v1 = fma2(c2, fma2(gi, gi, mul2(v0, minus)), v0);
+                // v rsqrt(v): 0 for 0, and not above the root where v has no normal reciprocal root
+                const float2 vf = v1.both();
+                const Two root = mul2(v1, Two(reciprocal_root(fmaxf(vf.x, 1.17549435e-38f)), reciprocal_root(fmaxf(vf.y, 1.17549435e-38f))));
+                const float2 den = fma2(root, inv_root, eps).both();
+                const Two p1 = fma2(mul2(m1, move), Two(reciprocal(den.x), reciprocal(den.y)), mul2(Two(to_float(p[n].t[i]), to_float(p[n].t[i + 1])), keep));
+                const float2 xf = p1.both(), mf = m1.both(), rf = root.both();
+                x[i] = xf.x;
+                x[i + 1] = xf.y;
+                first[n][i] = mf.x;
+                first[n][i + 1] = mf.y;
+                second[n][i] = BITS == 32 ? vf.x : rf.x;
+                second[n][i + 1] = BITS == 32 ? vf.y : rf.y;
+                if (BITS == 8) {
+                    m_top = fmaxf(m_top, fmaxf(fabsf(mf.x), fabsf(mf.y)));
+                    r_top = fmaxf(r_top, fmaxf(rf.x, rf.y));
+                }
+            }
+            const int i = (n * 32 + lane) * V;
+            store_values<T, V>(param + i, vec, left - i, x);
+        }
+        if constexpr (BITS == 32) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                store_values<float, V>(ms + (n * 32 + lane) * V, true, 0, first[n]);
+                store_values<float, V>(vs + (n * 32 + lane) * V, true, 0, second[n]);
+            }
+        } else {
+            // a scale below the smallest normal number has no reciprocal: the block's moments are then zeros
+            float m_new = warp_max(m_top) * (1.0f / 448.0f), r_new = warp_max(r_top) * (1.0f / 448.0f);
+            if (m_new < 1.17549435e-38f) m_new = 0.0f;
+            if (r_new < 1.17549435e-38f) r_new = 0.0f;
+            const float mi = m_new > 0.0f ? __fdividef(1.0f, m_new) : 0.0f, ri = r_new > 0.0f ? __fdividef(1.0f, r_new) : 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < V; i += 2) {
+                    const float2 f = mul2(Two(first[n][i], first[n][i + 1]), Two(mi)).both(), r = mul2(Two(second[n][i], second[n][i + 1]), Two(ri)).both();
+                    first[n][i] = f.x;
+                    first[n][i + 1] = f.y;
+                    second[n][i] = r.x > 0.0f ? fmaxf(r.x, 0.001953125f) : r.x;
+                    second[n][i + 1] = r.y > 0.0f ? fmaxf(r.y, 0.001953125f) : r.y;
+                }
+                store_codes<V>(ms + (n * 32 + lane) * V, first[n]);
+                store_codes<V>(vs + (n * 32 + lane) * V, second[n]);
+            }
+            if (lane == 0) {
+                tab.m_scale[b] = m_new;
+                tab.v_scale[b] = r_new;
             }
         }
     }
+};
+
+// A warp takes one block of 256 values and a CTA eight.  Warps that walk over several blocks, with or without the next one's loads on
+// their way, took up to twice as long (bf16 with 8-bit moments, 2^27 values: 271 us so, 339 to 541 us otherwise): new CTAs keep more
+// loads in flight.  The registers are held to what lets 40 (fp32) or 48 (16-bit) warps be there with 8-bit moments.
+template <typename T, int BITS, int CAP>
+__global__ void __launch_bounds__(kWarps * 32, BITS == 32 ? 1 : sizeof(T) == 4 ? 5 : 6) adamw_kernel(const __grid_constant__ AdamwTable<CAP> tab)
+{
+    const unsigned b = tab.base + blockIdx.x * kWarps + (threadIdx.x >> 5), end = tab.base + tab.blocks;
+    if (b >= end) return;
+    int at = 0, hi = tab.count;                 // the last tensor that starts at b or before
+    while (hi - at > 1) {
+        const int mid = (at + hi) >> 1;
+        if (tab.entry[mid].first <= b) at = mid;
+        else hi = mid;
+    }
+    Part<T, BITS> part;
+    part.load(tab, at, b, threadIdx.x & 31);
+    part.step(tab, b, threadIdx.x & 31);
 }
 
 template <typename T, int BITS, int CAP>
-void launch_adamw(AdamwTable<CAP> &tab, const DeviceInfo &di, cudaStream_t stream)
+void launch_adamw(const AdamwTable<CAP> &tab, cudaStream_t stream)
 {
-    // four blocks per warp where that leaves every SM several CTAs, else one
-    tab.per_cta = tab.blocks >= unsigned(di.sm_count) * kWarps * 4 * 8 ? kWarps * 4 : kWarps;
-    const unsigned grid = (tab.blocks + unsigned(tab.per_cta) - 1) / unsigned(tab.per_cta);
+    const unsigned grid = (tab.blocks + kWarps - 1) / kWarps;
     adamw_kernel<T, BITS, CAP><<<grid, kWarps * 32, 0, stream>>>(tab);
     count_launch();
 }
 
 template <int CAP>
-void launch_adamw(AdamwTable<CAP> &tab, int type, int bits, const DeviceInfo &di, cudaStream_t stream)
+void launch_adamw(const AdamwTable<CAP> &tab, int type, int bits, cudaStream_t stream)
 {
-    if (type == AXC_TYPE_FLOAT32) bits == 32 ? launch_adamw<float, 32>(tab, di, stream) : launch_adamw<float, 8>(tab, di, stream);
-    else if (type == AXC_TYPE_BFLOAT16) bits == 32 ? launch_adamw<__nv_bfloat16, 32>(tab, di, stream) : launch_adamw<__nv_bfloat16, 8>(tab, di, stream);
-    else bits == 32 ? launch_adamw<__half, 32>(tab, di, stream) : launch_adamw<__half, 8>(tab, di, stream);
+    if (type == AXC_TYPE_FLOAT32) bits == 32 ? launch_adamw<float, 32>(tab, stream) : launch_adamw<float, 8>(tab, stream);
+    else if (type == AXC_TYPE_BFLOAT16) bits == 32 ? launch_adamw<__nv_bfloat16, 32>(tab, stream) : launch_adamw<__nv_bfloat16, 8>(tab, stream);
+    else bits == 32 ? launch_adamw<__half, 32>(tab, stream) : launch_adamw<__half, 8>(tab, stream);
 }
 
 // The tensors in as many launches as their tables need.
 template <int CAP>
-void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t count, const DeviceInfo &di, cudaStream_t stream)
+void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t count, cudaStream_t stream)
 {
     const double root = sqrt(1.0 - pow(d.beta2, double(d.step))), first_left = 1.0 - pow(d.beta1, double(d.step));
     long long block = 0;
@@ -266,7 +340,7 @@ void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t
             e.step_size = float(tensors[at].lr / first_left);
             e.pad = 0;
         }
-        if (tab.count > 0) launch_adamw<CAP>(tab, d.type, d.state_bits, di, stream);
+        if (tab.count > 0) launch_adamw<CAP>(tab, d.type, d.state_bits, stream);
     }
 }
 
@@ -311,8 +385,8 @@ extern "C" int axc_adamw_step(const axc_adamw_desc *desc, const axc_adamw_tensor
     int prev = 0;
     AXC_CUDA(cudaGetDevice(&prev));
     if (prev != device) AXC_CUDA(cudaSetDevice(device));
-    if (count <= kSmallTable) run_adamw<kSmallTable>(d, tensors, count, di, cudaStream_t(stream));
-    else run_adamw<kLargeTable>(d, tensors, count, di, cudaStream_t(stream));
+    if (count <= kSmallTable) run_adamw<kSmallTable>(d, tensors, count, cudaStream_t(stream));
+    else run_adamw<kLargeTable>(d, tensors, count, cudaStream_t(stream));
     const cudaError_t e = cudaGetLastError();
     if (prev != device) cudaSetDevice(prev);
     return e == cudaSuccess ? AXC_OK : cuda_failed(e);
