@@ -2,7 +2,8 @@
 
 Every source is compiled to an object of its own, in parallel, then linked.  `build_library(check=True)` builds the
 debug flavour libaxconv_check.so (-DAXC_BOUNDS_CHECK: every computed shared-memory address and global index is checked
-before use, violations are recorded instead of trapping)."""
+before use, violations are recorded instead of trapping).  `build_binding()` builds the module that takes torch tensors to the
+library, _axc_torch.so."""
 import concurrent.futures
 import os
 import subprocess
@@ -17,11 +18,30 @@ SOURCES = ["axc_api.cu", "axc_conv.cu", "axc_sched.cu", "axc_xtab.cu", "axc_dept
            "axc_adamw.cu", "axc_gemm.cu", "axc_dense.cu", "axc_entropy.cu"]
 
 
+BINDING = os.path.join(HERE, "_axc_torch.so")
+
+
+def build_binding(force=False):
+    """The module between torch tensors and the library (csrc/axc_torch.cpp): CPython and ATen, no CUDA code."""
+    source = os.path.join(CSRC, "axc_torch.cpp")
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(map(os.path.getmtime, (source, os.path.join(INCLUDE, "axconv.h")))):
+        return BINDING
+    import sysconfig
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    includes = [INCLUDE, os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], cuda]
+    subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, source, "-o", BINDING] + ["-I" + i for i in includes] +
+                   ["-L" + os.path.join(home, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"], check=True)
+    return BINDING
+
+
 def needs_build(lib=LIB):
     if not os.path.exists(lib):
         return True
     t = os.path.getmtime(lib)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "axconv.h")]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")] + [os.path.join(INCLUDE, "axconv.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
 

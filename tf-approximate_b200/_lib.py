@@ -40,29 +40,6 @@ class DebugOut(C.Structure):
     _fields_ = [("qinput", C.c_void_p), ("qfilter", C.c_void_p), ("acc", C.c_void_p)]
 
 
-class AdamwTensor(C.Structure):
-    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("count", C.c_int64), ("lr", C.c_double), ("weight_decay", C.c_double)]
-
-
-class AdamwDesc(C.Structure):
-    _fields_ = [("type", C.c_int32), ("state_bits", C.c_int32), ("step", C.c_int64), ("beta1", C.c_double), ("beta2", C.c_double),
-                ("eps", C.c_double), ("grad_scale", C.c_float), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
-                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p)]
-
-
-class DenseDesc(C.Structure):
-    _fields_ = ([(n, C.c_int64) for n in ("rows", "inputs", "units")] +
-                [(n, C.c_int32) for n in ("type", "bias_type", "activation", "kernel_gradient_transposed")] +
-                [(n, C.c_int64) for n in ("x_row_stride", "x_column_stride", "kernel_row_stride", "kernel_column_stride", "residual_row_stride")])
-
-
-class EntropyDesc(C.Structure):
-    _fields_ = ([(n, C.c_int64) for n in ("rows", "inputs", "classes")] +
-                [(n, C.c_int32) for n in ("type", "bias_type", "reduction", "kernel_gradient_transposed")] +
-                [(n, C.c_int64) for n in ("ignore_index", "scratch_limit", "x_row_stride", "x_column_stride", "kernel_row_stride", "kernel_column_stride")] +
-                [("grad_scale", C.c_float)])
-
-
 _lib = None
 
 
@@ -125,13 +102,6 @@ def load():
     L.axc_column_sums.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
     L.axc_quant_props.argtypes = [C.c_float, C.c_float, C.POINTER(C.c_float)]
     L.axc_adamw_state_blocks.argtypes = [C.POINTER(C.c_int64), C.c_int32, C.POINTER(C.c_int64)]
-    L.axc_adamw_step.argtypes = [C.POINTER(AdamwDesc), C.c_void_p, C.c_int32, C.c_int, C.c_void_p]
-    L.axc_dense_workspace_bytes.argtypes = [C.POINTER(DenseDesc), C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
-    L.axc_dense_forward.argtypes = [C.POINTER(DenseDesc)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_int, C.c_void_p]
-    L.axc_dense_backward.argtypes = [C.POINTER(DenseDesc)] + [C.c_void_p] * 9 + [C.c_size_t, C.c_int, C.c_void_p]
-    L.axc_matrix_status.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_int, C.c_void_p]
-    L.axc_entropy_workspace_bytes.argtypes = [C.POINTER(EntropyDesc), C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]
-    L.axc_entropy.argtypes = [C.POINTER(EntropyDesc)] + [C.c_void_p] * 10 + [C.c_size_t, C.c_int, C.c_void_p]
     L.axc_status_string.argtypes = [C.c_int]
     L.axc_status_string.restype = C.c_char_p
     L.axc_last_cuda_error.restype = C.c_int
@@ -140,3 +110,32 @@ def load():
     L.axc_measure_lookup_peak.argtypes = [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p, C.POINTER(C.c_double)]
     _lib = L
     return L
+
+
+_binding = None
+
+
+def binding():
+    """The module between torch tensors and the loaded library (csrc/axc_torch.cpp)."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+
+        import torch  # noqa: F401  the module's symbols come from torch's libraries
+        from . import errors
+        if not os.path.exists(_build.BINDING):
+            raise RuntimeError("_axc_torch.so is not built (%s): run `python -c \"import __graft_entry__ as g; g.build()\"` at the "
+                               "repository root; there is no CPU fallback" % _build.BINDING)
+        L = load()
+        spec = importlib.util.spec_from_file_location("_axc_torch", _build.BINDING)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+
+        def raise_for_status(status, what):
+            errors.raise_for_status(status, what, "cudaError %d" % L.axc_last_cuda_error() if status == 100 else "")
+
+        names = ("axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes",
+                 "axc_entropy", "axc_adamw_step")
+        module.init(tuple(C.cast(getattr(L, n), C.c_void_p).value for n in names), errors.InvalidArgumentError, errors.InternalError, raise_for_status)
+        _binding = module
+    return _binding

@@ -7,7 +7,6 @@ import torch
 
 from . import _lib
 from .errors import InvalidArgumentError, raise_for_status
-from .ops import _cuda_detail
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _BLOCK = 256             # AXC_ADAMW_BLOCK
@@ -52,9 +51,10 @@ class AdamW:
             raise InvalidArgumentError("parameters must be float32, bfloat16 or float16 CUDA tensors")
         self.device, self.dtype, self.state_bits = first.device, first.dtype, state_bits
         self.betas, self.eps, self.step_count = tuple(betas), eps, 0
-        self._index = first.get_device()
+        for p in self.params:
+            if not isinstance(p, torch.Tensor) or p.dtype is not self.dtype or p.device != self.device or not p.is_contiguous():
+                raise InvalidArgumentError("every parameter must be a contiguous %s tensor on %s" % (self.dtype, self.device))
         self._counts = [p.numel() for p in self.params]
-        self._check(self.params, "parameter")
         n, blocks = len(self.params), C.c_int64()
         raise_for_status(_lib.load().axc_adamw_state_blocks((C.c_int64 * n)(*self._counts), n, C.byref(blocks)), "AdamW")
         self._table = np.zeros(n, dtype=_TENSOR)
@@ -69,16 +69,6 @@ class AdamW:
             self.exp_avg_scale = torch.zeros(blocks.value, dtype=torch.float32, device=self.device)
             self.exp_avg_sq_root_scale = torch.zeros(blocks.value, dtype=torch.float32, device=self.device)
 
-    def _check(self, tensors, what):
-        """Nothing that the kernel could read or write out of place: it is given addresses."""
-        T = torch.Tensor
-        if set(map(T.get_device, tensors)) != {self._index} or {t.dtype for t in tensors} != {self.dtype}:
-            raise InvalidArgumentError("every %s must be a %s tensor on %s" % (what, self.dtype, self.device))
-        if list(map(T.numel, tensors)) != self._counts:
-            raise InvalidArgumentError("a %s has another size than the parameter" % what)
-        if what == "parameter" and not all(map(T.is_contiguous, tensors)):
-            raise InvalidArgumentError("parameters must be contiguous")
-
     def set_lr(self, lr):
         """One learning rate for every parameter, from the next step on."""
         self._table["lr"] = lr
@@ -87,36 +77,14 @@ class AdamW:
         for p in self.params:
             p.grad = None
 
-    @torch.no_grad()
     def step(self, grads=None, grad_scale=1.0):
         """One step with `grads`, in the order of the parameters (default: their .grad; None: left as it is), times `grad_scale`."""
-        T, params = torch.Tensor, self.params
-        grads = [p.grad for p in params] if grads is None else list(grads)
-        if len(grads) != len(params):
-            raise InvalidArgumentError("%d gradients for %d parameters" % (len(grads), len(params)))
-        self._check(params, "parameter")
-        missing = [i for i, g in enumerate(grads) if g is None]
-        for i in missing:
-            grads[i] = params[i]
-        self._check(grads, "gradient")
-        if not all(map(T.is_contiguous, grads)):
-            for i, (g, p) in enumerate(zip(grads, params)):
-                if not g.is_contiguous():
-                    if g.shape != p.shape:
-                        raise InvalidArgumentError("a gradient has another shape than the parameter")
-                    grads[i] = g.contiguous()
-        table = self._table
-        table["param"], table["grad"] = list(map(T.data_ptr, params)), list(map(T.data_ptr, grads))
-        if missing:
-            table["grad"][missing] = 0
-        if self.state_bits == 32:
-            states = (self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), None, None)
-        else:
-            states = (self.exp_avg.data_ptr(), self.exp_avg_sq_root.data_ptr(), self.exp_avg_scale.data_ptr(), self.exp_avg_sq_root_scale.data_ptr())
-        desc = _lib.AdamwDesc(_TYPES[self.dtype], self.state_bits, self.step_count + 1, self.betas[0], self.betas[1], self.eps, grad_scale, *states)
-        st = _lib.load().axc_adamw_step(C.byref(desc), table.ctypes.data, len(params), self._index,
-                                        C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
-        raise_for_status(st, "AdamW", _cuda_detail() if st == 100 else "")
+        if grads is not None and not isinstance(grads, list):
+            grads = list(grads)
+        eight = self.state_bits == 8
+        _lib.binding().adamw_step(self.params, grads, self._table.ctypes.data, self.exp_avg, _TYPES[self.dtype], self.state_bits, self.step_count + 1,
+                                  (self.betas[0], self.betas[1], self.eps, grad_scale), self.exp_avg_sq_root if eight else self.exp_avg_sq,
+                                  self.exp_avg_scale if eight else None, self.exp_avg_sq_root_scale if eight else None)
         self.step_count += 1
 
     _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
