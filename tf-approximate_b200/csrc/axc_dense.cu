@@ -49,6 +49,7 @@ __device__ __forceinline__ void load_group(const T *at, long long left, Group<T>
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part)
 {
+    after_previous();
     constexpr int V = Group<T>::V, kRows = (ACT == kActNone ? 8 : 4) / (VEC ? 1 : 2), kApart = VEC ? 1 : 32;
     __shared__ float sums[8][32 * V];
     const int group = threadIdx.x & 31, r0 = threadIdx.x >> 5, first_column = VEC ? group * V : group;
@@ -141,9 +142,10 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
     }
 }
 
-__global__ void __launch_bounds__(256) slope_sums_kernel(const float *__restrict__ part, long long columns, int shares, float scale, const float *scale_dev,
+__global__ void __launch_bounds__(256) slope_sums_kernel(const float *part, long long columns, int shares, float scale, const float *scale_dev,
                                                          void *sums, int type)
 {
+    after_previous();
     const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
     if (c >= columns) return;
     float s = 0.0f;
@@ -162,22 +164,19 @@ int shares_of(long long rows, long long columns)
 }
 
 template <typename T, bool VEC>
-void launch_slope(const Slope &s, float *part, int shares, cudaStream_t stream)
+int launch_slope(const Slope &s, float *part, int shares, Queue &q)
 {
     const long long columns = s.planes && s.line > s.columns ? s.line : s.columns;
     const dim3 grid(unsigned((columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
-    if (!s.kept) slope_kernel<T, kActNone, VEC><<<grid, 256, 0, stream>>>(s, part);
-    else if (s.activation == kActRelu) slope_kernel<T, kActRelu, VEC><<<grid, 256, 0, stream>>>(s, part);
-    else if (s.activation == kActGelu) slope_kernel<T, kActGelu, VEC><<<grid, 256, 0, stream>>>(s, part);
-    else slope_kernel<T, kActSilu, VEC><<<grid, 256, 0, stream>>>(s, part);
-    count_launch();
+    return launch(q, !s.kept ? slope_kernel<T, kActNone, VEC> : s.activation == kActRelu ? slope_kernel<T, kActRelu, VEC>
+                     : s.activation == kActGelu ? slope_kernel<T, kActGelu, VEC> : slope_kernel<T, kActSilu, VEC>, grid, 256, 0, 1, s, part);
 }
 
 }  // namespace
 
 size_t slope_scratch(long long rows, long long columns) { return size_t(shares_of(rows, columns)) * size_t(columns) * 4; }
 
-int slope(const Slope &s, void *scratch, const DeviceInfo &di, cudaStream_t stream)
+int slope(const Slope &s, void *scratch, const DeviceInfo &di, Queue &q)
 {
     (void)di;
     if (s.columns == 0 || (s.rows == 0 && !s.sums)) return AXC_OK;
@@ -187,14 +186,12 @@ int slope(const Slope &s, void *scratch, const DeviceInfo &di, cudaStream_t stre
     const uintptr_t all = reinterpret_cast<uintptr_t>(s.dy) | reinterpret_cast<uintptr_t>(s.kept) | reinterpret_cast<uintptr_t>(s.same);
     const long long size = s.type == kFloat32 ? 4 : 2;
     const bool vec = (all & 15u) == 0 && s.dy_line * size % 16 == 0 && (s.padded || s.columns * size % 16 == 0) && s.plane * size % 16 == 0;
-    if (s.type == kFloat32) vec ? launch_slope<float, true>(s, part, shares, stream) : launch_slope<float, false>(s, part, shares, stream);
-    else if (s.type == kBfloat16) vec ? launch_slope<__nv_bfloat16, true>(s, part, shares, stream) : launch_slope<__nv_bfloat16, false>(s, part, shares, stream);
-    else vec ? launch_slope<__half, true>(s, part, shares, stream) : launch_slope<__half, false>(s, part, shares, stream);
-    if (s.sums) {
-        slope_sums_kernel<<<unsigned((s.columns + 255) / 256), 256, 0, stream>>>(part, s.columns, shares, s.scale, s.scale_dev, s.sums, s.sums_type);
-        count_launch();
-    }
-    return AXC_OK;
+    int rc;
+    if (s.type == kFloat32) rc = vec ? launch_slope<float, true>(s, part, shares, q) : launch_slope<float, false>(s, part, shares, q);
+    else if (s.type == kBfloat16) rc = vec ? launch_slope<__nv_bfloat16, true>(s, part, shares, q) : launch_slope<__nv_bfloat16, false>(s, part, shares, q);
+    else rc = vec ? launch_slope<__half, true>(s, part, shares, q) : launch_slope<__half, false>(s, part, shares, q);
+    if (rc || !s.sums) return rc;
+    return launch(q, slope_sums_kernel, dim3(unsigned((s.columns + 255) / 256)), 256, 0, 1, part, s.columns, shares, s.scale, s.scale_dev, s.sums, s.sums_type);
 }
 
 namespace {
@@ -258,7 +255,7 @@ int leave(int rc, int device, int prev)
 }
 
 int forward(const axc_dense_desc &d, const void *x, const void *kernel, const void *bias, const void *residual, void *y, void *pre, char *ws,
-            const DeviceInfo &di, cudaStream_t stream)
+            const DeviceInfo &di, Queue &q)
 {
     const Parts parts = parts_of(d, false, x, kernel, di);
     Gemm g = {};
@@ -269,8 +266,8 @@ int forward(const axc_dense_desc &d, const void *x, const void *kernel, const vo
     g.bf16 = d.type != kFloat16;
     int rc = AXC_OK;
     if (d.inputs > 0) {
-        rc = make_operand(x_of(d, x), ws + parts.x, &g.a, di, stream);
-        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &g.b, di, stream);
+        rc = make_operand(x_of(d, x), ws + parts.x, &g.a, di, q);
+        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &g.b, di, q);
         if (rc) return rc;
     }
     g.fin.alpha = 1.0f;
@@ -284,11 +281,11 @@ int forward(const axc_dense_desc &d, const void *x, const void *kernel, const vo
     g.fin.out_type = d.type;
     g.fin.out_line = d.units;
     g.fin.pre = pre;
-    return gemm(g, ws + parts.scratch, reinterpret_cast<unsigned *>(ws), true, di, stream);
+    return gemm(g, ws + parts.scratch, reinterpret_cast<unsigned *>(ws), true, di, q);
 }
 
 int backward(const axc_dense_desc &d, const void *dy, const void *x, const void *kernel, const void *kept, void *dx, void *dkernel, void *dbias,
-             void *dresidual, char *ws, const DeviceInfo &di, cudaStream_t stream)
+             void *dresidual, char *ws, const DeviceInfo &di, Queue &q)
 {
     const Parts parts = parts_of(d, true, x, kernel, di);
     const int planes = d.type == kFloat32 ? 3 : 1;
@@ -321,12 +318,12 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
     s.sums_type = d.bias_type;
     s.scale = 1.0f;
     int rc = AXC_OK;
-    if (s.same || s.planes || s.sums) rc = slope(s, ws + parts.part, di, stream);
+    if (s.same || s.planes || s.sums) rc = slope(s, ws + parts.part, di, q);
     if (rc) return rc;
     bool first = true;
     Operand operand = {};
     if (dx) {
-        if (d.units > 0) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &operand, di, stream);
+        if (d.units > 0) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &operand, di, q);
         if (rc) return rc;
         Gemm g = {};
         g.m = d.rows;
@@ -340,12 +337,12 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
         g.fin.out = dx;
         g.fin.out_type = d.type;
         g.fin.out_line = d.inputs;
-        rc = gemm(g, ws + parts.scratch, status, first, di, stream);
+        rc = gemm(g, ws + parts.scratch, status, first, di, q);
         if (rc) return rc;
         first = false;
     }
     if (dkernel) {
-        if (d.rows > 0) rc = make_operand(x_of(d, x), ws + parts.x, &operand, di, stream);
+        if (d.rows > 0) rc = make_operand(x_of(d, x), ws + parts.x, &operand, di, q);
         if (rc) return rc;
         Gemm g = {};
         g.k = d.rows;
@@ -366,11 +363,11 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
             g.b = transposed(dz);
         }
         g.fin.out_line = g.n;
-        rc = gemm(g, ws + parts.scratch, status, first, di, stream);
+        rc = gemm(g, ws + parts.scratch, status, first, di, q);
         if (rc) return rc;
         first = false;
     }
-    if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), stream));
+    if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
     return AXC_OK;
 }
 
@@ -408,7 +405,8 @@ extern "C" int axc_dense_forward(const axc_dense_desc *desc, const void *x, cons
     int prev = 0;
     rc = enter(device, &di, &prev);
     if (rc) return rc;
-    return leave(forward(d, x, kernel, bias, residual, y, pre, static_cast<char *>(workspace), di, cudaStream_t(stream)), device, prev);
+    Queue q = {cudaStream_t(stream)};
+    return leave(forward(d, x, kernel, bias, residual, y, pre, static_cast<char *>(workspace), di, q), device, prev);
 }
 
 extern "C" int axc_dense_backward(const axc_dense_desc *desc, const void *dy, const void *x, const void *kernel, const void *kept, void *dx, void *dkernel,
@@ -429,7 +427,8 @@ extern "C" int axc_dense_backward(const axc_dense_desc *desc, const void *dy, co
     int prev = 0;
     rc = enter(device, &di, &prev);
     if (rc) return rc;
-    return leave(backward(d, dy, x, kernel, kept, dx, dkernel, dbias, dresidual, static_cast<char *>(workspace), di, cudaStream_t(stream)), device, prev);
+    Queue q = {cudaStream_t(stream)};
+    return leave(backward(d, dy, x, kernel, kept, dx, dkernel, dbias, dresidual, static_cast<char *>(workspace), di, q), device, prev);
 }
 
 extern "C" int axc_matrix_status(const void *workspace, int32_t *status, int device, void *stream)

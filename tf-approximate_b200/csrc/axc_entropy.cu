@@ -60,6 +60,7 @@ __device__ __forceinline__ float block_sum(float v, float *shared)
 template <int FORM>
 __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
 {
+    after_previous();
     __shared__ float shared[8];
     const long long row = blockIdx.x;
     const float2 *stats = A.stats + row * A.segments;
@@ -132,9 +133,10 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
 }
 
 // The rows' losses added in a fixed order, and the factor of the gradients; one block.
-__global__ void __launch_bounds__(1024) loss_kernel(const float *__restrict__ row_loss, const long long *__restrict__ labels, long long rows, long long ignore,
+__global__ void __launch_bounds__(1024) loss_kernel(const float *row_loss, const long long *labels, long long rows, long long ignore,
                                                     int mean, float grad_factor, float *loss, float *alpha)
 {
+    after_previous();
     __shared__ float shared[32];
     float sum = 0.0f, count = 0.0f, low = 0.0f;                 // compensated: a sum may run over a million rows
     for (long long i = threadIdx.x; i < rows; i += 1024) {
@@ -222,7 +224,7 @@ int check_desc(const axc_entropy_desc *d)
 }
 
 int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const void *kernel, const void *bias, const long long *labels, float *loss, float *row_loss,
-            void *dx, void *dkernel, void *dbias, char *ws, const DeviceInfo &di, cudaStream_t stream)
+            void *dx, void *dkernel, void *dbias, char *ws, const DeviceInfo &di, Queue &q)
 {
     const int planes = d.type == kFloat32 ? 3 : 1;
     const float stored = d.type == kFloat16 ? kHalfScale : 1.0f;
@@ -237,8 +239,8 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
     Operand ox = {}, ok = {};
     int rc = AXC_OK;
     if (d.rows > 0) {
-        rc = make_operand(x_of(d, x), ws + l.x, &ox, di, stream);
-        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + l.kernel, &ok, di, stream);
+        rc = make_operand(x_of(d, x), ws + l.x, &ox, di, q);
+        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + l.kernel, &ok, di, q);
         if (rc) return rc;
         g.m = d.rows;
         g.n = d.classes;
@@ -255,7 +257,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
         e.stats = reinterpret_cast<float2 *>(ws + l.stats);
         e.segments = l.segments;
         e.label_logit = label_logit;
-        rc = gemm_entropy(g, e, false, status, true, di, stream);
+        rc = gemm_entropy(g, e, false, status, true, di, q);
         if (rc) return rc;
         RowArgs r = {};
         r.rows = d.rows;
@@ -274,15 +276,11 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
         r.gradient = reinterpret_cast<uint16_t *>(ws + l.gradient);
         r.plane = l.line * d.rows;
         const unsigned grid = unsigned(d.rows);
-        if (!l.kept) row_kernel<0><<<grid, 256, 0, stream>>>(r);
-        else if (d.type == kBfloat16) row_kernel<1><<<grid, 256, 0, stream>>>(r);
-        else if (d.type == kFloat16) row_kernel<2><<<grid, 256, 0, stream>>>(r);
-        else row_kernel<3><<<grid, 256, 0, stream>>>(r);
-        count_launch();
-    } else AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), stream));
-    loss_kernel<<<1, 1024, 0, stream>>>(row_loss, labels, d.rows, d.ignore_index, d.reduction == AXC_REDUCE_MEAN, d.grad_scale / stored, loss, alpha);
-    count_launch();
-    if (!l.gradients) return AXC_OK;
+        rc = launch(q, !l.kept ? row_kernel<0> : d.type == kBfloat16 ? row_kernel<1> : d.type == kFloat16 ? row_kernel<2> : row_kernel<3>, dim3(grid), 256, 0, 1, r);
+        if (rc) return rc;
+    } else AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
+    rc = launch(q, loss_kernel, dim3(1), 1024, 0, 1, row_loss, labels, d.rows, d.ignore_index, int(d.reduction == AXC_REDUCE_MEAN), d.grad_scale / stored, loss, alpha);
+    if (rc || !l.gradients) return rc;
     const size_t size = type_size(d.type);
     float *dx_sum = reinterpret_cast<float *>(ws + l.dx);
     const long long dx_line = (d.inputs + 3) / 4 * 4;
@@ -304,7 +302,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             e.lse = lse;
             e.row_scale = row_scale;
             e.column0 = int(c0);
-            rc = gemm_entropy(again, e, true, status, false, di, stream);
+            rc = gemm_entropy(again, e, true, status, false, di, q);
             if (rc) return rc;
         }
         const Operand dl = {ws + l.gradient, l.line, l.line * d.rows, false};
@@ -326,7 +324,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             p.fin.out = last ? dx : dx_sum;
             p.fin.out_type = last ? d.type : kFloat32;
             p.fin.out_line = last ? d.inputs : dx_line;
-            rc = gemm(p, ws + l.scratch, status, false, di, stream);
+            rc = gemm(p, ws + l.scratch, status, false, di, q);
             if (rc) return rc;
             p.fin.addend = nullptr;
         }
@@ -348,7 +346,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
                 p.fin.out = static_cast<char *>(dkernel) + size_t(c0) * size;
                 p.fin.out_line = d.classes;
             }
-            rc = gemm(p, ws + l.scratch, status, false, di, stream);
+            rc = gemm(p, ws + l.scratch, status, false, di, q);
             if (rc) return rc;
         }
         if (dbias) {
@@ -365,7 +363,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             s.sums_type = d.bias_type;
             s.scale = 1.0f;
             s.scale_dev = alpha;
-            rc = slope(s, ws + l.part, di, stream);
+            rc = slope(s, ws + l.part, di, q);
             if (rc) return rc;
         }
     }
@@ -407,8 +405,8 @@ extern "C" int axc_entropy(const axc_entropy_desc *desc, const void *x, const vo
     int prev = 0;
     AXC_CUDA(cudaGetDevice(&prev));
     if (prev != device) AXC_CUDA(cudaSetDevice(device));
-    rc = entropy(d, l, x, kernel, bias, reinterpret_cast<const long long *>(labels), loss, row_loss, dx, dkernel, dbias, static_cast<char *>(workspace), di,
-                 cudaStream_t(stream));
+    Queue q = {cudaStream_t(stream)};
+    rc = entropy(d, l, x, kernel, bias, reinterpret_cast<const long long *>(labels), loss, row_loss, dx, dkernel, dbias, static_cast<char *>(workspace), di, q);
     const cudaError_t e = cudaGetLastError();
     if (prev != device) cudaSetDevice(prev);
     return rc != AXC_OK ? rc : e == cudaSuccess ? AXC_OK : cuda_failed(e);

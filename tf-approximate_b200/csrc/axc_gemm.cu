@@ -19,6 +19,8 @@
 // kernel, which also applies what follows the product.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "axc_gemm.h"
 #include "axc_mma.cuh"
 
@@ -405,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     const int worker = int(blockIdx.x) / CG, workers = int(gridDim.x) / CG;
     const int units = P.tiles_m * P.tiles_n * P.splits;
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        if (P.first && blockIdx.x == 0) *P.status = 0u;        // a wait runs out after a second, not before this
         for (int i = 0; i < P.stages; ++i) {
             mma::barrier_init(full + 8 * i, 1);
             mma::barrier_init(empty + 8 * i, 1);
@@ -426,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     mma::fence_after();
     const unsigned tmem = head->tmem;
     asm volatile("griddepcontrol.wait;" ::: "memory");          // operands may come from the kernel before
+    if (P.first && blockIdx.x == 0 && threadIdx.x == 0) *P.status = 0u;        // a wait runs out after a second, not before this
     bool ok = true;
 
     // The loading and the multiplying warp run as a whole and one of their threads acts, so that what it hands over is computed once for
@@ -593,10 +596,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 }
 
 // The partial sums of a split product, added in the order of the splits, and what follows the product
-__global__ void __launch_bounds__(256) finish_kernel(const float *__restrict__ part, long long stride, long long part_line, int splits, int lines,
+__global__ void __launch_bounds__(256) finish_kernel(const float *part, long long stride, long long part_line, int splits, int lines,
                                                      int columns, const Finish f)
 {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous();
     const int quads = (columns + 3) / 4;
     const long long total = (long long)lines * quads;
     const float alpha = f.alpha * (f.alpha_dev ? *f.alpha_dev : 1.0f);
@@ -691,52 +694,46 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
 }
 
 template <int CG, int BN, int MODE, int PLANES>
-int launch(GemmArgs &P, long long units, const DeviceInfo &di, cudaStream_t stream)
+int launch_gemm(GemmArgs &P, long long units, const DeviceInfo &di, Queue &q)
 {
     const unsigned stage = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
     const unsigned lines = PLANES == 3 ? 8 * 1024 : 8 * 4096;
     P.stages = int((kSmem - kHeader - 1024 - lines) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const unsigned smem = kHeader + 1024 + lines + unsigned(P.stages) * stage;
-    AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+    static std::atomic<unsigned long long> ready{0};           // devices on which the kernel may have all shared memory
+    int device = 0;
+    AXC_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (!(ready.load(std::memory_order_acquire) & bit) || !bit) {
+        AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+        ready.fetch_or(bit, std::memory_order_release);
+    }
     const long long workers = di.sm_count / CG;
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((units < workers ? units : workers) * CG));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    AXC_CUDA(cudaLaunchKernelEx(&cfg, gemm_kernel<CG, BN, MODE, PLANES>, P));
-    count_launch();
-    return AXC_OK;
+    return launch(q, gemm_kernel<CG, BN, MODE, PLANES>, dim3(unsigned((units < workers ? units : workers) * CG)), kThreads, smem, CG, P);
 }
 
 template <int MODE, int PLANES>
-int launch_tiles(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, cudaStream_t stream)
+int launch_tiles(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, Queue &q)
 {
     if constexpr (PLANES == 1) {
-        if (plan.bn == 256) return plan.cg == 2 ? launch<2, 256, MODE, 1>(P, units, di, stream) : launch<1, 256, MODE, 1>(P, units, di, stream);
+        if (plan.bn == 256) return plan.cg == 2 ? launch_gemm<2, 256, MODE, 1>(P, units, di, q) : launch_gemm<1, 256, MODE, 1>(P, units, di, q);
     } else {
-        if (plan.cg == 2) return launch<2, 128, MODE, 3>(P, units, di, stream);
+        if (plan.cg == 2) return launch_gemm<2, 128, MODE, 3>(P, units, di, q);
     }
-    if (plan.bn == 128) return launch<1, 128, MODE, PLANES>(P, units, di, stream);
-    if (plan.bn == 64) return launch<1, 64, MODE, PLANES>(P, units, di, stream);
+    if (plan.bn == 128) return launch_gemm<1, 128, MODE, PLANES>(P, units, di, q);
+    if (plan.bn == 64) return launch_gemm<1, 64, MODE, PLANES>(P, units, di, q);
     if constexpr (MODE == kStore || MODE == kPartial) {
-        if (plan.bn == 32) return launch<1, 32, MODE, PLANES>(P, units, di, stream);
-        return launch<1, 16, MODE, PLANES>(P, units, di, stream);
+        if (plan.bn == 32) return launch_gemm<1, 32, MODE, PLANES>(P, units, di, q);
+        return launch_gemm<1, 16, MODE, PLANES>(P, units, di, q);
     }
     return AXC_INTERNAL;
 }
 
 template <int MODE>
-int launch_plan(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, cudaStream_t stream)
+int launch_plan(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, Queue &q)
 {
-    return P.planes == 3 ? launch_tiles<MODE, 3>(P, plan, units, di, stream) : launch_tiles<MODE, 1>(P, plan, units, di, stream);
+    return P.planes == 3 ? launch_tiles<MODE, 3>(P, plan, units, di, q) : launch_tiles<MODE, 1>(P, plan, units, di, q);
 }
 
 int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, GemmArgs *P)
@@ -766,12 +763,10 @@ int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, Gem
     return AXC_OK;
 }
 
-int launch_finish(const float *part, long long stride, long long line, int splits, const Gemm &g, const DeviceInfo &di, cudaStream_t stream)
+int launch_finish(const float *part, long long stride, long long line, int splits, const Gemm &g, const DeviceInfo &di, Queue &q)
 {
     const long long work = ceil_div(g.m * ceil_div(g.n, 4), 256), most = (long long)di.sm_count * 8;
-    finish_kernel<<<unsigned(work < most ? work : most), 256, 0, stream>>>(part, stride, line, splits, int(g.m), int(g.n), g.fin);
-    count_launch();
-    return AXC_OK;
+    return launch(q, finish_kernel, dim3(unsigned(work < most ? work : most)), 256, 0, 1, part, stride, line, splits, int(g.m), int(g.n), g.fin);
 }
 
 }  // namespace
@@ -783,12 +778,12 @@ size_t gemm_scratch(long long m, long long n, long long k, int planes, const Dev
     return plan.splits > 1 ? size_t(plan.splits) * size_t(m) * size_t((n + 3) / 4 * 4) * 4 : 0;
 }
 
-int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream)
+int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
 {
     if (g.m == 0 || g.n == 0) return AXC_OK;
     if (g.k == 0) {                                             // sums of nothing
-        if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), stream));
-        return launch_finish(nullptr, 0, 0, 0, g, di, stream);
+        if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
+        return launch_finish(nullptr, 0, 0, 0, g, di, q);
     }
     const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, true, di.sm_count);
     GemmArgs P = {};
@@ -796,16 +791,16 @@ int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const Devic
     if (rc) return rc;
     const long long units = (long long)P.tiles_m * P.tiles_n * plan.splits;
     if (units > 0x7fffffffll) return AXC_INVALID_ARGUMENT;
-    if (plan.splits == 1) return launch_plan<kStore>(P, plan, units, di, stream);
+    if (plan.splits == 1) return launch_plan<kStore>(P, plan, units, di, q);
     P.part = static_cast<float *>(scratch);
     P.part_line = (g.n + 3) / 4 * 4;
     P.part_stride = P.part_line * g.m;
-    rc = launch_plan<kPartial>(P, plan, units, di, stream);
+    rc = launch_plan<kPartial>(P, plan, units, di, q);
     if (rc) return rc;
-    return launch_finish(P.part, P.part_stride, P.part_line, plan.splits, g, di, stream);
+    return launch_finish(P.part, P.part_stride, P.part_line, plan.splits, g, di, q);
 }
 
-int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream)
+int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
 {
     if (g.m == 0 || g.n == 0) return AXC_OK;
     const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, false, false, di.sm_count);
@@ -815,7 +810,7 @@ int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *s
     const long long units = (long long)P.tiles_m * P.tiles_n;
     if (units > 0x7fffffffll) return AXC_INVALID_ARGUMENT;
     P.ent = e;
-    return gradient ? launch_plan<kGradient>(P, plan, units, di, stream) : launch_plan<kEntropy>(P, plan, units, di, stream);
+    return gradient ? launch_plan<kGradient>(P, plan, units, di, q) : launch_plan<kEntropy>(P, plan, units, di, q);
 }
 
 // ---- operands -----------------------------------------------------------------------------------------------------------
@@ -824,9 +819,10 @@ namespace {
 // Copies a matrix into lines of a multiple of 8 values, 16-bit types as they are, fp32 as three bf16 planes: the value rounded to
 // bf16, the rest rounded again, and what is left then, which bf16 holds exactly.
 template <bool SPLIT>
-__global__ void __launch_bounds__(256) lay_out_kernel(const void *__restrict__ src, int type, long long outer, long long inner, long long outer_stride,
-                                                      long long inner_stride, uint16_t *__restrict__ dst, long long line, long long plane)
+__global__ void __launch_bounds__(256) lay_out_kernel(const void *src, int type, long long outer, long long inner, long long outer_stride,
+                                                      long long inner_stride, uint16_t *dst, long long line, long long plane)
 {
+    after_previous();
     const long long groups = line / 8, total = outer * groups;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long o = i / groups, c = (i - o * groups) * 8;
@@ -835,10 +831,10 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const void *__restrict__ s
         for (int j = 0; j < 8; ++j) {
             const long long at = o * outer_stride + (c + j) * inner_stride;
             if (SPLIT) {
-                float x = c + j < inner ? __ldg(static_cast<const float *>(src) + at) : 0.0f;
+                float x = c + j < inner ? static_cast<const float *>(src)[at] : 0.0f;
 #pragma unroll
                 for (int p = 0; p < 3; ++p) out[p].h[j] = split_term(x, x);
-            } else out[0].h[j] = c + j < inner ? __ldg(static_cast<const uint16_t *>(src) + at) : uint16_t(0);
+            } else out[0].h[j] = c + j < inner ? static_cast<const uint16_t *>(src)[at] : uint16_t(0);
         }
 #pragma unroll
         for (int p = 0; p < (SPLIT ? 3 : 1); ++p) *reinterpret_cast<uint4 *>(dst + p * plane + o * line + c) = out[p].w;
@@ -866,7 +862,7 @@ size_t operand_bytes(const Matrix &x)
     return (outer * ((inner + 7) / 8 * 8) * 2 * (x.type == kFloat32 ? 3 : 1) + 255) / 256 * 256;
 }
 
-int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, cudaStream_t stream)
+int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, Queue &q)
 {
     if (readable_in_place(x)) {
         const bool by_columns = x.column_stride == 1 && x.row_stride % 8 == 0 && x.row_stride >= x.columns;
@@ -878,14 +874,9 @@ int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo 
     *out = {scratch, line, outer * line, !in};
     const long long work = ceil_div(outer * (line / 8), 256);
     const unsigned grid = unsigned(work < di.sm_count * 16 ? work : di.sm_count * 16);
-    if (x.type == kFloat32)
-        lay_out_kernel<true><<<grid, 256, 0, stream>>>(x.data, x.type, outer, inner, in ? x.row_stride : x.column_stride, in ? x.column_stride : x.row_stride,
-                                                       static_cast<uint16_t *>(scratch), line, outer * line);
-    else
-        lay_out_kernel<false><<<grid, 256, 0, stream>>>(x.data, x.type, outer, inner, in ? x.row_stride : x.column_stride, in ? x.column_stride : x.row_stride,
-                                                        static_cast<uint16_t *>(scratch), line, outer * line);
-    count_launch();
-    return AXC_OK;
+    const long long outer_stride = in ? x.row_stride : x.column_stride, inner_stride = in ? x.column_stride : x.row_stride;
+    return launch(q, x.type == kFloat32 ? lay_out_kernel<true> : lay_out_kernel<false>, dim3(grid), 256, 0, 1, x.data, x.type, outer, inner, outer_stride,
+                  inner_stride, static_cast<uint16_t *>(scratch), line, outer * line);
 }
 
 }  // namespace axc

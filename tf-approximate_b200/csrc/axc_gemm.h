@@ -8,6 +8,47 @@
 namespace axc {
 
 enum { kFloat32 = AXC_TYPE_FLOAT32, kBfloat16 = AXC_TYPE_BFLOAT16, kFloat16 = AXC_TYPE_FLOAT16 };
+// The launches of a call.  Every kernel after the first may start while the one before it ends: it waits for that one, whole and
+// visible, before it touches memory (after_previous), so that only its set-up overlaps.
+struct Queue {
+    cudaStream_t stream;
+    bool first = true;
+};
+template <typename... Params, typename... Args>
+inline int launch(Queue &q, void (*kernel)(Params...), dim3 grid, unsigned threads, unsigned smem, unsigned cluster, Args &&...args)
+{
+    cudaLaunchAttribute attr[2] = {};
+    unsigned n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (!q.first) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    q.first = false;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = q.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    AXC_CUDA(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
+    count_launch();
+    return AXC_OK;
+}
+// First in every kernel that `launch` starts: the next kernel may come, the one before is over.
+__device__ __forceinline__ void after_previous()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 inline size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
 
 template <typename T> __device__ __forceinline__ float widen(T x);
@@ -22,9 +63,9 @@ template <> __device__ __forceinline__ __half narrow<__half>(float x) { return _
 // element i of an array of `type`
 __device__ __forceinline__ float load_as_float(const void *p, long long i, int type)
 {
-    if (type == kFloat32) return __ldg(static_cast<const float *>(p) + i);
-    if (type == kBfloat16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(p) + i));
-    return __half2float(__ldg(static_cast<const __half *>(p) + i));
+    if (type == kFloat32) return *(static_cast<const float *>(p) + i);
+    if (type == kBfloat16) return __bfloat162float(*(static_cast<const __nv_bfloat16 *>(p) + i));
+    return __half2float(*(static_cast<const __half *>(p) + i));
 }
 __device__ __forceinline__ void store_from_float(void *p, long long i, int type, float x)
 {
@@ -123,9 +164,9 @@ struct Gemm {
 // Scratch for the partial sums of a product whose k is split; 0 where it is not.
 size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di);
 // `first`: of the products of a call; it clears the status word.
-int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream);
+int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, Queue &q);
 // Tiles of logits, never split; `gradient`: the second pass of the piecewise form.
-int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, cudaStream_t stream);
+int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, Queue &q);
 
 // Gradient of an activation and the sums of its columns, in one pass over dy [rows, columns]:
 //   dz = dy * act'(kept);  to `same` (dy's type and layout) and / or to the 16-bit planes of an operand, where given;
@@ -147,7 +188,7 @@ struct Slope {
     const float *scale_dev;
 };
 size_t slope_scratch(long long rows, long long columns);       // partial sums
-int slope(const Slope &s, void *scratch, const DeviceInfo &di, cudaStream_t stream);
+int slope(const Slope &s, void *scratch, const DeviceInfo &di, Queue &q);
 
 // ---- operands -----------------------------------------------------------------------------------------------------------
 // A matrix in the caller's memory: element (r, c) at data[r * row_stride + c * column_stride]
@@ -160,7 +201,7 @@ struct Matrix {
 bool readable_in_place(const Matrix &x);
 size_t operand_bytes(const Matrix &x);          // scratch that operand() fills, 0 where it reads in place
 // The matrix as an operand whose rows are x's rows (or, transposed, x's columns); copies and splits into `scratch` as needed.
-int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, cudaStream_t stream);
+int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, Queue &q);
 inline Operand transposed(Operand o)
 {
     o.rows_contiguous = !o.rows_contiguous;
