@@ -116,6 +116,21 @@ def test_strides_and_alignment(built, dtype):
         check_dense(x, w, rand(n), r, None, dtype, rand(n, t).t())
 
 
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9])
+def test_few_rows(built, rows, dtype, order):
+    """The kernels for up to 8 rows: short and long inputs, few units and many, off the 16-byte grid."""
+    import torch
+    for k, n in ((1, 5), (31, 260), (2048, 1000), (4100, 9999), (8192, 72), (264, 19000)):
+        x, w, b, r, g = make(rows, k, n, dtype, order, 3)
+        grad = torch.randn(rows, n, device="cuda", generator=g).to(x.dtype)
+        check_dense(x, w, b, r, "silu" if k % 2 else None, dtype, grad)
+    big = torch.randn(2 * rows, 301, device="cuda", generator=g).to(x.dtype)
+    x, w, b, r, _ = make(rows, 300, 500, dtype, order, 4)
+    check_dense(big[::2, 1:], w[:, 1:], b[1:], None, "gelu", dtype, r[:, 1:])
+
+
 def test_bias_of_another_type_and_leading_dimensions(built):
     import torch
     import tf_approximate_b200 as ax

@@ -39,7 +39,7 @@ def check_entropy(x, w, b, labels, dtype, reduction="mean", scale=1.0, limit=Non
     size = xd.abs() @ wd.abs() + (torch.where(torch.isfinite(b), b, torch.zeros_like(b)).double().abs() if b is not None else 0.0)
     e = size.amax(1) * sum_error(x.shape[1], dtype) + (logits.abs().nan_to_num(0.0, 0.0, 0.0).amax(1) + 1) * 2.0 ** -22     # per row
     off_row = 2 * e + 2.0 ** -19
-    got_loss, got_rows = ax.dense_cross_entropy(x, w, labels, b, reduction=reduction, row_losses=True)
+    got_loss, got_rows = ax.dense_cross_entropy(x, w, labels, b, reduction=reduction, row_losses=True, scratch_limit=limit)
     assert torch.equal(got_loss, loss)
     assert bool(((got_rows.double() - rows).abs() <= off_row).all())
     assert abs(float(loss) - float(rows.sum()) / count) <= float((off_row * valid).sum()) / count + 2.0 ** -20 * float(rows.sum()) / count + 1e-30
@@ -84,12 +84,13 @@ def test_few_pieces(built, dtype):
         check_entropy(x, w, b, labels, dtype, limit=200 * classes * (6 if dtype == "float32" else 2))
 
 
-@pytest.mark.parametrize("limit", [None, 1])
+@pytest.mark.parametrize("rows,limit", [(140, None), (140, 1), (1600, None)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_extreme_logits_and_masked_classes(built, dtype, limit):
+def test_extreme_logits_and_masked_classes(built, dtype, rows, limit):
+    """Few logits, pieces of the classes, kept exponentials."""
     import torch
     import tf_approximate_b200 as ax
-    x, w, b, labels = make(140, 64, 700, dtype, "in_out", scale=100.0)      # logits of some hundreds
+    x, w, b, labels = make(rows, 64, 700, dtype, "in_out", scale=100.0)      # logits of some hundreds
     check_entropy(x, w, b, labels, dtype, limit=limit)
     low = float(torch.finfo(b.dtype).min)
     for masked in (float("-inf"), low):
@@ -102,12 +103,12 @@ def test_extreme_logits_and_masked_classes(built, dtype, limit):
         assert bool((dw[:, 64:200] == 0).all()) and bool((db[64:200] == 0).all()) and bool(torch.isfinite(dx).all())
 
 
-@pytest.mark.parametrize("limit", [None, 1])
+@pytest.mark.parametrize("rows,limit", [(77, None), (77, 1), (4000, None)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
-def test_rows_without_label(built, dtype, limit):
+def test_rows_without_label(built, dtype, rows, limit):
     import torch
     import tf_approximate_b200 as ax
-    x, w, b, labels = make(77, 40, 300, dtype, "out_in")
+    x, w, b, labels = make(rows, 40, 300, dtype, "out_in")
     for reduction in ("mean", "sum"):
         loss, dx, dw, db = ax.dense_cross_entropy_gradients(x, w, torch.full_like(labels, -100), b, reduction=reduction, scratch_limit=limit)
         assert float(loss) == 0.0 and not bool(dx.any()) and not bool(dw.any()) and not bool(db.any())
@@ -120,24 +121,24 @@ def test_rows_without_label(built, dtype, limit):
     assert bool(torch.isfinite(check))
 
 
-@pytest.mark.parametrize("limit", [None, 1])
-def test_labels_that_are_no_class(built, limit):
+@pytest.mark.parametrize("rows,limit", [(77, None), (77, 1), (4000, None)])
+def test_labels_that_are_no_class(built, rows, limit):
     import torch
     import tf_approximate_b200 as ax
     for wrong in (-1, 300, 1 << 40, -(1 << 40)):
-        x, w, b, labels = make(77, 40, 300, "bfloat16", "in_out", ignored=0.0)
+        x, w, b, labels = make(rows, 40, 300, "bfloat16", "in_out", ignored=0.0)
         labels[5] = wrong
         loss, dx, dw, db = ax.dense_cross_entropy_gradients(x, w, labels, b, scratch_limit=limit)
-        _, rows = ax.dense_cross_entropy(x, w, labels, b, row_losses=True)
-        assert bool(torch.isnan(loss)) and torch.isnan(rows).nonzero()[:, 0].tolist() == [5]
+        _, losses = ax.dense_cross_entropy(x, w, labels, b, row_losses=True)
+        assert bool(torch.isnan(loss)) and torch.isnan(losses).nonzero()[:, 0].tolist() == [5]
         assert torch.isnan(dx).any(1).nonzero()[:, 0].tolist() == [5] and bool(torch.isnan(dw).any())
 
 
 def test_logits_that_are_not_finite(built):
     import torch
     import tf_approximate_b200 as ax
-    for value in (float("nan"), float("inf")):
-        x, w, b, labels = make(150, 64, 300, "bfloat16", "in_out", ignored=0.0)
+    for value, count in ((float("nan"), 150), (float("inf"), 150), (float("nan"), 4000), (float("inf"), 4000)):
+        x, w, b, labels = make(count, 64, 300, "bfloat16", "in_out", ignored=0.0)
         b[100] = value
         loss, rows = ax.dense_cross_entropy(x, w, labels, b, row_losses=True)
         assert not bool(torch.isfinite(loss)) and not bool(torch.isfinite(rows[labels != 100]).any())

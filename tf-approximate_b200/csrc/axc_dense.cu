@@ -1,6 +1,6 @@
 // The exact dense layer: y = act(x kernel + bias + residual), and its gradients.  The products are those of axc_gemm.cu; here are
 // the pass over the output's gradient between them, and the entry points.
-#include "axc_gemm.h"
+#include "axc_rows.h"
 
 namespace axc {
 namespace {
@@ -213,7 +213,7 @@ Matrix kernel_of(const axc_dense_desc &d, const void *k) { return {k, d.units, d
 Matrix dy_of(const axc_dense_desc &d, const void *dy) { return {dy, d.rows, d.units, d.units, 1, d.type}; }
 
 // Where the parts of a call's workspace lie.
-struct Parts {
+struct Room {
     size_t x, kernel, dz, part, scratch, total;
 };
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
@@ -222,10 +222,15 @@ size_t largest(size_t a, size_t b) { return a > b ? a : b; }
 // Addresses that no tensor has stand for unknown ones: sized for a copy of every operand.
 const void *const kUnknown = reinterpret_cast<const void *>(uintptr_t(2));
 
-Parts parts_of(const axc_dense_desc &d, bool backward, const void *x, const void *kernel, const DeviceInfo &di)
+Room room_of(const axc_dense_desc &d, bool backward, const void *x, const void *kernel, const DeviceInfo &di)
 {
     const int planes = d.type == kFloat32 ? 3 : 1;
-    Parts p;
+    Room p;
+    if (!backward && few_rows(x_of(d, x), kernel_of(d, kernel))) {
+        p.x = p.kernel = p.dz = p.part = p.scratch = 256;
+        p.total = p.scratch + up(few_rows_scratch(x_of(d, x), kernel_of(d, kernel), di));
+        return p;
+    }
     p.x = 256;
     p.kernel = p.x + up(operand_bytes(x_of(d, x)));
     p.dz = p.kernel + up(operand_bytes(kernel_of(d, kernel)));
@@ -257,19 +262,13 @@ int leave(int rc, int device, int prev)
 int forward(const axc_dense_desc &d, const void *x, const void *kernel, const void *bias, const void *residual, void *y, void *pre, char *ws,
             const DeviceInfo &di, Queue &q)
 {
-    const Parts parts = parts_of(d, false, x, kernel, di);
+    const Room parts = room_of(d, false, x, kernel, di);
     Gemm g = {};
     g.m = d.rows;
     g.n = d.units;
     g.k = d.inputs;
     g.planes = d.type == kFloat32 ? 3 : 1;
     g.bf16 = d.type != kFloat16;
-    int rc = AXC_OK;
-    if (d.inputs > 0) {
-        rc = make_operand(x_of(d, x), ws + parts.x, &g.a, di, q);
-        if (rc == AXC_OK) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &g.b, di, q);
-        if (rc) return rc;
-    }
     g.fin.alpha = 1.0f;
     g.fin.bias = bias;
     g.fin.bias_type = d.bias_type;
@@ -281,13 +280,19 @@ int forward(const axc_dense_desc &d, const void *x, const void *kernel, const vo
     g.fin.out_type = d.type;
     g.fin.out_line = d.units;
     g.fin.pre = pre;
+    if (few_rows(x_of(d, x), kernel_of(d, kernel)))
+        return few_rows_product(x_of(d, x), kernel_of(d, kernel), g.fin, ws + parts.scratch, reinterpret_cast<unsigned *>(ws), di, q);
+    if (d.inputs > 0) {
+        const int rc = make_operands(x_of(d, x), ws + parts.x, &g.a, kernel_of(d, kernel), ws + parts.kernel, &g.b, di, q);
+        if (rc) return rc;
+    }
     return gemm(g, ws + parts.scratch, reinterpret_cast<unsigned *>(ws), true, di, q);
 }
 
 int backward(const axc_dense_desc &d, const void *dy, const void *x, const void *kernel, const void *kept, void *dx, void *dkernel, void *dbias,
              void *dresidual, char *ws, const DeviceInfo &di, Queue &q)
 {
-    const Parts parts = parts_of(d, true, x, kernel, di);
+    const Room parts = room_of(d, true, x, kernel, di);
     const int planes = d.type == kFloat32 ? 3 : 1;
     const long long line = (d.units + 7) / 8 * 8;
     unsigned *status = reinterpret_cast<unsigned *>(ws);
@@ -321,10 +326,11 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
     if (s.same || s.planes || s.sums) rc = slope(s, ws + parts.part, di, q);
     if (rc) return rc;
     bool first = true;
-    Operand operand = {};
+    Operand ox = {}, ok = {};
+    const Matrix none = {};
+    rc = make_operands(dkernel ? x_of(d, x) : none, ws + parts.x, &ox, dx ? kernel_of(d, kernel) : none, ws + parts.kernel, &ok, di, q);
+    if (rc) return rc;
     if (dx) {
-        if (d.units > 0) rc = make_operand(kernel_of(d, kernel), ws + parts.kernel, &operand, di, q);
-        if (rc) return rc;
         Gemm g = {};
         g.m = d.rows;
         g.n = d.inputs;
@@ -332,7 +338,7 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
         g.planes = planes;
         g.bf16 = d.type != kFloat16;
         g.a = dz;
-        g.b = transposed(operand);
+        g.b = transposed(ok);
         g.fin.alpha = 1.0f;
         g.fin.out = dx;
         g.fin.out_type = d.type;
@@ -342,8 +348,6 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
         first = false;
     }
     if (dkernel) {
-        if (d.rows > 0) rc = make_operand(x_of(d, x), ws + parts.x, &operand, di, q);
-        if (rc) return rc;
         Gemm g = {};
         g.k = d.rows;
         g.planes = planes;
@@ -355,11 +359,11 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
             g.m = d.units;
             g.n = d.inputs;
             g.a = transposed(dz);
-            g.b = transposed(operand);
+            g.b = transposed(ox);
         } else {
             g.m = d.inputs;
             g.n = d.units;
-            g.a = transposed(operand);
+            g.a = transposed(ox);
             g.b = transposed(dz);
         }
         g.fin.out_line = g.n;
@@ -384,8 +388,8 @@ extern "C" int axc_dense_workspace_bytes(const axc_dense_desc *desc, const void 
     if (rc) return rc;
     if (!x) x = kUnknown;
     if (!kernel) kernel = kUnknown;
-    if (forward) *forward = parts_of(*desc, false, x, kernel, di).total;
-    if (backward) *backward = parts_of(*desc, true, x, kernel, di).total;
+    if (forward) *forward = room_of(*desc, false, x, kernel, di).total;
+    if (backward) *backward = room_of(*desc, true, x, kernel, di).total;
     return AXC_OK;
 }
 
@@ -401,7 +405,7 @@ extern "C" int axc_dense_forward(const axc_dense_desc *desc, const void *x, cons
     DeviceInfo di;
     rc = device_info(device, &di);
     if (rc) return rc;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < parts_of(d, false, x, kernel, di).total) return AXC_INTERNAL;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < room_of(d, false, x, kernel, di).total) return AXC_INTERNAL;
     int prev = 0;
     rc = enter(device, &di, &prev);
     if (rc) return rc;
@@ -423,7 +427,7 @@ extern "C" int axc_dense_backward(const axc_dense_desc *desc, const void *dy, co
     DeviceInfo di;
     rc = device_info(device, &di);
     if (rc) return rc;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < parts_of(d, true, x, kernel, di).total) return AXC_INTERNAL;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < room_of(d, true, x, kernel, di).total) return AXC_INTERNAL;
     int prev = 0;
     rc = enter(device, &di, &prev);
     if (rc) return rc;

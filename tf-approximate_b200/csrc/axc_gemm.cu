@@ -6,7 +6,7 @@
 // memory, and eight warps take finished sums out while the next tile's are being made in the other half of the tensor memory.
 //   pairs, 256 x 256 tiles    each SM loads 128 rows of a and half of b: 64 bytes of shared memory written and as many read per
 //                             clock, half of what a lone SM needs for 128 x 256
-//   lone CTAs, 128 x N tiles  for products with too few tiles to fill the GPU, and for few rows (then the weights are `a`)
+//   lone CTAs, 128 x N tiles  for products with too few tiles to fill the GPU
 //
 // fp32 operands are split exactly into three bf16 terms, x = x0 + x1 + x2, each 2^-8 of the one before; six of the nine products
 // of terms are summed (x2 y0, x1 y1, x0 y2, x1 y0, x0 y1, x0 y0), the three left out are below 2^-24 of x y.
@@ -45,7 +45,6 @@ struct GemmArgs {
     unsigned a_box_rows, b_box_rows;           // a box has that many rows (k contiguous), or 64 (rows contiguous)
     bool a_rows, b_rows;
     unsigned shape;
-    bool swapped;                              // m runs along the output's lines: out[n][m]
     Finish fin;
     EntropyArgs ent;
     float *part;                               // [split][line][part_line]
@@ -58,16 +57,6 @@ struct Header {                                // in shared memory
     uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2];
     unsigned tmem;
 };
-
-// `exact`: for fp32 results
-__device__ __forceinline__ float activate(float z, int act, bool exact)
-{
-    if (act == kActRelu) return max_keep_nan(z, 0.0f);
-    float bell;
-    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f, bell)));
-    if (act == kActSilu) return z * reciprocal(1.0f + __expf(-z));
-    return z;
-}
 
 // ---- lines of 32 rows between a warp's registers and memory --------------------------------------------------------------
 // A lane has a row of the sums, memory wants neighbouring lanes to have neighbouring values: 16 bytes stored by every lane to its own
@@ -212,25 +201,9 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
     const Finish &f = P.fin;
     if (n0 >= P.n) return;
     const bool exact = f.out_type == kFloat32;
-    const int row = row0 + L.lane;
     float v[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = alpha * __uint_as_float(x[i]);
-    if (P.swapped) {                           // neighbouring lanes have neighbouring values
-        if (row >= P.m) return;
-        const float bias = f.bias ? load_as_float(f.bias, row, f.bias_type) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            if (n0 + i < P.n) {
-                float z = v[i] + bias;
-                if (f.addend) z += load_as_float(f.addend, (long long)(n0 + i) * f.addend_line + row, f.addend_type);
-                const long long at = (long long)(n0 + i) * f.out_line + row;
-                if (f.pre) store_from_float(f.pre, at, f.out_type, z);
-                store_from_float(f.out, at, f.out_type, activate(z, f.activation, exact));
-            }
-        }
-        return;
-    }
     if (f.bias) {
         const ColumnValues<W> bias(f.bias, f.bias_type, n0, P.n, L.lane);
 #pragma unroll
@@ -291,13 +264,6 @@ __device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, un
 {
     if (n0 >= P.n) return;
     float *part = P.part + (long long)split * P.part_stride;
-    if (P.swapped) {
-        if (row0 + L.lane >= P.m) return;
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (n0 + i < P.n) part[(long long)(n0 + i) * P.part_line + row0 + L.lane] = __uint_as_float(x[i]);
-        return;
-    }
     float v[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = __uint_as_float(x[i]);
@@ -617,11 +583,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float *part, long lon
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (c + j < columns) {
-                float z = alpha * v[j];
-                if (f.bias) z += load_as_float(f.bias, c + j, f.bias_type);
-                if (f.addend) z += load_as_float(f.addend, line * f.addend_line + c + j, f.addend_type);
-                if (f.pre) store_from_float(f.pre, line * f.out_line + c + j, f.out_type, z);
-                store_from_float(f.out, line * f.out_line + c + j, f.out_type, activate(z, f.activation, true));
+                finish_value(f, alpha * v[j], line, c + j);
             }
         }
     }
@@ -653,40 +615,38 @@ bool make_map(const Operand &o, long long rows, long long k, int planes, bool bf
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a product is cut up: CTAs per tile, columns of a tile, splits of k; and whether the operands change places, so that the longer
-// of m and n runs over the 128 lanes.
+// How a product is cut up: CTAs per tile, columns of a tile, splits of k.
 struct Plan {
     int cg, bn, splits;
-    bool swapped;
 };
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, bool may_swap, int sms)
+// The cheapest of the tiles and splits by an estimate in clocks.  A stage takes what its matrix instructions take (2 for each column of
+// a tile; 225 where the tile is narrow, which its copies need), a wave of tiles 3000 more until its sums are out, the product another 3000
+// for its first bytes and its last tile; a split one 1500 and its partial sums' way to L2 and back.  Of all tiles and splits measured
+// for 18 products from 1024 x 64 x 10 to 2048 x 2048 x 2048, in bf16 and fp32, the one chosen so was the fastest for 15 and at most 7 %
+// slower for the others.  (Tiles of b's rows by a's, with the rows of the output along the lanes, were never faster by more than 10 %.)
+Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, int sms)
 {
-    Plan best = {1, 128, 1, false};
+    Plan best = {1, 128, 1};
     double least = 1e300;
     const long long steps = ceil_div(k > 0 ? k : 1, kStageK);
-    for (int swapped = 0; swapped < (may_swap ? 2 : 1); ++swapped) {
-        const long long tall = swapped ? n : m, wide = swapped ? m : n;
-        for (int c = 0; c < 6; ++c) {
-            static const int kCg[6] = {2, 1, 1, 1, 1, 1}, kBn[6] = {256, 256, 128, 64, 32, 16};
-            // clocks of a stage: the matrix instructions, or the copies that feed a narrow tile
-            static const double kClocks[6] = {540, 620, 330, 220, 190, 180};
-            const int cg = kCg[c], bn = planes == 3 && cg == 2 ? 128 : kBn[c];
-            if (!may_swap && bn < 64) continue;                 // segments of 64 columns
-            if (planes == 3 && bn == 256) continue;             // its sums do not fit into registers
-            const long long tiles = ceil_div(tall, 128 * cg) * ceil_div(wide, bn);
-            const int workers = sms / cg;
-            for (int splits = 1; splits <= (may_split ? 16 : 1); splits *= 2) {
-                if (splits > 1 && steps / splits < 4) break;
-                const double waves = double(ceil_div(tiles * splits, workers));
-                double clocks = waves * (double(ceil_div(steps, splits)) * (planes == 3 ? (cg == 2 ? 270 : kClocks[c]) * 6 : kClocks[c]) + 600) + 4000;
-                if (splits > 1) clocks += 4500 + double(m) * n * splits * 8 / 3000;
-                if (clocks < least * 0.97) {
-                    least = clocks;
-                    best = {cg, bn, splits, swapped != 0};
-                }
+    for (int c = 0; c < 6; ++c) {
+        static const int kCg[6] = {2, 1, 1, 1, 1, 1}, kBn[6] = {256, 256, 128, 64, 32, 16};
+        const int cg = kCg[c], bn = planes == 3 && cg == 2 ? 128 : kBn[c];
+        if (!may_split && bn < 64) continue;                    // logits: segments of 64 columns
+        if (planes == 3 && bn == 256) continue;                 // its sums do not fit into registers
+        // a lone SM has to bring in twice the bytes of a pair for the same products: 1.1
+        const double columns = cg == 1 ? 2.2 * bn : 2.0 * bn, stage = (planes == 3 ? 6 : 1) * (columns > 225 ? columns : 225);
+        const long long tiles = ceil_div(m, 128 * cg) * ceil_div(n, bn);
+        for (int splits = 1; splits <= (may_split ? 16 : 1); splits *= 2) {
+            if (splits > 1 && steps / splits < 2) break;
+            double clocks = double(ceil_div(tiles * splits, sms / cg)) * (double(ceil_div(steps, splits)) * stage + 3000) + 3000 + 20 * bn;
+            if (splits > 1) clocks += 1500 + double(m) * n * splits * 8 / 2700;
+            if (clocks < least) {
+                least = clocks;
+                best = {cg, bn, splits};
             }
         }
     }
@@ -738,14 +698,13 @@ int launch_plan(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo
 
 int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, GemmArgs *P)
 {
-    const Operand &a = plan.swapped ? g.b : g.a, &b = plan.swapped ? g.a : g.b;
-    const long long tall = plan.swapped ? g.n : g.m, wide = plan.swapped ? g.m : g.n;
-    if (tall > 0x7fffff00ll || wide > 0x7fffff00ll || g.k > 0x7fffff00ll) return AXC_INVALID_ARGUMENT;
+    const Operand &a = g.a, &b = g.b;
+    if (g.m > 0x7fffff00ll || g.n > 0x7fffff00ll || g.k > 0x7fffff00ll) return AXC_INVALID_ARGUMENT;
     const unsigned b_rows_per_cta = unsigned(plan.bn / plan.cg);
-    P->m = int(tall);
-    P->n = int(wide);
-    P->tiles_m = int(ceil_div(tall, 128 * plan.cg));
-    P->tiles_n = int(ceil_div(wide, plan.bn));
+    P->m = int(g.m);
+    P->n = int(g.n);
+    P->tiles_m = int(ceil_div(g.m, 128 * plan.cg));
+    P->tiles_n = int(ceil_div(g.n, plan.bn));
     P->splits = plan.splits;
     P->k_steps = int(ceil_div(g.k, kStageK));
     P->planes = g.planes;
@@ -754,28 +713,47 @@ int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, Gem
     P->a_bytes = 128 * 128;
     P->b_bytes = (b.rows_contiguous && b_rows_per_cta < 64 ? 64u : b_rows_per_cta) * 128u;
     P->shape = mma::instruction_shape(128 * plan.cg, plan.bn, g.bf16, a.rows_contiguous, b.rows_contiguous);
-    P->swapped = plan.swapped;
     P->fin = g.fin;
     P->status = status;
     P->first = first;
-    if (!make_map(a, tall, g.k, g.planes, g.bf16, 128, &P->map_a) || !make_map(b, wide, g.k, g.planes, g.bf16, b_rows_per_cta, &P->map_b))
+    if (!make_map(a, g.m, g.k, g.planes, g.bf16, 128, &P->map_a) || !make_map(b, g.n, g.k, g.planes, g.bf16, b_rows_per_cta, &P->map_b))
         return AXC_INTERNAL;
     return AXC_OK;
 }
 
-int launch_finish(const float *part, long long stride, long long line, int splits, const Gemm &g, const DeviceInfo &di, Queue &q)
-{
-    const long long work = ceil_div(g.m * ceil_div(g.n, 4), 256), most = (long long)di.sm_count * 8;
-    return launch(q, finish_kernel, dim3(unsigned(work < most ? work : most)), 256, 0, 1, part, stride, line, splits, int(g.m), int(g.n), g.fin);
-}
-
 }  // namespace
+
+int finish_parts(const Parts &parts, long long lines, long long columns, const Finish &f, const DeviceInfo &di, Queue &q)
+{
+    const long long work = ceil_div(lines * ceil_div(columns, 4), 256), most = (long long)di.sm_count * 8;
+    return launch(q, finish_kernel, dim3(unsigned(work < most ? work : most)), 256, 0, 1, parts.data, parts.stride, parts.line, parts.count, int(lines),
+                  int(columns), f);
+}
 
 size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di)
 {
     if (m == 0 || n == 0 || k == 0) return 0;
-    const Plan plan = choose_plan(m, n, k, planes, true, true, di.sm_count);
+    const Plan plan = choose_plan(m, n, k, planes, true, di.sm_count);
     return plan.splits > 1 ? size_t(plan.splits) * size_t(m) * size_t((n + 3) / 4 * 4) * 4 : 0;
+}
+
+size_t gemm_parts_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di)
+{
+    const Plan plan = choose_plan(m, n, k, planes, true, di.sm_count);
+    return size_t(plan.splits) * size_t(m) * size_t((n + 3) / 4 * 4) * 4;
+}
+
+int gemm_parts(const Gemm &g, void *scratch, Parts *parts, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
+{
+    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, di.sm_count);
+    GemmArgs P = {};
+    const int rc = fill_args(g, plan, status, first, &P);
+    if (rc) return rc;
+    P.part = static_cast<float *>(scratch);
+    P.part_line = (g.n + 3) / 4 * 4;
+    P.part_stride = P.part_line * g.m;
+    *parts = {P.part, P.part_line, P.part_stride, plan.splits};
+    return launch_plan<kPartial>(P, plan, (long long)P.tiles_m * P.tiles_n * plan.splits, di, q);
 }
 
 int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
@@ -783,27 +761,26 @@ int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const Devic
     if (g.m == 0 || g.n == 0) return AXC_OK;
     if (g.k == 0) {                                             // sums of nothing
         if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
-        return launch_finish(nullptr, 0, 0, 0, g, di, q);
+        return finish_parts(Parts{}, g.m, g.n, g.fin, di, q);
     }
-    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, true, di.sm_count);
+    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, di.sm_count);
+    if (plan.splits > 1) {
+        Parts parts;
+        const int rc = gemm_parts(g, scratch, &parts, status, first, di, q);
+        return rc ? rc : finish_parts(parts, g.m, g.n, g.fin, di, q);
+    }
     GemmArgs P = {};
-    int rc = fill_args(g, plan, status, first, &P);
+    const int rc = fill_args(g, plan, status, first, &P);
     if (rc) return rc;
-    const long long units = (long long)P.tiles_m * P.tiles_n * plan.splits;
+    const long long units = (long long)P.tiles_m * P.tiles_n;
     if (units > 0x7fffffffll) return AXC_INVALID_ARGUMENT;
-    if (plan.splits == 1) return launch_plan<kStore>(P, plan, units, di, q);
-    P.part = static_cast<float *>(scratch);
-    P.part_line = (g.n + 3) / 4 * 4;
-    P.part_stride = P.part_line * g.m;
-    rc = launch_plan<kPartial>(P, plan, units, di, q);
-    if (rc) return rc;
-    return launch_finish(P.part, P.part_stride, P.part_line, plan.splits, g, di, q);
+    return launch_plan<kStore>(P, plan, units, di, q);
 }
 
 int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
 {
     if (g.m == 0 || g.n == 0) return AXC_OK;
-    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, false, false, di.sm_count);
+    const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, false, di.sm_count);
     GemmArgs P = {};
     int rc = fill_args(g, plan, status, first, &P);
     if (rc) return rc;
@@ -816,28 +793,50 @@ int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *s
 // ---- operands -----------------------------------------------------------------------------------------------------------
 namespace {
 
-// Copies a matrix into lines of a multiple of 8 values, 16-bit types as they are, fp32 as three bf16 planes: the value rounded to
-// bf16, the rest rounded again, and what is left then, which bf16 holds exactly.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256) lay_out_kernel(const void *src, int type, long long outer, long long inner, long long outer_stride,
-                                                      long long inner_stride, uint16_t *dst, long long line, long long plane)
+// What lay_out_kernel copies: `outer` lines of `inner` values
+struct Layout {
+    const void *src;
+    uint16_t *dst;
+    long long outer, inner, outer_stride, inner_stride, line, plane;
+    bool split;
+};
+
+// Copies one matrix or two into lines of a multiple of 8 values, 16-bit types as they are, fp32 as three bf16 planes: the value rounded
+// to bf16, the rest rounded again, and what is left then, which bf16 holds exactly.  The first `blocks` blocks have the first matrix.
+__global__ void __launch_bounds__(256) lay_out_kernel(const Layout one, const Layout two, int blocks)
 {
     after_previous();
-    const long long groups = line / 8, total = outer * groups;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const bool second = int(blockIdx.x) >= blocks;
+    const Layout &m = second ? two : one;
+    const long long groups = m.line / 8, total = m.outer * groups, stride = (long long)(second ? gridDim.x - blocks : blocks) * 256;
+    for (long long i = (long long)(blockIdx.x - (second ? blocks : 0)) * 256 + threadIdx.x; i < total; i += stride) {
         const long long o = i / groups, c = (i - o * groups) * 8;
-        union { uint16_t h[8]; uint4 w; } out[SPLIT ? 3 : 1];
+        uint16_t *to = m.dst + o * m.line + c;
+        const long long from = o * m.outer_stride + c * m.inner_stride;
+        union { uint16_t h[8]; uint4 w; } out[3];
+        if (m.split) {
+            const float *src = static_cast<const float *>(m.src) + from;
+            float x[8];
+            if (m.inner_stride == 1 && c + 8 <= m.inner && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+                const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long long at = o * outer_stride + (c + j) * inner_stride;
-            if (SPLIT) {
-                float x = c + j < inner ? static_cast<const float *>(src)[at] : 0.0f;
+                for (int j = 0; j < 8; ++j) x[j] = c + j < m.inner ? src[j * m.inner_stride] : 0.0f;
+            }
 #pragma unroll
-                for (int p = 0; p < 3; ++p) out[p].h[j] = split_term(x, x);
-            } else out[0].h[j] = c + j < inner ? static_cast<const uint16_t *>(src)[at] : uint16_t(0);
+            for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) out[p].h[j] = split_term(x[j], x[j]);
+                *reinterpret_cast<uint4 *>(to + p * m.plane) = out[p].w;
+            }
+        } else {
+            const uint16_t *src = static_cast<const uint16_t *>(m.src) + from;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[0].h[j] = c + j < m.inner ? src[j * m.inner_stride] : uint16_t(0);
+            *reinterpret_cast<uint4 *>(to) = out[0].w;
         }
-#pragma unroll
-        for (int p = 0; p < (SPLIT ? 3 : 1); ++p) *reinterpret_cast<uint4 *>(dst + p * plane + o * line + c) = out[p].w;
     }
 }
 
@@ -862,21 +861,43 @@ size_t operand_bytes(const Matrix &x)
     return (outer * ((inner + 7) / 8 * 8) * 2 * (x.type == kFloat32 ? 3 : 1) + 255) / 256 * 256;
 }
 
-int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, Queue &q)
+namespace {
+
+// The operand, and in `copy` how it gets there (outer = 0: it is read in place)
+Operand plan_operand(const Matrix &x, void *scratch, Layout *copy)
 {
+    *copy = {};
+    if (x.rows == 0 || x.columns == 0) return {nullptr, 8, 0, false};
     if (readable_in_place(x)) {
         const bool by_columns = x.column_stride == 1 && x.row_stride % 8 == 0 && x.row_stride >= x.columns;
-        *out = {x.data, by_columns ? x.row_stride : x.column_stride, 0, !by_columns};
-        return AXC_OK;
+        return {x.data, by_columns ? x.row_stride : x.column_stride, 0, !by_columns};
     }
     const bool in = columns_inner(x);
-    const long long inner = in ? x.columns : x.rows, outer = in ? x.rows : x.columns, line = (inner + 7) / 8 * 8;
-    *out = {scratch, line, outer * line, !in};
-    const long long work = ceil_div(outer * (line / 8), 256);
-    const unsigned grid = unsigned(work < di.sm_count * 16 ? work : di.sm_count * 16);
-    const long long outer_stride = in ? x.row_stride : x.column_stride, inner_stride = in ? x.column_stride : x.row_stride;
-    return launch(q, x.type == kFloat32 ? lay_out_kernel<true> : lay_out_kernel<false>, dim3(grid), 256, 0, 1, x.data, x.type, outer, inner, outer_stride,
-                  inner_stride, static_cast<uint16_t *>(scratch), line, outer * line);
+    copy->src = x.data;
+    copy->dst = static_cast<uint16_t *>(scratch);
+    copy->inner = in ? x.columns : x.rows;
+    copy->outer = in ? x.rows : x.columns;
+    copy->outer_stride = in ? x.row_stride : x.column_stride;
+    copy->inner_stride = in ? x.column_stride : x.row_stride;
+    copy->line = (copy->inner + 7) / 8 * 8;
+    copy->plane = copy->outer * copy->line;
+    copy->split = x.type == kFloat32;
+    return {scratch, copy->line, copy->plane, !in};
+}
+
+}  // namespace
+
+int make_operands(const Matrix &x, void *x_scratch, Operand *ox, const Matrix &y, void *y_scratch, Operand *oy, const DeviceInfo &di, Queue &q)
+{
+    Layout one, two;
+    *ox = plan_operand(x, x_scratch, &one);
+    *oy = plan_operand(y, y_scratch, &two);
+    const long long most = (long long)di.sm_count * 16;
+    long long a = ceil_div(one.outer * (one.line / 8), 256), b = ceil_div(two.outer * (two.line / 8), 256);
+    if (a + b == 0) return AXC_OK;
+    if (a > most) a = most;
+    if (b > most) b = most;
+    return launch(q, lay_out_kernel, dim3(unsigned(a + b)), 256, 0, 1, one, two, int(a));
 }
 
 }  // namespace axc

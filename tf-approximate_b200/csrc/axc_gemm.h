@@ -137,6 +137,26 @@ struct Finish {
     void *pre;                  // NULL, or where the activation's argument goes (out_type, out_line)
 };
 
+// `exact`: for fp32 results
+__device__ __forceinline__ float activate(float z, int act, bool exact)
+{
+    if (act == kActRelu) return max_keep_nan(z, 0.0f);
+    float bell;
+    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f, bell)));
+    if (act == kActSilu) return z * reciprocal(1.0f + __expf(-z));
+    return z;
+}
+
+// One value of an output: line, column
+__device__ __forceinline__ void finish_value(const Finish &f, float z, long long line, long long column)
+{
+    if (f.bias) z += load_as_float(f.bias, column, f.bias_type);
+    if (f.addend) z += load_as_float(f.addend, line * f.addend_line + column, f.addend_type);
+    const long long at = line * f.out_line + column;
+    if (f.pre) store_from_float(f.pre, at, f.out_type, z);
+    store_from_float(f.out, at, f.out_type, activate(z, f.activation, f.out_type == kFloat32));
+}
+
 // What the cross entropy makes of a tile of logits; see axc_entropy.cu.
 struct EntropyArgs {
     const void *bias;
@@ -165,6 +185,15 @@ struct Gemm {
 size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di);
 // `first`: of the products of a call; it clears the status word.
 int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, Queue &q);
+// The sums alone, as `count` parts that are to be added in order: part i of out[r, c] at data[i * stride + r * line + c].
+struct Parts {
+    const float *data;
+    long long line, stride;
+    int count;
+};
+int finish_parts(const Parts &parts, long long lines, long long columns, const Finish &f, const DeviceInfo &di, Queue &q);
+size_t gemm_parts_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di);
+int gemm_parts(const Gemm &g, void *scratch, Parts *parts, unsigned *status, bool first, const DeviceInfo &di, Queue &q);
 // Tiles of logits, never split; `gradient`: the second pass of the piecewise form.
 int gemm_entropy(const Gemm &g, const EntropyArgs &e, bool gradient, unsigned *status, bool first, const DeviceInfo &di, Queue &q);
 
@@ -200,8 +229,8 @@ struct Matrix {
 // Whether the tensor cores can read it where it is (16-bit, one unit stride, lines of a multiple of 16 bytes, aligned).
 bool readable_in_place(const Matrix &x);
 size_t operand_bytes(const Matrix &x);          // scratch that operand() fills, 0 where it reads in place
-// The matrix as an operand whose rows are x's rows (or, transposed, x's columns); copies and splits into `scratch` as needed.
-int make_operand(const Matrix &x, void *scratch, Operand *out, const DeviceInfo &di, Queue &q);
+// Two matrices as operands whose rows are theirs; copies and splits into the scratch as needed, in one launch.
+int make_operands(const Matrix &x, void *x_scratch, Operand *ox, const Matrix &y, void *y_scratch, Operand *oy, const DeviceInfo &di, Queue &q);
 inline Operand transposed(Operand o)
 {
     o.rows_contiguous = !o.rows_contiguous;
