@@ -623,10 +623,11 @@ struct Plan {
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // The cheapest of the tiles and splits by an estimate in clocks.  A stage takes what its matrix instructions take (2 for each column of
-// a tile; 225 where the tile is narrow, which its copies need), a wave of tiles 3000 more until its sums are out, the product another 3000
-// for its first bytes and its last tile; a split one 1500 and its partial sums' way to L2 and back.  Of all tiles and splits measured
-// for 18 products from 1024 x 64 x 10 to 2048 x 2048 x 2048, in bf16 and fp32, the one chosen so was the fastest for 15 and at most 7 %
-// slower for the others.  (Tiles of b's rows by a's, with the rows of the output along the lanes, were never faster by more than 10 %.)
+// a tile, 390 at least) or what its bytes take (114 a clock and SM when all SMs have tiles, in proportion when few have), whichever is
+// more; a wave of tiles 3400 more until its sums are out, the product another 4500 for its first bytes and its last tile; a split one 7600
+// for the second kernel and its partial sums' way to L2 and back.  Fitted to all tiles and splits measured for 34 products, in bf16 from
+// 4 x 2048 x 1000 to 8192 x 8192 x 2048 and 2047 x 50001 x 1024, in fp32 from 64 x 300 x 64 to 2000 x 2000 x 2000: the one chosen so was
+// the fastest or within 2 % of it for 31, 3 to 12 % slower for the others (3000 x 3000 x 700: 27.6 us instead of 24.6).
 Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, int sms)
 {
     Plan best = {1, 128, 1};
@@ -637,13 +638,14 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
         const int cg = kCg[c], bn = planes == 3 && cg == 2 ? 128 : kBn[c];
         if (!may_split && bn < 64) continue;                    // logits: segments of 64 columns
         if (planes == 3 && bn == 256) continue;                 // its sums do not fit into registers
-        // a lone SM has to bring in twice the bytes of a pair for the same products: 1.1
-        const double columns = cg == 1 ? 2.2 * bn : 2.0 * bn, stage = (planes == 3 ? 6 : 1) * (columns > 225 ? columns : 225);
-        const long long tiles = ceil_div(m, 128 * cg) * ceil_div(n, bn);
+        const double products = (planes == 3 ? 6 : 1) * (bn > 195 ? 2.0 * bn : 390.0), bytes = planes * (double(m < 128 ? m : 128) + bn / cg) * 128;
+        const long long tiles = ceil_div(m, 128 * cg) * ceil_div(n, bn), workers = sms / cg;
         for (int splits = 1; splits <= (may_split ? 16 : 1); splits *= 2) {
             if (splits > 1 && steps / splits < 2) break;
-            double clocks = double(ceil_div(tiles * splits, sms / cg)) * (double(ceil_div(steps, splits)) * stage + 3000) + 3000 + 20 * bn;
-            if (splits > 1) clocks += 1500 + double(m) * n * splits * 8 / 2700;
+            const long long units = tiles * splits;
+            const double copies = bytes / 114 * double(units < workers ? units : workers) / double(workers), stage = products > copies ? products : copies;
+            double clocks = double(ceil_div(units, workers)) * (double(ceil_div(steps, splits)) * stage + 3400) + 4500 + 8 * bn;
+            if (splits > 1) clocks += 7600 + double(m) * n * splits * 8 / 7400;
             if (clocks < least) {
                 least = clocks;
                 best = {cg, bn, splits};
