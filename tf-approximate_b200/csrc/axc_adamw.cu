@@ -82,6 +82,12 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return d;
 }
+__device__ __forceinline__ Two add2(Two a, Two b)
+{
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
 __device__ __forceinline__ Two mul2(Two a, Two b)
 {
     Two d;
@@ -147,6 +153,12 @@ __device__ __forceinline__ void store_codes(uint8_t *at, const float (&x)[V])
     for (int i = 0; i < V / 2; ++i) u.c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
     __stcs(reinterpret_cast<typename Word<V>::type *>(at), u.w);
 }
+// At most 2 kNear where a quotient is within kNear units in the last place of the middle between two codes: e4m3 has 3 bits of fraction,
+// the middle has the next one and no more.  (Below the normal codes, 3.5e-5 of the block's largest value, the middles are others: there a
+// quotient that close to one, 1 in a million, may get the other code.)
+constexpr unsigned kNear = 8;
+__device__ __forceinline__ unsigned edge(float q) { return (__float_as_uint(q) + (kNear - 0x80000u)) & 0xfffffu; }
+
 __device__ __forceinline__ float warp_max(float x)
 {
 #pragma unroll
@@ -164,6 +176,7 @@ struct Part {
     Packed<State, V> m[N], v[N];
     float m_scale = 0.0f, v_scale = 0.0f, decay, step_size;
     T *param;
+    const T *grad;
     long long left;                            // values of the tensor from the block's first on; 0: a tensor without a gradient
     bool vec;
 
@@ -174,7 +187,7 @@ struct Part {
         const long long first = (long long)(b - e.first) * kBlock;
         left = e.count - first;
         param = static_cast<T *>(e.param) + first;
-        const T *grad = static_cast<const T *>(e.grad) + first;
+        grad = static_cast<const T *>(e.grad) + first;
         decay = e.decay;
         step_size = e.step_size;
         vec = left >= kBlock && ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & (V * sizeof(T) - 1)) == 0;
@@ -194,30 +207,38 @@ struct Part {
         }
     }
 
+    // The moments of values i and i + 1, each operation rounded by itself
     template <int CAP>
-    __device__ __forceinline__ void step(const AdamwTable<CAP> &tab, unsigned b, int lane) const
+    __device__ __forceinline__ void moments(const AdamwTable<CAP> &tab, int n, int i, Two &m1, Two &v1) const
+    {
+        const Two minus(-1.0f), gi = mul2(Two(to_float(g[n].t[i]), to_float(g[n].t[i + 1])), Two(tab.grad_scale));
+        Two m0, v0;
+        if constexpr (BITS == 32) {
+            m0 = Two(m[n].t[i], m[n].t[i + 1]);
+            v0 = Two(v[n].t[i], v[n].t[i + 1]);
+        } else {
+            m0 = decode<V>(m[n], i / 2, Two(m_scale));
+            v0 = decode<V>(v[n], i / 2, Two(v_scale));
+            v0 = mul2(v0, v0);
+        }
+        m1 = add2(m0, mul2(Two(tab.c1), fma2(m0, minus, gi)));
+        v1 = add2(v0, mul2(Two(tab.c2), fma2(v0, minus, mul2(gi, gi))));
+    }
+
+    template <int CAP>
+    __device__ __forceinline__ void step(const AdamwTable<CAP> &tab, unsigned b, int lane)
     {
         if (left <= 0) return;
         State *ms = static_cast<State *>(tab.m) + size_t(b) * kBlock, *vs = static_cast<State *>(tab.v) + size_t(b) * kBlock;
-        float first[N][V], second[N][V], m_top = 0.0f, r_top = 0.0f;
-        const Two minus(-1.0f), c1(tab.c1), c2(tab.c2), grad_scale(tab.grad_scale), inv_root(tab.inv_root), eps(tab.eps), keep(decay), move(-step_size);
-        const Two ms2(m_scale), vs2(v_scale);
+        float first[N][V], second[N][V], m_top = 0.0f, v_top = 0.0f;
+        const Two inv_root(tab.inv_root), eps(tab.eps), keep(decay), move(-step_size);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             float x[V];
 #pragma unroll
             for (int i = 0; i < V; i += 2) {
-                const Two gi = mul2(Two(to_float(g[n].t[i]), to_float(g[n].t[i + 1])), grad_scale);
-                Two m0, v0;
-                if constexpr (BITS == 32) {
-                    m0 = Two(m[n].t[i], m[n].t[i + 1]);
-                    v0 = Two(v[n].t[i], v[n].t[i + 1]);
-                } else {
-                    m0 = decode<V>(m[n], i / 2, ms2);
-                    v0 = decode<V>(v[n], i / 2, vs2);
-                    v0 = mul2(v0, v0);
-                }
-                const Two m1 = fma2(c1, fma2(m0, minus, gi), m0), v1 = fma2(c2, fma2(gi, gi, mul2(v0, minus)), v0);
+                Two m1, v1;
+                moments(tab, n, i, m1, v1);
                 // v rsqrt(v): 0 for 0, and not above the root where v has no normal reciprocal root
                 const float2 vf = v1.both();
                 const Two root = mul2(v1, Two(reciprocal_root(fmaxf(vf.x, 1.17549435e-38f)), reciprocal_root(fmaxf(vf.y, 1.17549435e-38f))));
@@ -232,7 +253,7 @@ struct Part {
                 second[n][i + 1] = BITS == 32 ? vf.y : rf.y;
                 if (BITS == 8) {
                     m_top = fmaxf(m_top, fmaxf(fabsf(mf.x), fabsf(mf.y)));
-                    r_top = fmaxf(r_top, fmaxf(rf.x, rf.y));
+                    v_top = fmaxf(v_top, fmaxf(vf.x, vf.y));
                 }
             }
             const int i = (n * 32 + lane) * V;
@@ -246,20 +267,49 @@ struct Part {
             }
         } else {
             // a scale below the smallest normal number has no reciprocal: the block's moments are then zeros
-            float m_new = warp_max(m_top) * (1.0f / 448.0f), r_new = warp_max(r_top) * (1.0f / 448.0f);
+            float m_new = warp_max(m_top) * (1.0f / 448.0f), r_new = __fsqrt_rn(warp_max(v_top)) * (1.0f / 448.0f);
             if (m_new < 1.17549435e-38f) m_new = 0.0f;
             if (r_new < 1.17549435e-38f) r_new = 0.0f;
             const float mi = m_new > 0.0f ? __fdividef(1.0f, m_new) : 0.0f, ri = r_new > 0.0f ? __fdividef(1.0f, r_new) : 0.0f;
+            unsigned near_edge = 0xffffffffu;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
                     const float2 f = mul2(Two(first[n][i], first[n][i + 1]), Two(mi)).both(), r = mul2(Two(second[n][i], second[n][i + 1]), Two(ri)).both();
+                    near_edge = min(min(near_edge, edge(f.x)), min(edge(f.y), min(edge(r.x), edge(r.y))));
                     first[n][i] = f.x;
                     first[n][i + 1] = f.y;
                     second[n][i] = r.x > 0.0f ? fmaxf(r.x, 0.001953125f) : r.x;
                     second[n][i + 1] = r.y > 0.0f ? fmaxf(r.y, 0.001953125f) : r.y;
                 }
+            // The quotients are a few units in the last place off.  Where that could take one over the edge between two codes, the lane's are
+            // computed again, rounded at every step: the codes are those of the formula to the bit, as its definition has them.
+            // (What that takes is read again rather than kept in registers.)
+            if (near_edge <= 2 * kNear) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int at = (n * 32 + lane) * V;
+                    load_values<T, V>(grad + at, vec, left - at, g[n]);
+                    load_values<State, V>(ms + at, true, 0, m[n]);
+                    load_values<State, V>(vs + at, true, 0, v[n]);
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) {
+                        Two m1, v1;
+                        moments(tab, n, i, m1, v1);
+                        const float2 mf = m1.both(), vf = v1.both();
+                        first[n][i] = m_new > 0.0f ? __fdiv_rn(mf.x, m_new) : 0.0f;
+                        first[n][i + 1] = m_new > 0.0f ? __fdiv_rn(mf.y, m_new) : 0.0f;
+                        const float rx = r_new > 0.0f ? __fdiv_rn(__fsqrt_rn(vf.x), r_new) : 0.0f, ry = r_new > 0.0f ? __fdiv_rn(__fsqrt_rn(vf.y), r_new) : 0.0f;
+                        second[n][i] = rx > 0.0f ? fmaxf(rx, 0.001953125f) : rx;
+                        second[n][i + 1] = ry > 0.0f ? fmaxf(ry, 0.001953125f) : ry;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
                 store_codes<V>(ms + (n * 32 + lane) * V, first[n]);
                 store_codes<V>(vs + (n * 32 + lane) * V, second[n]);
             }
@@ -272,10 +322,10 @@ struct Part {
 };
 
 // A warp takes one block of 256 values and a CTA eight.  Warps that walk over several blocks, with or without the next one's loads on
-// their way, took up to twice as long (bf16 with 8-bit moments, 2^27 values: 271 us so, 339 to 541 us otherwise): new CTAs keep more
-// loads in flight.  The registers are held to what lets 40 (fp32) or 48 (16-bit) warps be there with 8-bit moments.
+// their way, took up to twice as long (bf16 with 8-bit moments, 2^27 values: 276 us so, 339 to 541 us otherwise): new CTAs keep more
+// loads in flight.  The registers are held to what lets 40 warps be there with 8-bit moments.
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kWarps * 32, BITS == 32 ? 1 : sizeof(T) == 4 ? 5 : 6) adamw_kernel(const __grid_constant__ AdamwTable<CAP> tab)
+__global__ void __launch_bounds__(kWarps * 32, BITS == 32 ? 1 : 5) adamw_kernel(const __grid_constant__ AdamwTable<CAP> tab)
 {
     const unsigned b = tab.base + blockIdx.x * kWarps + (threadIdx.x >> 5), end = tab.base + tab.blocks;
     if (b >= end) return;

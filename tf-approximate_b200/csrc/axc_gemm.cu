@@ -13,7 +13,11 @@
 //
 // Sums are fp32.  The tensor cores cut a sum off at 24 bits at every step of 16 k (measured: 2e-8 of it on average, always towards
 // zero), which 16-bit results do not show.  For fp32 the sums of every 64 k, the small products first, are taken out and added in
-// registers, with rounding: an error of 1e-7 instead of 2e-5 at k = 16384; the eight warps do that while the next 64 k run.
+// registers, with rounding: an error of 1e-7 instead of 2e-5 at k = 16384; the eight warps do that while the next 64 k run.  So are the
+// sums of 256 k (512 where k is over 1536) for 16-bit operands whose result a ReLU cuts: the sign of a sum near zero decides about a whole
+// gradient there.  Of 4.25 million sums of 1030 products about one had another sign than the exact sum; with runs of 512 one in four such
+// products has one, with 256 one in sixteen.  That costs 10 % (1531 x 1032 x 2776: 18.9 to 20.8 us; 4096 x 4096 x 4096 in runs of 512: 97 to
+// 107, of 256: 129).
 //
 // Products whose tiles are too few have k split over CTAs; the partial sums are added in a fixed order by a second
 // kernel, which also applies what follows the product.
@@ -28,7 +32,7 @@ namespace axc {
 namespace {
 
 constexpr int kStageK = 64;                    // k of a stage: 128 bytes, a swizzled line
-constexpr int kThreads = 384;                  // warps: 0 loads, 1 multiplies, 2 holds the tensor memory, 4 to 11 take the sums out
+constexpr int kThreads = 320;                  // warps: 0 loads and holds the tensor memory, 1 multiplies, 2 to 9 take the sums out
 constexpr unsigned kHeader = 1024;             // barriers and such, before the stages
 constexpr unsigned kSmem = 227 * 1024;
 constexpr int kMaxStages = 12;
@@ -51,6 +55,7 @@ struct GemmArgs {
     long long part_line, part_stride;
     unsigned *status;
     bool first;                                // of a call: clears the status
+    int run;                                   // CLOSE, 16-bit operands: stages between two takings out
 };
 
 struct Header {                                // in shared memory
@@ -355,13 +360,15 @@ __device__ __forceinline__ void place_of(const GemmArgs &P, int tile, int &tm, i
     tn = (tile - group * per) / rows;
 }
 
-// CG: CTAs per tile.  BN: columns of a tile.  MODE: what becomes of the sums.  PLANES: terms of an operand.
-template <int CG, int BN, int MODE, int PLANES>
+// CG: CTAs per tile.  BN: columns of a tile.  MODE: what becomes of the sums.  PLANES: terms of an operand.  CLOSE: sums are taken out and
+// added in registers on the way.
+template <int CG, int BN, int MODE, int PLANES, bool CLOSE>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs P)
 {
     constexpr int TM = 128 * CG;
     constexpr unsigned kColumns = BN < 32 ? 32 : BN;           // tensor memory of one tile's sums
     constexpr int kBuffers = 2, kUnits = PLANES == 3 ? 2 : 8;
+    const int run = PLANES == 3 ? 1 : P.run;                   // stages between two takings out, a power of two
     extern __shared__ char raw[];
     const unsigned base = (mma::smem_address(raw) + 1023u) & ~1023u;
     Header *head = reinterpret_cast<Header *>(raw + (base - mma::smem_address(raw)));
@@ -387,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         mma::prefetch_map(&P.map_a);
         mma::prefetch_map(&P.map_b);
     }
-    if (warp == 2) mma::tmem_alloc<CG>(mma::smem_address(&head->tmem), kColumns * kBuffers);
+    if (warp == 0) mma::tmem_alloc<CG>(mma::smem_address(&head->tmem), kColumns * kBuffers);
     mma::fence_before();
     if (CG == 2) mma::cluster_sync();
     else __syncthreads();
@@ -444,7 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
             unsigned d = 0;
             for (int k = k0; k < k1; ++k) {
-                if (PLANES == 3 || k == k0) {
+                const bool opens = CLOSE ? ((k - k0) & (run - 1)) == 0 : k == k0, closes = k + 1 == k1 || (CLOSE && ((k - k0) & (run - 1)) == run - 1);
+                if (opens) {
                     if (!(ok = mma::barrier_wait(sums_empty + 8 * buffer, sums_phase))) break;
                     d = tmem + unsigned(buffer) * kColumns;
                 }
@@ -458,32 +466,32 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
                         for (int j = 0; j < kStageK / 16; ++j)
                             mma::multiply<CG>(d, mma::operand(a + j * step_a, chunk_a), mma::operand(b + j * step_b, chunk_b), P.shape,
-                                              (PLANES == 1 && k > k0) || q > 0 || j > 0);
+                                              !opens || q > 0 || j > 0);
                     }
                     mma::commit<CG>(empty + 8 * s);
-                    if (PLANES == 3 || k + 1 == k1) mma::commit<CG>(sums_full + 8 * buffer);
+                    if (closes) mma::commit<CG>(sums_full + 8 * buffer);
                 }
                 __syncwarp();
                 if (++s == P.stages) s = 0, phase ^= 1u;
-                if (PLANES == 3 || k + 1 == k1) {
+                if (closes) {
                     if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
                 }
             }
         }
-    } else if (warp >= 4) {
-        // warps 4 to 7 take the first half of the columns, 8 to 11 the second; a warp reaches the 32 lanes of its place in four
+    } else if (warp >= 2) {
+        // warps 2 to 5 take the first half of the columns, 6 to 9 the second; a warp reaches the 32 lanes of its place in four
         constexpr int kHalves = BN >= 128 ? 2 : 1;
-        const int half = (warp - 4) >> 2, quarter = warp & 3;
+        const int half = (warp - 2) >> 2, quarter = warp & 3;
         const float alpha = MODE == kStore ? P.fin.alpha * (P.fin.alpha_dev ? *P.fin.alpha_dev : 1.0f) : 1.0f;
         int buffer = 0;
         unsigned phase = 0;
-        constexpr int kMine = BN / kHalves, W = kMine < 32 ? 16 : kMine < 64 || (PLANES == 3 && MODE != kEntropy) ? 32 : 64;
+        constexpr int kMine = BN / kHalves, W = kMine < 32 ? 16 : kMine < 64 || (CLOSE && MODE != kEntropy) ? 32 : 64;
         for (int u = worker; u < units && ok; u += workers) {
             int tm, tn;
             place_of(P, u / P.splits, tm, tn);
             const int split = u % P.splits;
             const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + half * kMine;
-            const Lines L = {lines + unsigned(warp - 4) * kUnits * 512u, lane, min(32, P.m - row0)};
+            const Lines L = {lines + unsigned(warp - 2) * kUnits * 512u, lane, min(32, P.m - row0)};
             const int of_lane = row0 + lane < P.m ? row0 + lane : P.m - 1;
             const long long label = MODE == kEntropy ? P.ent.labels[of_lane] : 0;
             auto take = [&](unsigned (&x)[W], int c) {
@@ -493,14 +501,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 else entropy_segment<kUnits>(P, L, x, row0, n0 + c, label);
             };
             const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
-            if constexpr (PLANES == 3) {
+            if constexpr (CLOSE) {
                 const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
                 unsigned sum[kMine / W][W];
 #pragma unroll
                 for (int c = 0; c < kMine / W; ++c)
 #pragma unroll
                     for (int i = 0; i < W; ++i) sum[c][i] = 0u;
-                for (int k = k0; k < k1; ++k) {
+                for (int k = k0; k < k1; k += run) {
                     if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
                     mma::fence_after();
                     __syncwarp();
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     mma::fence_before();
     if (CG == 2) mma::cluster_sync();
     else __syncthreads();
-    if (warp == 2) {
+    if (warp == 0) {
         mma::fence_after();
         mma::tmem_free<CG>(tmem, kColumns * kBuffers);
     }
@@ -655,7 +663,7 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
     return best;
 }
 
-template <int CG, int BN, int MODE, int PLANES>
+template <int CG, int BN, int MODE, int PLANES, bool CLOSE>
 int launch_gemm(GemmArgs &P, long long units, const DeviceInfo &di, Queue &q)
 {
     const unsigned stage = unsigned(PLANES) * (P.a_bytes + P.b_bytes);
@@ -668,26 +676,26 @@ int launch_gemm(GemmArgs &P, long long units, const DeviceInfo &di, Queue &q)
     AXC_CUDA(cudaGetDevice(&device));
     const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
     if (!(ready.load(std::memory_order_acquire) & bit) || !bit) {
-        AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+        AXC_CUDA(cudaFuncSetAttribute(gemm_kernel<CG, BN, MODE, PLANES, CLOSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
         ready.fetch_or(bit, std::memory_order_release);
     }
     const long long workers = di.sm_count / CG;
-    return launch(q, gemm_kernel<CG, BN, MODE, PLANES>, dim3(unsigned((units < workers ? units : workers) * CG)), kThreads, smem, CG, P);
+    return launch(q, gemm_kernel<CG, BN, MODE, PLANES, CLOSE>, dim3(unsigned((units < workers ? units : workers) * CG)), kThreads, smem, CG, P);
 }
 
-template <int MODE, int PLANES>
+template <int MODE, int PLANES, bool CLOSE>
 int launch_tiles(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, Queue &q)
 {
     if constexpr (PLANES == 1) {
-        if (plan.bn == 256) return plan.cg == 2 ? launch_gemm<2, 256, MODE, 1>(P, units, di, q) : launch_gemm<1, 256, MODE, 1>(P, units, di, q);
+        if (plan.bn == 256) return plan.cg == 2 ? launch_gemm<2, 256, MODE, 1, CLOSE>(P, units, di, q) : launch_gemm<1, 256, MODE, 1, CLOSE>(P, units, di, q);
     } else {
-        if (plan.cg == 2) return launch_gemm<2, 128, MODE, 3>(P, units, di, q);
+        if (plan.cg == 2) return launch_gemm<2, 128, MODE, 3, true>(P, units, di, q);
     }
-    if (plan.bn == 128) return launch_gemm<1, 128, MODE, PLANES>(P, units, di, q);
-    if (plan.bn == 64) return launch_gemm<1, 64, MODE, PLANES>(P, units, di, q);
+    if (plan.bn == 128) return launch_gemm<1, 128, MODE, PLANES, CLOSE>(P, units, di, q);
+    if (plan.bn == 64) return launch_gemm<1, 64, MODE, PLANES, CLOSE>(P, units, di, q);
     if constexpr (MODE == kStore || MODE == kPartial) {
-        if (plan.bn == 32) return launch_gemm<1, 32, MODE, PLANES>(P, units, di, q);
-        return launch_gemm<1, 16, MODE, PLANES>(P, units, di, q);
+        if (plan.bn == 32) return launch_gemm<1, 32, MODE, PLANES, CLOSE>(P, units, di, q);
+        return launch_gemm<1, 16, MODE, PLANES, CLOSE>(P, units, di, q);
     }
     return AXC_INTERNAL;
 }
@@ -695,7 +703,11 @@ int launch_tiles(GemmArgs &P, const Plan &plan, long long units, const DeviceInf
 template <int MODE>
 int launch_plan(GemmArgs &P, const Plan &plan, long long units, const DeviceInfo &di, Queue &q)
 {
-    return P.planes == 3 ? launch_tiles<MODE, 3>(P, plan, units, di, q) : launch_tiles<MODE, 1>(P, plan, units, di, q);
+    if (P.planes == 3) return launch_tiles<MODE, 3, true>(P, plan, units, di, q);
+    if constexpr (MODE == kStore || MODE == kPartial) {
+        if (P.fin.activation == kActRelu) return launch_tiles<MODE, 1, true>(P, plan, units, di, q);
+    }
+    return launch_tiles<MODE, 1, false>(P, plan, units, di, q);
 }
 
 int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, GemmArgs *P)
@@ -718,6 +730,7 @@ int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, Gem
     P->fin = g.fin;
     P->status = status;
     P->first = first;
+    P->run = P->k_steps <= 24 ? 4 : 8;
     if (!make_map(a, g.m, g.k, g.planes, g.bf16, 128, &P->map_a) || !make_map(b, g.n, g.k, g.planes, g.bf16, b_rows_per_cta, &P->map_b))
         return AXC_INTERNAL;
     return AXC_OK;
