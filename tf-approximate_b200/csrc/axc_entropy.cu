@@ -8,7 +8,7 @@
 //   pieces   the logits of a piece of the classes are computed again, with the log-sum-exp at hand, and become the gradient in the
 //            tile's last step: 8 T D V operations, scratch for one piece
 // Where the logits are few (2^20, of at most 8192 classes) their product is split over CTAs like any other, and the pass over the rows
-// adds the parts up in shared memory and does all the rest: 128 CTAs instead of 32 for 256 x 2048 x 1000, 14.2 to %SMALL% us.
+// adds the parts up in shared memory and does all the rest: 128 CTAs instead of 32 for 256 x 2048 x 1000, 14.2 to 8.3 us.
 // The kept exponentials are fp16 for bf16 operands (rounded to 2^-12, the gradient to 2^-9), fp32 for others.
 // For fp16 the stored gradient is (softmax - onehot) 2^14, whose smallest normal value is 3.7e-9; the products' factor takes it out.
 #include "axc_gemm.h"
@@ -39,6 +39,11 @@ struct RowArgs {
     Parts parts;
     const void *bias;
     int bias_type, planes, bf16;
+    // the call's result
+    unsigned *done;                            // rows that are done
+    int mean;
+    float grad_factor;
+    float *loss, *alpha;
 };
 
 __device__ __forceinline__ float block_max(float v, float *shared)
@@ -62,6 +67,35 @@ __device__ __forceinline__ float block_sum(float v, float *shared)
     float r = 0.0f;
     for (int i = 0; i < int(blockDim.x >> 5); ++i) r += shared[i];
     return r;
+}
+
+// The last block to come here adds the rows' losses up, in an order that does not depend on which block that is, and leaves the loss
+// and the factor of the gradients.  Compensated: a sum may run over a million rows.
+__device__ __forceinline__ void add_losses(const RowArgs &A, float *shared)
+{
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        __threadfence();                       // this thread wrote the row's loss
+        last = atomicAdd(A.done, 1u) == gridDim.x - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    float sum = 0.0f, count = 0.0f, low = 0.0f;
+    for (long long i = threadIdx.x; i < A.rows; i += 256) {
+        if (A.labels[i] == A.ignore) continue;
+        const float y = __ldcg(A.row_loss + i) - low, t = sum + y;
+        low = isfinite(t) ? (t - sum) - y : 0.0f;
+        sum = t;
+        count += 1.0f;
+    }
+    sum = block_sum(sum, shared);
+    count = block_sum(count, shared);
+    if (threadIdx.x == 0) {
+        const float share = A.mean ? (count > 0.0f ? 1.0f / count : 0.0f) : 1.0f;
+        *A.loss = sum * share;
+        *A.alpha = A.grad_factor * share;
+    }
 }
 
 // One block per row: its log-sum-exp and loss; FORM 0: no more, 1: fp16 exponentials in place to bf16 gradients, 2: fp32 to fp16,
@@ -95,8 +129,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
             A.row_scale[row] = scale;
         }
     }
-    if (FORM == 0) return;
-    const int groups = int(A.line / 8);
+    const int groups = FORM == 0 ? 0 : int(A.line / 8);
     for (int i = threadIdx.x; i < groups; i += 256) {
         const int c = i * 8;
         const float first = stats[c / kSegment].x;
@@ -139,6 +172,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
             *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
+    add_losses(A, shared);
 }
 
 // The same for few logits, from the parts of their sums.
@@ -168,8 +202,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
     const bool counts = label != A.ignore, known = label >= 0 && label < A.classes;
     const float lse = base + logf(sum), scale = !counts ? 0.0f : known ? A.stored : NAN, factor = scale / sum;
     if (threadIdx.x == 0) A.row_loss[row] = !counts ? 0.0f : known ? lse - logits[label] : NAN;
-    if (!A.gradient) return;
-    for (int c = int(threadIdx.x) * 8; c < A.line; c += 2048) {
+    for (int c = A.gradient ? int(threadIdx.x) * 8 : int(A.line); c < A.line; c += 2048) {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -191,29 +224,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
             *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
-}
-
-// The rows' losses added in a fixed order, and the factor of the gradients; one block.
-__global__ void __launch_bounds__(1024) loss_kernel(const float *row_loss, const long long *labels, long long rows, long long ignore,
-                                                    int mean, float grad_factor, float *loss, float *alpha)
-{
-    after_previous();
-    __shared__ float shared[32];
-    float sum = 0.0f, count = 0.0f, low = 0.0f;                 // compensated: a sum may run over a million rows
-    for (long long i = threadIdx.x; i < rows; i += 1024) {
-        if (labels[i] == ignore) continue;
-        const float y = row_loss[i] - low, t = sum + y;
-        low = isfinite(t) ? (t - sum) - y : 0.0f;
-        sum = t;
-        count += 1.0f;
-    }
-    sum = block_sum(sum, shared);
-    count = block_sum(count, shared);
-    if (threadIdx.x == 0) {
-        const float share = mean ? (count > 0.0f ? 1.0f / count : 0.0f) : 1.0f;
-        *loss = sum * share;
-        *alpha = grad_factor * share;
-    }
+    add_losses(A, shared);
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
@@ -344,11 +355,19 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
         r.bf16 = g.bf16;
         r.plane = l.line * d.rows;
         const unsigned grid = unsigned(d.rows);
+        r.done = status + 1;
+        r.mean = d.reduction == AXC_REDUCE_MEAN;
+        r.grad_factor = d.grad_scale / stored;
+        r.loss = loss;
+        r.alpha = alpha;
         rc = launch(q, l.few ? few_kernel : !l.kept ? row_kernel<0> : d.type == kBfloat16 ? row_kernel<1> : d.type == kFloat16 ? row_kernel<2> : row_kernel<3>, dim3(grid), 256, 0, 1, r);
         if (rc) return rc;
-    } else AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
-    rc = launch(q, loss_kernel, dim3(1), 1024, 0, 1, row_loss, labels, d.rows, d.ignore_index, int(d.reduction == AXC_REDUCE_MEAN), d.grad_scale / stored, loss, alpha);
-    if (rc || !l.gradients) return rc;
+    } else {                                   // a sum over nothing
+        AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
+        AXC_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), q.stream));
+        AXC_CUDA(cudaMemsetAsync(alpha, 0, sizeof(float), q.stream));
+    }
+    if (!l.gradients) return AXC_OK;
     const size_t size = type_size(d.type);
     float *dx_sum = reinterpret_cast<float *>(ws + l.dx);
     const long long dx_line = (d.inputs + 3) / 4 * 4;

@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     mma::fence_after();
     const unsigned tmem = head->tmem;
     asm volatile("griddepcontrol.wait;" ::: "memory");          // operands may come from the kernel before
-    if (P.first && blockIdx.x == 0 && threadIdx.x == 0) *P.status = 0u;        // a wait runs out after a second, not before this
+    // a wait runs out after a second, not before this; the word behind the status counts what a later kernel has done
+    if (P.first && blockIdx.x == 0 && threadIdx.x == 0) P.status[0] = P.status[1] = 0u;
     bool ok = true;
 
     // The loading and the multiplying warp run as a whole and one of their threads acts, so that what it hands over is computed once for
