@@ -642,6 +642,7 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
     Plan best = {1, 128, 1};
     double least = 1e300;
     const long long steps = ceil_div(k > 0 ? k : 1, kStageK);
+    const double memory = (double(m) + double(n)) * double(k) * 2 * planes / 3400;         // the operands, once, at memory's rate
     for (int c = 0; c < 6; ++c) {
         static const int kCg[6] = {2, 1, 1, 1, 1, 1}, kBn[6] = {256, 256, 128, 64, 32, 16};
         const int cg = kCg[c], bn = planes == 3 && cg == 2 ? 128 : kBn[c];
@@ -653,7 +654,9 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
             if (splits > 1 && steps / splits < 2) break;
             const long long units = tiles * splits;
             const double copies = bytes / 114 * double(units < workers ? units : workers) / double(workers), stage = products > copies ? products : copies;
-            double clocks = double(ceil_div(units, workers)) * (double(ceil_div(steps, splits)) * stage + 3400) + 4500 + 8 * bn;
+            double clocks = double(ceil_div(units, workers)) * (double(ceil_div(steps, splits)) * stage + 3400);
+            if (clocks < memory) clocks = memory;
+            clocks += 4500 + 8 * bn;
             if (splits > 1) clocks += 7600 + double(m) * n * splits * 8 / 7400;
             if (clocks < least) {
                 least = clocks;
