@@ -636,7 +636,8 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 // more; a wave of tiles 3400 more until its sums are out, the product another 4500 for its first bytes and its last tile; a split one 7600
 // for the second kernel and its partial sums' way to L2 and back.  Fitted to all tiles and splits measured for 34 products, in bf16 from
 // 4 x 2048 x 1000 to 8192 x 8192 x 2048 and 2047 x 50001 x 1024, in fp32 from 64 x 300 x 64 to 2000 x 2000 x 2000: the one chosen so was
-// the fastest or within 2 % of it for 31, 3 to 12 % slower for the others (3000 x 3000 x 700: 27.6 us instead of 24.6).
+// the fastest or within 2 % of it for 30, 3 to 12 % slower for three (3000 x 3000 x 700: 27.6 us instead of 24.6) and 29 % for 4 x 4096 x
+// 16384 (37 instead of 28.7: so few rows of a are the same few lines of memory for every CTA).
 Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, int sms)
 {
     Plan best = {1, 128, 1};

@@ -3,9 +3,11 @@
 //   inputs contiguous  a warp has 1 or 4 units and walks along their inputs, 16 bytes a lane; the rows of x come through L1
 //   units contiguous   (fp32) a lane has 16 bytes of neighbouring units, the warps and the blocks of a column share the inputs, and their
 //                      sums are added in a fixed order (shared memory, then the second kernel of split products)
-// 16-bit kernels with more than two rows, or with units contiguous, are quicker on the tensor cores.  us for 4096 inputs x 16384 units:
-//   bf16, inputs contiguous   1 row 24.1, 2 rows 34, 4 rows 43; tensor cores 27.8       (reading it once: 20.5)
-//   fp32                      inputs contiguous 43.9 to 112 for 1 to 8 rows, tensor cores 201; units contiguous %SUM%   (41.0)
+// 16-bit kernels with more than two rows, or with units contiguous, are as quick or quicker on the tensor cores.  us for 4096 inputs x
+// 16384 units, and 2048 x 1000:
+//   bf16, inputs contiguous   1 row 24.1, 2 rows 34, 4 rows 43 (tensor cores 34 to 37; reading it once: 20.5); 4.1, 4.6, 6.7 (9.3)
+//   fp32, inputs contiguous   44 to 112 for 1 to 8 rows (tensor cores 215; 41.0); 5.1 to 10.9 (17.7)
+//   fp32, units contiguous    67 to 112 (226; 41.0); 10.1 to 11.8 (18.1)
 #include "axc_rows.h"
 
 namespace axc {
