@@ -167,6 +167,10 @@ def test_refusals(built):
     for grads in ([], [torch.zeros(5, device="cuda")], [torch.zeros(4, 6)], [torch.zeros(4, 6, device="cuda").half()]):
         with pytest.raises(ax.InvalidArgumentError):
             opt.step(grads)
+    opt.params.append(p.clone())
+    with pytest.raises(ax.InvalidArgumentError):
+        opt.step([p, p])
+    opt.params.pop()
     assert opt.step_count == 0
     with pytest.raises(ax.InvalidArgumentError):
         opt.load_state_dict(ax.AdamW([p], state_bits=8).state_dict())

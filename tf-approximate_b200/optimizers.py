@@ -79,6 +79,8 @@ class AdamW:
 
     def step(self, grads=None, grad_scale=1.0):
         """One step with `grads`, in the order of the parameters (default: their .grad; None: left as it is), times `grad_scale`."""
+        if len(self.params) != len(self._counts):
+            raise InvalidArgumentError("the optimizer's parameters are those it was made with")
         if grads is not None and not isinstance(grads, list):
             grads = list(grads)
         eight = self.state_bits == 8
