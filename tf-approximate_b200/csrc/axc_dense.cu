@@ -10,6 +10,8 @@ namespace {
 // the V columns of a group, 2 to 8 rows in flight, packed until they are needed.  Lines that do not start on 16 bytes are read value by
 // value, the V values of a thread 32 apart, so that neighbouring lanes still read neighbouring ones.  The sums of the block's 8 rows are
 // added in shared memory, those of the blocks by a second kernel, in a fixed order.  Bound by reading dy and kept and writing dz once.
+// Nothing is read or written behind the last column (packed groups: S.padded or columns that are whole groups): the operand's tensor maps end
+// there, so what its lines have up to a multiple of 8 values does not matter.
 // ------------------------------------------------------------------------------------------------
 constexpr int kShares = 64;                    // blocks that share the rows, at most
 
@@ -58,9 +60,7 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
-    // operand lines are a multiple of 8 values: zeros behind the last column
-    const long long mine = S.planes ? S.line - c : left;
-    if (mine > 0) {
+    if (left > 0) {
         const T *dy = static_cast<const T *>(S.dy) + (begin + r0) * S.dy_line + c, *kept = static_cast<const T *>(S.kept) + (begin + r0) * S.columns + c;
         for (long long r = begin + r0; r < end; r += 8 * kRows, dy += 8 * kRows * S.dy_line, kept += 8 * kRows * S.columns) {
             Group<T> g[kRows], k[ACT != kActNone ? kRows : 1];
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                         else {
 #pragma unroll
                             for (int i = 0; i < V; ++i)
-                                if (32 * i < mine) operand[32 * i] = u.t[i];
+                                if (32 * i < left) operand[32 * i] = u.t[i];
                         }
                     }
                 }
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                         else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (32 * i < mine) to[32 * i] = u.h[i];
+                                if (32 * i < left) to[32 * i] = u.h[i];
                         }
                     }
                 }
@@ -166,8 +166,7 @@ int shares_of(long long rows, long long columns)
 template <typename T, bool VEC>
 int launch_slope(const Slope &s, float *part, int shares, Queue &q)
 {
-    const long long columns = s.planes && s.line > s.columns ? s.line : s.columns;
-    const dim3 grid(unsigned((columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
+    const dim3 grid(unsigned((s.columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
     return launch(q, !s.kept ? slope_kernel<T, kActNone, VEC> : s.activation == kActRelu ? slope_kernel<T, kActRelu, VEC>
                      : s.activation == kActGelu ? slope_kernel<T, kActGelu, VEC> : slope_kernel<T, kActSilu, VEC>, grid, 256, 0, 1, s, part);
 }
