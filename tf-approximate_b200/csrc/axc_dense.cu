@@ -13,8 +13,6 @@ namespace {
 // Nothing is read or written behind the last column (packed groups: S.padded or columns that are whole groups): the operand's tensor maps end
 // there, so what its lines have up to a multiple of 8 values does not matter.
 // ------------------------------------------------------------------------------------------------
-constexpr int kShares = 64;                    // blocks that share the rows, at most
-
 template <int ACT, bool EXACT>
 __device__ __forceinline__ float slope_of(float kept)
 {
@@ -153,16 +151,6 @@ __global__ void __launch_bounds__(256) slope_sums_kernel(const float *part, long
     store_from_float(sums, c, type, s * scale * (scale_dev ? *scale_dev : 1.0f));
 }
 
-int shares_of(long long rows, long long columns)
-{
-    // about eight blocks for every SM, of at least 32 rows each
-    long long shares = (rows + 31) / 32;
-    const long long across = columns / 256 + 1, most = 1184 / across + 1;
-    if (shares > most) shares = most;
-    if (shares > kShares) shares = kShares;
-    return int(shares < 1 ? 1 : shares);
-}
-
 template <typename T, bool VEC>
 int launch_slope(const Slope &s, float *part, int shares, Queue &q)
 {
@@ -173,13 +161,11 @@ int launch_slope(const Slope &s, float *part, int shares, Queue &q)
 
 }  // namespace
 
-size_t slope_scratch(long long rows, long long columns) { return size_t(shares_of(rows, columns)) * size_t(columns) * 4; }
-
-int slope(const Slope &s, void *scratch, const DeviceInfo &di, Queue &q)
+int slope(const Slope &s, void *scratch, size_t room, Queue &q)
 {
-    (void)di;
     if (s.columns == 0 || (s.rows == 0 && !s.sums)) return AXC_OK;
-    const int shares = shares_of(s.rows, s.columns);
+    if (s.sums && room < slope_scratch(s.rows, s.columns)) return AXC_INTERNAL;
+    const int shares = column_shares(s.rows, s.columns);
     float *part = s.sums ? static_cast<float *>(scratch) : nullptr;
     // whole groups of 16 bytes, in every line of every tensor
     const uintptr_t all = reinterpret_cast<uintptr_t>(s.dy) | reinterpret_cast<uintptr_t>(s.kept) | reinterpret_cast<uintptr_t>(s.same);
@@ -322,7 +308,7 @@ int backward(const axc_dense_desc &d, const void *dy, const void *x, const void 
     s.sums_type = d.bias_type;
     s.scale = 1.0f;
     int rc = AXC_OK;
-    if (s.same || s.planes || s.sums) rc = slope(s, ws + parts.part, di, q);
+    if (s.same || s.planes || s.sums) rc = slope(s, ws + parts.part, parts.scratch - parts.part, q);
     if (rc) return rc;
     bool first = true;
     Operand ox = {}, ok = {};

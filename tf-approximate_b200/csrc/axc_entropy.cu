@@ -256,13 +256,7 @@ Layout layout_of(const axc_entropy_desc &d, bool gradients, const void *x, const
     l.few = d.classes <= kFewClasses && d.rows * d.classes <= kFewLogits && (d.scratch_limit == 0 || d.scratch_limit >= kFewLogits * 64);
     l.kept = gradients && !l.few && size_t(d.rows) * size_t(whole) * (keep_bytes + gradient_bytes) <= limit;
     l.piece = whole;
-    if (gradients && !l.kept && !l.few) {
-        // as few pieces as the limit allows, of equal size, at least 256 classes
-        const size_t each = size_t(d.rows) * 2 * planes, most = limit / (each ? each : 1) / 256 * 256;
-        const long long cap = most < 256 ? 256 : (long long)most < whole ? (long long)most : whole;
-        const long long pieces = (whole + cap - 1) / cap;
-        l.piece = ((whole + pieces - 1) / pieces + 255) / 256 * 256;
-    }
+    if (gradients && !l.kept && !l.few) l.piece = classes_of_piece(d.rows, whole, planes, limit);
     l.line = l.piece < whole ? l.piece : whole;
     l.x = 256;
     l.kernel = l.x + up(operand_bytes(x_of(d, x)));
@@ -275,14 +269,13 @@ Layout layout_of(const axc_entropy_desc &d, bool gradients, const void *x, const
     if (gradients) l.dx = (l.kept && d.type == kBfloat16 ? l.keep + up(size_t(d.rows) * l.line * 2) : l.gradient + up(size_t(d.rows) * l.line * 2 * planes));
     const bool pieces = gradients && !l.kept && !l.few;
     l.part = l.dx + (pieces ? up(size_t(d.rows) * size_t((d.inputs + 3) / 4 * 4) * 4) : 0);
-    l.scratch = l.part + (gradients ? up(slope_scratch(d.rows, l.line)) : 0);
+    l.scratch = l.part + (gradients ? up(slope_scratch_of_pieces(d.rows, d.classes, pieces ? l.piece : d.classes)) : 0);
     size_t most = 0;
     if (gradients) {
-        // pieces are equal but for the last
-        const long long sizes[2] = {!pieces || l.piece > d.classes ? d.classes : l.piece, !pieces ? d.classes : d.classes - (d.classes - 1) / l.piece * l.piece};
-        for (int i = 0; i < 2; ++i) {
-            most = largest(most, gemm_scratch(d.rows, d.inputs, sizes[i], planes, di));
-            most = largest(most, d.kernel_gradient_transposed ? gemm_scratch(sizes[i], d.inputs, d.rows, planes, di) : gemm_scratch(d.inputs, sizes[i], d.rows, planes, di));
+        const PieceSizes sizes = piece_sizes(d.classes, pieces ? l.piece : d.classes);
+        for (const long long n : sizes.n) {
+            most = largest(most, gemm_scratch(d.rows, d.inputs, n, planes, di));
+            most = largest(most, d.kernel_gradient_transposed ? gemm_scratch(n, d.inputs, d.rows, planes, di) : gemm_scratch(d.inputs, n, d.rows, planes, di));
         }
     }
     if (l.few) most = largest(most, gemm_parts_scratch(d.rows, d.classes, d.inputs, planes, di));
@@ -451,7 +444,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             s.sums_type = d.bias_type;
             s.scale = 1.0f;
             s.scale_dev = alpha;
-            rc = slope(s, ws + l.part, di, q);
+            rc = slope(s, ws + l.part, l.scratch - l.part, q);
             if (rc) return rc;
         }
     }

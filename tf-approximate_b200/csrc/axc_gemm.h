@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include "axc_internal.h"
+#include "axc_pieces.h"
 
 namespace axc {
 
@@ -216,8 +217,8 @@ struct Slope {
     float scale;
     const float *scale_dev;
 };
-size_t slope_scratch(long long rows, long long columns);       // partial sums
-int slope(const Slope &s, void *scratch, const DeviceInfo &di, Queue &q);
+// `room`: bytes of the scratch, slope_scratch(rows, columns) at least; less is refused.
+int slope(const Slope &s, void *scratch, size_t room, Queue &q);
 
 // ---- operands -----------------------------------------------------------------------------------------------------------
 // A matrix in the caller's memory: element (r, c) at data[r * row_stride + c * column_stride]
