@@ -112,10 +112,11 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                 }
                 if (S.planes && sizeof(T) == 4) {
                     uint16_t *to = S.planes + row * S.line + c;
+#pragma unroll
                     for (int p = 0; p < 3; ++p, to += S.plane) {
                         union { uint2 w; uint16_t h[4]; } u;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(d[i], d[i]);
+                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(d[i], d[i], p);
                         if (VEC) *reinterpret_cast<uint2 *>(to) = u.w;
                         else {
 #pragma unroll

@@ -9,7 +9,8 @@
 //   lone CTAs, 128 x N tiles  for products with too few tiles to fill the GPU
 //
 // fp32 operands are split exactly into three bf16 terms, x = x0 + x1 + x2, each 2^-8 of the one before; six of the nine products
-// of terms are summed (x2 y0, x1 y1, x0 y2, x1 y0, x0 y1, x0 y0), the three left out are below 2^-24 of x y.
+// of terms are summed (x2 y0, x1 y1, x0 y2, x1 y0, x0 y1, x0 y0), the three left out are below 2^-24 of x y.  Infinities are split so that
+// their products are those of the values (split_term).
 //
 // Sums are fp32.  The tensor cores cut a sum off at 24 bits at every step of 16 k (measured: 2e-8 of it on average, always towards
 // zero), which 16-bit results do not show.  For fp32 the sums of every 64 k, the small products first, are taken out and added in
@@ -848,7 +849,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const Layout one, const La
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) out[p].h[j] = split_term(x[j], x[j]);
+                for (int j = 0; j < 8; ++j) out[p].h[j] = split_term(x[j], x[j], p);
                 *reinterpret_cast<uint4 *>(to + p * m.plane) = out[p].w;
             }
         } else {

@@ -101,18 +101,24 @@ __device__ __forceinline__ float erf_16bit(float x, float &bell)
     return copysignf(fmaf(-poly, bell, 1.0f), x);
 }
 
-// The next bf16 term of x, and in `rest` what it leaves.  A value beyond bf16's range keeps its largest finite term; infinities and
-// NaNs are whole in their first term.
-__device__ __forceinline__ uint16_t split_term(float x, float &rest)
+// bf16 term `p` of three of x, and in `rest` what is left of x for the terms after it.  A value beyond bf16's range keeps its largest finite
+// term.  An infinity is (1, 0, inf) with its sign: of the six products of terms that are summed, the third one is in that with the other
+// operand's first term alone, so that inf meets no term that is zero because the value needs no more of them; its own first term
+// stands for it where the other operand is infinite, too.  A NaN is whole in its first term.
+__device__ __forceinline__ uint16_t split_term(float x, float &rest, int p)
 {
+    if (isinf(x)) {
+        rest = x;
+        return __bfloat16_as_ushort(__float2bfloat16_rn(p == 0 ? copysignf(1.0f, x) : p == 1 ? 0.0f : x));
+    }
     __nv_bfloat16 h = __float2bfloat16_rn(x);
-    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __float2bfloat16_rz(x);
+    if (isinf(__bfloat162float(h))) h = __float2bfloat16_rz(x);
     rest = isfinite(x) ? x - __bfloat162float(h) : 0.0f;
     return __bfloat16_as_ushort(h);
 }
 
 // A matrix of `rows` x `k` as the tensor cores read it: 16-bit values (bf16, or fp16), either k or the rows contiguous, 16-byte
-// aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_planes).
+// aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_term).
 struct Operand {
     const void *data;
     long long line;             // values from one line to the next
