@@ -245,6 +245,18 @@ int leave(int rc, int device, int prev)
     return rc != AXC_OK ? rc : e == cudaSuccess ? AXC_OK : cuda_failed(e);
 }
 
+// A call without outputs: no more than its status.  Without a workspace there is nothing to do, not even a device to look for.
+int nothing(void *workspace, size_t bytes, int device, void *stream)
+{
+    if (!workspace || bytes < sizeof(unsigned)) return AXC_OK;
+    DeviceInfo di;
+    int prev = 0;
+    const int rc = enter(device, &di, &prev);
+    if (rc) return rc;
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, sizeof(unsigned), cudaStream_t(stream));
+    return leave(e == cudaSuccess ? AXC_OK : cuda_failed(e), device, prev);
+}
+
 int forward(const axc_dense_desc &d, const void *x, const void *kernel, const void *bias, const void *residual, void *y, void *pre, char *ws,
             const DeviceInfo &di, Queue &q)
 {
@@ -386,7 +398,7 @@ extern "C" int axc_dense_forward(const axc_dense_desc *desc, const void *x, cons
     int rc = check_desc(desc);
     if (rc) return rc;
     const axc_dense_desc &d = *desc;
-    if (d.rows == 0 || d.units == 0) return AXC_OK;
+    if (d.rows == 0 || d.units == 0) return nothing(workspace, workspace_bytes, device, stream);
     if (!y || (d.inputs > 0 && (!x || !kernel))) return AXC_INVALID_ARGUMENT;
     DeviceInfo di;
     rc = device_info(device, &di);
@@ -409,7 +421,7 @@ extern "C" int axc_dense_backward(const axc_dense_desc *desc, const void *dy, co
     const bool some = d.rows > 0 && d.units > 0;
     if (some && (!dy || (d.activation != kActNone && !kept))) return AXC_INVALID_ARGUMENT;
     if (d.inputs > 0 && some && ((dx && !kernel) || (dkernel && !x))) return AXC_INVALID_ARGUMENT;
-    if (d.rows == 0 && d.units == 0) return AXC_OK;
+    if (d.rows == 0 && d.units == 0) return nothing(workspace, workspace_bytes, device, stream);
     DeviceInfo di;
     rc = device_info(device, &di);
     if (rc) return rc;

@@ -779,10 +779,9 @@ int gemm_parts(const Gemm &g, void *scratch, Parts *parts, unsigned *status, boo
 
 int gemm(const Gemm &g, void *scratch, unsigned *status, bool first, const DeviceInfo &di, Queue &q)
 {
-    if (g.m == 0 || g.n == 0) return AXC_OK;
-    if (g.k == 0) {                                             // sums of nothing
+    if (g.m == 0 || g.n == 0 || g.k == 0) {                     // nothing, or sums of nothing: no kernel that would clear the status
         if (first) AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));
-        return finish_parts(Parts{}, g.m, g.n, g.fin, di, q);
+        return g.m == 0 || g.n == 0 ? AXC_OK : finish_parts(Parts{}, g.m, g.n, g.fin, di, q);
     }
     const Plan plan = choose_plan(g.m, g.n, g.k, g.planes, true, di.sm_count);
     if (plan.splits > 1) {
