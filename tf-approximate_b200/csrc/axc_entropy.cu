@@ -2,11 +2,12 @@
 //   l = x kernel + bias,  loss_t = log sum_v exp(l_tv) - l_t,label,  dl = w (softmax(l) - onehot),  dx = dl kernel^T,  dkernel = x^T dl
 // The logits never reach memory.  One pass of matrix tiles over the classes (axc_gemm.cu) leaves, for every row and segment of 64
 // classes, the largest logit and the sum of exponentials relative to it.  A pass over the rows joins them to the row's
-// log-sum-exp.  Then one of two forms gives the gradient of the logits, 16-bit values that are rounded once:
+// largest logit and sum (never to their one number log sum_v exp(l_tv): it is rounded to a part of the logits' size, which may be all
+// that there is of a small loss or gradient).  Then one of two forms gives the gradient of the logits, 16-bit values that are rounded once:
 //   kept     the exponentials, relative to their segment's largest logit, were kept in scratch, and the pass over the rows turns them
 //            into the gradient: 6 T D V operations, 2 bytes of scratch per logit (bf16; 6 for fp16, 10 for fp32)
-//   pieces   the logits of a piece of the classes are computed again, with the log-sum-exp at hand, and become the gradient in the
-//            tile's last step: 8 T D V operations, scratch for one piece
+//   pieces   the logits of a piece of the classes are computed again, with the row's largest logit and sum at hand, and become the gradient
+//            in the tile's last step: 8 T D V operations, scratch for one piece
 // Where the logits are few (2^20, of at most 8192 classes) their product is split over CTAs like any other, and the pass over the rows
 // adds the parts up in shared memory and does all the rest: 128 CTAs instead of 32 for 256 x 2048 x 1000, 14.2 to 8.3 us.
 // The kept exponentials are fp16 for bf16 operands (rounded to 2^-12, the gradient to 2^-9), fp32 for others.
@@ -28,7 +29,9 @@ struct RowArgs {
     long long ignore;
     const float2 *stats;
     int segments;
-    float *label_logit, *lse, *row_scale, *row_loss;
+    float *label_logit;
+    float2 *softmax;                           // see EntropyArgs
+    float *row_scale, *row_loss;
     float stored;                              // scale of the stored gradient
     // kept form
     void *keep;
@@ -98,7 +101,7 @@ __device__ __forceinline__ void add_losses(const RowArgs &A, float *shared)
     }
 }
 
-// One block per row: its log-sum-exp and loss; FORM 0: no more, 1: fp16 exponentials in place to bf16 gradients, 2: fp32 to fp16,
+// One block per row: its largest logit, sum and loss; FORM 0: no more, 1: fp16 exponentials in place to bf16 gradients, 2: fp32 to fp16,
 // 3: fp32 to three bf16 planes.  Bound by reading and writing the exponentials once.
 template <int FORM>
 __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
@@ -119,13 +122,13 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
     sum = block_sum(sum, shared);
     const long long label = A.labels[row];
     const bool counts = label != A.ignore, known = label >= 0 && label < A.classes;
-    const float lse = base + logf(sum);
     // a label outside the classes shows in the loss and in every gradient
     const float scale = !counts ? 0.0f : known ? A.stored : NAN;
     if (threadIdx.x == 0) {
-        A.row_loss[row] = !counts ? 0.0f : known ? lse - A.label_logit[row] : NAN;
-        if (FORM == 0 && A.lse) {
-            A.lse[row] = lse;
+        // the largest logit comes off the label's first: the logits' size does not decide what is left of a small loss
+        A.row_loss[row] = !counts ? 0.0f : known ? logf(sum) - (A.label_logit[row] - base) : NAN;
+        if (FORM == 0 && A.softmax) {
+            A.softmax[row] = make_float2(base, 1.0f / sum);
             A.row_scale[row] = scale;
         }
     }
@@ -200,8 +203,8 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
     sum = block_sum(sum, shared);
     const long long label = A.labels[row];
     const bool counts = label != A.ignore, known = label >= 0 && label < A.classes;
-    const float lse = base + logf(sum), scale = !counts ? 0.0f : known ? A.stored : NAN, factor = scale / sum;
-    if (threadIdx.x == 0) A.row_loss[row] = !counts ? 0.0f : known ? lse - logits[label] : NAN;
+    const float scale = !counts ? 0.0f : known ? A.stored : NAN, factor = scale / sum;
+    if (threadIdx.x == 0) A.row_loss[row] = !counts ? 0.0f : known ? logf(sum) - (logits[label] - base) : NAN;
     for (int c = A.gradient ? int(threadIdx.x) * 8 : int(A.line); c < A.line; c += 2048) {
         float v[8];
 #pragma unroll
@@ -262,7 +265,7 @@ Layout layout_of(const axc_entropy_desc &d, bool gradients, const void *x, const
     l.kernel = l.x + up(operand_bytes(x_of(d, x)));
     l.stats = l.kernel + up(operand_bytes(kernel_of(d, kernel)));
     l.rows = l.stats + up(size_t(d.rows) * l.segments * 8);
-    l.keep = l.rows + 4 * up(size_t(d.rows) * 4) + 256;
+    l.keep = l.rows + 5 * up(size_t(d.rows) * 4) + 256;
     l.gradient = l.keep + (l.kept ? up(size_t(d.rows) * l.line * keep_bytes) : 0);
     if (gradients && l.kept && d.type == kBfloat16) l.gradient = l.keep;
     l.dx = l.keep;
@@ -299,9 +302,10 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
     const float stored = d.type == kFloat16 ? kHalfScale : 1.0f;
     unsigned *status = reinterpret_cast<unsigned *>(ws);
     const size_t per_row = up(size_t(d.rows) * 4);
-    float *label_logit = reinterpret_cast<float *>(ws + l.rows), *lse = reinterpret_cast<float *>(ws + l.rows + per_row);
-    float *row_scale = reinterpret_cast<float *>(ws + l.rows + 2 * per_row), *alpha = reinterpret_cast<float *>(ws + l.rows + 4 * per_row);
-    if (!row_loss) row_loss = reinterpret_cast<float *>(ws + l.rows + 3 * per_row);
+    float2 *softmax = reinterpret_cast<float2 *>(ws + l.rows);
+    float *label_logit = reinterpret_cast<float *>(ws + l.rows + 2 * per_row), *row_scale = reinterpret_cast<float *>(ws + l.rows + 3 * per_row);
+    float *alpha = reinterpret_cast<float *>(ws + l.rows + 5 * per_row);
+    if (!row_loss) row_loss = reinterpret_cast<float *>(ws + l.rows + 4 * per_row);
     Gemm g = {};
     g.planes = planes;
     g.bf16 = d.type != kFloat16;
@@ -335,7 +339,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
         r.stats = e.stats;
         r.segments = l.segments;
         r.label_logit = label_logit;
-        r.lse = l.gradients ? lse : nullptr;
+        r.softmax = l.gradients ? softmax : nullptr;
         r.row_scale = row_scale;
         r.row_loss = row_loss;
         r.stored = stored;
@@ -380,7 +384,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
             e.keep = ws + l.gradient;
             e.line = l.line;
             e.plane = l.line * d.rows;
-            e.lse = lse;
+            e.softmax = softmax;
             e.row_scale = row_scale;
             e.column0 = int(c0);
             rc = gemm_entropy(again, e, true, status, false, di, q);

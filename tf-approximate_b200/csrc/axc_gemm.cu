@@ -317,14 +317,15 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &
     if (e.keep) store_row<64, N>(L, v, e.keep, e.keep_fp32 ? kFloat32 : kFloat16, e.line, row0, n0, int(e.line));
 }
 
-// W logits of a row and what the loss's gradient is there: row_scale * (exp(logit - lse) - [label])
+// W logits of a row and what the loss's gradient is there: row_scale * (exp(logit - largest) / sum - [label])
 template <int W, int N>
 __device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0)
 {
     const EntropyArgs &e = P.ent;
     if (n0 >= e.line) return;
     const int row = row0 + L.lane < P.m ? row0 + L.lane : P.m - 1;
-    const float lse = e.lse[row], scale = e.row_scale[row];
+    const float2 softmax = e.softmax[row];
+    const float scale = e.row_scale[row];
     const long long label = e.labels[row] - e.column0 - n0;
     float v[W];
 #pragma unroll
@@ -340,7 +341,7 @@ __device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines 
     }
     // a row without a label stays out, whatever its logits are
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = scale != 0.0f ? scale * (__expf(v[i] - lse) - (label == i ? 1.0f : 0.0f)) : 0.0f;
+    for (int i = 0; i < W; ++i) v[i] = scale != 0.0f ? scale * (__expf(v[i] - softmax.x) * softmax.y - (label == i ? 1.0f : 0.0f)) : 0.0f;
     uint16_t *keep = static_cast<uint16_t *>(e.keep);
     const int type = (P.shape >> 7 & 1) ? kBfloat16 : kFloat16;
     for (int plane = 0; plane < P.planes; ++plane) {

@@ -175,7 +175,7 @@ struct EntropyArgs {
     float2 *stats;              // [rows][segments] {largest logit, sum of exponentials relative to it}
     int segments;
     float *label_logit;
-    const float *lse;           // gradient only
+    const float2 *softmax;      // gradient only: a row's largest logit, and 1 / its sum of exponentials relative to that
     const float *row_scale;     // gradient only: 0 for rows without a label, else the scale of the stored gradient
     int column0;                // gradient only: first class of this piece
 };
