@@ -2,12 +2,21 @@
 convolutions go through a truth table.  The reference takes both from its host framework (Keras Dense, sparse softmax cross
 entropy with logits); here they are matrix kernels on the tensor cores behind include/axconv.h."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .errors import InvalidArgumentError
 
 _ACTIVATIONS = {None: 0, "none": 0, "linear": 0, "relu": 1, "gelu": 2, "silu": 3}
 _REDUCTIONS = {"mean": 0, "sum": 1}
+
+
+def _differentiated(*tensors):
+    """Whether autograd has to see the call: a gradient may be asked for, or tensors may have tangents of forward mode, which the autograd
+    functions refuse (they have no rule for it) and a direct call would drop."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _activation(name):
@@ -54,7 +63,7 @@ class _DenseFn(torch.autograd.Function):
 
 def dense(x, kernel, bias=None, residual=None, activation=None):
     """activation(x kernel + bias + residual), differentiable once; see `dense_forward`."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, kernel, bias, residual)):
+    if _differentiated(x, kernel, bias, residual):
         return _DenseFn.apply(x, kernel, bias, residual, activation)
     return _lib.binding().dense_forward(x, kernel, bias, residual, _activation(activation), None)[0]
 
@@ -97,7 +106,7 @@ def dense_cross_entropy(x, kernel, labels, bias=None, ignore_index=-100, reducti
     """Softmax cross entropy of a dense classifier; see `dense_cross_entropy_gradients`.  Differentiable once: the gradients are
     computed with the loss and kept until backward, so float16 operands want a loss scale there (`dense_cross_entropy_gradients`
     has one).  row_losses: (loss, the rows' own losses), without gradients."""
-    if not row_losses and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, kernel, bias)):
+    if not row_losses and _differentiated(x, kernel, bias):
         return _EntropyFn.apply(x, kernel, bias, labels, ignore_index, reduction, scratch_limit)
     loss, rows, _, _, _ = _entropy(x, kernel, labels, bias, ignore_index, reduction, 1.0, scratch_limit, bool(row_losses), (False, False, False), False)
     return (loss, rows) if row_losses else loss
