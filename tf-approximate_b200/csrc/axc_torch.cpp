@@ -350,6 +350,11 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
         table[i].grad = g.const_data_ptr();
     }
     check(g_entry.adamw(&d, table, int32_t(count), device, stream_of(like)), "AdamW");
+    // a graph that saved a parameter's value from before the step is refused its backward pass
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(a[0], i));
+        if (table[i].grad && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();        // (tensors of inference mode have no counter)
+    }
     Py_RETURN_NONE;
     AXC_TORCH_END
 }
