@@ -327,13 +327,13 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
         invalid(std::to_string(PyList_GET_SIZE(a[1])) + " gradients for " + std::to_string(count) + " parameters");
     const int device = like.device().index();
     std::vector<at::Tensor> copies;
-    auto fits = [&](const at::Tensor &t, int64_t values, const char *what) {
+    auto fits = [&](const at::Tensor &t, const char *what) {
         if (!t.is_cuda() || t.device().index() != device || type_of(t) != type) invalid(std::string("every ") + what + " must be a tensor of the optimizer's type and device");
-        if (t.numel() != values) invalid(std::string("a ") + what + " has another size than the parameter");
     };
     for (Py_ssize_t i = 0; i < count; ++i) {
         const at::Tensor p = tensor_of(PyList_GET_ITEM(a[0], i), "parameter", false);
-        fits(p, table[i].count, "parameter");
+        fits(p, "parameter");
+        if (p.numel() != table[i].count) invalid("a parameter has another size than it had when the optimizer was made");
         if (!p.is_contiguous()) invalid("parameters must be contiguous");
         at::Tensor g;
         if (given) g = tensor_of(PyList_GET_ITEM(a[1], i), "gradient", true);
@@ -341,9 +341,9 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
         table[i].param = p.mutable_data_ptr();
         table[i].grad = nullptr;
         if (!g.defined()) continue;
-        fits(g, table[i].count, "gradient");
+        fits(g, "gradient");
+        if (g.sizes() != p.sizes()) invalid("a gradient has another shape than its parameter: " + text_of(g.sizes()) + " for " + text_of(p.sizes()));
         if (!g.is_contiguous()) {
-            if (g.sizes() != p.sizes()) invalid("a gradient has another shape than the parameter");
             g = g.contiguous();
             copies.push_back(g);
         }
