@@ -307,7 +307,6 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (n != 11 || !PyList_Check(a[0]) || (a[1] != Py_None && !PyList_Check(a[1]))) invalid("adamw_step takes 11 arguments");
     c10::NoGradGuard no_grad;
     axc_adamw_tensor *table = static_cast<axc_adamw_tensor *>(PyLong_AsVoidPtr(a[2]));
-    const at::Tensor like = tensor_of(a[3], "moments", false);            // its device is the parameters'
     const int type = int(PyLong_AsLong(a[4]));
     axc_adamw_desc d = {};
     d.type = type;
@@ -316,20 +315,34 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (!PyArg_ParseTuple(a[7], "dddf", &d.beta1, &d.beta2, &d.eps, &d.grad_scale)) throw Raised();
     const at::Tensor m = tensor_of(a[3], "moments", false), v = tensor_of(a[8], "moments", false), ms = tensor_of(a[9], "scales", true),
                      vs = tensor_of(a[10], "scales", true);
-    d.exp_avg = out_address(m);
-    d.exp_avg_sq = out_address(v);
-    d.exp_avg_scale = static_cast<float *>(out_address(ms));
-    d.exp_avg_sq_scale = static_cast<float *>(out_address(vs));
     if (PyErr_Occurred()) throw Raised();
     const Py_ssize_t count = PyList_GET_SIZE(a[0]);
     const bool given = a[1] != Py_None;
     if (given && PyList_GET_SIZE(a[1]) != count)
         invalid(std::to_string(PyList_GET_SIZE(a[1])) + " gradients for " + std::to_string(count) + " parameters");
-    const int device = like.device().index();
+    const int device = m.device().index();                                // the parameters'
     std::vector<at::Tensor> copies;
     auto fits = [&](const at::Tensor &t, const char *what) {
         if (!t.is_cuda() || t.device().index() != device || type_of(t) != type) invalid(std::string("every ") + what + " must be a tensor of the optimizer's type and device");
     };
+    // the moments are attributes that a caller can replace: they are what the kernels take them for, or nothing is launched
+    int64_t blocks = 0;
+    for (Py_ssize_t i = 0; i < count; ++i) blocks += table[i].count / AXC_ADAMW_BLOCK + (table[i].count % AXC_ADAMW_BLOCK != 0);
+    auto holds = [&](const at::Tensor &t, int64_t values, at::ScalarType scalar) {
+        if (!t.defined() || !t.is_cuda() || t.device().index() != device || t.scalar_type() != scalar || t.numel() != values || !t.is_contiguous())
+            invalid("the optimizer's moments are not the tensors that it made");
+    };
+    const at::ScalarType state = d.state_bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+    holds(m, blocks * AXC_ADAMW_BLOCK, state);
+    holds(v, blocks * AXC_ADAMW_BLOCK, state);
+    if (d.state_bits == 8) {
+        holds(ms, blocks, at::kFloat);
+        holds(vs, blocks, at::kFloat);
+    }
+    d.exp_avg = out_address(m);
+    d.exp_avg_sq = out_address(v);
+    d.exp_avg_scale = static_cast<float *>(out_address(ms));
+    d.exp_avg_sq_scale = static_cast<float *>(out_address(vs));
     for (Py_ssize_t i = 0; i < count; ++i) {
         const at::Tensor p = tensor_of(PyList_GET_ITEM(a[0], i), "parameter", false);
         fits(p, "parameter");
@@ -349,7 +362,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
         }
         table[i].grad = g.const_data_ptr();
     }
-    check(g_entry.adamw(&d, table, int32_t(count), device, stream_of(like)), "AdamW");
+    check(g_entry.adamw(&d, table, int32_t(count), device, stream_of(m)), "AdamW");
     // a graph that saved a parameter's value from before the step is refused its backward pass
     for (Py_ssize_t i = 0; i < count; ++i) {
         const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(a[0], i));
