@@ -54,6 +54,9 @@ class AdamW:
         for p in self.params:
             if not isinstance(p, torch.Tensor) or p.dtype is not self.dtype or p.device != self.device or not p.is_contiguous():
                 raise InvalidArgumentError("every parameter must be a contiguous %s tensor on %s" % (self.dtype, self.device))
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(begin < end for (begin, _), (_, end) in zip(spans[1:], spans)):
+            raise InvalidArgumentError("parameters share memory: a step would change it twice at the same time")
         self._counts = [p.numel() for p in self.params]
         n, blocks = len(self.params), C.c_int64()
         raise_for_status(_lib.load().axc_adamw_state_blocks((C.c_int64 * n)(*self._counts), n, C.byref(blocks)), "AdamW")
