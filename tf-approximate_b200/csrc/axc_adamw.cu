@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <float.h>
 
 #include <type_traits>
 
@@ -56,10 +57,12 @@ __device__ __forceinline__ float reciprocal(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float reciprocal_root(float x)
+// also of a value below the normal ones, and inf of inf: a gradient whose square leaves fp32's range still steps as the formula has it (2^29 bf16 values
+// with 8-bit moments: 1235 us, 1195 with the root that takes values below the normal ones for 0)
+__device__ __forceinline__ float square_root(float x)
 {
     float r;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -212,17 +215,18 @@ struct Part {
     __device__ __forceinline__ void moments(const AdamwTable<CAP> &tab, int n, int i, Two &m1, Two &v1) const
     {
         const Two minus(-1.0f), gi = mul2(Two(to_float(g[n].t[i]), to_float(g[n].t[i + 1])), Two(tab.grad_scale));
-        Two m0, v0;
+        Two m0, v0, v0_finite;
         if constexpr (BITS == 32) {
             m0 = Two(m[n].t[i], m[n].t[i + 1]);
             v0 = Two(v[n].t[i], v[n].t[i + 1]);
+            v0_finite = Two(fminf(v[n].t[i], FLT_MAX), fminf(v[n].t[i + 1], FLT_MAX));          // what is infinite stays so
         } else {
             m0 = decode<V>(m[n], i / 2, Two(m_scale));
             v0 = decode<V>(v[n], i / 2, Two(v_scale));
-            v0 = mul2(v0, v0);
+            v0_finite = v0 = mul2(v0, v0);
         }
         m1 = add2(m0, mul2(Two(tab.c1), fma2(m0, minus, gi)));
-        v1 = add2(v0, mul2(Two(tab.c2), fma2(v0, minus, mul2(gi, gi))));
+        v1 = add2(v0, mul2(Two(tab.c2), fma2(v0_finite, minus, mul2(gi, gi))));
     }
 
     template <int CAP>
@@ -239,9 +243,8 @@ struct Part {
             for (int i = 0; i < V; i += 2) {
                 Two m1, v1;
                 moments(tab, n, i, m1, v1);
-                // v rsqrt(v): 0 for 0, and not above the root where v has no normal reciprocal root
                 const float2 vf = v1.both();
-                const Two root = mul2(v1, Two(reciprocal_root(fmaxf(vf.x, 1.17549435e-38f)), reciprocal_root(fmaxf(vf.y, 1.17549435e-38f))));
+                const Two root(square_root(vf.x), square_root(vf.y));
                 const float2 den = fma2(root, inv_root, eps).both();
                 const Two p1 = fma2(mul2(m1, move), Two(reciprocal(den.x), reciprocal(den.y)), mul2(Two(to_float(p[n].t[i]), to_float(p[n].t[i + 1])), keep));
                 const float2 xf = p1.both(), mf = m1.both(), rf = root.both();
