@@ -20,8 +20,8 @@ __device__ __forceinline__ float slope_of(float kept)
     if (ACT == kActGelu) {
         if (EXACT) return 0.5f * (1.0f + erff(kept * 0.70710678f)) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
         float bell;
-        const float e = erf_16bit(kept * 0.70710678f, bell);
-        return fmaf(0.5f, e, fmaf(kept * bell, 0.39894228f, 0.5f));
+        const float below = normal_16bit(kept, bell);
+        return fmaf(kept * bell, 0.39894228f, below);
     }
     const float s = reciprocal(1.0f + __expf(-kept));
     return s * fmaf(kept, 1.0f - s, 1.0f);

@@ -91,14 +91,17 @@ __device__ __forceinline__ float reciprocal(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// erf as Abramowitz and Stegun's 7.1.26 has it: 1.5e-7 off at most, which no 16-bit result shows, at a third of the cost of erff;
-// and exp(-x^2), which it is made of
-__device__ __forceinline__ float erf_16bit(float x, float &bell)
+// For 16-bit results: Phi(z), the normal distribution below z, and bell = exp(-z^2 / 2), which it is made of.  The smaller side, erfc(|z| / sqrt 2) / 2,
+// is bell times a polynomial in t = 1 / (1 + 0.435 |z| / sqrt 2), as Hastings has it, with coefficients of its own: the least largest RELATIVE error for
+// |z| up to 13 (an exchange over 20 000 points: 3.7e-6, one more with the operations' rounding), so that GELU's tail, which is
+// that side times z, is as good as the rest.  A third of the cost of erff.
+__device__ __forceinline__ float normal_16bit(float z, float &bell)
 {
-    const float a = fabsf(x), t = reciprocal(fmaf(0.3275911f, a, 1.0f));
-    bell = __expf(-a * a);
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    return copysignf(fmaf(-poly, bell, 1.0f), x);
+    const float a = fabsf(z), t = reciprocal(fmaf(0.30759144f, a, 1.0f));
+    bell = __expf(-0.5f * a * a);
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.0758679435f, 0.191902518f), 0.00506413169f), 0.137423128f), 0.118498363f), 0.122977965f);
+    const float side = poly * bell;
+    return z < 0.0f ? side : 1.0f - side;
 }
 
 // bf16 term `p` of three of x, and in `rest` what is left of x for the terms after it.  A value beyond bf16's range keeps its largest finite
@@ -149,7 +152,7 @@ __device__ __forceinline__ float activate(float z, int act, bool exact)
 {
     if (act == kActRelu) return max_keep_nan(z, 0.0f);
     float bell;
-    if (act == kActGelu) return 0.5f * z * (1.0f + (exact ? erff(z * 0.70710678f) : erf_16bit(z * 0.70710678f, bell)));
+    if (act == kActGelu) return exact ? 0.5f * z * (1.0f + erff(z * 0.70710678f)) : z * normal_16bit(z, bell);
     if (act == kActSilu) return z * reciprocal(1.0f + __expf(-z));
     return z;
 }
