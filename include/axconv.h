@@ -430,6 +430,8 @@ int axc_debug_bounds_record(int device, uint32_t out4[4]);
  * tables in global memory, and the convolution); negative: the built-in limit of about a second.  With 0 every wait runs
  * out at once: the kernels finish, the outputs are not valid, and axc_conv2d_plan_info reports status 3. */
 int axc_debug_wait_polls(int device, int32_t expand, int32_t convolution);
+/* The same for the waits of the matrix kernels (dense layer, cross entropy), whose status axc_matrix_status reads. */
+int axc_debug_matrix_wait_polls(int device, int32_t polls);
 
 /* Measures what one SM sustains in conflict-free 16-bit shared-memory loads - the operation a table MAC of the
  * dense kernels costs (the reference does the same lookup through a texture fetch,

@@ -768,6 +768,22 @@ int axc_debug_wait_polls(int device, int32_t expand, int32_t convolution)
 #endif
 }
 
+int axc_debug_matrix_wait_polls(int device, int32_t polls)
+{
+#ifndef AXC_BOUNDS_CHECK
+    (void)device; (void)polls;
+    return AXC_UNIMPLEMENTED;
+#else
+    int prev = 0;
+    AXC_CUDA(cudaGetDevice(&prev));
+    if (prev != device) AXC_CUDA(cudaSetDevice(device));
+    cudaError_t e = cudaDeviceSynchronize();
+    const int rc = e == cudaSuccess ? axc::set_matrix_wait_polls(polls) : axc::cuda_failed(e);
+    if (prev != device) cudaSetDevice(prev);
+    return rc;
+#endif
+}
+
 int axc_quant_props(float min_value, float max_value, float out3[3])
 {
     if (!out3) return AXC_INVALID_ARGUMENT;

@@ -39,6 +39,14 @@ constexpr unsigned kSmem = 227 * 1024;
 constexpr int kMaxStages = 12;
 constexpr int kSegment = 64;                   // columns whose exponentials share a largest logit
 
+// Polls after which a wait gives up.  The debug flavour reads them from device memory, so that a test can make the waits run out.
+#ifdef AXC_BOUNDS_CHECK
+__device__ int g_wait_polls = mma::kWaitPolls;
+#define AXC_MATRIX_POLLS (*(volatile int *)&g_wait_polls)
+#else
+#define AXC_MATRIX_POLLS mma::kWaitPolls
+#endif
+
 enum { kStore = 0, kPartial = 1, kEntropy = 2, kGradient = 3 };
 
 struct GemmArgs {
@@ -406,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     // a wait runs out after a second, not before this; the word behind the status counts what a later kernel has done
     if (P.first && blockIdx.x == 0 && threadIdx.x == 0) P.status[0] = P.status[1] = 0u;
     bool ok = true;
+    const int polls = AXC_MATRIX_POLLS;
 
     // The loading and the multiplying warp run as a whole and one of their threads acts, so that what it hands over is computed once for
     // the warp: with a branch around the loop the 4 matrix instructions of a stage took 660 clocks instead of 512, the issuing thread's own.
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             const int k0 = int((long long)P.k_steps * split / P.splits), k1 = int((long long)P.k_steps * (split + 1) / P.splits);
             const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
             for (int k = k0; k < k1; ++k) {
-                if (!(ok = mma::barrier_wait(empty + 8 * s, phase))) break;
+                if (!(ok = mma::barrier_wait(empty + 8 * s, phase, polls))) break;
                 if (leader) {
                     if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
                     unsigned at = ring + unsigned(s) * stage_bytes;
@@ -456,10 +465,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             for (int k = k0; k < k1; ++k) {
                 const bool opens = CLOSE ? ((k - k0) & (run - 1)) == 0 : k == k0, closes = k + 1 == k1 || (CLOSE && ((k - k0) & (run - 1)) == run - 1);
                 if (opens) {
-                    if (!(ok = mma::barrier_wait(sums_empty + 8 * buffer, sums_phase))) break;
+                    if (!(ok = mma::barrier_wait(sums_empty + 8 * buffer, sums_phase, polls))) break;
                     d = tmem + unsigned(buffer) * kColumns;
                 }
-                if (!(ok = mma::barrier_wait(full + 8 * s, phase))) break;
+                if (!(ok = mma::barrier_wait(full + 8 * s, phase, polls))) break;
                 mma::fence_after();
                 const unsigned at = (ring + unsigned(s) * stage_bytes) >> 4, plane = (P.a_bytes + P.b_bytes) >> 4;
                 if (leader) {
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int i = 0; i < W; ++i) sum[c][i] = 0u;
                 for (int k = k0; k < k1; k += run) {
-                    if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
+                    if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase, polls))) break;
                     mma::fence_after();
                     __syncwarp();
                     if (half < kHalves) {
@@ -537,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                     for (int c = 0; c < kMine / W; ++c) take(sum[c], c * W);
                 }
             } else {
-                if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase))) break;
+                if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase, polls))) break;
                 mma::fence_after();
                 __syncwarp();
                 if (half < kHalves) {
@@ -744,6 +753,15 @@ int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, Gem
 }
 
 }  // namespace
+
+#ifdef AXC_BOUNDS_CHECK
+int set_matrix_wait_polls(int polls)
+{
+    const int value = polls < 0 ? mma::kWaitPolls : polls;
+    AXC_CUDA(cudaMemcpyToSymbol(g_wait_polls, &value, sizeof(value)));
+    return AXC_OK;
+}
+#endif
 
 int finish_parts(const Parts &parts, long long lines, long long columns, const Finish &f, const DeviceInfo &di, Queue &q)
 {

@@ -50,10 +50,10 @@ __device__ __forceinline__ void barrier_arrive_cluster(unsigned bar)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The whole warp waits for the phase `parity`; false, in all its threads, when it did not come within the limit.
-__device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity)
+// The whole warp waits for the phase `parity`; false, in all its threads, when it did not come within `polls`.
+__device__ __forceinline__ bool barrier_wait(unsigned bar, unsigned parity, int polls)
 {
-    for (int it = 0; it < kWaitPolls; ++it) {
+    for (int it = 0; it < polls; ++it) {
         unsigned done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
