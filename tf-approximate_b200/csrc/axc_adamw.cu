@@ -48,6 +48,7 @@ struct AdamwTable {
     void *m, *v;
     float *m_scale, *v_scale;
     AdamwEntry entry[CAP];
+    unsigned state_blocks;                     // of the moments of all tensors
 };
 constexpr int kSmallTable = 96, kLargeTable = 800;
 
@@ -118,10 +119,11 @@ union Packed {
     T t[V];
     __device__ Packed() {}
 };
+// (`left`: how many there are from `at` on)
 template <typename T, int V>
 __device__ __forceinline__ void load_values(const T *at, bool vec, long long left, Packed<T, V> &x)
 {
-    if (vec) x.w = __ldcs(reinterpret_cast<const typename Word<V * sizeof(T)>::type *>(at));
+    if (vec && AXC_GLOBAL_OK(V - 1, left, 481u)) x.w = __ldcs(reinterpret_cast<const typename Word<V * sizeof(T)>::type *>(at));
     else {
 #pragma unroll
         for (int i = 0; i < V; ++i) x.t[i] = i < left ? at[i] : T(0);
@@ -133,7 +135,7 @@ __device__ __forceinline__ void store_values(T *at, bool vec, long long left, co
     Packed<T, V> u;
 #pragma unroll
     for (int i = 0; i < V; ++i) u.t[i] = from_float<T>(x[i]);
-    if (vec) __stcs(reinterpret_cast<typename Word<V * sizeof(T)>::type *>(at), u.w);
+    if (vec && AXC_GLOBAL_OK(V - 1, left, 482u)) __stcs(reinterpret_cast<typename Word<V * sizeof(T)>::type *>(at), u.w);
     else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -149,8 +151,9 @@ __device__ __forceinline__ Two decode(const Packed<uint8_t, V> &codes, int i, Tw
     return mul2(Two(f.x, f.y), scale);
 }
 template <int V>
-__device__ __forceinline__ void store_codes(uint8_t *at, const float (&x)[V])
+__device__ __forceinline__ void store_codes(uint8_t *at, long long left, const float (&x)[V])
 {
+    if (!AXC_GLOBAL_OK(V - 1, left, 483u)) return;
     union { typename Word<V>::type w; __nv_fp8x2_storage_t c[V / 2]; } u;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) u.c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
@@ -183,12 +186,16 @@ struct Part {
     long long left;                            // values of the tensor from the block's first on; 0: a tensor without a gradient
     bool vec;
 
+    // values of the moments from block b on
+    template <int CAP>
+    static __device__ __forceinline__ long long in_state(const AdamwTable<CAP> &tab, unsigned b) { return ((long long)tab.state_blocks - b) * kBlock; }
+
     template <int CAP>
     __device__ __forceinline__ void load(const AdamwTable<CAP> &tab, int at, unsigned b, int lane)
     {
         const AdamwEntry &e = tab.entry[at];
         const long long first = (long long)(b - e.first) * kBlock;
-        left = e.count - first;
+        left = AXC_GLOBAL_OK(at, tab.count, 486u) ? e.count - first : 0;
         param = static_cast<T *>(e.param) + first;
         grad = static_cast<const T *>(e.grad) + first;
         decay = e.decay;
@@ -201,12 +208,14 @@ struct Part {
             const int i = (n * 32 + lane) * V;
             load_values<T, V>(grad + i, vec, left - i, g[n]);
             load_values<T, V>(param + i, vec, left - i, p[n]);
-            load_values<State, V>(ms + i, true, 0, m[n]);
-            load_values<State, V>(vs + i, true, 0, v[n]);
+            load_values<State, V>(ms + i, true, in_state(tab, b) - i, m[n]);
+            load_values<State, V>(vs + i, true, in_state(tab, b) - i, v[n]);
         }
         if constexpr (BITS == 8) {
-            m_scale = tab.m_scale[b];
-            v_scale = tab.v_scale[b];
+            if (AXC_GLOBAL_OK(b, tab.state_blocks, 485u)) {
+                m_scale = tab.m_scale[b];
+                v_scale = tab.v_scale[b];
+            }
         }
     }
 
@@ -265,8 +274,9 @@ struct Part {
         if constexpr (BITS == 32) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                store_values<float, V>(ms + (n * 32 + lane) * V, true, 0, first[n]);
-                store_values<float, V>(vs + (n * 32 + lane) * V, true, 0, second[n]);
+                const int i = (n * 32 + lane) * V;
+                store_values<float, V>(ms + i, true, in_state(tab, b) - i, first[n]);
+                store_values<float, V>(vs + i, true, in_state(tab, b) - i, second[n]);
             }
         } else {
             // a scale below the smallest normal number has no reciprocal: the block's moments are then zeros
@@ -294,8 +304,8 @@ struct Part {
                 for (int n = 0; n < N; ++n) {
                     const int at = (n * 32 + lane) * V;
                     load_values<T, V>(grad + at, vec, left - at, g[n]);
-                    load_values<State, V>(ms + at, true, 0, m[n]);
-                    load_values<State, V>(vs + at, true, 0, v[n]);
+                    load_values<State, V>(ms + at, true, in_state(tab, b) - at, m[n]);
+                    load_values<State, V>(vs + at, true, in_state(tab, b) - at, v[n]);
                 }
 #pragma unroll
                 for (int n = 0; n < N; ++n)
@@ -313,10 +323,11 @@ struct Part {
             }
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                store_codes<V>(ms + (n * 32 + lane) * V, first[n]);
-                store_codes<V>(vs + (n * 32 + lane) * V, second[n]);
+                const int i = (n * 32 + lane) * V;
+                store_codes<V>(ms + i, in_state(tab, b) - i, first[n]);
+                store_codes<V>(vs + i, in_state(tab, b) - i, second[n]);
             }
-            if (lane == 0) {
+            if (lane == 0 && AXC_GLOBAL_OK(b, tab.state_blocks, 484u)) {
                 tab.m_scale[b] = m_new;
                 tab.v_scale[b] = r_new;
             }
@@ -361,7 +372,7 @@ void launch_adamw(const AdamwTable<CAP> &tab, int type, int bits, cudaStream_t s
 
 // The tensors in as many launches as their tables need.
 template <int CAP>
-void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t count, cudaStream_t stream)
+void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t count, int64_t blocks, cudaStream_t stream)
 {
     const double root = sqrt(1.0 - pow(d.beta2, double(d.step))), first_left = 1.0 - pow(d.beta1, double(d.step));
     long long block = 0;
@@ -377,6 +388,7 @@ void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t
         tab.m_scale = d.exp_avg_scale;
         tab.v_scale = d.exp_avg_sq_scale;
         tab.base = tab.blocks = 0;
+        tab.state_blocks = unsigned(blocks);
         tab.count = 0;
         for (; at < count && tab.count < CAP; ++at) {
             const long long first = block;
@@ -398,6 +410,9 @@ void run_adamw(const axc_adamw_desc &d, const axc_adamw_tensor *tensors, int32_t
 }
 
 }  // namespace
+
+AXC_DEFINE_BOUNDS_READER(bounds_record_adamw)
+
 }  // namespace axc
 
 extern "C" int axc_adamw_state_blocks(const int64_t *counts, int32_t tensors, int64_t *blocks)
@@ -438,8 +453,8 @@ extern "C" int axc_adamw_step(const axc_adamw_desc *desc, const axc_adamw_tensor
     int prev = 0;
     AXC_CUDA(cudaGetDevice(&prev));
     if (prev != device) AXC_CUDA(cudaSetDevice(device));
-    if (count <= kSmallTable) run_adamw<kSmallTable>(d, tensors, count, cudaStream_t(stream));
-    else run_adamw<kLargeTable>(d, tensors, count, cudaStream_t(stream));
+    if (count <= kSmallTable) run_adamw<kSmallTable>(d, tensors, count, blocks, cudaStream_t(stream));
+    else run_adamw<kLargeTable>(d, tensors, count, blocks, cudaStream_t(stream));
     const cudaError_t e = cudaGetLastError();
     if (prev != device) cudaSetDevice(prev);
     return e == cudaSuccess ? AXC_OK : cuda_failed(e);

@@ -736,15 +736,16 @@ int axc_debug_bounds_record(int device, uint32_t out4[4])
     AXC_CUDA(cudaGetDevice(&prev));
     if (prev != device) AXC_CUDA(cudaSetDevice(device));
     cudaError_t e = cudaDeviceSynchronize();
-    unsigned parts[4][4] = {};
+    int (*const readers[])(unsigned[4]) = {axc::bounds_record_sched, axc::bounds_record_conv, axc::bounds_record_depthwise, axc::bounds_record_xtab,
+                                           axc::bounds_record_adamw, axc::bounds_record_gemm, axc::bounds_record_dense, axc::bounds_record_rows,
+                                           axc::bounds_record_entropy};
+    constexpr int kParts = int(sizeof(readers) / sizeof(readers[0]));
+    unsigned parts[kParts][4] = {};
     int rc = e == cudaSuccess ? AXC_OK : axc::cuda_failed(e);
-    if (rc == AXC_OK) rc = axc::bounds_record_sched(parts[0]);
-    if (rc == AXC_OK) rc = axc::bounds_record_conv(parts[1]);
-    if (rc == AXC_OK) rc = axc::bounds_record_depthwise(parts[2]);
-    if (rc == AXC_OK) rc = axc::bounds_record_xtab(parts[3]);
+    for (int t = 0; t < kParts && rc == AXC_OK; ++t) rc = readers[t](parts[t]);
     if (prev != device) cudaSetDevice(prev);
     out4[0] = out4[1] = out4[2] = out4[3] = 0;
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < kParts; ++t) {
         if (parts[t][0] != 0 && out4[0] == 0) { out4[1] = parts[t][1]; out4[2] = parts[t][2]; out4[3] = parts[t][3]; }
         out4[0] += parts[t][0];
     }

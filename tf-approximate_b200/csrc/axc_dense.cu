@@ -35,19 +35,33 @@ union Group {                                  // 16 bytes of values
     __device__ Group() {}
 };
 
-// V columns of a row: neighbours at `at`, or 32 apart, those below `left`
+// V columns of a row: neighbours at `at`, or 32 apart, those below `left`.  base, count: all there is (debug flavour).
 template <bool VEC, typename T>
-__device__ __forceinline__ void load_group(const T *at, long long left, Group<T> &g)
+__device__ __forceinline__ void load_group(const T *at, long long left, Group<T> &g, const T *base, long long count)
 {
-    if (VEC) g.w = __ldcs(reinterpret_cast<const uint4 *>(at));
-    else {
+    if (VEC) {
+        if (AXC_VALUES_OK(at, Group<T>::V, base, count, 401u)) g.w = __ldcs(reinterpret_cast<const uint4 *>(at));
+        else g.w = make_uint4(0u, 0u, 0u, 0u);
+    } else {
 #pragma unroll
-        for (int i = 0; i < Group<T>::V; ++i) g.t[i] = 32 * i < left ? at[32 * i] : narrow<T>(0.0f);
+        for (int i = 0; i < Group<T>::V; ++i) g.t[i] = 32 * i < left && AXC_VALUES_OK(at + 32 * i, 1, base, count, 402u) ? at[32 * i] : narrow<T>(0.0f);
+    }
+}
+// The same way out
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_group(T *at, long long left, const Group<T> &g, const T *base, long long count)
+{
+    if (VEC) {
+        if (AXC_VALUES_OK(at, Group<T>::V, base, count, 403u)) *reinterpret_cast<uint4 *>(at) = g.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < Group<T>::V; ++i)
+            if (32 * i < left && AXC_VALUES_OK(at + 32 * i, 1, base, count, 404u)) at[32 * i] = g.t[i];
     }
 }
 
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part)
+__global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *part, long long part_values)
 {
     after_previous();
     constexpr int V = Group<T>::V, kRows = (ACT == kActNone ? 8 : 4) / (VEC ? 1 : 2), kApart = VEC ? 1 : 32;
@@ -65,8 +79,8 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
                 const int step = r + 8 * q < end ? 8 * q : 0;      // behind the last row: the first one again, not used
-                load_group<VEC>(dy + step * S.dy_line, left, g[q]);
-                if constexpr (ACT != kActNone) load_group<VEC>(kept + step * S.columns, left, k[q]);
+                load_group<VEC>(dy + step * S.dy_line, left, g[q], static_cast<const T *>(S.dy), S.dy_values());
+                if constexpr (ACT != kActNone) load_group<VEC>(kept + step * S.columns, left, k[q], static_cast<const T *>(S.kept), S.tensor_values());
             }
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
@@ -77,7 +91,7 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                 for (int i = 0; i < V; ++i) d[i] = widen(g[q].t[i]);
                 for (int p = 1; p < S.dy_planes; ++p) {
                     Group<T> more;
-                    load_group<VEC>(dy + 8 * q * S.dy_line + p * S.plane, left, more);
+                    load_group<VEC>(dy + 8 * q * S.dy_line + p * S.plane, left, more, static_cast<const T *>(S.dy), S.dy_values());
 #pragma unroll
                     for (int i = 0; i < V; ++i) d[i] += widen(more.t[i]);
                 }
@@ -91,24 +105,9 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                     Group<T> u;
 #pragma unroll
                     for (int i = 0; i < V; ++i) u.t[i] = narrow<T>(d[i]);
-                    T *to = static_cast<T *>(S.same) + row * S.columns + c;
-                    if (S.same) {
-                        if (VEC) *reinterpret_cast<uint4 *>(to) = u.w;
-                        else {
-#pragma unroll
-                            for (int i = 0; i < V; ++i)
-                                if (32 * i < left) to[32 * i] = u.t[i];
-                        }
-                    }
-                    T *operand = reinterpret_cast<T *>(S.planes) + row * S.line + c;
-                    if (S.planes && sizeof(T) == 2) {
-                        if (VEC) *reinterpret_cast<uint4 *>(operand) = u.w;
-                        else {
-#pragma unroll
-                            for (int i = 0; i < V; ++i)
-                                if (32 * i < left) operand[32 * i] = u.t[i];
-                        }
-                    }
+                    T *same = static_cast<T *>(S.same), *operand = reinterpret_cast<T *>(S.planes);
+                    if (S.same) store_group<VEC>(same + row * S.columns + c, left, u, same, S.tensor_values());
+                    if (S.planes && sizeof(T) == 2) store_group<VEC>(operand + row * S.line + c, left, u, operand, S.operand_values());
                 }
                 if (S.planes && sizeof(T) == 4) {
                     uint16_t *to = S.planes + row * S.line + c;
@@ -117,11 +116,12 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                         union { uint2 w; uint16_t h[4]; } u;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) u.h[i] = split_term(d[i], d[i], p);
-                        if (VEC) *reinterpret_cast<uint2 *>(to) = u.w;
-                        else {
+                        if (VEC) {
+                            if (AXC_VALUES_OK(to, 4, S.planes, 3 * S.operand_values(), 405u)) *reinterpret_cast<uint2 *>(to) = u.w;
+                        } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (32 * i < left) to[32 * i] = u.h[i];
+                                if (32 * i < left && AXC_VALUES_OK(to + 32 * i, 1, S.planes, 3 * S.operand_values(), 406u)) to[32 * i] = u.h[i];
                         }
                     }
                 }
@@ -137,30 +137,34 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
 #pragma unroll
         for (int k = 1; k < 8; ++k) s += sums[k][i];
         const long long column = (long long)blockIdx.x * 32 * V + i;
-        if (column < S.columns) part[(long long)blockIdx.y * S.columns + column] = s;
+        const long long at = (long long)blockIdx.y * S.columns + column;
+        if (column < S.columns && AXC_GLOBAL_OK(at, part_values, 407u)) part[at] = s;
     }
 }
 
-__global__ void __launch_bounds__(256) slope_sums_kernel(const float *part, long long columns, int shares, float scale, const float *scale_dev,
-                                                         void *sums, int type)
+__global__ void __launch_bounds__(256) slope_sums_kernel(const float *part, long long part_values, long long columns, int shares, float scale,
+                                                         const float *scale_dev, void *sums, int type)
 {
     after_previous();
     const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
     if (c >= columns) return;
     float s = 0.0f;
-    for (int k = 0; k < shares; ++k) s += part[k * columns + c];
+    for (int k = 0; k < shares; ++k)
+        if (AXC_GLOBAL_OK(k * columns + c, part_values, 408u)) s += part[k * columns + c];
     store_from_float(sums, c, type, s * scale * (scale_dev ? *scale_dev : 1.0f));
 }
 
 template <typename T, bool VEC>
-int launch_slope(const Slope &s, float *part, int shares, Queue &q)
+int launch_slope(const Slope &s, float *part, long long part_values, int shares, Queue &q)
 {
     const dim3 grid(unsigned((s.columns + 32 * Group<T>::V - 1) / (32 * Group<T>::V)), unsigned(shares));
     return launch(q, !s.kept ? slope_kernel<T, kActNone, VEC> : s.activation == kActRelu ? slope_kernel<T, kActRelu, VEC>
-                     : s.activation == kActGelu ? slope_kernel<T, kActGelu, VEC> : slope_kernel<T, kActSilu, VEC>, grid, 256, 0, 1, s, part);
+                     : s.activation == kActGelu ? slope_kernel<T, kActGelu, VEC> : slope_kernel<T, kActSilu, VEC>, grid, 256, 0, 1, s, part, part_values);
 }
 
 }  // namespace
+
+AXC_DEFINE_BOUNDS_READER(bounds_record_dense)
 
 int slope(const Slope &s, void *scratch, size_t room, Queue &q)
 {
@@ -168,16 +172,17 @@ int slope(const Slope &s, void *scratch, size_t room, Queue &q)
     if (s.sums && room < slope_scratch(s.rows, s.columns)) return AXC_INTERNAL;
     const int shares = column_shares(s.rows, s.columns);
     float *part = s.sums ? static_cast<float *>(scratch) : nullptr;
+    const long long values = (long long)(room / sizeof(float));
     // whole groups of 16 bytes, in every line of every tensor
     const uintptr_t all = reinterpret_cast<uintptr_t>(s.dy) | reinterpret_cast<uintptr_t>(s.kept) | reinterpret_cast<uintptr_t>(s.same);
     const long long size = s.type == kFloat32 ? 4 : 2;
     const bool vec = (all & 15u) == 0 && s.dy_line * size % 16 == 0 && (s.padded || s.columns * size % 16 == 0) && s.plane * size % 16 == 0;
     int rc;
-    if (s.type == kFloat32) rc = vec ? launch_slope<float, true>(s, part, shares, q) : launch_slope<float, false>(s, part, shares, q);
-    else if (s.type == kBfloat16) rc = vec ? launch_slope<__nv_bfloat16, true>(s, part, shares, q) : launch_slope<__nv_bfloat16, false>(s, part, shares, q);
-    else rc = vec ? launch_slope<__half, true>(s, part, shares, q) : launch_slope<__half, false>(s, part, shares, q);
+    if (s.type == kFloat32) rc = vec ? launch_slope<float, true>(s, part, values, shares, q) : launch_slope<float, false>(s, part, values, shares, q);
+    else if (s.type == kBfloat16) rc = vec ? launch_slope<__nv_bfloat16, true>(s, part, values, shares, q) : launch_slope<__nv_bfloat16, false>(s, part, values, shares, q);
+    else rc = vec ? launch_slope<__half, true>(s, part, values, shares, q) : launch_slope<__half, false>(s, part, values, shares, q);
     if (rc || !s.sums) return rc;
-    return launch(q, slope_sums_kernel, dim3(unsigned((s.columns + 255) / 256)), 256, 0, 1, part, s.columns, shares, s.scale, s.scale_dev, s.sums, s.sums_type);
+    return launch(q, slope_sums_kernel, dim3(unsigned((s.columns + 255) / 256)), 256, 0, 1, part, values, s.columns, shares, s.scale, s.scale_dev, s.sums, s.sums_type);
 }
 
 namespace {

@@ -111,7 +111,8 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
     const long long row = blockIdx.x;
     const float2 *stats = A.stats + row * A.segments;
     float top = -INFINITY;
-    for (int i = threadIdx.x; i < A.segments; i += 256) top = fmaxf(top, stats[i].x);
+    for (int i = threadIdx.x; i < A.segments; i += 256)
+        if (AXC_GLOBAL_OK(row * A.segments + i, A.rows * A.segments, 461u)) top = fmaxf(top, stats[i].x);
     top = block_max(top, shared);
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
     const int groups = FORM == 0 ? 0 : int(A.line / 8);
     for (int i = threadIdx.x; i < groups; i += 256) {
         const int c = i * 8;
+        if (!AXC_GLOBAL_OK(c / kSegment, A.segments, 462u) || !AXC_GLOBAL_OK(row * A.line + c + 7, A.rows * A.line, 463u)) continue;
         const float first = stats[c / kSegment].x;
         float factor = scale / sum;
         if (first != -INFINITY) factor *= __expf(first - base);
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
                     v[2 * j + 1] -= t.y;
                 }
             }
-            *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+            if (AXC_VALUES_OK(to, 8, A.gradient, A.rows * A.line + (FORM == 3 ? 2 : 0) * A.plane, 464u)) *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
     add_losses(A, shared);
@@ -189,6 +191,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
     bool nan = false;
     for (int c = threadIdx.x; c < classes; c += 256) {
         const float *at = A.parts.data + row * A.parts.line + c;
+        if (!AXC_GLOBAL_OK(c, kFewClasses, 465u) || !AXC_VALUES_OK(at + (A.parts.count - 1) * A.parts.stride, 1, A.parts.data, A.parts.count * A.parts.stride, 466u)) continue;
         float l = at[0];
         for (int i = 1; i < A.parts.count; ++i) l += at[i * A.parts.stride];
         if (A.bias) l += load_as_float(A.bias, c, A.bias_type);
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
                     v[2 * j + 1] -= t.y;
                 }
             }
-            *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+            if (AXC_VALUES_OK(to, 8, A.gradient, A.rows * A.line + (A.planes - 1) * A.plane, 467u)) *reinterpret_cast<uint4 *>(to) = make_uint4(u[0], u[1], u[2], u[3]);
         }
     }
     add_losses(A, shared);
@@ -456,6 +459,9 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
 }
 
 }  // namespace
+
+AXC_DEFINE_BOUNDS_READER(bounds_record_entropy)
+
 }  // namespace axc
 
 extern "C" int axc_entropy_workspace_bytes(const axc_entropy_desc *desc, const void *x, const void *kernel, int device, size_t *loss_only, size_t *gradients)

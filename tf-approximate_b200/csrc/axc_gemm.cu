@@ -81,33 +81,42 @@ struct Lines {
     unsigned stage;                            // the warp's shared memory
     int lane, rows;                            // rows of the 32 that exist
 };
+// What the lines are a part of (debug flavour)
+struct Whole {
+    const char *base;
+    long long bytes;
+};
 
 template <int N>
 __device__ __forceinline__ unsigned unit_at(unsigned stage, int row, int unit) { return stage + unsigned(row * N + (unit ^ (row & (N - 1)))) * 16u; }
 
 // Lines that do not start on 16 bytes: value by value, neighbouring lanes neighbouring ones, several on their way at a time.
 template <int N, typename Pointer, typename Move>
-__device__ __forceinline__ void single_values(const Lines &L, Pointer lines, long long line, int left, int size, Move move)
+__device__ __forceinline__ void single_values(const Lines &L, Pointer lines, long long line, int left, int size, const Whole &all, Move move)
 {
     const int in_row = N * 16 / size;          // a power of two, 8 to 64
 #pragma unroll 8
     for (int i = 0; i < in_row; ++i) {
         const int at = i * 32 + L.lane, r = at / in_row, b = (at & (in_row - 1)) * size;
-        if (r < L.rows && b < left) move(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), lines + r * line + b, size);
+        if (r < L.rows && b < left && AXC_VALUES_OK(lines + r * line + b, size, all.base, all.bytes, 431u) &&
+            AXC_SHARED_OK(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), unsigned(size), L.stage, L.stage + N * 512u, 432u))
+            move(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), lines + r * line + b, size);
     }
 }
 
 // `bytes`: how many of a row exist; aligned: all rows start on 16 bytes
 template <int M, int N>
-__device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M], char *out, long long line, int bytes, int size, bool aligned)
+__device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M], char *out, long long line, int bytes, int size, bool aligned, const Whole &all)
 {
 #pragma unroll
     for (int part = 0; part < M; part += N) {
         __syncwarp();
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int u = 0; u < N; ++u) {
+            if (!AXC_SHARED_OK(unit_at<N>(L.stage, L.lane, u), 16u, L.stage, L.stage + N * 512u, 433u)) continue;
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, L.lane, u)), "r"(q[part + u].x), "r"(q[part + u].y),
                          "r"(q[part + u].z), "r"(q[part + u].w) : "memory");
+        }
         __syncwarp();
         char *to = out + part * 16;
         const int left = bytes - part * 16;
@@ -117,10 +126,10 @@ __device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M],
                 const int r = (i * 32 + L.lane) / N, u = L.lane % N;
                 uint4 w;
                 asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(unit_at<N>(L.stage, r, u)));
-                if (r < L.rows) *reinterpret_cast<uint4 *>(to + r * line + u * 16) = w;
+                if (r < L.rows && AXC_VALUES_OK(to + r * line + u * 16, 16, all.base, all.bytes, 434u)) *reinterpret_cast<uint4 *>(to + r * line + u * 16) = w;
             }
         } else {
-            single_values<N>(L, to, line, left, size, [](unsigned from, char *at, int size) {
+            single_values<N>(L, to, line, left, size, all, [](unsigned from, char *at, int size) {
                 if (size == 2) {
                     unsigned short h;
                     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from));
@@ -137,7 +146,7 @@ __device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M],
 
 // The other way: M units of the lane's row, zeros where there is nothing.
 template <int M, int N>
-__device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const char *in, long long line, int bytes, int size, bool aligned)
+__device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const char *in, long long line, int bytes, int size, bool aligned, const Whole &all)
 {
 #pragma unroll
     for (int part = 0; part < M; part += N) {
@@ -149,11 +158,12 @@ __device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const 
             for (int i = 0; i < N; ++i) {
                 const int r = (i * 32 + L.lane) / N, u = L.lane % N;
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (r < L.rows) w = *reinterpret_cast<const uint4 *>(from + r * line + u * 16);
+                if (r < L.rows && AXC_VALUES_OK(from + r * line + u * 16, 16, all.base, all.bytes, 435u)) w = *reinterpret_cast<const uint4 *>(from + r * line + u * 16);
+                if (!AXC_SHARED_OK(unit_at<N>(L.stage, r, u), 16u, L.stage, L.stage + N * 512u, 436u)) continue;
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, r, u)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
             }
         } else {
-            single_values<N>(L, from, line, left, size, [](unsigned to, const char *at, int size) {
+            single_values<N>(L, from, line, left, size, all, [](unsigned to, const char *at, int size) {
                 if (size == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(*reinterpret_cast<const unsigned short *>(at)) : "memory");
                 else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<const unsigned *>(at)) : "memory");
             });
@@ -168,20 +178,21 @@ __device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const 
 
 __device__ __forceinline__ bool lines_aligned(const void *base, long long line_bytes) { return ((reinterpret_cast<uintptr_t>(base) | uintptr_t(line_bytes)) & 15u) == 0; }
 
-// W fp32 values of every lane's row, as `type`; columns n0 .. of n
+// W fp32 values of every lane's row, as `type`; columns n0 .. of n; values: all that there are from `base` on
 template <int W, int N>
-__device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], void *base, int type, long long line, int row0, int n0, int n)
+__device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], void *base, int type, long long line, int row0, int n0, int n, long long values)
 {
     const int size = type == kFloat32 ? 4 : 2, left = n - n0;
     char *out = static_cast<char *>(base) + (row0 * line + n0) * size;
     const bool aligned = lines_aligned(base, line * size);
     const int bytes = (left < W ? left : W) * size;
+    const Whole all = {static_cast<const char *>(base), values * size};
     if (type == kFloat32) {
         uint4 q[W / 4];
 #pragma unroll
         for (int i = 0; i < W / 4; ++i)
             q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
-        store_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, out, line * 4, bytes, 4, aligned);
+        store_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, out, line * 4, bytes, 4, aligned, all);
     } else {
         const bool bf16 = type == kBfloat16;
         uint4 q[W / 8];
@@ -189,7 +200,7 @@ __device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], v
         for (int i = 0; i < W / 8; ++i)
             q[i] = make_uint4(pack2(v[8 * i], v[8 * i + 1], bf16), pack2(v[8 * i + 2], v[8 * i + 3], bf16), pack2(v[8 * i + 4], v[8 * i + 5], bf16),
                               pack2(v[8 * i + 6], v[8 * i + 7], bf16));
-        store_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, out, line * 2, bytes, 2, aligned);
+        store_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, out, line * 2, bytes, 2, aligned, all);
     }
 }
 
@@ -202,7 +213,7 @@ struct ColumnValues {
 #pragma unroll
         for (int i = 0; i < (W < 32 ? 1 : W / 32); ++i) {
             const int c = n0 + 32 * i + lane;
-            mine[i] = values && c < n ? load_as_float(values, c, type) : 0.0f;
+            mine[i] = values && c < n && AXC_GLOBAL_OK(c, n, 437u) ? load_as_float(values, c, type) : 0.0f;
         }
     }
     __device__ __forceinline__ float column(int i) const { return __shfl_sync(0xffffffffu, mine[i / 32], i & 31); }
@@ -227,9 +238,10 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
         const int size = f.addend_type == kFloat32 ? 4 : 2, left = P.n - n0, bytes = (left < W ? left : W) * size;
         const char *in = static_cast<const char *>(f.addend) + ((long long)row0 * f.addend_line + n0) * size;
         const bool aligned = lines_aligned(f.addend, f.addend_line * size);
+        const Whole all = {static_cast<const char *>(f.addend), f.addend_values() * size};
         if (size == 4) {
             uint4 q[W / 4];
-            load_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, in, f.addend_line * 4, bytes, 4, aligned);
+            load_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, in, f.addend_line * 4, bytes, 4, aligned, all);
 #pragma unroll
             for (int i = 0; i < W / 4; ++i) {
                 v[4 * i] += __uint_as_float(q[i].x);
@@ -239,7 +251,7 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
             }
         } else {
             uint4 q[W / 8];
-            load_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, in, f.addend_line * 2, bytes, 2, aligned);
+            load_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, in, f.addend_line * 2, bytes, 2, aligned, all);
 #pragma unroll
             for (int i = 0; i < W / 8; ++i) {
                 const unsigned u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
@@ -253,7 +265,7 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
             }
         }
     }
-    if (f.pre) store_row<W, N>(L, v, f.pre, f.out_type, f.out_line, row0, n0, P.n);
+    if (f.pre) store_row<W, N>(L, v, f.pre, f.out_type, f.out_line, row0, n0, P.n, f.out_values());
     if (f.activation == kActRelu) {
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActRelu, exact);
@@ -269,7 +281,7 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActSilu, exact);
     }
-    store_row<W, N>(L, v, f.out, f.out_type, f.out_line, row0, n0, P.n);
+    store_row<W, N>(L, v, f.out, f.out_type, f.out_line, row0, n0, P.n, f.out_values());
 }
 
 // Partial sums in the order of the output's lines
@@ -281,7 +293,7 @@ __device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, un
     float v[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] = __uint_as_float(x[i]);
-    store_row<W, N>(L, v, part, kFloat32, P.part_line, row0, n0, P.n);
+    store_row<W, N>(L, v, part, kFloat32, P.part_line, row0, n0, P.n, (P.splits - split) * P.part_stride);
 }
 
 // One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
@@ -308,7 +320,7 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &
     for (int i = 4; i < 64; ++i) top4[i & 3] = max_keep_nan(top4[i & 3], v[i]);
     const float top = max_keep_nan(max_keep_nan(top4[0], top4[1]), max_keep_nan(top4[2], top4[3]));
     label -= n0;
-    if (row < P.m && label >= 0 && label < kSegment && n0 + label < P.n) {
+    if (row < P.m && label >= 0 && label < kSegment && n0 + label < P.n && AXC_GLOBAL_OK(row, P.m, 438u)) {
         float mine = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 64; ++i) mine = fmaxf(mine, i == int(label) ? v[i] : -INFINITY);
@@ -321,8 +333,9 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &
         v[i] = __expf(v[i] - base);
         sum4[i & 3] += v[i];
     }
-    if (row < P.m) e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
-    if (e.keep) store_row<64, N>(L, v, e.keep, e.keep_fp32 ? kFloat32 : kFloat16, e.line, row0, n0, int(e.line));
+    if (row < P.m && AXC_GLOBAL_OK((long long)row * e.segments + n0 / kSegment, (long long)P.m * e.segments, 439u))
+        e.stats[(long long)row * e.segments + n0 / kSegment] = make_float2(top, (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+    if (e.keep) store_row<64, N>(L, v, e.keep, e.keep_fp32 ? kFloat32 : kFloat16, e.line, row0, n0, int(e.line), P.m * e.line);
 }
 
 // W logits of a row and what the loss's gradient is there: row_scale * (exp(logit - largest) / sum - [label])
@@ -353,7 +366,7 @@ __device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines 
     uint16_t *keep = static_cast<uint16_t *>(e.keep);
     const int type = (P.shape >> 7 & 1) ? kBfloat16 : kFloat16;
     for (int plane = 0; plane < P.planes; ++plane) {
-        store_row<W, N>(L, v, keep, type, e.line, row0, n0, int(e.line));
+        store_row<W, N>(L, v, keep, type, e.line, row0, n0, int(e.line), P.m * e.line);
         if (P.planes == 3) {
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
@@ -434,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 if (leader) {
                     if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
                     unsigned at = ring + unsigned(s) * stage_bytes;
-                    for (int p = 0; p < PLANES; ++p) {
+                    // (a stage that is not loaded runs the waits out)
+                    for (int p = 0; p < PLANES && AXC_SHARED_OK(at, 1024u, ring, ring + unsigned(P.stages) * stage_bytes, 440u); ++p) {
                         if (P.a_rows) {
                             for (int r = 0; r < 128; r += 64) mma::load_box<CG>(at + unsigned(r) * 128u, &P.map_a, signal + 8 * s, row_a + r, k * kStageK, p);
                         } else mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kStageK, row_a, p);
@@ -593,6 +607,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float *part, long lon
         const long long line = i / quads;
         const int c = int(i - line * quads) * 4;
         const float *at = part + line * part_line + c;
+        if (!AXC_VALUES_OK(at + (splits > 0 ? splits - 1 : 0) * stride, splits > 0 ? 4 : 0, part, splits * stride, 426u)) continue;
         float4 s = splits > 0 ? *reinterpret_cast<const float4 *>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int k = 1; k < splits; ++k) {
@@ -743,7 +758,7 @@ int fill_args(const Gemm &g, const Plan &plan, unsigned *status, bool first, Gem
     P->a_bytes = 128 * 128;
     P->b_bytes = (b.rows_contiguous && b_rows_per_cta < 64 ? 64u : b_rows_per_cta) * 128u;
     P->shape = mma::instruction_shape(128 * plan.cg, plan.bn, g.bf16, a.rows_contiguous, b.rows_contiguous);
-    P->fin = g.fin;
+    P->fin = sized(g.fin, g.m, g.n);
     P->status = status;
     P->first = first;
     P->run = P->k_steps <= 24 ? 4 : 8;
@@ -767,8 +782,10 @@ int finish_parts(const Parts &parts, long long lines, long long columns, const F
 {
     const long long work = ceil_div(lines * ceil_div(columns, 4), 256), most = (long long)di.sm_count * 8;
     return launch(q, finish_kernel, dim3(unsigned(work < most ? work : most)), 256, 0, 1, parts.data, parts.stride, parts.line, parts.count, int(lines),
-                  int(columns), f);
+                  int(columns), sized(f, lines, columns));
 }
+
+AXC_DEFINE_BOUNDS_READER(bounds_record_gemm)
 
 size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di)
 {
@@ -852,6 +869,10 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const Layout one, const La
         const long long o = i / groups, c = (i - o * groups) * 8;
         uint16_t *to = m.dst + o * m.line + c;
         const long long from = o * m.outer_stride + c * m.inner_stride;
+        [[maybe_unused]] const long long values = (m.outer - 1) * m.outer_stride + (m.inner - 1) * m.inner_stride + 1;
+        if (!AXC_GLOBAL_OK(from + ((c + 8 < m.inner ? c + 8 : m.inner) - 1 - c) * m.inner_stride, values, 424u) ||
+            !AXC_GLOBAL_OK(o * m.line + c + 7 + (m.split ? 2 : 0) * m.plane, m.outer * m.line * (m.split ? 3 : 1), 425u))
+            continue;
         union { uint16_t h[8]; uint4 w; } out[3];
         if (m.split) {
             const float *src = static_cast<const float *>(m.src) + from;

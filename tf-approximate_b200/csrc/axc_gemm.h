@@ -145,7 +145,16 @@ struct Finish {
     int out_type;
     long long out_line;
     void *pre;                  // NULL, or where the activation's argument goes (out_type, out_line)
+    long long lines, columns;   // of the output; set by the products
+    __host__ __device__ long long out_values() const { return (lines - 1) * out_line + columns; }
+    __host__ __device__ long long addend_values() const { return (lines - 1) * addend_line + columns; }
 };
+inline Finish sized(Finish f, long long lines, long long columns)
+{
+    f.lines = lines;
+    f.columns = columns;
+    return f;
+}
 
 // `exact`: for fp32 results
 __device__ __forceinline__ float activate(float z, int act, bool exact)
@@ -160,9 +169,10 @@ __device__ __forceinline__ float activate(float z, int act, bool exact)
 // One value of an output: line, column
 __device__ __forceinline__ void finish_value(const Finish &f, float z, long long line, long long column)
 {
-    if (f.bias) z += load_as_float(f.bias, column, f.bias_type);
-    if (f.addend) z += load_as_float(f.addend, line * f.addend_line + column, f.addend_type);
+    if (f.bias && AXC_GLOBAL_OK(column, f.columns, 421u)) z += load_as_float(f.bias, column, f.bias_type);
+    if (f.addend && AXC_GLOBAL_OK(line * f.addend_line + column, f.addend_values(), 422u)) z += load_as_float(f.addend, line * f.addend_line + column, f.addend_type);
     const long long at = line * f.out_line + column;
+    if (!AXC_GLOBAL_OK(at, f.out_values(), 423u)) return;
     if (f.pre) store_from_float(f.pre, at, f.out_type, z);
     store_from_float(f.out, at, f.out_type, activate(z, f.activation, f.out_type == kFloat32));
 }
@@ -225,6 +235,10 @@ struct Slope {
     int sums_type;
     float scale;
     const float *scale_dev;
+    // values of dy, and of a tensor or operand that has a line for every row
+    __host__ __device__ long long dy_values() const { return (rows - 1) * dy_line + (padded ? dy_line : columns) + (dy_planes - 1) * plane; }
+    __host__ __device__ long long tensor_values() const { return rows * columns; }
+    __host__ __device__ long long operand_values() const { return rows * line; }
 };
 // `room`: bytes of the scratch, slope_scratch(rows, columns) at least; less is refused.
 int slope(const Slope &s, void *scratch, size_t room, Queue &q);

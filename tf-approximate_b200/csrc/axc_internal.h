@@ -29,19 +29,22 @@ __device__ __forceinline__ bool shared_ok(unsigned addr, unsigned bytes, unsigne
 {
     unsigned window;
     asm("mov.u32 %0, %%aggr_smem_size;" : "=r"(window));      // user + reserved shared memory of this CTA
-    hi = hi < window ? hi : window;
-    return bounds_note(addr >= lo && addr + bytes <= hi && (addr & (bytes - 1u)) == 0u, site, addr);
+    // (in a cluster the bits from 2^24 on are the CTA's rank)
+    return bounds_note(addr >= lo && addr + bytes <= hi && (addr & 0xffffffu) + bytes <= window && (addr & (bytes - 1u)) == 0u, site, addr);
 }
 __device__ __forceinline__ bool global_ok(long long index, long long count, unsigned site)
 {
     return bounds_note(index >= 0 && index < count, site, (unsigned long long)index);
 }
 }  // namespace axc
+// `n` values at `at` are among the `count` values from `base` on
+#define AXC_VALUES_OK(at, n, base, count, site) (::axc::global_ok((at) - (base), (long long)(count) - (long long)(n) + 1, (site)))
 #define AXC_SHARED_OK(addr, bytes, lo, hi, site) (::axc::shared_ok((addr), (bytes), (lo), (hi), (site)))
 #define AXC_GLOBAL_OK(index, count, site) (::axc::global_ok((index), (count), (site)))
 #else
 #define AXC_SHARED_OK(addr, bytes, lo, hi, site) (true)
 #define AXC_GLOBAL_OK(index, count, site) (true)
+#define AXC_VALUES_OK(at, n, base, count, site) (true)
 #endif
 
 namespace axc {
@@ -69,6 +72,11 @@ int bounds_record_sched(unsigned out4[4]);
 int bounds_record_conv(unsigned out4[4]);
 int bounds_record_depthwise(unsigned out4[4]);
 int bounds_record_xtab(unsigned out4[4]);
+int bounds_record_adamw(unsigned out4[4]);
+int bounds_record_gemm(unsigned out4[4]);
+int bounds_record_dense(unsigned out4[4]);
+int bounds_record_rows(unsigned out4[4]);
+int bounds_record_entropy(unsigned out4[4]);
 int set_wait_polls(int expand, int convolution);      // debug flavour only
 int set_matrix_wait_polls(int polls);                 // debug flavour only
 

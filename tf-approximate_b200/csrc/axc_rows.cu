@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(256) rows_dot_kernel(const RowsArgs A)
     const long long u0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
     if (u0 >= A.units) return;
     const T *x = static_cast<const T *>(A.x), *w[U];
+    [[maybe_unused]] const long long x_values = (A.rows - 1) * A.x_line + A.inputs, kernel_values = (A.units - 1) * A.kernel_line + A.inputs;
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = static_cast<const T *>(A.kernel) + (u0 + u < A.units ? u0 + u : A.units - 1) * A.kernel_line;
     float sum[U][R];
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(256) rows_dot_kernel(const RowsArgs A)
             for (int u = 0; u < U; ++u) {
                 const long long k = k0 + 32 * V * i;
                 if (k < A.inputs) {
+                    if (!AXC_VALUES_OK(w[u] + k, V, static_cast<const T *>(A.kernel), kernel_values, 441u)) continue;
                     if constexpr (VEC) b[i][u].w[0] = __ldcs(reinterpret_cast<const uint4 *>(w[u] + k));
                     else b[i][u].t[0] = w[u][k];
                 }
@@ -58,6 +60,7 @@ __global__ void __launch_bounds__(256) rows_dot_kernel(const RowsArgs A)
             for (int r = 0; r < R; ++r) {
                 Values<T, V> a;
                 const T *from = x + (r < A.rows ? r : A.rows - 1) * A.x_line + k;
+                if (!AXC_VALUES_OK(from, V, x, x_values, 442u)) continue;
                 if constexpr (VEC) a.w[0] = *reinterpret_cast<const uint4 *>(from);
                 else a.t[0] = *from;
 #pragma unroll
@@ -90,6 +93,7 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(const RowsArgs A, float *
     const long long c = ((long long)blockIdx.x * 32 + lane) * V;
     const long long begin = A.inputs * blockIdx.y / gridDim.y, end = A.inputs * (blockIdx.y + 1) / gridDim.y;
     const T *x = static_cast<const T *>(A.x), *kernel = static_cast<const T *>(A.kernel);
+    [[maybe_unused]] const long long x_values = (A.rows - 1) * A.x_line + A.inputs, kernel_values = (A.inputs - 1) * A.kernel_line + A.units;
     float sum[R][V];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -98,7 +102,10 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(const RowsArgs A, float *
     for (long long k0 = begin + warp * 32; k0 < end; k0 += 256) {
         float mine[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) mine[r] = k0 + lane < end ? widen(x[(r < A.rows ? r : A.rows - 1) * A.x_line + k0 + lane]) : 0.0f;
+        for (int r = 0; r < R; ++r) {
+            const long long at = (r < A.rows ? r : A.rows - 1) * A.x_line + k0 + lane;
+            mine[r] = k0 + lane < end && AXC_GLOBAL_OK(at, x_values, 443u) ? widen(x[at]) : 0.0f;
+        }
 #pragma unroll
         for (int i0 = 0; i0 < 32; i0 += 8) {
             Values<T, V> b[8];
@@ -109,11 +116,11 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(const RowsArgs A, float *
                 for (int j = 0; j < V; ++j) b[i].t[j] = narrow<T>(0.0f);
                 if (k < end) {
                     const T *from = kernel + k * A.kernel_line + c;
-                    if (VEC && c + V <= A.units) b[i].w[0] = __ldcs(reinterpret_cast<const uint4 *>(from));
+                    if (VEC && c + V <= A.units && AXC_VALUES_OK(from, V, kernel, kernel_values, 444u)) b[i].w[0] = __ldcs(reinterpret_cast<const uint4 *>(from));
                     else {
 #pragma unroll
                         for (int j = 0; j < V; ++j)
-                            if (c + j < A.units) b[i].t[j] = from[j];
+                            if (c + j < A.units && AXC_VALUES_OK(from + j, 1, kernel, kernel_values, 445u)) b[i].t[j] = from[j];
                     }
                 }
             }
@@ -140,8 +147,10 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(const RowsArgs A, float *
             for (int k = 1; k < 8; ++k) s += sums[k][i];
             const long long column = (long long)blockIdx.x * 32 * V + i;
             if (column < A.units) {
-                if (gridDim.y > 1) part[blockIdx.y * part_stride + r * part_line + column] = s;
-                else finish_value(A.fin, s, r, column);
+                if (gridDim.y > 1) {
+                    const long long at = blockIdx.y * part_stride + r * part_line + column;
+                    if (AXC_GLOBAL_OK(at, gridDim.y * part_stride, 446u)) part[at] = s;
+                } else finish_value(A.fin, s, r, column);
             }
         }
     }
@@ -198,6 +207,8 @@ int shares_of(const Matrix &x, const Matrix &kernel, const DeviceInfo &di)
 
 }  // namespace
 
+AXC_DEFINE_BOUNDS_READER(bounds_record_rows)
+
 bool few_rows(const Matrix &x, const Matrix &kernel)
 {
     if (x.rows == 0 || x.columns == 0 || (x.column_stride != 1 && x.columns > 1)) return false;
@@ -214,7 +225,8 @@ size_t few_rows_scratch(const Matrix &x, const Matrix &kernel, const DeviceInfo 
 int few_rows_product(const Matrix &x, const Matrix &kernel, const Finish &f, void *scratch, unsigned *status, const DeviceInfo &di, Queue &q)
 {
     const bool dot = inputs_contiguous(kernel);
-    RowsArgs A = {x.data, kernel.data, int(x.rows), x.columns, kernel.rows, x.row_stride, dot ? kernel.row_stride : kernel.column_stride, f, status};
+    RowsArgs A = {x.data, kernel.data, int(x.rows), x.columns, kernel.rows, x.row_stride, dot ? kernel.row_stride : kernel.column_stride,
+                  sized(f, x.rows, kernel.rows), status};
     const long long size = (long long)type_size(x.type);
     const uintptr_t all = reinterpret_cast<uintptr_t>(kernel.data) | uintptr_t(A.kernel_line * size) | (dot ? reinterpret_cast<uintptr_t>(x.data) | uintptr_t(A.x_line * size) : 0);
     const bool vec = all % 16 == 0 && (!dot || x.columns * size % 16 == 0);
