@@ -74,7 +74,8 @@ at::Tensor tensor_of(PyObject *o, const char *name, bool optional)
 {
     if (o == Py_None && optional) return at::Tensor();
     if (!THPVariable_Check(o)) invalid(std::string(name) + " must be a torch tensor");
-    return THPVariable_Unpack(o);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    return t.is_neg() ? t.resolve_neg() : t;               // the imaginary part of a conjugate: its memory holds the other sign
 }
 PyObject *wrap(const at::Tensor &t)
 {
@@ -345,12 +346,13 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     d.exp_avg_sq_scale = static_cast<float *>(out_address(vs));
     for (Py_ssize_t i = 0; i < count; ++i) {
         const at::Tensor p = tensor_of(PyList_GET_ITEM(a[0], i), "parameter", false);
+        if (p.unsafeGetTensorImpl() != THPVariable_Unpack(PyList_GET_ITEM(a[0], i)).unsafeGetTensorImpl()) invalid("a parameter whose memory holds the other sign");
         fits(p, "parameter");
         if (p.numel() != table[i].count) invalid("a parameter has another size than it had when the optimizer was made");
         if (!p.is_contiguous()) invalid("parameters must be contiguous");
         at::Tensor g;
         if (given) g = tensor_of(PyList_GET_ITEM(a[1], i), "gradient", true);
-        else g = p.grad();
+        else g = p.grad().defined() && p.grad().is_neg() ? p.grad().resolve_neg() : p.grad();
         table[i].param = p.mutable_data_ptr();
         table[i].grad = nullptr;
         if (!g.defined()) continue;
