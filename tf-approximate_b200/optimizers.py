@@ -100,9 +100,18 @@ class AdamW:
                 **{k: getattr(self, k).clone() for k in self._STATES if hasattr(self, k)}}
 
     def load_state_dict(self, state):
+        """Takes over a state of `state_dict`, as a whole or not at all."""
+        names = [k for k in self._STATES if hasattr(self, k)]
+        if not isinstance(state, dict) or not {"step_count", "state_bits", "counts", *names} <= state.keys():
+            raise InvalidArgumentError("the state is not one of an optimizer with %d-bit moments" % self.state_bits)
         if state["state_bits"] != self.state_bits or list(state["counts"]) != self._counts:
             raise InvalidArgumentError("the state belongs to other parameters or has another number of bits")
-        for k in self._STATES:
-            if hasattr(self, k):
-                getattr(self, k).copy_(state[k])
+        for k in names:
+            mine, other = getattr(self, k), state[k]
+            if not isinstance(other, torch.Tensor) or other.shape != mine.shape or other.dtype is not mine.dtype:
+                raise InvalidArgumentError("the state's %s must be a %s tensor of shape %s" % (k, mine.dtype, tuple(mine.shape)))
+        if int(state["step_count"]) < 0:
+            raise InvalidArgumentError("a number of steps must not be negative")
+        for k in names:
+            getattr(self, k).copy_(state[k])
         self.step_count = int(state["step_count"])
