@@ -16,7 +16,7 @@ def _differentiated(*tensors):
     functions refuse (they have no rule for it) and a direct call would drop."""
     if forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
 
 
 def _activation(name):
