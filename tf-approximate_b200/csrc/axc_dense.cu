@@ -405,6 +405,7 @@ extern "C" int axc_dense_forward(const axc_dense_desc *desc, const void *x, cons
     const axc_dense_desc &d = *desc;
     if (d.rows == 0 || d.units == 0) return nothing(workspace, workspace_bytes, device, stream);
     if (!y || (d.inputs > 0 && (!x || !kernel))) return AXC_INVALID_ARGUMENT;
+    if (!aligned_to(type_size(d.type), x, kernel, residual, y, pre) || !aligned_to(type_size(d.bias_type), bias)) return AXC_INVALID_ARGUMENT;
     DeviceInfo di;
     rc = device_info(device, &di);
     if (rc) return rc;
@@ -426,6 +427,7 @@ extern "C" int axc_dense_backward(const axc_dense_desc *desc, const void *dy, co
     const bool some = d.rows > 0 && d.units > 0;
     if (some && (!dy || (d.activation != kActNone && !kept))) return AXC_INVALID_ARGUMENT;
     if (d.inputs > 0 && some && ((dx && !kernel) || (dkernel && !x))) return AXC_INVALID_ARGUMENT;
+    if (!aligned_to(type_size(d.type), dy, x, kernel, kept, dx, dkernel, dresidual) || !aligned_to(type_size(d.bias_type), dbias)) return AXC_INVALID_ARGUMENT;
     if (d.rows == 0 && d.units == 0) return nothing(workspace, workspace_bytes, device, stream);
     DeviceInfo di;
     rc = device_info(device, &di);

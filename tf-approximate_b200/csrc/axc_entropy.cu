@@ -487,6 +487,9 @@ extern "C" int axc_entropy(const axc_entropy_desc *desc, const void *x, const vo
     if (rc) return rc;
     const axc_entropy_desc &d = *desc;
     if (!loss || !kernel || (d.rows > 0 && (!x || !labels))) return AXC_INVALID_ARGUMENT;
+    if (!aligned_to(type_size(d.type), x, kernel, dx, dkernel) || !aligned_to(type_size(d.bias_type), bias, dbias) || !aligned_to(sizeof(float), loss, row_loss) ||
+        !aligned_to(sizeof(int64_t), labels))
+        return AXC_INVALID_ARGUMENT;
     DeviceInfo di;
     rc = device_info(device, &di);
     if (rc) return rc;

@@ -51,6 +51,12 @@ __device__ __forceinline__ void after_previous()
 }
 
 inline size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
+// Whether every address is a multiple of `size`: what a kernel cannot load or store elsewhere (NULL is)
+template <typename... P>
+inline bool aligned_to(size_t size, P... p)
+{
+    return ((uintptr_t(0) | ... | reinterpret_cast<uintptr_t>(p)) % size) == 0;
+}
 
 template <typename T> __device__ __forceinline__ float widen(T x);
 template <> __device__ __forceinline__ float widen<float>(float x) { return x; }
