@@ -18,12 +18,11 @@ __device__ __forceinline__ float slope_of(float kept)
 {
     if (ACT == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
     if (ACT == kActGelu) {
-        if (EXACT) return 0.5f * (1.0f + erff(kept * 0.70710678f)) + kept * __expf(-0.5f * kept * kept) * 0.39894228f;
         float bell;
-        const float below = normal_16bit(kept, bell);
+        const float below = normal_below(kept, bell, EXACT);
         return fmaf(kept * bell, 0.39894228f, below);
     }
-    const float s = reciprocal(1.0f + __expf(-kept));
+    const float s = sigmoid(kept, EXACT);
     return s * fmaf(kept, 1.0f - s, 1.0f);
 }
 

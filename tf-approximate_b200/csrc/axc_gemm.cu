@@ -279,7 +279,7 @@ __device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, un
         }
     } else if (f.activation == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActSilu, exact);
+        for (int i = 0; i < W; ++i) v[i] = exact ? activate(v[i], kActSilu, true) : activate(v[i], kActSilu, false);
     }
     store_row<W, N>(L, v, f.out, f.out_type, f.out_line, row0, n0, P.n, f.out_values());
 }

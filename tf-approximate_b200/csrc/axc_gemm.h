@@ -97,18 +97,40 @@ __device__ __forceinline__ float reciprocal(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// For 16-bit results: Phi(z), the normal distribution below z, and bell = exp(-z^2 / 2), which it is made of.  The smaller side, erfc(|z| / sqrt 2) / 2,
-// is bell times a polynomial in t = 1 / (1 + 0.435 |z| / sqrt 2), as Hastings has it, with coefficients of its own: the least largest RELATIVE error for
-// |z| up to 13 (an exchange over 20 000 points: 3.7e-6, one more with the operations' rounding), so that GELU's tail, which is
-// that side times z, is as good as the rest.  A third of the cost of erff.
-__device__ __forceinline__ float normal_16bit(float z, float &bell)
+// Phi(z), the normal distribution below z, and bell = exp(-z^2 / 2), which it is made of.  The smaller side, erfc(|z| / sqrt 2) / 2, is bell times a
+// polynomial in t = 1 / (1 + p |z| / sqrt 2), as Hastings has it, with coefficients of its own: the least largest RELATIVE error for |z| up to 13 (an
+// exchange over 20 000 points), so that GELU's tail, which is that side times z, is as good as the rest; 1 + erf has lost it.
+//   exact    fp32 results: p = 0.375, nine terms, 1.1e-8, six units of 2^-24 with its operations' rounding; expf, whose argument's rounding is z^2 units
+//   else     16-bit results: p = 0.435, six terms, 3.7e-6, and an exponential good to 2^-20 of itself
+__device__ __forceinline__ float normal_below(float z, float &bell, bool exact)
 {
-    const float a = fabsf(z), t = reciprocal(fmaf(0.30759144f, a, 1.0f));
-    bell = __expf(-0.5f * a * a);
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.0758679435f, 0.191902518f), 0.00506413169f), 0.137423128f), 0.118498363f), 0.122977965f);
+    const float a = fabsf(z);
+    float poly;
+    if (exact) {
+        const float t = reciprocal(fmaf(0.265165031f, a, 1.0f));
+        bell = expf(-0.5f * a * a);
+        poly = fmaf(t, 0.0308483057f, -0.144037679f);
+        poly = fmaf(t, poly, 0.21694687f);
+        poly = fmaf(t, poly, -0.115538195f);
+        poly = fmaf(t, poly, 0.137422055f);
+        poly = fmaf(t, poly, 0.0605194829f);
+        poly = fmaf(t, poly, 0.102715209f);
+        poly = fmaf(t, poly, 0.105316751f);
+        poly = t * fmaf(t, poly, 0.105807208f);
+    } else {
+        const float t = reciprocal(fmaf(0.30759144f, a, 1.0f));
+        bell = __expf(-0.5f * a * a);
+        poly = fmaf(t, -0.0758679435f, 0.191902518f);
+        poly = fmaf(t, poly, 0.00506413169f);
+        poly = fmaf(t, poly, 0.137423128f);
+        poly = fmaf(t, poly, 0.118498363f);
+        poly = t * fmaf(t, poly, 0.122977965f);
+    }
     const float side = poly * bell;
     return z < 0.0f ? side : 1.0f - side;
 }
+// 1 / (1 + exp(-z))
+__device__ __forceinline__ float sigmoid(float z, bool exact) { return reciprocal(1.0f + (exact ? expf(-z) : __expf(-z))); }
 
 // bf16 term `p` of three of x, and in `rest` what is left of x for the terms after it.  A value beyond bf16's range keeps its largest finite
 // term.  An infinity is (1, 0, inf) with its sign: of the six products of terms that are summed, the third one is in that with the other
@@ -167,8 +189,8 @@ __device__ __forceinline__ float activate(float z, int act, bool exact)
 {
     if (act == kActRelu) return max_keep_nan(z, 0.0f);
     float bell;
-    if (act == kActGelu) return exact ? 0.5f * z * (1.0f + erff(z * 0.70710678f)) : z * normal_16bit(z, bell);
-    if (act == kActSilu) return z * reciprocal(1.0f + __expf(-z));
+    if (act == kActGelu) return z * normal_below(z, bell, exact);
+    if (act == kActSilu) return z * sigmoid(z, exact);
     return z;
 }
 
