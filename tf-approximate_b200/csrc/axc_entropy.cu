@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
     float sum = 0.0f;
     for (int i = threadIdx.x; i < A.segments; i += 256) {
         const float2 s = stats[i];
-        sum += s.x == -INFINITY ? s.y : s.y * __expf(s.x - base);
+        sum += s.x == -INFINITY ? s.y : s.y * exponential(s.x - base, FORM == 3 || (FORM == 0 && A.planes == 3));
     }
     sum = block_sum(sum, shared);
     const long long label = A.labels[row];
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
         if (!AXC_GLOBAL_OK(c / kSegment, A.segments, 462u) || !AXC_GLOBAL_OK(row * A.line + c + 7, A.rows * A.line, 463u)) continue;
         const float first = stats[c / kSegment].x;
         float factor = scale / sum;
-        if (first != -INFINITY) factor *= __expf(first - base);
+        if (first != -INFINITY) factor *= exponential(first - base, FORM == 3);
         if (!counts) factor = 0.0f;
         float v[8];
         if (FORM == 1) {
@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(256) row_kernel(const RowArgs A)
 }
 
 // The same for few logits, from the parts of their sums.
+template <bool EXACT>
 __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
 {
     after_previous();
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
     top = block_max(top, shared);
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = nan ? NAN : 0.0f;
-    for (int c = threadIdx.x; c < classes; c += 256) sum += __expf(logits[c] - base);
+    for (int c = threadIdx.x; c < classes; c += 256) sum += exponential(logits[c] - base, EXACT);
     sum = block_sum(sum, shared);
     const long long label = A.labels[row];
     const bool counts = label != A.ignore, known = label >= 0 && label < A.classes;
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(256) few_kernel(const RowArgs A)
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[j] = counts && c + j < classes ? __expf(logits[c + j < classes ? c + j : 0] - base) * factor : 0.0f;
+            v[j] = counts && c + j < classes ? exponential(logits[c + j < classes ? c + j : 0] - base, EXACT) * factor : 0.0f;
             if (c + j == label && counts) v[j] -= scale;
         }
         uint16_t *to = A.gradient + row * A.line + c;
@@ -360,7 +361,7 @@ int entropy(const axc_entropy_desc &d, const Layout &l, const void *x, const voi
         r.grad_factor = d.grad_scale / stored;
         r.loss = loss;
         r.alpha = alpha;
-        rc = launch(q, l.few ? few_kernel : !l.kept ? row_kernel<0> : d.type == kBfloat16 ? row_kernel<1> : d.type == kFloat16 ? row_kernel<2> : row_kernel<3>, dim3(grid), 256, 0, 1, r);
+        rc = launch(q, l.few ? (planes == 3 ? few_kernel<true> : few_kernel<false>) : !l.kept ? row_kernel<0> : d.type == kBfloat16 ? row_kernel<1> : d.type == kFloat16 ? row_kernel<2> : row_kernel<3>, dim3(grid), 256, 0, 1, r);
         if (rc) return rc;
     } else {                                   // a sum over nothing
         AXC_CUDA(cudaMemsetAsync(status, 0, sizeof(unsigned), q.stream));

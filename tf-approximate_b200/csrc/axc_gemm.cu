@@ -298,7 +298,7 @@ __device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, un
 
 // One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
 // A segment of -inf has the exponentials 0 (relative to 0, not to itself); one with a NaN has nothing else.  `label`: the row's.
-template <int N>
+template <int N, bool EXACT>
 __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &L, unsigned (&x)[64], int row0, int n0, long long label)
 {
     const EntropyArgs &e = P.ent;
@@ -330,7 +330,7 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &
     float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 64; ++i) {
-        v[i] = __expf(v[i] - base);
+        v[i] = exponential(v[i] - base, EXACT);
         sum4[i & 3] += v[i];
     }
     if (row < P.m && AXC_GLOBAL_OK((long long)row * e.segments + n0 / kSegment, (long long)P.m * e.segments, 439u))
@@ -339,7 +339,7 @@ __device__ __forceinline__ void entropy_segment(const GemmArgs &P, const Lines &
 }
 
 // W logits of a row and what the loss's gradient is there: row_scale * (exp(logit - largest) / sum - [label])
-template <int W, int N>
+template <int W, int N, bool EXACT>
 __device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0)
 {
     const EntropyArgs &e = P.ent;
@@ -362,7 +362,7 @@ __device__ __forceinline__ void gradient_columns(const GemmArgs &P, const Lines 
     }
     // a row without a label stays out, whatever its logits are
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = scale != 0.0f ? scale * (__expf(v[i] - softmax.x) * softmax.y - (label == i ? 1.0f : 0.0f)) : 0.0f;
+    for (int i = 0; i < W; ++i) v[i] = scale != 0.0f ? scale * (exponential(v[i] - softmax.x, EXACT) * softmax.y - (label == i ? 1.0f : 0.0f)) : 0.0f;
     uint16_t *keep = static_cast<uint16_t *>(e.keep);
     const int type = (P.shape >> 7 & 1) ? kBfloat16 : kFloat16;
     for (int plane = 0; plane < P.planes; ++plane) {
@@ -523,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             auto take = [&](unsigned (&x)[W], int c) {
                 if constexpr (MODE == kStore) finish_row<W, kUnits>(P, L, x, row0, n0 + c, alpha);
                 else if constexpr (MODE == kPartial) store_part<W, kUnits>(P, L, x, row0, n0 + c, split);
-                else if constexpr (MODE == kGradient) gradient_columns<W, kUnits>(P, L, x, row0, n0 + c);
-                else entropy_segment<kUnits>(P, L, x, row0, n0 + c, label);
+                else if constexpr (MODE == kGradient) gradient_columns<W, kUnits, PLANES == 3>(P, L, x, row0, n0 + c);
+                else entropy_segment<kUnits, PLANES == 3>(P, L, x, row0, n0 + c, label);
             };
             const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
             if constexpr (CLOSE) {

@@ -97,6 +97,9 @@ __device__ __forceinline__ float reciprocal(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// exp(x) of a softmax, x <= 0: exact for fp32 operands; the other one is off by some |x| 2^-23 of itself
+__device__ __forceinline__ float exponential(float x, bool exact) { return exact ? expf(x) : __expf(x); }
+
 // Phi(z), the normal distribution below z, and bell = exp(-z^2 / 2), which it is made of.  The smaller side, erfc(|z| / sqrt 2) / 2, is bell times a
 // polynomial in t = 1 / (1 + p |z| / sqrt 2), as Hastings has it, with coefficients of its own: the least largest RELATIVE error for |z| up to 13 (an
 // exchange over 20 000 points), so that GELU's tail, which is that side times z, is as good as the rest; 1 + erf has lost it.
