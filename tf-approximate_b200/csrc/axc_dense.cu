@@ -110,11 +110,13 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const Slope S, float *par
                 }
                 if (S.planes && sizeof(T) == 4) {
                     uint16_t *to = S.planes + row * S.line + c;
+                    unsigned t[2][3];
+                    split_terms(d[0], d[1], t[0]);
+                    split_terms(d[2], d[3], t[1]);
 #pragma unroll
                     for (int p = 0; p < 3; ++p, to += S.plane) {
                         union { uint2 w; uint16_t h[4]; } u;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) u.h[i] = split_term(d[i], d[i], p);
+                        u.w = make_uint2(t[0][p], t[1][p]);
                         if (VEC) {
                             if (AXC_VALUES_OK(to, 4, S.planes, 3 * S.operand_values(), 405u)) *reinterpret_cast<uint2 *>(to) = u.w;
                         } else {

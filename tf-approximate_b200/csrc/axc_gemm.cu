@@ -10,7 +10,7 @@
 //
 // fp32 operands are split exactly into three bf16 terms, x = x0 + x1 + x2, each 2^-8 of the one before; six of the nine products
 // of terms are summed (x2 y0, x1 y1, x0 y2, x1 y0, x0 y1, x0 y0), the three left out are below 2^-24 of x y.  Infinities are split so that
-// their products are those of the values (split_term).
+// their products are those of the values (split_terms).
 //
 // Sums are fp32.  The tensor cores cut a sum off at 24 bits at every step of 16 k (measured: 2e-8 of it on average, always towards
 // zero), which 16-bit results do not show.  For fp32 the sums of every 64 k, the small products first, are taken out and added in
@@ -873,7 +873,6 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const Layout one, const La
         if (!AXC_GLOBAL_OK(from + ((c + 8 < m.inner ? c + 8 : m.inner) - 1 - c) * m.inner_stride, values, 424u) ||
             !AXC_GLOBAL_OK(o * m.line + c + 7 + (m.split ? 2 : 0) * m.plane, m.outer * m.line * (m.split ? 3 : 1), 425u))
             continue;
-        union { uint16_t h[8]; uint4 w; } out[3];
         if (m.split) {
             const float *src = static_cast<const float *>(m.src) + from;
             float x[8];
@@ -885,17 +884,17 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const Layout one, const La
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = c + j < m.inner ? src[j * m.inner_stride] : 0.0f;
             }
+            unsigned t[4][3];
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
+            for (int j = 0; j < 4; ++j) split_terms(x[2 * j], x[2 * j + 1], t[j]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) out[p].h[j] = split_term(x[j], x[j], p);
-                *reinterpret_cast<uint4 *>(to + p * m.plane) = out[p].w;
-            }
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(to + p * m.plane) = make_uint4(t[0][p], t[1][p], t[2][p], t[3][p]);
         } else {
             const uint16_t *src = static_cast<const uint16_t *>(m.src) + from;
+            union { uint16_t h[8]; uint4 w; } out;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[0].h[j] = c + j < m.inner ? src[j * m.inner_stride] : uint16_t(0);
-            *reinterpret_cast<uint4 *>(to) = out[0].w;
+            for (int j = 0; j < 8; ++j) out.h[j] = c + j < m.inner ? src[j * m.inner_stride] : uint16_t(0);
+            *reinterpret_cast<uint4 *>(to) = out.w;
         }
     }
 }

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "axc_internal.h"
 #include "axc_pieces.h"
@@ -135,24 +136,29 @@ __device__ __forceinline__ float normal_below(float z, float &bell, bool exact)
 // 1 / (1 + exp(-z))
 __device__ __forceinline__ float sigmoid(float z, bool exact) { return reciprocal(1.0f + (exact ? expf(-z) : __expf(-z))); }
 
-// bf16 term `p` of three of x, and in `rest` what is left of x for the terms after it.  A value beyond bf16's range keeps its largest finite
-// term.  An infinity is (1, 0, inf) with its sign: of the six products of terms that are summed, the third one is in that with the other
-// operand's first term alone, so that inf meets no term that is zero because the value needs no more of them; its own first term
-// stands for it where the other operand is infinite, too.  A NaN is whole in its first term.
-__device__ __forceinline__ uint16_t split_term(float x, float &rest, int p)
+// The three bf16 terms of x and of y, x in the low half: the value rounded, the rest rounded again, and what is left then, which bf16
+// holds exactly.  A value beyond bf16's range has its largest finite term first.  An infinity is (1, 0, inf) with its sign: of the six products of terms
+// that are summed, the third one is in that with the other operand's first term alone, so that inf meets no term that is zero because
+// the value needs no more of them; its own first term stands for it where the other operand is infinite, too.  NaN likewise.
+__device__ __forceinline__ void split_terms(float x, float y, unsigned (&term)[3])
 {
-    if (isinf(x)) {
-        rest = x;
-        return __bfloat16_as_ushort(__float2bfloat16_rn(p == 0 ? copysignf(1.0f, x) : p == 1 ? 0.0f : x));
+    constexpr float kLargest = 3.38953139e38f;                 // of bf16
+    const bool fx = fabsf(x) <= FLT_MAX, fy = fabsf(y) <= FLT_MAX;
+    float rx = fx ? x : copysignf(1.0f, x), ry = fy ? y : copysignf(1.0f, y);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const float hx = p == 0 ? fminf(fmaxf(rx, -kLargest), kLargest) : p == 2 && !fx ? x : rx;
+        const float hy = p == 0 ? fminf(fmaxf(ry, -kLargest), kLargest) : p == 2 && !fy ? y : ry;
+        const __nv_bfloat162 h = __floats2bfloat162_rn(hx, hy);
+        term[p] = reinterpret_cast<const unsigned &>(h);
+        const float2 back = __bfloat1622float2(h);
+        rx -= back.x;
+        ry -= back.y;
     }
-    __nv_bfloat16 h = __float2bfloat16_rn(x);
-    if (isinf(__bfloat162float(h))) h = __float2bfloat16_rz(x);
-    rest = isfinite(x) ? x - __bfloat162float(h) : 0.0f;
-    return __bfloat16_as_ushort(h);
 }
 
 // A matrix of `rows` x `k` as the tensor cores read it: 16-bit values (bf16, or fp16), either k or the rows contiguous, 16-byte
-// aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_term).
+// aligned lines.  fp32 matrices are three such planes whose sum is the value to the bit (see split_terms).
 struct Operand {
     const void *data;
     long long line;             // values from one line to the next
