@@ -16,7 +16,11 @@ def _differentiated(*tensors):
     functions refuse (they have no rule for it) and a direct call would drop."""
     if forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                return True
+    return False
 
 
 def _activation(name):
