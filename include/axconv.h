@@ -341,14 +341,15 @@ enum { AXC_ACTIVATION_NONE = 0, AXC_ACTIVATION_RELU = 1, AXC_ACTIVATION_GELU = 2
 /* The exact dense layer:  y = act(x kernel + bias + residual),  x [rows, inputs], kernel [inputs, units], any strides (elements);
  * bias [units]; residual [rows, units] with unit stride along a row; y [rows, units] contiguous, all of one type but the bias.
  * Sums and everything up to y's rounding are fp32; fp32 operands go through the tensor cores as three bf16 terms each, to about
- * fp32's own precision (2^-22 of the largest products).
+ * fp32's own precision (2^-22 of the largest products); infinities and NaNs among them give what their products are.
  * pre (may be NULL): z = x kernel + bias + residual in y's type, which the gradient of gelu (the exact one, with erf) and silu needs.
  * backward: dz = dy act'(kept) with kept = z, for relu y;  dx = dz kernel^T, dkernel = x^T dz ([units, inputs] in memory where
  * kernel_gradient_transposed), dbias = column sums of dz, dresidual = dz; outputs contiguous, any may be NULL.  dy [rows, units]
  * contiguous.
  * Workspace: axc_dense_workspace_bytes for the tensors' addresses (NULL: enough for any), 256-byte aligned, nothing kept in it.  Calls only
  * enqueue kernels (and a memset): capturable.  axc_matrix_status reads the workspace's status word after the stream is idle: 0, or 3
- * where a wait inside a kernel ran out; the output is then not valid. */
+ * where a wait inside a kernel ran out; the output is then not valid.  Nothing else reports that: asking costs a wait for the stream.
+ * Addresses must be multiples of their type's size. */
 typedef struct {
     int64_t rows, inputs, units;
     int32_t type, bias_type, activation, kernel_gradient_transposed;
@@ -390,7 +391,9 @@ int axc_entropy(const axc_entropy_desc *desc, const void *x, const void *kernel,
  * The moments of the tensors lie one after the other in the caller's buffers, each tensor's at a multiple of AXC_ADAMW_BLOCK values
  * (axc_adamw_state_blocks: how many blocks in all), zeros before the first step; 16-byte aligned.
  * state_bits 32: fp32, exp_avg = m, exp_avg_sq = v.  state_bits 8: e4m3 codes, one byte each, with one fp32 scale per block;
- * exp_avg_sq then holds the codes of sqrt(v).  step counts from 1.  Only the calls' own kernels are enqueued: capturable. */
+ * exp_avg_sq then holds the codes of sqrt(v).  step counts from 1.
+ * Only the calls' own kernels are enqueued, so that a call can be captured; the rates and both bias corrections are numbers in the launch, and a
+ * replayed graph repeats those of the step that was captured: a loop of replays has to update the launch's parameters, or call. */
 enum { AXC_ADAMW_BLOCK = 256 };
 typedef struct {
     void *param;

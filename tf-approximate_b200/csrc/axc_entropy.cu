@@ -10,8 +10,14 @@
 //            in the tile's last step: 8 T D V operations, scratch for one piece
 // Where the logits are few (2^20, of at most 8192 classes) their product is split over CTAs like any other, and the pass over the rows
 // adds the parts up in shared memory and does all the rest: 128 CTAs instead of 32 for 256 x 2048 x 1000, 14.2 to 8.3 us.
-// The kept exponentials are fp16 for bf16 operands (rounded to 2^-12, the gradient to 2^-9), fp32 for others.
-// For fp16 the stored gradient is (softmax - onehot) 2^14, whose smallest normal value is 3.7e-9; the products' factor takes it out.
+// Roundings, for 16-bit operands; fp32 ones have none (fp32 exponentials, the gradient as three bf16 terms):
+//   exponentials kept for bf16 are fp16: 2 bytes a logit written and read instead of 4 (the pass over 2 GiB of them is 721 us of 11 to 13 ms for 8192 x
+//                  2048 x 131072).  To 2^-12 of themselves down to 2^-14 of their segment's largest, to 2^-25 of that one below: a class below 2^-25 of
+//                  the largest of its segment of 64 gets no gradient, where its segment's largest one is rounded by 2^-9 of itself.  Kept for fp16: fp32
+//   gradient       dl is rounded once to bf16 (2^-9), or to fp16 (2^-12) times 2^14, so that its smallest normal value is 3.7e-9 (the products' factor takes
+//                  the 2^14 out), before both products and the bias's sum: the matrix units multiply 16-bit values at full rate, a second term would
+//                  double the products.  dx and dkernel are then off by 0.0019 instead of the 0.0017 that their own rounding to bf16 makes
+//   __expf         16-bit operands' exponentials are good to 2^-19 for |x| up to 20, which the two above hide
 #include "axc_gemm.h"
 
 namespace axc {

@@ -18,7 +18,8 @@
 // sums of 256 k (512 where k is over 1536) for 16-bit operands whose result a ReLU cuts: the sign of a sum near zero decides about a whole
 // gradient there.  Of 4.25 million sums of 1030 products about one had another sign than the exact sum; with runs of 512 one in four such
 // products has one, with 256 one in sixteen.  That costs 10 % (1531 x 1032 x 2776: 18.9 to 20.8 us; 4096 x 4096 x 4096 in runs of 512: 97 to
-// 107, of 256: 129).
+// 107, of 256: 129).  Longer sums would want the shorter runs as much; they have the longer ones for their price alone, 10 instead
+// of 33 %.  (128 sums a thread spill in the tiles of 256 columns: 88 to 92 bytes written and 860 to 908 read, 344 and 256 in the split form.)
 //
 // Products whose tiles are too few have k split over CTAs; the partial sums are added in a fixed order by a second
 // kernel, which also applies what follows the product.

@@ -66,7 +66,8 @@ class _DenseFn(torch.autograd.Function):
 
 
 def dense(x, kernel, bias=None, residual=None, activation=None):
-    """activation(x kernel + bias + residual), differentiable once; see `dense_forward`."""
+    """activation(x kernel + bias + residual), differentiable once, in reverse mode; see `dense_forward`.  Does not wait for the call: only
+    `dense_forward` and `dense_backward` with `check` ask whether a wait inside the kernels ran out."""
     if _differentiated(x, kernel, bias, residual):
         return _DenseFn.apply(x, kernel, bias, residual, activation)
     return _lib.binding().dense_forward(x, kernel, bias, residual, _activation(activation), None)[0]
@@ -107,9 +108,9 @@ class _EntropyFn(torch.autograd.Function):
 
 
 def dense_cross_entropy(x, kernel, labels, bias=None, ignore_index=-100, reduction="mean", row_losses=False, scratch_limit=None):
-    """Softmax cross entropy of a dense classifier; see `dense_cross_entropy_gradients`.  Differentiable once: the gradients are
-    computed with the loss and kept until backward, so float16 operands want a loss scale there (`dense_cross_entropy_gradients`
-    has one).  row_losses: (loss, the rows' own losses), without gradients."""
+    """Softmax cross entropy of a dense classifier; see `dense_cross_entropy_gradients`.  Differentiable once, in reverse mode: the gradients
+    are computed with the loss and kept, in the operands' types, until backward multiplies them by its fp32 factor, so that small gradients of
+    float16 operands are lost before a loss scale reaches them (`dense_cross_entropy_gradients` has one that comes before that rounding).  row_losses: (loss, the rows' own losses), without gradients."""
     if not row_losses and _differentiated(x, kernel, bias):
         return _EntropyFn.apply(x, kernel, bias, labels, ignore_index, reduction, scratch_limit)
     loss, rows, _, _, _ = _entropy(x, kernel, labels, bias, ignore_index, reduction, 1.0, scratch_limit, bool(row_losses), (False, False, False), False)

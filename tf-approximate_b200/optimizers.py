@@ -24,7 +24,9 @@ class AdamW:
       state_bits=32   exp_avg, exp_avg_sq: fp32
       state_bits=8    exp_avg, exp_avg_sq_root: float8_e4m3fn, with exp_avg_scale and exp_avg_sq_root_scale, one fp32 value for each 256;
                       the second moment is held as its root, which is what the step divides by
-    `step_count` counts the steps; a parameter without a gradient is left as it is, its moments too."""
+    `step_count` counts the steps; a parameter without a gradient is left as it is, its moments too.  A step raises the version counter of
+    the parameters that it changes.  One that is captured into a CUDA graph repeats its own step's rates and bias corrections when it is
+    replayed."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32):
         groups = list(params)
@@ -81,7 +83,8 @@ class AdamW:
             p.grad = None
 
     def step(self, grads=None, grad_scale=1.0):
-        """One step with `grads`, in the order of the parameters (default: their .grad; None: left as it is), times `grad_scale`."""
+        """One step with `grads`, in the order of the parameters (default: their .grad; None: left as it is), times
+        `grad_scale`.  A gradient has its parameter's shape, and any strides."""
         if len(self.params) != len(self._counts):
             raise InvalidArgumentError("the optimizer's parameters are those it was made with")
         if grads is not None and not isinstance(grads, list):
