@@ -383,6 +383,16 @@ int axc_entropy_workspace_bytes(const axc_entropy_desc *desc, const void *x, con
 int axc_entropy(const axc_entropy_desc *desc, const void *x, const void *kernel, const void *bias, const int64_t *labels, float *loss, float *row_loss,
                 void *dx, void *dkernel, void *dbias, void *workspace, size_t workspace_bytes, int device, void *stream);
 
+/* out = factor * x in fp32, rounded once to the tensor's type, for tensors of any of the types, four of them a launch: the gradients of a loss times the
+ * factor that its own gradient is, one float in device memory.  out may be x. */
+typedef struct {
+    const void *x;
+    void *out;
+    int64_t count;
+    int32_t type;
+} axc_scale_tensor;
+int axc_scale(const axc_scale_tensor *tensors, int32_t count, const float *factor, int device, void *stream);
+
 /* One step of AdamW over many tensors, in one launch per 800 of them:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  g = grad_scale * gradient
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)

@@ -17,7 +17,7 @@ SYMBOLS = [
     "axc_add_residual", "axc_max_pool_same", "axc_conv2d_forward_fused", "axc_depthwise_conv2d_forward_fused", "axc_tensor_range", "axc_fake_quant", "axc_column_sums", "axc_conv2d_forward_sharded", "axc_gather_outputs",
     "axc_qconv2d_workspace_bytes", "axc_qconv2d_fast_workspace_bytes", "axc_qconv2d_route", "axc_qconv2d_forward", "axc_quantized_zero_point", "axc_quantized_output_range",
     "axc_adamw_state_blocks", "axc_adamw_step",
-    "axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes", "axc_entropy",
+    "axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes", "axc_entropy", "axc_scale",
 ]
 
 
@@ -135,7 +135,7 @@ def binding():
             errors.raise_for_status(status, what, "cudaError %d" % L.axc_last_cuda_error() if status == 100 else "")
 
         names = ("axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes",
-                 "axc_entropy", "axc_adamw_step")
+                 "axc_entropy", "axc_adamw_step", "axc_scale")
         module.init(tuple(C.cast(getattr(L, n), C.c_void_p).value for n in names), errors.InvalidArgumentError, errors.InternalError, raise_for_status)
         _binding = module
     return _binding

@@ -24,6 +24,7 @@ struct Entry {
     decltype(&axc_entropy_workspace_bytes) entropy_bytes;
     decltype(&axc_entropy) entropy;
     decltype(&axc_adamw_step) adamw;
+    decltype(&axc_scale) scale;
 };
 Entry g_entry = {};
 PyObject *g_invalid = nullptr, *g_internal = nullptr, *g_raise = nullptr;    // exception classes; raise_for_status(status, what)
@@ -300,6 +301,34 @@ PyObject *entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
     AXC_TORCH_END
 }
 
+// scaled(factor, tensor or None, ...) -> a tuple of their products with the factor, a tensor of one value; tensors without gaps
+PyObject *scaled(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    AXC_TORCH_BEGIN
+    if (n < 1) invalid("scaled takes a factor");
+    c10::NoGradGuard no_grad;
+    at::Tensor factor = tensor_of(a[0], "factor", false);
+    if (!factor.is_cuda() || factor.numel() != 1) invalid("the factor must be one value on a CUDA device");
+    if (factor.scalar_type() != at::kFloat) factor = factor.to(at::kFloat);
+    std::vector<at::Tensor> x(n - 1), out(n - 1);
+    std::vector<axc_scale_tensor> table;
+    for (Py_ssize_t i = 0; i + 1 < n; ++i) {
+        x[i] = tensor_of(a[i + 1], "tensor", true);
+        if (!x[i].defined()) continue;
+        if (type_of(x[i]) < 0 || x[i].device() != factor.device()) invalid("a float32, bfloat16 or float16 tensor on the factor's device expected");
+        if (!x[i].is_non_overlapping_and_dense()) x[i] = x[i].contiguous();
+        out[i] = at::empty_like(x[i]);
+        if (out[i].strides() != x[i].strides()) x[i] = x[i].contiguous(), out[i] = at::empty_like(x[i], at::MemoryFormat::Contiguous);
+        table.push_back({address(x[i]), out_address(out[i]), x[i].numel(), type_of(x[i])});
+    }
+    check(g_entry.scale(table.data(), int32_t(table.size()), static_cast<const float *>(address(factor)), factor.device().index(), stream_of(factor)), "scale");
+    PyObject *r = PyTuple_New(n - 1);
+    if (!r) throw Raised();
+    for (Py_ssize_t i = 0; i + 1 < n; ++i) PyTuple_SET_ITEM(r, i, wrap(out[i]));
+    return r;
+    AXC_TORCH_END
+}
+
 // adamw_step(params, grads or None, the table's address, exp_avg, type, state_bits, step, (beta1, beta2, eps, grad_scale), exp_avg_sq, its scales)
 // params and grads: lists; the table's entries have counts and rates already.
 PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
@@ -381,9 +410,9 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 // init(addresses of the entry points, InvalidArgumentError, InternalError, raise_for_status)
 PyObject *init(PyObject *, PyObject *args)
 {
-    unsigned long long p[7];
+    unsigned long long p[8];
     PyObject *i, *e, *r;
-    if (!PyArg_ParseTuple(args, "(KKKKKKK)OOO", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &i, &e, &r)) return nullptr;
+    if (!PyArg_ParseTuple(args, "(KKKKKKKK)OOO", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &i, &e, &r)) return nullptr;
     g_entry.dense_bytes = reinterpret_cast<decltype(g_entry.dense_bytes)>(p[0]);
     g_entry.dense_forward = reinterpret_cast<decltype(g_entry.dense_forward)>(p[1]);
     g_entry.dense_backward = reinterpret_cast<decltype(g_entry.dense_backward)>(p[2]);
@@ -391,6 +420,7 @@ PyObject *init(PyObject *, PyObject *args)
     g_entry.entropy_bytes = reinterpret_cast<decltype(g_entry.entropy_bytes)>(p[4]);
     g_entry.entropy = reinterpret_cast<decltype(g_entry.entropy)>(p[5]);
     g_entry.adamw = reinterpret_cast<decltype(g_entry.adamw)>(p[6]);
+    g_entry.scale = reinterpret_cast<decltype(g_entry.scale)>(p[7]);
     Py_INCREF(i);
     Py_INCREF(e);
     Py_INCREF(r);
@@ -404,6 +434,7 @@ PyMethodDef g_methods[] = {{"init", init, METH_VARARGS, nullptr},
                            {"dense_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense_forward)), METH_FASTCALL, nullptr},
                            {"dense_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense_backward)), METH_FASTCALL, nullptr},
                            {"entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entropy)), METH_FASTCALL, nullptr},
+                           {"scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scaled)), METH_FASTCALL, nullptr},
                            {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_step)), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_axc_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

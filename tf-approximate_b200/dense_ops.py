@@ -103,8 +103,8 @@ class _EntropyFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        # one dimension, not none: the product with the fp32 factor is then computed in fp32 and rounded once, when it is stored
-        return tuple(None if t is None else torch.mul(t, grad.reshape(1), out=torch.empty_like(t)) for t in ctx.saved_tensors) + (None,) * 4
+        # fp32 products, rounded once (torch would round the factor to the gradients' type first)
+        return _lib.binding().scaled(grad, *ctx.saved_tensors) + (None,) * 4
 
 
 def dense_cross_entropy(x, kernel, labels, bias=None, ignore_index=-100, reduction="mean", row_losses=False, scratch_limit=None):
