@@ -422,6 +422,43 @@ typedef struct {
 int axc_adamw_state_blocks(const int64_t *counts, int32_t tensors, int64_t *blocks);
 int axc_adamw_step(const axc_adamw_desc *desc, const axc_adamw_tensor *tensors, int32_t count, int device, void *stream);
 
+/* Group norm of tensors with their channels last, with the shortcut and the activation that follow it:
+ *   xhat = (x - mean) r, r = 1 / sqrt(var + epsilon), over a sample's places and a group's channels (var: over all of them, not less one)
+ *   z = xhat scale + offset + residual,  y = act(z)
+ * x, residual, y, dy, dx, dresidual [samples, places, channels] contiguous, of one type; scale, offset [channels], each of its own type, NULL for
+ * ones and zeros; channels a multiple of groups.  statistics: {mean, r} for [samples, groups], fp32, 8-byte aligned, which the backward pass reads.
+ * backward: dz = dy act'(z), z computed again;  dscale, doffset: sums of dz xhat and of dz over samples and places, in their parameters' types;
+ * dresidual = dz;  dx = r (dz scale - S1 / m - xhat S2 / m), S1 and S2 the group's sums of dz scale and dz scale xhat, m its values.  Outputs may be
+ * NULL.  Without samples or places nothing is written but zeros to dscale and doffset.
+ * Sums are fp32 in a fixed order.  Workspace: 256-byte aligned, nothing kept in it; it may be NULL where 0 bytes are needed.  Calls only enqueue
+ * kernels: capturable.  Addresses must be multiples of their type's size; tensors that all start on 16 bytes are read faster. */
+typedef struct {
+    int64_t samples, places, channels, groups;
+    int32_t type, scale_type, offset_type, activation;
+    float epsilon;
+} axc_norm_desc;
+int axc_group_norm_workspace_bytes(const axc_norm_desc *desc, int device, size_t *forward, size_t *backward);
+int axc_group_norm_forward(const axc_norm_desc *desc, const void *x, const void *scale, const void *offset, const void *residual, void *y, float *statistics,
+                           void *workspace, size_t workspace_bytes, int device, void *stream);
+int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy, const void *x, const float *statistics, const void *scale, const void *offset,
+                            const void *residual, void *dx, void *dscale, void *doffset, void *dresidual, void *workspace, size_t workspace_bytes, int device,
+                            void *stream);
+
+/* Dropout whose mask is computed, and computed again for the gradient, instead of stored:
+ *   y[i] = (bits[i] >= share ? x[i] * factor : 0) + residual[i],  share = rate 2^16 rounded, factor = 2^16 / (2^16 - share)  (0 for share 2^16)
+ * bits: 16 of the random generator Philox 4x32 with 10 rounds (Salmon, Moraes, Dror, Shaw 2011) under the key `seed` (low word first); values 8 j to
+ * 8 j + 7 have the four words, low half first, of the counter {j low, j high, offset low, offset high}.  The mask depends on neither the type nor the
+ * address.  A dropped value is 0 whatever it was.  offset_device: NULL, or one int64 in device memory that is read in place of `offset`, so that a
+ * captured call can have another mask at every replay.  x, residual, y: `count` values of one type; residual may be NULL; y may be x or residual.
+ * The gradient of x is this call on y's gradient, without a residual. */
+typedef struct {
+    int64_t count;
+    int32_t type;
+    double rate;
+    uint64_t seed, offset;
+} axc_dropout_desc;
+int axc_dropout(const axc_dropout_desc *desc, const void *x, const void *residual, void *y, const int64_t *offset_device, int device, void *stream);
+
 /* ---- quantisation parameters: Nudge + UpdateVarQuantProps
  *      (tf2/src/approx_ops_types.h:29-49, 135-152).  out3 = {scale, 1/scale, nudged_min}. */
 int axc_quant_props(float min_value, float max_value, float out3[3]);

@@ -18,6 +18,7 @@ SYMBOLS = [
     "axc_qconv2d_workspace_bytes", "axc_qconv2d_fast_workspace_bytes", "axc_qconv2d_route", "axc_qconv2d_forward", "axc_quantized_zero_point", "axc_quantized_output_range",
     "axc_adamw_state_blocks", "axc_adamw_step",
     "axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes", "axc_entropy", "axc_scale",
+    "axc_group_norm_workspace_bytes", "axc_group_norm_forward", "axc_group_norm_backward", "axc_dropout",
 ]
 
 
@@ -135,7 +136,8 @@ def binding():
             errors.raise_for_status(status, what, "cudaError %d" % L.axc_last_cuda_error() if status == 100 else "")
 
         names = ("axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes",
-                 "axc_entropy", "axc_adamw_step", "axc_scale")
+                 "axc_entropy", "axc_adamw_step", "axc_scale", "axc_group_norm_workspace_bytes", "axc_group_norm_forward", "axc_group_norm_backward",
+                 "axc_dropout")
         module.init(tuple(C.cast(getattr(L, n), C.c_void_p).value for n in names), errors.InvalidArgumentError, errors.InternalError, raise_for_status)
         _binding = module
     return _binding

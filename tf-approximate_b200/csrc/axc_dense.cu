@@ -18,19 +18,6 @@ namespace {
 // They make bf16 GELU's results off by 0.0024 in all, where the rounding of the results alone makes 0.0017; a linear layer has none of it.  fp32
 // has neither.
 // ------------------------------------------------------------------------------------------------
-template <int ACT, bool EXACT>
-__device__ __forceinline__ float slope_of(float kept)
-{
-    if (ACT == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
-    if (ACT == kActGelu) {
-        float bell;
-        const float below = normal_below(kept, bell, EXACT);
-        return fmaf(kept * bell, 0.39894228f, below);
-    }
-    const float s = sigmoid(kept, EXACT);
-    return s * fmaf(kept, 1.0f - s, 1.0f);
-}
-
 template <typename T>
 union Group {                                  // 16 bytes of values
     static constexpr int V = 16 / sizeof(T);

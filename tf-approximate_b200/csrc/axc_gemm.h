@@ -203,6 +203,20 @@ __device__ __forceinline__ float activate(float z, int act, bool exact)
     return z;
 }
 
+// The activation's slope at its argument, for relu at its argument or its value
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float slope_of(float kept)
+{
+    if (ACT == kActRelu) return kept > 0.0f ? 1.0f : (kept != kept ? kept : 0.0f);
+    if (ACT == kActGelu) {
+        float bell;
+        const float below = normal_below(kept, bell, EXACT);
+        return fmaf(kept * bell, 0.39894228f, below);
+    }
+    const float s = sigmoid(kept, EXACT);
+    return s * fmaf(kept, 1.0f - s, 1.0f);
+}
+
 // One value of an output: line, column
 __device__ __forceinline__ void finish_value(const Finish &f, float z, long long line, long long column)
 {

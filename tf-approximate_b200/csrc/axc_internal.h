@@ -77,6 +77,8 @@ int bounds_record_gemm(unsigned out4[4]);
 int bounds_record_dense(unsigned out4[4]);
 int bounds_record_rows(unsigned out4[4]);
 int bounds_record_entropy(unsigned out4[4]);
+int bounds_record_norm(unsigned out4[4]);
+int bounds_record_dropout(unsigned out4[4]);
 int set_wait_polls(int expand, int convolution);      // debug flavour only
 int set_matrix_wait_polls(int polls);                 // debug flavour only
 

@@ -1,0 +1,221 @@
+// How group norm's kernels cut up their tensors, and a thread's way through its part.  Plain arithmetic, in a header of its own so that it can be checked without a GPU
+// over any number of sizes: the workspace's size, the shared memory and the launches come from here.
+#pragma once
+#include <stddef.h>
+
+#ifdef __CUDACC__
+#define AXC_BOTH __host__ __device__ __forceinline__
+#else
+#define AXC_BOTH inline
+#endif
+
+namespace axc {
+
+constexpr int kNormThreads = 256;              // of a block, at most
+constexpr int kNormCluster = 8;                // blocks that share a span, at most
+constexpr long long kNormSmem = 226 * 1024;    // of a block, at most
+
+struct NormShape {
+    long long samples, places, channels, groups;
+    int size;                                  // bytes of a value
+    bool aligned;                              // every tensor starts on 16 bytes
+    long long each() const { return channels / groups; }
+    long long values() const { return samples * places * channels; }
+};
+
+// Resident: a span, which is a sample's channels of one or several whole groups, stays in the shared memory of a cluster of `blocks` blocks between
+// the sums over it and what is computed of them.  Else the tensors are read twice, in blocks of `span` channels and a share of the places each.
+struct NormPlan {
+    bool resident;
+    int vec;                                   // values that a thread moves at a time: 16 bytes of them, or one
+    int threads, span, blocks;
+    long long shares;                          // not resident: blocks that share a sample's places
+    unsigned smem;
+};
+
+inline long long norm_gcd(long long a, long long b)
+{
+    while (b) {
+        const long long t = a % b;
+        a = b;
+        b = t;
+    }
+    return a;
+}
+
+// Threads of `threads` that take part, so that each keeps its `vec` channels from one step to the next: as many as are a multiple of what the
+// channels' order repeats after.  0: it repeats after more than all of them.
+inline int norm_active(int threads, int span, int vec)
+{
+    const long long period = span / norm_gcd(span, vec);
+    return period > threads ? 0 : int(threads / period * period);
+}
+
+// Steps that the threads take for the places of a block, one more where a sample starts inside 16 bytes
+inline long long norm_steps(long long places, int span, int vec, int active)
+{
+    const long long all = places * span + vec - 1, each = (long long)active * vec;
+    return (all + each - 1) / each;
+}
+
+AXC_BOTH size_t norm_up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// Shared memory of a resident block: `kept` bytes for each value, a pair of sums for each of the threads' channels, four floats for each group
+// (a pair for the cluster's blocks to read, a pair of results).
+inline long long norm_smem(long long places, int span, int vec, int active, int kept, long long groups, int sums)
+{
+    return norm_steps(places, span, vec, active) * active * vec * kept + 32 + (long long)active * vec * 8 + (long long)span * 8 * sums + groups * 16;
+}
+
+// Channels at a time where the tensors are read twice
+inline int norm_columns(const NormShape &s, int *vec)
+{
+    const int wide = 16 / s.size;
+    *vec = s.aligned && (s.channels % wide == 0 || norm_active(kNormThreads, int(s.channels < (1 << 20) ? s.channels : (1 << 20)), wide) > 0) ? wide : 1;
+    const long long most = (long long)kNormThreads * *vec;
+    if (s.channels % *vec) return int(s.channels);            // lines that start anywhere: whole ones
+    return int(s.channels < most ? s.channels : most);
+}
+
+// `kept`: bytes that stay in shared memory for each value; `moved`: bytes read and written for each; `sums`: 1 where sums of single channels are kept,
+// too (the backward pass).
+//
+// The estimate, in us: all bytes at memory's rate, or the blocks' own times in as many rounds as the SMs take them, whichever is more, and one block's
+// time.  A block takes 3 us for its start, its two exchanges and its end, 1 more in a cluster, and its bytes at what an SM moves with the blocks that
+// fit on it (20 bytes a ns for each, 44 at most).  Pieces of a line below 64 bytes are charged for the rest of what memory moves.
+inline NormPlan norm_plan(const NormShape &s, int kept, int moved, int sums, int sms)
+{
+    NormPlan best = {};
+    double least = 1e300;
+    const int wide = 16 / s.size;
+    const long long each = s.each();
+    for (int v = 0; v < 2; ++v) {
+        const int vec = v == 0 ? wide : 1;
+        if (vec > 1 && !s.aligned) continue;
+        for (long long k = 1; k <= s.groups; ++k) {
+            if (s.groups % k) continue;
+            const long long span = each * k;
+            if (span > (long long)kNormThreads * vec) break;
+            if (span < s.channels && (span % vec || s.channels % vec)) continue;
+            for (int threads = 64; threads <= kNormThreads; threads *= 2) {
+                const int active = norm_active(threads, int(span), vec);
+                if (!active) continue;
+                for (int blocks = 1; blocks <= kNormCluster && blocks <= s.places; ++blocks) {
+                    const long long places = (s.places + blocks - 1) / blocks;
+                    if (places * span > (1ll << 20)) continue;
+                    const long long smem = norm_smem(places, int(span), vec, active, kept, k, sums);
+                    if (smem > kNormSmem) continue;
+                    const double line = double(span) * s.size, waste = span == s.channels || line >= 64 ? 1.0 : line >= 32 ? 1.15 : 32 / line;
+                    long long fit = kNormSmem / (smem + 1024);
+                    if (fit > 768 / threads) fit = 768 / threads;
+                    const double units = double(s.samples) * double(s.groups / k) * blocks;
+                    // a thread has four accesses on their way
+                    double rate = double(fit) * threads * vec * s.size * 4 / 800.0;
+                    if (rate > 44) rate = 44;
+                    const double bytes = double(places) * double(span) * moved * waste * (vec == 1 ? 2.0 : 1.0);
+                    const double own = 3.0 + (blocks > 1 ? 1.0 : 0.0) + bytes * double(fit) / rate / 1000.0;
+                    const double rounds = units / (double(sms) * double(fit)), cover = units < sms ? units / sms : 1.0;
+                    const double memory = double(s.values()) * moved * waste / (6.5e6 * cover);
+                    const double time = (rounds * own > memory ? rounds * own : memory) + own * (rounds < 1 ? 1.0 - rounds + 1e-3 : 0.5);
+                    if (time < least) {
+                        least = time;
+                        best = {true, vec, threads, int(span), blocks, 0, unsigned(smem)};
+                    }
+                }
+            }
+        }
+    }
+    if (best.resident) return best;
+    int vec = 1;
+    const int span = norm_columns(s, &vec);
+    best.vec = vec;
+    best.threads = kNormThreads;
+    best.span = span;
+    // six blocks for every SM, of 32 KiB at least
+    const long long across = s.samples * ((s.channels + span - 1) / span), most = s.places * span * s.size / (32 * 1024) + 1;
+    long long shares = ((long long)sms * 6 + across - 1) / (across ? across : 1);
+    if (shares > most) shares = most;
+    if (shares > s.places) shares = s.places;
+    if (shares < 1) shares = 1;
+    const long long fewest = (s.places * span >> 30) + 1;     // a block counts its values in 32 bits
+    best.shares = shares < fewest ? fewest : shares;
+    return best;
+}
+
+// Bytes of scratch: pairs of fp32 sums for every sample and channel, and share; group sums behind them
+inline size_t norm_pad(size_t bytes) { return (bytes + 255) / 256 * 256; }
+inline size_t norm_part_bytes(const NormShape &s, const NormPlan &p)
+{
+    return p.resident ? 0 : norm_pad(size_t(s.samples) * size_t(p.shares) * size_t(s.channels) * 8);
+}
+inline size_t norm_sums_bytes(const NormShape &s) { return norm_pad(size_t(s.samples) * size_t(s.channels) * 8); }
+inline size_t norm_group_bytes(const NormShape &s) { return norm_pad(size_t(s.samples) * size_t(s.groups) * 8); }
+
+// ---- in the kernels ------------------------------------------------------------------------------------------------------------
+// A thread's way through the places and channels of its block: `count` vectors, the j-th with the values o + j * each .. of the block's own
+// (place by place, `total` of them), at at + j * step from the sample's start.
+template <int V>
+struct Walk {
+    int o, each, count, total;
+    long long at, step;
+    AXC_BOTH Walk(int thread, int active, int shift, int places, int span, long long channels, long long place0, int channel0)
+    {
+        each = active * V;
+        o = thread * V - shift;
+        total = places * span;
+        count = thread < active && o < total ? (total - 1 - o) / each + 1 : 0;
+        if (span == channels) {
+            at = place0 * channels + o;
+            step = each;
+        } else {
+            at = (place0 + o / span) * channels + channel0 + o % span;
+            step = (each / span) * channels;
+        }
+    }
+    AXC_BOTH bool whole(int j) const
+    {
+        if (V == 1) return true;
+        const int s = o + j * each;
+        return s >= 0 && s + V <= total;
+    }
+    AXC_BOTH bool has(int j, int i) const
+    {
+        const int s = o + j * each + i;
+        return s >= 0 && s < total;
+    }
+};
+// Thread t's channel i is entry t * V + i; a span's channel l has the entries (l + shift) mod span + k * span.
+struct Entries {
+    int span, shift, copies, each, rest, base;
+    AXC_BOTH Entries(int active, int vec, int span_, int shift_, int total)
+    {
+        span = span_;
+        shift = shift_;
+        each = active * vec;
+        copies = each / span;
+        base = total / each;
+        rest = total - base * each;
+    }
+    AXC_BOTH int entry(int l, int copy) const
+    {
+        const int e = l + shift;
+        return (e < span ? e : e % span) + copy * span;
+    }
+    // values that were added up in it
+    AXC_BOTH float values(int entry) const
+    {
+        int o = entry - shift;
+        if (o < 0) o += each;
+        return float(base + (o < rest ? 1 : 0));
+    }
+};
+
+// local channel of a thread's value i
+template <int V>
+AXC_BOTH int local_channel(const Walk<V> &w, int span, int i)
+{
+    const int o = w.o + i;
+    return o < 0 ? (o + (V + span - 1) / span * span) % span : o % span;
+}
+
+}  // namespace axc

@@ -9,6 +9,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cstring>
 #include <string>
 #include <vector>
 
@@ -25,6 +26,10 @@ struct Entry {
     decltype(&axc_entropy) entropy;
     decltype(&axc_adamw_step) adamw;
     decltype(&axc_scale) scale;
+    decltype(&axc_group_norm_workspace_bytes) norm_bytes;
+    decltype(&axc_group_norm_forward) norm_forward;
+    decltype(&axc_group_norm_backward) norm_backward;
+    decltype(&axc_dropout) dropout;
 };
 Entry g_entry = {};
 PyObject *g_invalid = nullptr, *g_internal = nullptr, *g_raise = nullptr;    // exception classes; raise_for_status(status, what)
@@ -407,20 +412,164 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     AXC_TORCH_END
 }
 
+// ---- group norm ------------------------------------------------------------------------------------------------------------------
+struct Norm {
+    at::Tensor x, scale, offset, residual;
+    axc_norm_desc d;
+    int device;
+};
+
+at::Tensor of_channels(PyObject *p, const char *name, const at::Tensor &x)
+{
+    const at::Tensor t = tensor_of(p, name, true);
+    if (!t.defined()) return t;
+    if (type_of(t) < 0 || t.device() != x.device() || t.dim() != 1 || t.size(0) != x.size(-1))
+        invalid(std::string(name) + " must be a float32, bfloat16 or float16 tensor of shape (" + std::to_string(x.size(-1)) + ",) on x's device");
+    return t.contiguous();
+}
+// a tensor of x's type, shape and device
+at::Tensor like_x(PyObject *p, const char *name, const at::Tensor &x, bool optional)
+{
+    const at::Tensor t = tensor_of(p, name, optional);
+    if (!t.defined()) return t;
+    if (t.scalar_type() != x.scalar_type() || t.device() != x.device() || t.sizes() != x.sizes())
+        invalid(std::string(name) + " must be a tensor of x's type, of shape " + text_of(x.sizes()) + " on x's device");
+    return t.contiguous();
+}
+
+Norm norm_of(PyObject *px, PyObject *groups, PyObject *scale, PyObject *offset, PyObject *residual, PyObject *activation, double epsilon)
+{
+    Norm n;
+    const at::Tensor x = tensor_of(px, "x", false);
+    if (!x.is_cuda() || type_of(x) < 0) invalid("x must be a float32, bfloat16 or float16 CUDA tensor (this build has no CPU kernel)");
+    if (x.dim() < 2 || x.size(-1) < 1) invalid("x [samples, ..., channels] expected, got " + text_of(x.sizes()));
+    n.d = {};
+    n.d.groups = PyLong_AsLongLong(groups);
+    if (PyErr_Occurred()) throw Raised();
+    if (n.d.groups < 1 || x.size(-1) % n.d.groups) invalid("the channels (" + std::to_string(x.size(-1)) + ") must be a multiple of the groups (" + std::to_string(n.d.groups) + ")");
+    if (!(epsilon >= 0.0 && epsilon <= 3.4e38)) invalid("epsilon must be finite and not negative");
+    n.scale = of_channels(scale, "scale", x);
+    n.offset = of_channels(offset, "offset", x);
+    n.residual = like_x(residual, "residual", x, true);
+    n.x = x.contiguous();
+    n.d.samples = x.size(0);
+    n.d.places = 1;
+    for (int64_t i = 1; i + 1 < x.dim(); ++i) n.d.places *= x.size(i);
+    n.d.channels = x.size(-1);
+    n.d.type = type_of(x);
+    n.d.scale_type = n.scale.defined() ? type_of(n.scale) : AXC_TYPE_FLOAT32;
+    n.d.offset_type = n.offset.defined() ? type_of(n.offset) : AXC_TYPE_FLOAT32;
+    n.d.activation = int(PyLong_AsLong(activation));
+    n.d.epsilon = float(epsilon);
+    n.device = x.device().index();
+    return n;
+}
+
+// group_norm_forward(x, groups, scale, offset, residual, activation, epsilon) -> (y, statistics)
+PyObject *group_norm_forward(PyObject *, PyObject *const *a, Py_ssize_t count)
+{
+    AXC_TORCH_BEGIN
+    if (count != 7) invalid("group_norm_forward takes 7 arguments");
+    c10::NoGradGuard no_grad;
+    const double epsilon = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred()) throw Raised();
+    const Norm n = norm_of(a[0], a[1], a[2], a[3], a[4], a[5], epsilon);
+    const at::Tensor y = at::empty(n.x.sizes(), n.x.options()), statistics = at::empty({n.d.samples, n.d.groups, 2}, n.x.options().dtype(at::kFloat));
+    size_t bytes = 0;
+    check(g_entry.norm_bytes(&n.d, n.device, &bytes, nullptr), "group norm");
+    const at::Tensor ws = bytes ? scratch(n.x, bytes) : at::Tensor();
+    check(g_entry.norm_forward(&n.d, address(n.x), address(n.scale), address(n.offset), address(n.residual), out_address(y), static_cast<float *>(out_address(statistics)),
+                               out_address(ws), bytes, n.device, stream_of(n.x)),
+          "group norm");
+    return Py_BuildValue("(NN)", wrap(y), wrap(statistics));
+    AXC_TORCH_END
+}
+
+// group_norm_backward(grad, x, statistics, groups, scale, offset, residual, activation, need_x, need_scale, need_offset, need_residual) -> (dx, dscale, doffset, dresidual)
+PyObject *group_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t count)
+{
+    AXC_TORCH_BEGIN
+    if (count != 12) invalid("group_norm_backward takes 12 arguments");
+    c10::NoGradGuard no_grad;
+    const Norm n = norm_of(a[1], a[3], a[4], a[5], a[6], a[7], 0.0);
+    const at::Tensor grad = like_x(a[0], "grad", n.x, false), statistics = tensor_of(a[2], "statistics", false);
+    if (statistics.scalar_type() != at::kFloat || statistics.device() != n.x.device() || statistics.dim() != 3 || statistics.size(0) != n.d.samples ||
+        statistics.size(1) != n.d.groups || statistics.size(2) != 2 || !statistics.is_contiguous())
+        invalid("statistics must be what the forward pass returned for these samples and groups");
+    at::Tensor dx, dscale, doffset, dresidual;
+    if (a[8] == Py_True) dx = at::empty(n.x.sizes(), n.x.options());
+    if (a[9] == Py_True && n.scale.defined()) dscale = at::empty(n.scale.sizes(), n.scale.options());
+    if (a[10] == Py_True && n.offset.defined()) doffset = at::empty(n.offset.sizes(), n.offset.options());
+    const bool with_residual = a[11] == Py_True && n.residual.defined(), same = with_residual && n.d.activation == AXC_ACTIVATION_NONE;
+    if (with_residual && !same) dresidual = at::empty(n.x.sizes(), n.x.options());
+    size_t bytes = 0;
+    check(g_entry.norm_bytes(&n.d, n.device, nullptr, &bytes), "group norm's gradients");
+    const at::Tensor ws = scratch(n.x, bytes);
+    check(g_entry.norm_backward(&n.d, address(grad), address(n.x), static_cast<const float *>(address(statistics)), address(n.scale), address(n.offset), address(n.residual),
+                                out_address(dx), out_address(dscale), out_address(doffset), out_address(dresidual), out_address(ws), bytes, n.device, stream_of(n.x)),
+          "group norm's gradients");
+    PyObject *r = nullptr;
+    if (same) {                                                // its gradient is the output's
+        Py_INCREF(a[0]);
+        r = a[0];
+    } else r = wrap(dresidual);
+    return Py_BuildValue("(NNNN)", wrap(dx), wrap(dscale), wrap(doffset), r);
+    AXC_TORCH_END
+}
+
+// dropout(x, rate, seed, offset: an int or one int64 on x's device, residual) -> y
+PyObject *dropout(PyObject *, PyObject *const *a, Py_ssize_t count)
+{
+    AXC_TORCH_BEGIN
+    if (count != 5) invalid("dropout takes 5 arguments");
+    c10::NoGradGuard no_grad;
+    at::Tensor x = tensor_of(a[0], "x", false);
+    if (!x.is_cuda() || type_of(x) < 0) invalid("x must be a float32, bfloat16 or float16 CUDA tensor (this build has no CPU kernel)");
+    axc_dropout_desc d = {};
+    d.rate = PyFloat_AsDouble(a[1]);
+    if (PyErr_Occurred()) throw Raised();
+    if (!(d.rate >= 0.0 && d.rate <= 1.0)) invalid("a rate must lie in [0, 1]");
+    auto word = [](PyObject *o, const char *what) {
+        if (!PyLong_Check(o)) invalid(std::string(what) + " must be an int in [0, 2^64)");
+        const unsigned long long v = PyLong_AsUnsignedLongLong(o);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            invalid(std::string(what) + " must be an int in [0, 2^64)");
+        }
+        return uint64_t(v);
+    };
+    d.seed = word(a[2], "a seed");
+    at::Tensor offset;
+    if (THPVariable_Check(a[3])) {
+        offset = THPVariable_Unpack(a[3]);
+        if (offset.scalar_type() != at::kLong || offset.numel() != 1 || offset.device() != x.device()) invalid("an offset that is a tensor must be one int64 on x's device");
+    } else d.offset = word(a[3], "an offset");
+    const at::Tensor residual = like_x(a[4], "residual", x, true);
+    x = x.contiguous();
+    d.count = x.numel();
+    d.type = type_of(x);
+    const at::Tensor y = at::empty(x.sizes(), x.options());
+    check(g_entry.dropout(&d, address(x), address(residual), out_address(y), static_cast<const int64_t *>(address(offset)), x.device().index(), stream_of(x)), "dropout");
+    return wrap(y);
+    AXC_TORCH_END
+}
+
 // init(addresses of the entry points, InvalidArgumentError, InternalError, raise_for_status)
 PyObject *init(PyObject *, PyObject *args)
 {
-    unsigned long long p[8];
-    PyObject *i, *e, *r;
-    if (!PyArg_ParseTuple(args, "(KKKKKKKK)OOO", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &i, &e, &r)) return nullptr;
-    g_entry.dense_bytes = reinterpret_cast<decltype(g_entry.dense_bytes)>(p[0]);
-    g_entry.dense_forward = reinterpret_cast<decltype(g_entry.dense_forward)>(p[1]);
-    g_entry.dense_backward = reinterpret_cast<decltype(g_entry.dense_backward)>(p[2]);
-    g_entry.status = reinterpret_cast<decltype(g_entry.status)>(p[3]);
-    g_entry.entropy_bytes = reinterpret_cast<decltype(g_entry.entropy_bytes)>(p[4]);
-    g_entry.entropy = reinterpret_cast<decltype(g_entry.entropy)>(p[5]);
-    g_entry.adamw = reinterpret_cast<decltype(g_entry.adamw)>(p[6]);
-    g_entry.scale = reinterpret_cast<decltype(g_entry.scale)>(p[7]);
+    PyObject *addresses, *i, *e, *r;
+    if (!PyArg_ParseTuple(args, "O!OOO", &PyTuple_Type, &addresses, &i, &e, &r)) return nullptr;
+    // (every entry is a function's address, in the order of Entry)
+    constexpr Py_ssize_t kEntries = sizeof(Entry) / sizeof(void *);
+    if (PyTuple_GET_SIZE(addresses) != kEntries) {
+        PyErr_Format(PyExc_ValueError, "%zd entry points expected", kEntries);
+        return nullptr;
+    }
+    void *p[kEntries];
+    for (Py_ssize_t k = 0; k < kEntries; ++k) p[k] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, k));
+    if (PyErr_Occurred()) return nullptr;
+    static_assert(sizeof(p) == sizeof(g_entry), "Entry has nothing but addresses");
+    std::memcpy(static_cast<void *>(&g_entry), p, sizeof(p));
     Py_INCREF(i);
     Py_INCREF(e);
     Py_INCREF(r);
@@ -436,6 +585,9 @@ PyMethodDef g_methods[] = {{"init", init, METH_VARARGS, nullptr},
                            {"entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entropy)), METH_FASTCALL, nullptr},
                            {"scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scaled)), METH_FASTCALL, nullptr},
                            {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_step)), METH_FASTCALL, nullptr},
+                           {"group_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_forward)), METH_FASTCALL, nullptr},
+                           {"group_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_backward)), METH_FASTCALL, nullptr},
+                           {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dropout)), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_axc_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

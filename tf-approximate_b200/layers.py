@@ -4,7 +4,7 @@ input and kernel, the table convolution, then bias and activation; the backward 
 convolution's (the reference registers `conv2d_backprop_input/filter` as the gradient, :264-302)."""
 import torch
 
-from . import dense_ops, ops
+from . import dense_ops, norm_ops, ops
 from .ops import approx_conv2d_with_min_max_vars
 
 
@@ -228,3 +228,49 @@ class Dense(torch.nn.Module):
         if self.activation not in (None, "none", "linear"):
             raise ops.InvalidArgumentError("the logits of a cross entropy have no activation")
         return dense_ops.dense_cross_entropy(inputs.to(self.kernel.dtype), self.kernel, labels, self.bias, ignore_index, reduction)
+
+
+class GroupNorm(torch.nn.Module):
+    """Group norm of tensors with their channels last, in the manner of Keras' GroupNormalization, with the activation that follows it (and, where
+    the call has one, the shortcut that is added before it): activation(normalised inputs * scale + offset + residual)."""
+
+    def __init__(self, channels, groups=32, activation=None, epsilon=1e-3, use_scale=True, use_offset=True, dtype=torch.float32):
+        super().__init__()
+        dense_ops._activation(activation)                       # refuses an unknown name here, not at the first call
+        if groups < 1 or channels < 1 or channels % groups:
+            raise ops.InvalidArgumentError("the channels (%d) must be a multiple of the groups (%d)" % (channels, groups))
+        self.groups, self.activation, self.epsilon = groups, activation, epsilon
+        self.scale = torch.nn.Parameter(torch.ones(channels, dtype=dtype)) if use_scale else None
+        self.offset = torch.nn.Parameter(torch.zeros(channels, dtype=dtype)) if use_offset else None
+
+    def forward(self, inputs, residual=None):
+        return norm_ops.group_norm(inputs, self.groups, self.scale, self.offset, residual, self.activation, self.epsilon)
+
+
+class Dropout(torch.nn.Module):
+    """Dropout without a stored mask, in the manner of the Keras layer; in evaluation the inputs pass.  `calls`, which picks the mask and counts up with
+    every call in training, is an int, or with `capturable` one int64 on the inputs' device that the call itself counts up, so that a captured step
+    has another mask at every replay.  seed: None for one of torch's."""
+
+    def __init__(self, rate, seed=None, capturable=False):
+        super().__init__()
+        if not 0.0 <= rate <= 1.0:
+            raise ops.InvalidArgumentError("a rate must lie in [0, 1]")
+        self.rate = float(rate)
+        self.seed = int(torch.randint(1 << 62, ()).item()) if seed is None else seed
+        self.capturable = capturable
+        if capturable:
+            self.register_buffer("calls", torch.zeros((), dtype=torch.int64))
+        else:
+            self.calls = 0
+
+    def forward(self, inputs, residual=None):
+        if not self.training:
+            return inputs if residual is None else inputs + residual
+        if self.capturable:
+            offset = self.calls.clone()                         # the backward pass reads this call's own
+            self.calls.add_(1)
+        else:
+            offset = self.calls
+            self.calls += 1
+        return norm_ops.dropout(inputs, self.rate, self.seed, offset, residual)
