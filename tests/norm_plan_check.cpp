@@ -27,17 +27,22 @@ static long long pick(long long lo, long long hi)
     } while (0)
 
 template <int V>
-static void block(const NormShape &s, const NormPlan &p, int active, int span, long long sample, long long place0, int places, int channel0, std::vector<unsigned char> &seen,
+static void block(const NormShape &s, const NormPlan &p, const Span &sp, long long sample, long long place0, int places, int channel0, std::vector<unsigned char> &seen,
                   long long steps)
 {
+    const int active = sp.active, span = sp.channels;
     const int shift = V == 1 || span < s.channels ? 0 : int((sample * s.places + place0) * s.channels & (V - 1));
-    const Entries E(active, V, span, shift, places * span);
+    const Entries E(sp, shift, places * span);
+    CHECK(places * (long long)span <= (1 << 20) + span);
     std::vector<int> count(size_t(active) * V), channel(size_t(active) * V, -1);
     CHECK(active > 0 && active <= p.threads && (active * V) % span == 0);
     for (int t = 0; t < p.threads; ++t) {
-        const Walk<V> w(t, active, shift, places, span, s.channels, place0, channel0);
+        const Walk<V> w(t, sp, shift, places, s.channels, place0, channel0);
         CHECK(steps < 0 || w.count <= steps);
         CHECK(t < active || w.count == 0);
+        int local[V], group[V];
+        local_channels<V>(w, sp, p.resident ? divider(unsigned(s.each())) : sp.by_channels, local, group);
+        CHECK(w.count == (t < active && w.o < w.total ? (w.total - 1 - w.o) / w.each + 1 : 0));
         for (int j = 0; j < w.count; ++j) {
             const long long first = sample * s.places * s.channels + w.at + j * w.step;
             if (w.whole(j)) CHECK(first % V == 0 || V == 1);
@@ -49,7 +54,8 @@ static void block(const NormShape &s, const NormPlan &p, int active, int span, l
                 }
                 CHECK(first + i >= sample * s.places * s.channels && first + i < (sample + 1) * s.places * s.channels);
                 const int c = int((first + i) % s.channels);
-                CHECK(c == channel0 + local_channel<V>(w, span, i));
+                CHECK(c == channel0 + local[i]);
+                CHECK(!p.resident || c / s.each() == (channel0 + group[i] * s.each()) / s.each());
                 ++seen[size_t(first + i)];
                 ++count[size_t(t) * V + i];
                 channel[size_t(t) * V + i] = c - channel0;
@@ -59,8 +65,9 @@ static void block(const NormShape &s, const NormPlan &p, int active, int span, l
     std::vector<unsigned char> used(size_t(active) * V);
     for (int l = 0; l < span; ++l)
         for (int k = 0; k < E.copies; ++k) {
-            const int e = E.entry(l, k);
+            const int e = E.first_entry(l) + k * span;
             CHECK(e >= 0 && e < active * V && !used[e]);
+            CHECK(e / span == k && E.place(e, k) == e + k && E.place(e, k) < entry_places(sp));
             used[e] = 1;
             CHECK(channel[e] == -1 || channel[e] == l);
             CHECK(int(E.values(e)) == count[e]);
@@ -69,7 +76,7 @@ static void block(const NormShape &s, const NormPlan &p, int active, int span, l
 }
 
 template <int V>
-static void whole(const NormShape &s, const NormPlan &p, int kept, int sums)
+static void whole(const NormShape &s, const NormPlan &p, int sums)
 {
     std::vector<unsigned char> seen(size_t(s.values()));
     const int spans = int((s.channels + p.span - 1) / p.span);
@@ -79,21 +86,27 @@ static void whole(const NormShape &s, const NormPlan &p, int kept, int sums)
             if (p.resident) {
                 CHECK(s.channels % p.span == 0 && p.span % s.each() == 0 && p.blocks >= 1 && p.blocks <= s.places);
                 const int active = norm_active(p.threads, p.span, p.vec), groups = int(p.span / s.each());
+                const Span sp = span_of(p.span, active, p.vec);
                 const long long steps = norm_steps((s.places + p.blocks - 1) / p.blocks, p.span, p.vec, active);
                 const size_t slots = size_t(steps) * active * p.vec;
-                const size_t used = sums ? norm_up16(slots * 4) + norm_up16(slots * s.size) + size_t(active) * p.vec * 8 + size_t(p.span) * 8 + size_t(groups) * 16
-                                         : norm_up16(slots * s.size) + size_t(active) * p.vec * 8 + size_t(groups) * 16;
-                CHECK(used <= p.smem && p.smem <= kNormSmem);
+                // as the kernels lay it out
+                const size_t data = (sums ? 2 : 1) * norm_up16(slots * s.size);
+                CHECK(data + size_t(entry_places(sp)) * 8 + size_t(p.span) * 8 * sums + size_t(groups) * 16 <= p.smem && p.smem <= kNormSmem);
+                const long long per = (s.places + p.blocks - 1) / p.blocks;
+                CHECK(per * (p.blocks - 1) < s.places);
                 for (int r = 0; r < p.blocks; ++r) {
-                    const long long p0 = s.places * r / p.blocks, p1 = s.places * (r + 1) / p.blocks;
-                    block<V>(s, p, active, p.span, n, p0, int(p1 - p0), channel0, seen, steps);
+                    const long long p0 = r * per, p1 = p0 + per < s.places ? p0 + per : s.places;
+                    block<V>(s, p, sp, n, p0, int(p1 - p0), channel0, seen, steps);
                 }
             } else {
                 const int span = int(s.channels - channel0 < p.span ? s.channels - channel0 : p.span);
-                const int active = span == p.span ? norm_active(p.threads, p.span, p.vec) : p.threads / (span / V) * (span / V);
+                const Span sp = span_of(span, norm_active(p.threads, span, p.vec), p.vec);
+                CHECK(entry_places(sp) <= 2 * kNormThreads * V);
+                const long long per = (s.places + p.shares - 1) / p.shares;
+                CHECK(per * (p.shares - 1) < s.places);
                 for (long long h = 0; h < p.shares; ++h) {
-                    const long long p0 = s.places * h / p.shares, p1 = s.places * (h + 1) / p.shares;
-                    block<V>(s, p, active, span, n, p0, int(p1 - p0), channel0, seen, -1);
+                    const long long p0 = h * per, p1 = p0 + per < s.places ? p0 + per : s.places;
+                    block<V>(s, p, sp, n, p0, int(p1 - p0), channel0, seen, -1);
                 }
             }
         }
@@ -114,13 +127,14 @@ int main(int argc, char **argv)
         s.size = pick(0, 1) ? 2 : 4;
         s.aligned = pick(0, 4) != 0;
         for (int backward = 0; backward < 2; ++backward) {
-            const NormPlan p = backward ? norm_plan(s, s.size + 4, 3 * s.size, 1, 148) : norm_plan(s, s.size, 2 * s.size, 0, 148);
+            const bool residual = pick(0, 1);
+            const NormPlan p = norm_plan(s, (1 + backward) * s.size, (backward ? residual ? 5 : 3 : residual ? 3 : 2) * s.size, backward, 148);
             ++(p.resident ? resident : twice);
             if (p.vec == 1) ++single;
             else if (s.channels % p.vec) ++loose;
-            if (p.vec == 8) whole<8>(s, p, s.size, backward);
-            else if (p.vec == 4) whole<4>(s, p, s.size, backward);
-            else whole<1>(s, p, s.size, backward);
+            if (p.vec == 8) whole<8>(s, p, backward);
+            else if (p.vec == 4) whole<4>(s, p, backward);
+            else whole<1>(s, p, backward);
         }
     }
     std::printf("resident %d, twice %d, single values %d, loose lines %d\n", resident, twice, single, loose);

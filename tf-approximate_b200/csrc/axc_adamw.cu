@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "axc_internal.h"
+#include "axc_two.cuh"
 
 namespace axc {
 namespace {
@@ -66,38 +67,6 @@ __device__ __forceinline__ float square_root(float x)
     float r;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
-}
-
-// Two fp32 values that one instruction computes with
-struct Two {
-    unsigned long long v;
-    __device__ __forceinline__ Two() {}
-    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
-    __device__ __forceinline__ float2 both() const
-    {
-        float2 f;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-        return f;
-    }
-};
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
-{
-    Two d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
-__device__ __forceinline__ Two add2(Two a, Two b)
-{
-    Two d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b)
-{
-    Two d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
 }
 
 __device__ __forceinline__ float to_float(float x) { return x; }

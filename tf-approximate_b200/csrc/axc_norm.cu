@@ -16,9 +16,11 @@
 // start anywhere, too (20 channels of fp16: 5 vectors hold two lines), as a whole tensor has no gaps.  A vector that sticks out of what a block
 // has, at its start or its end, is moved value by value.
 //
-// Sums are fp32.  Those of the variance are never of squares that nearly cancel: a thread adds the squares of a few values less their own mean, and
-// means and squares are joined pair by pair (Chan, Golub and LeVeque).  Every sum has a fixed order.
-// Between the two passes of the gradients dz stays fp32.  Nothing is rounded to fewer bits but the outputs.
+// Sums are fp32.  Those of the variance are never of squares that nearly cancel: a thread adds the squares of up to 32 values less the first of them,
+// and means and squared distances are joined by their means (Chan, Golub and LeVeque).  Every sum has a fixed order.
+// Roundings to 16 bits: the outputs, and dz of resident spans, which dx is made of (the sums take it before), as the dense layer's dz is: fp32
+// would take half as much shared memory again, which is what bounds how many loads are on their way (256 x 56 x 56 x 256 with a shortcut:
+// see below).  It makes dx off by 0.0024 in all where its own rounding alone makes 0.0017 (bf16).
 #include <atomic>
 #include <type_traits>
 #include <vector>
@@ -26,6 +28,7 @@
 #include "axc_gemm.h"
 #include "axc_mma.cuh"
 #include "axc_norm_plan.h"
+#include "axc_two.cuh"
 
 namespace axc {
 namespace {
@@ -38,10 +41,16 @@ struct NormArgs {
     long long samples, places, channels;
     int groups, each;                          // channels of a group: each
     float2 *statistics;                        // [samples][groups] {mean, r}
-    int span, spans, blocks, active;           // channels of a block's span, spans of a sample, blocks that share one
+    Span span, last;                           // of a block; the last one of a line may be narrower where the tensors are read twice
+    int spans, blocks;                         // spans of a line, blocks that share one
+    long long per;                             // places of a block; the last one has the rest
+    int steps, span_groups;                    // resident: steps that the threads take, groups of a span
+    bool whole_vectors;                        // a thread's channels are neighbours, and of one group
+    Span vectors;                              // then: the span's vectors in place of its channels
+    Divider by_group;                          // channels of a group
     long long shares;
     float2 *part;                              // [samples][shares][channels] sums of a share of the places
-    float2 *sums;                              // [samples][channels] {sum of dz, sum of dz xhat}
+    float2 *sums;                              // [samples][channels] {sum of dz, sum of dz xhat}; may be NULL
     float2 *group_sums;                        // [samples][groups] {S1 r / m, S2 r r / m}
     void *dscale, *doffset;
     __host__ __device__ long long values() const { return samples * places * channels; }
@@ -62,28 +71,70 @@ union Pack {
 template <typename T, int V>
 __device__ __forceinline__ int shift_of(const NormArgs &P, long long sample, long long place0)
 {
-    return V == 1 || P.span < P.channels ? 0 : int((sample * P.places + place0) * P.channels & (V - 1));
+    return V == 1 || P.span.channels < P.channels ? 0 : int((sample * P.places + place0) * P.channels & (V - 1));
 }
 
+// Pairs that hold V values; a single one has nothing beside it
+template <int V> constexpr int kPairs = (V + 1) / 2;
+
 template <typename T, int V>
-__device__ __forceinline__ void load(const T *sample, const Walk<V> &w, int j, Pack<T, V> &v, [[maybe_unused]] const T *base, [[maybe_unused]] long long count)
+__device__ __forceinline__ void widen_pairs(const Pack<T, V> &v, Two (&x)[kPairs<V>])
 {
-    const T *from = sample + w.at + j * w.step;
-    if (w.whole(j)) {
+    if constexpr (V == 1) x[0] = Two(widen(v.t[0]), 0.0f);
+    else {
+        const unsigned w[4] = {v.w.x, v.w.y, v.w.z, v.w.w};
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            if constexpr (sizeof(T) == 4) x[i] = Two(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) x[i] = Two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            else {
+                const float2 f = __half22float2(reinterpret_cast<const __half2 &>(w[i]));
+                x[i] = Two(f.x, f.y);
+            }
+        }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> narrow_pairs(const Two (&x)[kPairs<V>])
+{
+    Pack<T, V> v;
+    if constexpr (V == 1) v.t[0] = narrow<T>(x[0].both().x);
+    else {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = x[i].both();
+            if constexpr (sizeof(T) == 4) {
+                w[2 * i] = __float_as_uint(f.x);
+                w[2 * i + 1] = __float_as_uint(f.y);
+            } else w[i] = pack2(f.x, f.y, std::is_same<T, __nv_bfloat16>::value);
+        }
+        v.w = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+__device__ __forceinline__ void set_lane(Two &x, int lane, float v)
+{
+    const float2 f = x.both();
+    x = lane ? Two(f.x, v) : Two(v, f.y);
+}
+
+// The j-th vector of a tensor, at `from`: whole, or value by value where some are outside of the block's.  base, count: all there is.
+template <bool WHOLE, typename T, int V>
+__device__ __forceinline__ void load(const T *from, const Walk<V> &w, int j, Pack<T, V> &v, [[maybe_unused]] const T *base, [[maybe_unused]] long long count)
+{
+    if (WHOLE) {
         if (AXC_VALUES_OK(from, V, base, count, 501u)) v.w = *reinterpret_cast<const typename Bits<V * sizeof(T)>::type *>(from);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) v.t[i] = w.has(j, i) && AXC_VALUES_OK(from + i, 1, base, count, 502u) ? from[i] : narrow<T>(0.0f);
     }
 }
-template <typename T, int V>
-__device__ __forceinline__ void store(T *sample, const Walk<V> &w, int j, const float (&x)[V], [[maybe_unused]] T *base, [[maybe_unused]] long long count)
+template <bool WHOLE, typename T, int V>
+__device__ __forceinline__ void store(T *to, const Walk<V> &w, int j, const Two (&x)[kPairs<V>], [[maybe_unused]] T *base, [[maybe_unused]] long long count)
 {
-    T *to = sample + w.at + j * w.step;
-    Pack<T, V> v;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v.t[i] = narrow<T>(x[i]);
-    if (w.whole(j)) {
+    const Pack<T, V> v = narrow_pairs<T, V>(x);
+    if (WHOLE) {
         if (AXC_VALUES_OK(to, V, base, count, 503u)) *reinterpret_cast<typename Bits<V * sizeof(T)>::type *>(to) = v.w;
     } else {
 #pragma unroll
@@ -92,179 +143,309 @@ __device__ __forceinline__ void store(T *sample, const Walk<V> &w, int j, const 
     }
 }
 
-template <int V, bool EXACT>
-__device__ __forceinline__ void activate_all(float (&z)[V], int act)
+// body(whole, how many, the first) for all vectors of a thread, N whole ones at a time as long as there are so many
+template <int V, typename N, typename Body>
+__device__ __forceinline__ void batches(const Walk<V> &w, N n, Body body)
 {
-    if (act == kActNone) return;
-    if (act == kActRelu) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], kActRelu, EXACT);
-    } else if (act == kActGelu) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], kActGelu, EXACT);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], kActSilu, EXACT);
-    }
-}
-// d *= act'(z)
-template <int V, bool EXACT>
-__device__ __forceinline__ void slopes(float (&d)[V], const float (&z)[V], int act)
-{
-    if (act == kActNone) return;
-    if (act == kActRelu) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[i] *= slope_of<kActRelu, EXACT>(z[i]);
-    } else if (act == kActGelu) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[i] *= slope_of<kActGelu, EXACT>(z[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[i] *= slope_of<kActSilu, EXACT>(z[i]);
+    const std::integral_constant<int, 1> one;
+    int j = w.first;
+    for (; j + N::value <= w.end; j += N::value) body(std::true_type(), n, j);
+    for (; j < w.end; ++j) body(std::true_type(), one, j);
+    if constexpr (V > 1) {
+        if (w.first > 0) body(std::false_type(), one, 0);
+        if (w.end < w.count) body(std::false_type(), one, w.end);
     }
 }
 
-// Mean and sum of squared distances from it, for each of a thread's channels
-template <int V>
-struct Moments {
-    float n = 0.0f, mean[V], square[V];        // n: whole vectors so far
-    template <int N>
-    __device__ __forceinline__ void add(const float (&v)[N][V])
-    {
-        const float sum = n + N, w = __fdividef(float(N), sum), w2 = n * w;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float m = v[0][i], q = 0.0f;
-#pragma unroll
-            for (int k = 1; k < N; ++k) m += v[k][i];
-            m *= 1.0f / N;
-#pragma unroll
-            for (int k = 0; k < N; ++k) q = fmaf(v[k][i] - m, v[k][i] - m, q);
-            if (n == 0.0f) {
-                mean[i] = m;
-                square[i] = q;
-            } else {
-                const float d = m - mean[i];
-                mean[i] = fmaf(d, w, mean[i]);
-                square[i] = fmaf(d * d, w2, square[i] + q);
+// All vectors of a thread into its own places of shared memory, `stride` apart, asynchronously where there is a copy of that size: nothing waits
+// for one before the next is on its way, and what a thread has copied it alone reads, after wait_copies().
+template <typename T, int V, typename Word>
+__device__ __forceinline__ void fetch(const T *sample, const Walk<V> &w, Word *to, int stride, const T *base, long long count)
+{
+    constexpr int kBytes = V * sizeof(T);
+    if constexpr (kBytes >= 4) {
+        const T *from = sample + w.at + w.first * w.step;
+        unsigned place = mma::smem_address(to) + unsigned(w.first * stride) * unsigned(sizeof(Word));
+#pragma unroll 4
+        for (int j = w.first; j < w.end; ++j) {
+            if (AXC_VALUES_OK(from, V, base, count, 519u)) {
+                if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place), "l"(from) : "memory");
+                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(place), "l"(from) : "memory");
+            }
+            from += w.step;
+            place += unsigned(stride) * unsigned(sizeof(Word));
+        }
+        if constexpr (V > 1) {
+            for (int side = 0; side < 2; ++side) {
+                if (side == 0 ? w.first == 0 : w.end == w.count) continue;
+                const int j = side == 0 ? 0 : w.end;
+                Pack<T, V> v;
+                load<false>(sample + w.at + j * w.step, w, j, v, base, count);
+                to[j * stride] = v.w;
             }
         }
-        n = sum;
+    } else {
+        constexpr int N = 8;
+        for (int j = 0; j < w.count; j += N) {
+            Pack<T, V> v[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (j + k < w.count) load<true>(sample + w.at + (j + k) * w.step, w, j + k, v[k], base, count);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (j + k < w.count) to[(j + k) * stride] = v[k].w;
+        }
+    }
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// 1 / (1 + exp(-z)) for 16-bit results: 2^(-z log2 e), and both approximations good to 2^-22
+__device__ __forceinline__ Two sigmoid2(Two z)
+{
+    const float2 t = mul2(z, Two(-1.44269504f)).both();
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    const float2 d = add2(Two(e.x, e.y), Two(1.0f)).both();
+    return Two(reciprocal(d.x), reciprocal(d.y));
+}
+template <int H, bool EXACT>
+__device__ __forceinline__ void activate_pairs(Two (&z)[H], int act)
+{
+    if (act == kActNone) return;
+    if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if constexpr (EXACT) {
+                const float2 f = z[i].both();
+                z[i] = Two(activate(f.x, kActSilu, true), activate(f.y, kActSilu, true));
+            } else z[i] = mul2(z[i], sigmoid2(z[i]));
+        }
+    } else if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float2 f = z[i].both();
+            z[i] = Two(activate(f.x, kActRelu, EXACT), activate(f.y, kActRelu, EXACT));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float2 f = z[i].both();
+            z[i] = Two(activate(f.x, kActGelu, EXACT), activate(f.y, kActGelu, EXACT));
+        }
+    }
+}
+// d *= act'(z)
+template <int ACT, bool EXACT>
+__device__ __forceinline__ Two slope2(Two z)
+{
+    const float2 f = z.both();
+    return Two(slope_of<ACT, EXACT>(f.x), slope_of<ACT, EXACT>(f.y));
+}
+template <int H, bool EXACT>
+__device__ __forceinline__ void slopes(Two (&d)[H], const Two (&z)[H], int act)
+{
+    if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if constexpr (EXACT) d[i] = mul2(d[i], slope2<kActSilu, true>(z[i]));
+            else {
+                const Two s = sigmoid2(z[i]);
+                d[i] = mul2(d[i], mul2(s, fma2(z[i], fma2(s, Two(-1.0f), Two(1.0f)), Two(1.0f))));
+            }
+        }
+    } else if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) d[i] = mul2(d[i], slope2<kActRelu, EXACT>(z[i]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < H; ++i) d[i] = mul2(d[i], slope2<kActGelu, EXACT>(z[i]));
+    }
+}
+
+// Mean and sum of squared distances from it, for each of a thread's channels.  Values are counted from the first of a run of up to kRun, so the
+// sum of their squares is at most as many times that of the distances from the mean as the run has values, whatever they are: the difference
+// loses no more than that.  Runs are joined by their means.
+constexpr int kRun = 32;
+template <int V>
+struct Moments {
+    static constexpr int H = kPairs<V>;
+    float n = 0.0f;                            // whole vectors in the runs that are over
+    Two mean[H], square[H];
+    Two pivot[H], sum[H], squares[H];          // of this run
+    template <typename T>
+    __device__ __forceinline__ void open(const Pack<T, V> &v)
+    {
+        widen_pairs<T, V>(v, pivot);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            pivot[i] = mul2(pivot[i], Two(-1.0f));
+            sum[i] = squares[i] = Two(0.0f);
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void add(const Pack<T, V> &v)
+    {
+        Two x[H];
+        widen_pairs<T, V>(v, x);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const Two d = add2(x[i], pivot[i]);
+            sum[i] = add2(sum[i], d);
+            squares[i] = fma2(d, d, squares[i]);
+        }
+    }
+    // `k`: values of the run
+    __device__ __forceinline__ void close(float k)
+    {
+        const float all = n + k, w = __fdividef(k, all);
+        const Two share(__fdividef(1.0f, k)), minus(-1.0f), w1(w), w2(n * w);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const Two m = mul2(sum[i], share), q = fma2(mul2(m, minus), sum[i], squares[i]), at = fma2(pivot[i], minus, m);
+            if (n == 0.0f) {
+                mean[i] = at;
+                square[i] = q;
+            } else {
+                const Two d = fma2(mean[i], minus, at);
+                mean[i] = fma2(d, w1, mean[i]);
+                square[i] = fma2(mul2(d, d), w2, add2(square[i], q));
+            }
+        }
+        n = all;
     }
     // one value of channel i, which has had `k` so far
     __device__ __forceinline__ void add_one(int i, float v, float k)
     {
+        const float2 m2 = mean[i / 2].both(), s2 = square[i / 2].both();
+        float m = i & 1 ? m2.y : m2.x, s = i & 1 ? s2.y : s2.x;
         if (k == 0.0f) {
-            mean[i] = v;
-            square[i] = 0.0f;
+            m = v;
+            s = 0.0f;
         } else {
-            const float d = v - mean[i];
-            mean[i] += __fdividef(d, k + 1.0f);
-            square[i] = fmaf(d, v - mean[i], square[i]);
+            const float d = v - m;
+            m += __fdividef(d, k + 1.0f);
+            s = fmaf(d, v - m, s);
         }
+        set_lane(mean[i / 2], i & 1, m);
+        set_lane(square[i / 2], i & 1, s);
+    }
+    __device__ __forceinline__ float2 of(int i) const
+    {
+        const float2 m = mean[i / 2].both(), s = square[i / 2].both();
+        return i & 1 ? make_float2(m.y, fmaxf(s.y, 0.0f)) : make_float2(m.x, fmaxf(s.x, 0.0f));
     }
 };
 
-// x's moments, `chunk` vectors on their way at a time; keep(j, vector) sees every vector
-template <typename T, int V, typename Keep>
-__device__ __forceinline__ void take_moments(const T *sample, const Walk<V> &w, Moments<V> &mo, const T *base, long long count, Keep keep)
+// The moments of a thread's vectors; get(j, vector, whether it is whole) has the j-th, N of them at a time
+template <int N, typename T, int V, typename Get>
+__device__ __forceinline__ void take_moments(const Walk<V> &w, Moments<V> &mo, Get get)
 {
-    constexpr int N = V == 1 ? 8 : 4;
-    const int first = w.count > 0 && !w.whole(0) ? 1 : 0, end = w.count > first && !w.whole(w.count - 1) ? w.count - 1 : w.count;
-    int j = first;
-    for (; j + N <= end; j += N) {
-        Pack<T, V> v[N];
-        float f[N][V];
+    for (int j0 = w.first; j0 < w.end; j0 += kRun) {
+        const int end = min(j0 + kRun, w.end);
+        int j = j0;
+        for (; j + N <= end; j += N) {
+            Pack<T, V> v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) load(sample, w, j + k, v[k], base, count);
+            for (int k = 0; k < N; ++k) get(j + k, v[k], std::true_type());
+            if (j == j0) mo.open(v[0]);
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            keep(j + k, v[k]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[k][i] = widen(v[k].t[i]);
+            for (int k = 0; k < N; ++k) mo.add(v[k]);
         }
-        mo.add(f);
-    }
-    if (j < end) {
-        Pack<T, V> v[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < end) load(sample, w, j + k, v[k], base, count);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < end) {
-                float f[1][V];
-                keep(j + k, v[k]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[0][i] = widen(v[k].t[i]);
-                mo.add(f);
-            }
-    }
-    if (V > 1 && (first > 0 || end < w.count)) {
-        float had[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) had[i] = mo.n;
-        for (int side = 0; side < 2; ++side) {
-            if (side == 0 ? first == 0 : end == w.count) continue;
-            const int at = side == 0 ? 0 : end;
+        for (; j < end; ++j) {
             Pack<T, V> v;
-            load(sample, w, at, v, base, count);
-            keep(at, v);
+            get(j, v, std::true_type());
+            if (j == j0) mo.open(v);
+            mo.add(v);
+        }
+        mo.close(float(end - j0));
+    }
+    if constexpr (V > 1) {
+        if (w.first > 0 || w.end < w.count) {
+            float had[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (w.has(at, i)) {
-                    mo.add_one(i, widen(v.t[i]), had[i]);
-                    had[i] += 1.0f;
-                }
+            for (int i = 0; i < V; ++i) had[i] = mo.n;
+            for (int side = 0; side < 2; ++side) {
+                if (side == 0 ? w.first == 0 : w.end == w.count) continue;
+                const int at = side == 0 ? 0 : w.end;
+                Pack<T, V> v;
+                get(at, v, std::false_type());
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (w.has(at, i)) {
+                        mo.add_one(i, widen(v.t[i]), had[i]);
+                        had[i] += 1.0f;
+                    }
+            }
         }
     }
 }
 
 // ---- sums over the threads of a block ------------------------------------------------------------------------------------------
-// Lanes that share one of `items` sums: a power of two
+// Lanes that share one of `items` sums, as a power of two: all 32, or what the block's threads allow
 __device__ __forceinline__ int lanes_for(int items)
 {
-    int q = 32;
-    while (q > 1 && q * items > int(blockDim.x)) q >>= 1;
-    return q;
+    const int each = int(blockDim.x) >= 32 * items ? 5 : 31 - __clz(max(1, int(float(blockDim.x) / float(items))));
+    return each;
 }
-__device__ __forceinline__ float over_lanes(float x, int q)
+__device__ __forceinline__ float over_lanes(float x, int log2)
 {
-    for (int o = q >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+#pragma unroll
+    for (int o = 4; o >= 0; --o)
+        if (o < log2) x += __shfl_xor_sync(0xffffffffu, x, 1 << o);
     return x;
 }
 
-// {mean, squared distances} of `items` neighbouring sets of `each` channels, from the threads' entries: give(item, mean, square) in one thread
-template <typename Give>
-__device__ __forceinline__ void join_moments(const float2 *entries, const Entries &E, int items, int each, float values, Give give)
+// A thread's sums into their places
+template <int V, typename Get>
+__device__ __forceinline__ void give_entries(float2 *entries, const Span &s, Get get)
 {
-    const int q = lanes_for(items), lane = threadIdx.x & (q - 1), step = int(blockDim.x) / q;
+    int e = int(threadIdx.x) * V, copy = int(s.by_channels.of(unsigned(e))), left = s.channels - (e - copy * s.channels);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        entries[e + copy] = get(i);
+        ++e;
+        if (--left == 0) ++copy, left = s.channels;
+    }
+}
+
+// {mean, squared distances} of `items` neighbouring sets of `each` channels, from the threads' entries, `of_entry` values each for every one that the
+// entry counts: give(item, mean, square) in one thread
+template <typename Give>
+__device__ __forceinline__ void join_moments(const float2 *entries, const Entries &E, int items, int each, float values, float of_entry, Give give)
+{
+    const int log2 = lanes_for(items), q = 1 << log2, lane = threadIdx.x & (q - 1), step = int(blockDim.x) >> log2;
+    const float share = __fdividef(1.0f, values);
     for (int first = 0; first < items; first += step) {
-        const int item = first + int(threadIdx.x) / q;
+        const int item = first + (int(threadIdx.x) >> log2);
         const bool mine = item < items;
         float sum = 0.0f;
         if (mine) {
-            for (int d = 0; d < each; ++d)
+            for (int d = 0; d < each; ++d) {
+                const int e0 = E.first_entry(item * each + d);
                 for (int k = lane; k < E.copies; k += q) {
-                    const int e = E.entry(item * each + d, k);
-                    const float n = E.values(e);
-                    if (n > 0.0f) sum = fmaf(n, entries[e].x, sum);
+                    const int e = e0 + k * E.span;
+                    const float n = of_entry * E.values(e);
+                    if (n > 0.0f) sum = fmaf(n, entries[E.place(e, k)].x, sum);
                 }
+            }
         }
-        const float mean = __fdiv_rn(over_lanes(sum, q), values);
+        const float mean = over_lanes(sum, log2) * share;
         float square = 0.0f;
         if (mine) {
-            for (int d = 0; d < each; ++d)
+            for (int d = 0; d < each; ++d) {
+                const int e0 = E.first_entry(item * each + d);
                 for (int k = lane; k < E.copies; k += q) {
-                    const int e = E.entry(item * each + d, k);
-                    const float n = E.values(e);
+                    const int e = e0 + k * E.span;
+                    const float n = of_entry * E.values(e);
                     if (n > 0.0f) {
-                        const float off = entries[e].x - mean;
-                        square += fmaf(n * off, off, entries[e].y);
+                        const float2 f = entries[E.place(e, k)];
+                        square += fmaf(n * (f.x - mean), f.x - mean, f.y);
                     }
                 }
+            }
         }
-        square = over_lanes(square, q);
+        square = over_lanes(square, log2);
         if (mine && lane == 0) give(item, mean, square);
     }
 }
@@ -273,18 +454,20 @@ __device__ __forceinline__ void join_moments(const float2 *entries, const Entrie
 template <typename Give>
 __device__ __forceinline__ void join_sums(const float2 *entries, const Entries &E, Give give)
 {
-    const int q = lanes_for(E.span), lane = threadIdx.x & (q - 1), step = int(blockDim.x) / q;
+    const int log2 = lanes_for(E.span), q = 1 << log2, lane = threadIdx.x & (q - 1), step = int(blockDim.x) >> log2;
     for (int first = 0; first < E.span; first += step) {
-        const int l = first + int(threadIdx.x) / q;
+        const int l = first + (int(threadIdx.x) >> log2);
         float a = 0.0f, b = 0.0f;
-        if (l < E.span)
+        if (l < E.span) {
+            const float2 *from = entries + E.first_entry(l);
             for (int k = lane; k < E.copies; k += q) {
-                const float2 f = entries[E.entry(l, k)];
+                const float2 f = from[k * (E.span + 1)];
                 a += f.x;
                 b += f.y;
             }
-        a = over_lanes(a, q);
-        b = over_lanes(b, q);
+        }
+        a = over_lanes(a, log2);
+        b = over_lanes(b, log2);
         if (l < E.span && lane == 0) give(l, a, b);
     }
 }
@@ -299,77 +482,183 @@ __device__ __forceinline__ float2 of_block(const float2 *at, int rank)
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// The same for all blocks of the cluster, all of them on their way at once; what lies behind the last block is this block's own, not used
+__device__ __forceinline__ void of_all(const float2 *at, int blocks, float2 (&f)[kNormCluster])
+{
+#pragma unroll
+    for (int r = 0; r < kNormCluster; ++r) f[r] = of_block(at, r < blocks ? r : 0);
+}
+__device__ __forceinline__ float2 sum_of_all(const float2 *at, int blocks)
+{
+    float2 f[kNormCluster], sum = make_float2(0.0f, 0.0f);
+    of_all(at, blocks, f);
+#pragma unroll
+    for (int r = 0; r < kNormCluster; ++r)
+        if (r < blocks) {
+            sum.x += f[r].x;
+            sum.y += f[r].y;
+        }
+    return sum;
+}
+
 // Where a resident block is
 struct Place {
-    long long sample, place0;
-    int rank, span, channel0, places;
+    long long sample, sample0;
+    int rank, span, channel0, place0, places;
     __device__ __forceinline__ explicit Place(const NormArgs &P)
     {
-        rank = P.blocks > 1 ? int(mma::cluster_rank()) : 0;
-        const unsigned unit = blockIdx.x / unsigned(P.blocks);
-        sample = unit / unsigned(P.spans);
-        span = int(unit - unsigned(sample) * unsigned(P.spans));
-        channel0 = span * P.span;
-        place0 = P.places * rank / P.blocks;
-        places = int(P.places * (rank + 1) / P.blocks - place0);
+        unsigned unit = blockIdx.x, n;
+        rank = 0;
+        if (P.blocks > 1) {
+            rank = int(mma::cluster_rank());
+            asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(unit));
+        }
+        n = P.spans > 1 ? unit / unsigned(P.spans) : unit;
+        sample = n;
+        sample0 = sample * P.places * P.channels;
+        span = int(unit - n * unsigned(P.spans));
+        channel0 = span * P.span.channels;
+        place0 = rank * int(P.per);
+        places = min(int(P.per), int(P.places) - place0);
     }
 };
+
+// A parameter at V channels, `none` where there is none; in_line: the channels are neighbours
+template <int V>
+__device__ __forceinline__ void load_parameters(const void *from, int type, const int (&c)[V], bool in_line, [[maybe_unused]] long long count, float none, float (&out)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = none;
+    if (!from) return;
+    if (type == kFloat32 && in_line) {
+        const float *at = static_cast<const float *>(from) + c[0];
+        if (!AXC_VALUES_OK(at, V, static_cast<const float *>(from), count, 505u)) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = at[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (AXC_GLOBAL_OK(c[i], count, 506u)) out[i] = load_as_float(from, c[i], type);
+    }
+}
 
 // What a thread needs of its channels
 template <int V>
 struct Channels {
-    float mean[V], factor[V], offset[V];
-    // channel(i), group's {mean, r}(channel)
-    template <typename Channel, typename Stats>
-    __device__ __forceinline__ void fill(const NormArgs &P, Channel channel, Stats stats)
+    static constexpr int H = kPairs<V>;
+    Two less[H], factor[H], offset[H];         // less: the mean with its sign turned
+    // stats(group of the span): {mean, r}; in_line: the channels are neighbours, and of one group
+    template <typename Stats>
+    __device__ __forceinline__ void fill(const NormArgs &P, int channel0, const int (&local)[V], const int (&group)[V], bool in_line, Stats stats)
     {
+        int c[V];
+        float a[V], b[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = channel(i);
-            const float2 s = stats(c);
-            mean[i] = s.x;
-            factor[i] = s.y * (P.scale && AXC_GLOBAL_OK(c, P.channels, 505u) ? load_as_float(P.scale, c, P.scale_type) : 1.0f);
-            offset[i] = P.offset && AXC_GLOBAL_OK(c, P.channels, 506u) ? load_as_float(P.offset, c, P.offset_type) : 0.0f;
+        for (int i = 0; i < V; ++i) c[i] = channel0 + local[i];
+        load_parameters<V>(P.scale, P.scale_type, c, in_line, P.channels, 1.0f, a);
+        load_parameters<V>(P.offset, P.offset_type, c, in_line, P.channels, 0.0f, b);
+        const float2 s0 = stats(group[0]);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const int k = V > 1 ? i + 1 : i;
+            const float2 s = in_line ? s0 : stats(group[i]), t = in_line ? s0 : stats(group[k]);
+            less[i / 2] = Two(-s.x, -t.x);
+            factor[i / 2] = Two(a[i] * s.y, a[k] * t.y);
+            offset[i / 2] = Two(b[i], b[k]);
         }
     }
-    __device__ __forceinline__ float z(int i, float x) const { return fmaf(x - mean[i], factor[i], offset[i]); }
 };
 
 // y of one vector
 template <typename T, int V>
-__device__ __forceinline__ void finish(const NormArgs &P, const Channels<V> &ch, const Walk<V> &w, int j, const Pack<T, V> &x, long long sample0)
+__device__ __forceinline__ void output_of(const NormArgs &P, const Channels<V> &ch, const Pack<T, V> &x, const Pack<T, V> &residual, Two (&z)[kPairs<V>])
 {
-    float z[V];
+    constexpr int H = kPairs<V>;
+    widen_pairs<T, V>(x, z);
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = ch.z(i, widen(x.t[i]));
+    for (int i = 0; i < H; ++i) z[i] = fma2(add2(z[i], ch.less[i]), ch.factor[i], ch.offset[i]);
     if (P.residual) {
-        Pack<T, V> r;
-        load(static_cast<const T *>(P.residual) + sample0, w, j, r, static_cast<const T *>(P.residual), P.values());
+        Two r[H];
+        widen_pairs<T, V>(residual, r);
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] += widen(r.t[i]);
+        for (int i = 0; i < H; ++i) z[i] = add2(z[i], r[i]);
     }
-    activate_all<V, sizeof(T) == 4>(z, P.activation);
-    store(static_cast<T *>(P.y) + sample0, w, j, z, static_cast<T *>(P.y), P.values());
+    activate_pairs<H, sizeof(T) == 4>(z, P.activation);
 }
 
 // dz of one vector, and x less its mean
 template <typename T, int V>
-__device__ __forceinline__ void slope_at(const NormArgs &P, const Channels<V> &ch, const Pack<T, V> &x, const Pack<T, V> &dy, const Pack<T, V> &residual, float (&dz)[V],
-                                         float (&off)[V])
+__device__ __forceinline__ void slope_at(const NormArgs &P, const Channels<V> &ch, const Pack<T, V> &x, const Pack<T, V> &dy, const Pack<T, V> &residual,
+                                         Two (&dz)[kPairs<V>], Two (&off)[kPairs<V>])
 {
-    float z[V];
+    constexpr int H = kPairs<V>;
+    widen_pairs<T, V>(x, off);
+    widen_pairs<T, V>(dy, dz);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        off[i] = widen(x.t[i]) - ch.mean[i];
-        z[i] = fmaf(off[i], ch.factor[i], ch.offset[i]);
-        dz[i] = widen(dy.t[i]);
-    }
-    if (P.residual && P.activation != kActNone) {
+    for (int i = 0; i < H; ++i) off[i] = add2(off[i], ch.less[i]);
+    if (P.activation == kActNone) return;
+    Two z[H];
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] += widen(residual.t[i]);
+    for (int i = 0; i < H; ++i) z[i] = fma2(off[i], ch.factor[i], ch.offset[i]);
+    if (P.residual) {
+        Two r[H];
+        widen_pairs<T, V>(residual, r);
+#pragma unroll
+        for (int i = 0; i < H; ++i) z[i] = add2(z[i], r[i]);
     }
-    slopes<V, sizeof(T) == 4>(dz, z, P.activation);
+    slopes<H, sizeof(T) == 4>(dz, z, P.activation);
 }
+// Sums of dz and of dz (x - mean); values outside of a block's are left out (their x and dy are zeros, which is not enough)
+template <int V>
+struct Sums {
+    static constexpr int H = kPairs<V>;
+    Two dz[H], off[H];
+    __device__ __forceinline__ Sums()
+    {
+#pragma unroll
+        for (int i = 0; i < H; ++i) dz[i] = off[i] = Two(0.0f);
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void add(const Walk<V> &w, int j, Two (&d)[H], const Two (&o)[H])
+    {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if (!WHOLE) {
+                const float2 f = d[i].both();
+                d[i] = Two(w.has(j, 2 * i) ? f.x : 0.0f, w.has(j, 2 * i + 1) ? f.y : 0.0f);
+            }
+            dz[i] = add2(dz[i], d[i]);
+            off[i] = fma2(d[i], o[i], off[i]);
+        }
+    }
+    __device__ __forceinline__ float2 of(int i) const
+    {
+        const float2 a = dz[i / 2].both(), b = off[i / 2].both();
+        return i & 1 ? make_float2(a.y, b.y) : make_float2(a.x, b.x);
+    }
+};
+// dx = dz factor - first - (x - mean) second
+template <int V>
+struct Gradient {
+    static constexpr int H = kPairs<V>;
+    Two first[H], second[H];                   // both with their signs turned
+    template <typename Stats>
+    __device__ __forceinline__ void fill(const int (&group)[V], bool in_line, Stats stats)
+    {
+        const float2 s0 = stats(group[0]);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 s = in_line ? s0 : stats(group[i]), t = in_line ? s0 : stats(group[V > 1 ? i + 1 : i]);
+            first[i / 2] = Two(-s.x, -t.x);
+            second[i / 2] = Two(-s.y, -t.y);
+        }
+    }
+    __device__ __forceinline__ void of(const Channels<V> &ch, const Two (&off)[H], Two (&d)[H]) const
+    {
+#pragma unroll
+        for (int i = 0; i < H; ++i) d[i] = fma2(second[i], off[i], fma2(d[i], ch.factor[i], first[i]));
+    }
+};
 
 // ---- resident spans -------------------------------------------------------------------------------------------------------------
 template <typename T, int V>
@@ -378,63 +667,89 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_forward_kernel(const Nor
     after_previous();
     extern __shared__ __align__(16) char raw[];
     const Place at(P);
-    const int shift = shift_of<T, V>(P, at.sample, at.place0);
-    const Walk<V> w(threadIdx.x, P.active, shift, at.places, P.span, P.channels, at.place0, at.channel0);
-    const int steps = (int((P.places + P.blocks - 1) / P.blocks) * P.span + V - 1 + P.active * V - 1) / (P.active * V), groups = P.span / P.each;
+    const int shift = shift_of<T, V>(P, at.sample, at.place0), thread = threadIdx.x, groups = P.span_groups, stride = P.span.active;
+    const Walk<V> w(thread, P.span, shift, at.places, P.channels, at.place0, at.channel0);
     typedef typename Bits<V * sizeof(T)>::type Word;
-    Word *kept = reinterpret_cast<Word *>(raw);
-    float2 *entries = reinterpret_cast<float2 *>(raw + norm_up16(size_t(steps) * P.active * V * sizeof(T)));
-    float2 *mine = entries + P.active * V, *result = mine + groups;
-    const long long sample0 = at.sample * P.places * P.channels;
-    const T *x = static_cast<const T *>(P.x);
+    const size_t room = norm_up16(size_t(P.steps) * P.span.active * V * sizeof(T));
+    Word *kept = reinterpret_cast<Word *>(raw) + thread;
+    float2 *entries = reinterpret_cast<float2 *>(raw + room);
+    float2 *mine = entries + entry_places(P.span), *result = mine + groups;
+    const T *x = static_cast<const T *>(P.x), *residual = static_cast<const T *>(P.residual);
+    fetch<T, V>(x + at.sample0, w, kept, stride, x, P.values());
+    wait_copies();
     Moments<V> mo;
-    take_moments(x + sample0, w, mo, x, P.values(), [&](int j, const Pack<T, V> &v) { kept[j * P.active + int(threadIdx.x)] = v.w; });
-    if (int(threadIdx.x) < P.active) {
+    take_moments<2, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto) { v.w = kept[j * stride]; });
+    const float all = float(P.places) * float(P.each), part = float(at.places) * float(P.each);
+    if (P.whole_vectors) {
+        // a thread's channels are all of one group: one entry for them
+        if (thread < P.span.active) {
+            float mean = 0.0f, square = 0.0f;
+            if (w.count > 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) entries[threadIdx.x * V + i] = make_float2(mo.mean[i], mo.square[i]);
+                for (int i = 0; i < V; ++i) mean += mo.of(i).x;
+                mean *= 1.0f / V;
+#pragma unroll
+                for (int i = 0; i < V; ++i) square += fmaf(mo.n * (mo.of(i).x - mean), mo.of(i).x - mean, mo.of(i).y);
+            }
+            give_entries<1>(entries, P.vectors, [&](int) { return make_float2(mean, square); });
+        }
+        __syncthreads();
+        const Entries E(P.vectors, 0, at.places * P.vectors.channels);
+        join_moments(entries, E, groups, P.each / V, part, float(V), [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
+    } else {
+        if (thread < P.span.active) give_entries<V>(entries, P.span, [&](int i) { return mo.of(i); });
+        __syncthreads();
+        const Entries E(P.span, shift, w.total);
+        join_moments(entries, E, groups, P.each, part, 1.0f, [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
     }
-    __syncthreads();
-    const Entries E(P.active, V, P.span, shift, w.total);
-    join_moments(entries, E, groups, P.each, float(at.places) * float(P.each), [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
     __syncwarp();
     if (P.blocks > 1) mma::cluster_sync();
     else __syncthreads();
-    const float all = float(P.places) * float(P.each);
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+    for (int g = thread; g < groups; g += blockDim.x) {
         float2 f = mine[g];
         if (P.blocks > 1) {
+            float2 other[kNormCluster];
+            of_all(mine + g, P.blocks, other);
+            const float n = float(int(P.per)) * float(P.each), last = float(int(P.places) - int(P.per) * (P.blocks - 1)) * float(P.each);
             float sum = 0.0f, square = 0.0f;
-            for (int r = 0; r < P.blocks; ++r) {
-                const float n = float(P.places * (r + 1) / P.blocks - P.places * r / P.blocks) * float(P.each);
-                sum = fmaf(n, of_block(mine + g, r).x, sum);
-            }
+#pragma unroll
+            for (int r = 0; r < kNormCluster; ++r)
+                if (r < P.blocks) sum = fmaf(r + 1 < P.blocks ? n : last, other[r].x, sum);
             const float mean = __fdiv_rn(sum, all);
-            for (int r = 0; r < P.blocks; ++r) {
-                const float n = float(P.places * (r + 1) / P.blocks - P.places * r / P.blocks) * float(P.each);
-                const float2 other = of_block(mine + g, r);
-                square += fmaf(n * (other.x - mean), other.x - mean, other.y);
-            }
+#pragma unroll
+            for (int r = 0; r < kNormCluster; ++r)
+                if (r < P.blocks) square += fmaf((r + 1 < P.blocks ? n : last) * (other[r].x - mean), other[r].x - mean, other[r].y);
             f = make_float2(mean, square);
         }
         f.y = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(f.y, all) + P.epsilon));
         result[g] = f;
         const long long to = at.sample * P.groups + at.span * groups + g;
-        if (at.rank == 0 && P.statistics && AXC_GLOBAL_OK(to, P.samples * P.groups, 507u)) P.statistics[to] = f;
+        if (at.rank == 0 && AXC_GLOBAL_OK(to, P.samples * P.groups, 507u)) P.statistics[to] = f;
     }
     __syncthreads();
     if (P.blocks > 1) cluster_arrive();
+    int local[V], group[V];
+    local_channels<V>(w, P.span, P.by_group, local, group);
     Channels<V> ch;
-    ch.fill(P, [&](int i) { return at.channel0 + local_channel<V>(w, P.span, i); }, [&](int c) { return result[(c - at.channel0) / P.each]; });
-    constexpr int N = 4;
-    for (int j = 0; j < w.count; j += N) {
+    ch.fill(P, at.channel0, local, group, P.whole_vectors, [&](int g) { return result[g]; });
+    T *y = static_cast<T *>(P.y);
+    batches<V>(w, std::integral_constant<int, 4>(), [&](auto whole, auto n, int j) {
+        constexpr int N = decltype(n)::value;
+        const long long from = at.sample0 + w.at + j * w.step;
+        Pack<T, V> r[N];
+        if (P.residual) {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) {
-                Pack<T, V> v;
-                v.w = kept[(j + k) * P.active + int(threadIdx.x)];
-                finish<T, V>(P, ch, w, j + k, v, sample0);
-            }
-    }
+            for (int k = 0; k < N; ++k) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, r[k], residual, P.values());
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            Pack<T, V> v;
+            v.w = kept[(j + k) * stride];
+            Two z[kPairs<V>];
+            output_of<T, V>(P, ch, v, r[k], z);
+            store<decltype(whole)::value>(y + from + k * w.step, w, j + k, z, y, P.values());
+        }
+    });
     __syncwarp();
     if (P.blocks > 1) cluster_wait();          // what others read of this block's shared memory
 }
@@ -445,153 +760,112 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_backward_kernel(const No
     after_previous();
     extern __shared__ __align__(16) char raw[];
     const Place at(P);
-    const int shift = shift_of<T, V>(P, at.sample, at.place0);
-    const Walk<V> w(threadIdx.x, P.active, shift, at.places, P.span, P.channels, at.place0, at.channel0);
-    const int steps = (int((P.places + P.blocks - 1) / P.blocks) * P.span + V - 1 + P.active * V - 1) / (P.active * V), groups = P.span / P.each;
+    const int shift = shift_of<T, V>(P, at.sample, at.place0), thread = threadIdx.x, groups = P.span_groups, stride = P.span.active;
+    const Walk<V> w(thread, P.span, shift, at.places, P.channels, at.place0, at.channel0);
     typedef typename Bits<V * sizeof(T)>::type Word;
-    constexpr int kQuads = V >= 4 ? V / 4 : 1;
-    typedef typename Bits<V >= 4 ? 16 : 4>::type Quad;                         // four values of dz, or one
-    const int slots = steps * P.active;
-    Quad *kept_dz = reinterpret_cast<Quad *>(raw);
-    Word *kept = reinterpret_cast<Word *>(raw + norm_up16(size_t(slots) * V * 4));
-    float2 *entries = reinterpret_cast<float2 *>(raw + norm_up16(size_t(slots) * V * 4) + norm_up16(size_t(slots) * V * sizeof(T)));
-    float2 *channels = entries + P.active * V, *mine = channels + P.span, *result = mine + groups;
-    const long long sample0 = at.sample * P.places * P.channels, values = P.values();
-    const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
-    auto stats = [&](int c) {
-        const long long from = at.sample * P.groups + c / P.each;
-        return AXC_GLOBAL_OK(from, P.samples * P.groups, 508u) ? P.statistics[from] : make_float2(0.0f, 0.0f);
-    };
-    Channels<V> ch;
-    ch.fill(P, [&](int i) { return at.channel0 + local_channel<V>(w, P.span, i); }, stats);
-    float sum[V], sum_off[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = sum_off[i] = 0.0f;
     const bool with = P.residual && P.activation != kActNone;
-    constexpr int N = 2;
-    for (int j = 0; j < w.count; j += N) {
-        Pack<T, V> vx[N], vd[N], vr[N];
+    const size_t room = norm_up16(size_t(P.steps) * P.span.active * V * sizeof(T));
+    Word *kept = reinterpret_cast<Word *>(raw) + thread, *kept_dz = reinterpret_cast<Word *>(raw + room) + thread;      // dy's, first
+    float2 *entries = reinterpret_cast<float2 *>(raw + 2 * room);
+    float2 *channels = entries + entry_places(P.span), *mine = channels + P.span.channels, *result = mine + groups;
+    const long long values = P.values();
+    const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
+    fetch<T, V>(x + at.sample0, w, kept, stride, x, values);
+    fetch<T, V>(dy + at.sample0, w, kept_dz, stride, dy, values);
+    const float2 *statistics = P.statistics + at.sample * P.groups + at.span * groups;
+    [[maybe_unused]] const long long in_statistics = P.samples * P.groups - (at.sample * P.groups + at.span * groups);
+    auto stats = [&](int g) { return AXC_GLOBAL_OK(g, in_statistics, 508u) ? statistics[g] : make_float2(0.0f, 0.0f); };
+    int local[V], group[V];
+    local_channels<V>(w, P.span, P.by_group, local, group);
+    Channels<V> ch;
+    ch.fill(P, at.channel0, local, group, P.whole_vectors, stats);
+    Sums<V> sums;
+    T *dresidual = static_cast<T *>(P.dresidual);
+    wait_copies();
+    batches<V>(w, std::integral_constant<int, 4>(), [&](auto whole, auto n, int j) {
+        constexpr int N = decltype(n)::value;
+        const long long from = at.sample0 + w.at + j * w.step;
+        Pack<T, V> vr[N];
+        if (with) {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) {
-                load(x + sample0, w, j + k, vx[k], x, values);
-                load(dy + sample0, w, j + k, vd[k], dy, values);
-                if (with) load(residual + sample0, w, j + k, vr[k], residual, values);
-            }
+            for (int k = 0; k < N; ++k) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) {
-                float dz[V], off[V];
-                slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-                if (!w.whole(j + k)) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (!w.has(j + k, i)) dz[i] = off[i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    sum[i] += dz[i];
-                    sum_off[i] = fmaf(dz[i], off[i], sum_off[i]);
-                }
-                const int slot = (j + k) * P.active + int(threadIdx.x);
-                kept[slot] = vx[k].w;
-#pragma unroll
-                for (int q = 0; q < kQuads; ++q) {
-                    if constexpr (V >= 4)
-                        kept_dz[q * slots + slot] = make_uint4(__float_as_uint(dz[4 * q]), __float_as_uint(dz[4 * q + 1]), __float_as_uint(dz[4 * q + 2]),
-                                                               __float_as_uint(dz[4 * q + 3]));
-                    else kept_dz[slot] = __float_as_uint(dz[0]);
-                }
-                if (P.dresidual) store(static_cast<T *>(P.dresidual) + sample0, w, j + k, dz, static_cast<T *>(P.dresidual), values);
-            }
-    }
-    if (int(threadIdx.x) < P.active) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) entries[threadIdx.x * V + i] = make_float2(sum[i], sum_off[i]);
-    }
+        for (int k = 0; k < N; ++k) {
+            Pack<T, V> vx, vd;
+            vx.w = kept[(j + k) * stride];
+            vd.w = kept_dz[(j + k) * stride];
+            Two dz[kPairs<V>], off[kPairs<V>];
+            slope_at<T, V>(P, ch, vx, vd, vr[k], dz, off);
+            sums.template add<decltype(whole)::value>(w, j + k, dz, off);
+            if (P.activation != kActNone) kept_dz[(j + k) * stride] = narrow_pairs<T, V>(dz).w;
+            if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
+        }
+    });
+    if (thread < P.span.active) give_entries<V>(entries, P.span, [&](int i) { return sums.of(i); });
     __syncthreads();
-    const Entries E(P.active, V, P.span, shift, w.total);
-    join_sums(entries, E, [&](int l, float a, float b) { channels[l] = make_float2(a, b * stats(at.channel0 + l).y); });
+    const Entries E(P.span, shift, w.total);
+    join_sums(entries, E, [&](int l, float a, float b) { channels[l] = make_float2(a, b); });
     __syncthreads();
     {
-        const int q = lanes_for(groups), lane = threadIdx.x & (q - 1), step = int(blockDim.x) / q;
+        const int log2 = lanes_for(groups), q = 1 << log2, lane = thread & (q - 1), step = int(blockDim.x) >> log2;
         for (int first = 0; first < groups; first += step) {
-            const int g = first + int(threadIdx.x) / q;
+            const int g = first + (thread >> log2);
             float a = 0.0f, b = 0.0f;
             if (g < groups)
                 for (int d = lane; d < P.each; d += q) {
-                    const int c = at.channel0 + g * P.each + d;
+                    const int l = g * P.each + d, c = at.channel0 + l;
                     const float scale = P.scale && AXC_GLOBAL_OK(c, P.channels, 509u) ? load_as_float(P.scale, c, P.scale_type) : 1.0f;
-                    const float2 f = channels[g * P.each + d];
+                    const float2 f = channels[l];
                     a = fmaf(scale, f.x, a);
                     b = fmaf(scale, f.y, b);
                 }
-            a = over_lanes(a, q);
-            b = over_lanes(b, q);
+            a = over_lanes(a, log2);
+            b = over_lanes(b, log2);
             if (g < groups && lane == 0) mine[g] = make_float2(a, b);
         }
     }
     __syncwarp();
     if (P.blocks > 1) mma::cluster_sync();
     else __syncthreads();
-    const float all = float(P.places) * float(P.each);
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-        float2 f = mine[g];
-        if (P.blocks > 1) {
-            f = make_float2(0.0f, 0.0f);
-            for (int r = 0; r < P.blocks; ++r) {
-                const float2 other = of_block(mine + g, r);
-                f.x += other.x;
-                f.y += other.y;
-            }
-        }
-        const float r = stats(at.channel0 + g * P.each).y;
-        result[g] = make_float2(__fdiv_rn(f.x, all) * r, __fdiv_rn(f.y, all) * r * r);
+    const float share = __fdiv_rn(1.0f, float(P.places) * float(P.each));
+    for (int g = thread; g < groups; g += blockDim.x) {
+        const float2 f = P.blocks > 1 ? sum_of_all(mine + g, P.blocks) : mine[g];
+        const float r = stats(g).y;
+        // the sums are of dz and of dz (x - mean): r makes xhat of that
+        result[g] = make_float2(f.x * share * r, f.y * share * r * r * r);
     }
     // the sums of single channels, shared out among the cluster's blocks
-    for (int l = at.rank + int(threadIdx.x) * P.blocks; l < P.span; l += int(blockDim.x) * P.blocks) {
-        float2 f = channels[l];
-        if (P.blocks > 1) {
-            f = make_float2(0.0f, 0.0f);
-            for (int r = 0; r < P.blocks; ++r) {
-                const float2 other = of_block(channels + l, r);
-                f.x += other.x;
-                f.y += other.y;
-            }
+    if (P.sums) {
+        for (int l = at.rank + thread * P.blocks; l < P.span.channels; l += int(blockDim.x) * P.blocks) {
+            const float2 f = P.blocks > 1 ? sum_of_all(channels + l, P.blocks) : channels[l];
+            const long long to = at.sample * P.channels + at.channel0 + l;
+            if (AXC_GLOBAL_OK(to, P.samples * P.channels, 510u)) P.sums[to] = make_float2(f.x, f.y * stats(int(P.by_group.of(unsigned(l)))).y);
         }
-        const long long to = at.sample * P.channels + at.channel0 + l;
-        if (P.sums && AXC_GLOBAL_OK(to, P.samples * P.channels, 510u)) P.sums[to] = f;
     }
     __syncthreads();
     if (P.blocks > 1) cluster_arrive();
     if (P.dx) {
-        float first[V], second[V];
+        T *dx = static_cast<T *>(P.dx);
+        Gradient<V> gradient;
+        gradient.fill(group, P.whole_vectors, [&](int g) { return result[g]; });
+        batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
+            constexpr int N = decltype(n)::value;
+            const long long from = at.sample0 + w.at + j * w.step;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float2 f = result[local_channel<V>(w, P.span, i) / P.each];
-            first[i] = f.x;
-            second[i] = f.y;
-        }
-#pragma unroll 2
-        for (int j = 0; j < w.count; ++j) {
-            const int slot = j * P.active + int(threadIdx.x);
-            Pack<T, V> v;
-            v.w = kept[slot];
-            float dx[V];
+            for (int k = 0; k < N; ++k) {
+                Pack<T, V> v, vd;
+                v.w = kept[(j + k) * stride];
+                vd.w = kept_dz[(j + k) * stride];
+                Two d[kPairs<V>], off[kPairs<V>];
+                widen_pairs<T, V>(vd, d);
+                widen_pairs<T, V>(v, off);
 #pragma unroll
-            for (int q = 0; q < kQuads; ++q) {
-                if constexpr (V >= 4) {
-                    const uint4 d = kept_dz[q * slots + slot];
-                    dx[4 * q] = __uint_as_float(d.x);
-                    dx[4 * q + 1] = __uint_as_float(d.y);
-                    dx[4 * q + 2] = __uint_as_float(d.z);
-                    dx[4 * q + 3] = __uint_as_float(d.w);
-                } else dx[0] = __uint_as_float(kept_dz[slot]);
+                for (int i = 0; i < kPairs<V>; ++i) off[i] = add2(off[i], ch.less[i]);
+                gradient.of(ch, off, d);
+                store<decltype(whole)::value>(dx + from + k * w.step, w, j + k, d, dx, values);
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i) dx[i] = fmaf(-second[i], widen(v.t[i]) - ch.mean[i], fmaf(dx[i], ch.factor[i], -first[i]));
-            store(static_cast<T *>(P.dx) + sample0, w, j, dx, static_cast<T *>(P.dx), values);
-        }
+        });
     }
     __syncwarp();
     if (P.blocks > 1) cluster_wait();
@@ -600,52 +874,49 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_backward_kernel(const No
 // ---- tensors that are read twice -------------------------------------------------------------------------------------------------
 // Block -> sample, share of the places, columns
 struct Share {
-    long long sample, share, place0;
-    int channel0, span, places, active;
-    template <int V>
-    static __device__ __forceinline__ Share of(const NormArgs &P, long long block, std::integral_constant<int, V>)
+    long long sample, place0;
+    int share, channel0, places;
+    bool last;                                 // of a line's spans
+    __device__ __forceinline__ Share(const NormArgs &P, unsigned block)
     {
-        Share s;
-        const long long columns = P.spans;
-        s.channel0 = int(block % columns) * P.span;
-        block /= columns;
-        s.share = block % P.shares;
-        s.sample = block / P.shares;
-        s.span = int(P.channels - s.channel0 < P.span ? P.channels - s.channel0 : P.span);
-        s.place0 = P.places * s.share / P.shares;
-        s.places = int(P.places * (s.share + 1) / P.shares - s.place0);
-        // as norm_active has it; a narrower last span has a divisor of its own
-        s.active = s.span == P.span ? P.active : int(blockDim.x) / (s.span / V) * (s.span / V);
-        return s;
+        unsigned rest = P.spans > 1 ? block / unsigned(P.spans) : block;
+        const int span = int(block - rest * unsigned(P.spans));
+        const unsigned n = rest / unsigned(P.shares);
+        sample = n;
+        share = int(rest - n * unsigned(P.shares));
+        channel0 = span * P.span.channels;
+        last = span + 1 == P.spans;
+        place0 = share * P.per;
+        places = int(min(P.per, P.places - place0));
     }
+    __device__ __forceinline__ const Span &span(const NormArgs &P) const { return last ? P.last : P.span; }
 };
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads) norm_moments_kernel(const NormArgs P)
 {
     after_previous();
-    __shared__ float2 entries[kNormThreads * V];
-    const Share at = Share::of(P, blockIdx.x, std::integral_constant<int, V>());
+    __shared__ float2 entries[2 * kNormThreads * V];
+    const Share at(P, blockIdx.x);
+    const Span &span = at.span(P);
     const int shift = shift_of<T, V>(P, at.sample, at.place0);
-    const Walk<V> w(threadIdx.x, at.active, shift, at.places, at.span, P.channels, at.place0, at.channel0);
+    const Walk<V> w(threadIdx.x, span, shift, at.places, P.channels, at.place0, at.channel0);
     const T *x = static_cast<const T *>(P.x);
     Moments<V> mo;
-    take_moments(x + at.sample * P.places * P.channels, w, mo, x, P.values(), [](int, const Pack<T, V> &) {});
-    if (int(threadIdx.x) < at.active) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) entries[threadIdx.x * V + i] = make_float2(mo.mean[i], mo.square[i]);
-    }
+    const T *sample = x + at.sample * P.places * P.channels;
+    take_moments<V == 1 ? 8 : 4, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto whole) { load<decltype(whole)::value>(sample + w.at + j * w.step, w, j, v, x, P.values()); });
+    if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return mo.of(i); });
     __syncthreads();
-    const Entries E(at.active, V, at.span, shift, w.total);
+    const Entries E(span, shift, w.total);
     const long long to = (at.sample * P.shares + at.share) * P.channels + at.channel0;
-    join_moments(entries, E, at.span, 1, float(at.places), [&](int l, float mean, float square) {
+    join_moments(entries, E, span.channels, 1, float(at.places), 1.0f, [&](int l, float mean, float square) {
         if (AXC_GLOBAL_OK(to + l, P.samples * P.shares * P.channels, 511u)) P.part[to + l] = make_float2(mean, square);
     });
 }
 
 __device__ __forceinline__ float over_block(float x, float *room)
 {
-    x = over_lanes(x, 32);
+    x = over_lanes(x, 5);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = x;
     __syncthreads();
@@ -664,7 +935,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
     const float2 *part = P.part + sample * P.shares * P.channels + group * P.each;
     const long long entries = P.shares * P.each;
     const float all = float(P.places) * float(P.each);
-    auto values = [&](long long s) { return float(P.places * (s + 1) / P.shares - P.places * s / P.shares); };
+    const float of_share = float(P.per), of_last = float(P.places - P.per * (P.shares - 1));
+    auto values = [&](long long s) { return s + 1 < P.shares ? of_share : of_last; };
     [[maybe_unused]] const long long room_for = P.shares * P.channels - group * P.each;
     float sum = 0.0f, square = 0.0f;
     for (long long e = threadIdx.x; e < entries; e += kNormThreads) {
@@ -683,90 +955,89 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
 }
 
 template <int V>
-__device__ __forceinline__ void fill_channels(const NormArgs &P, const Share &at, const Walk<V> &w, Channels<V> &ch)
+__device__ __forceinline__ void fill_channels(const NormArgs &P, const Share &at, const Walk<V> &w, Channels<V> &ch, int (&group)[V])
 {
-    ch.fill(P, [&](int i) { return at.channel0 + local_channel<V>(w, at.span, i); },
-            [&](int c) {
-                const long long from = at.sample * P.groups + c / P.each;
-                return AXC_GLOBAL_OK(from, P.samples * P.groups, 514u) ? P.statistics[from] : make_float2(0.0f, 0.0f);
-            });
+    // (a span that starts inside a group counts its channels from there)
+    int local[V];
+    local_channels<V>(w, at.span(P), at.span(P).by_channels, local, group);
+#pragma unroll
+    for (int i = 0; i < V; ++i) group[i] = (at.channel0 + local[i]) / P.each;
+    const float2 *statistics = P.statistics + at.sample * P.groups;
+    ch.fill(P, at.channel0, local, group, false, [&](int g) { return AXC_GLOBAL_OK(g, P.groups, 514u) ? statistics[g] : make_float2(0.0f, 0.0f); });
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 2) norm_apply_kernel(const NormArgs P)
 {
     after_previous();
-    const Share at = Share::of(P, (long long)gridDim.x - 1 - blockIdx.x, std::integral_constant<int, V>());
-    const Walk<V> w(threadIdx.x, at.active, shift_of<T, V>(P, at.sample, at.place0), at.places, at.span, P.channels, at.place0, at.channel0);
+    const Share at(P, gridDim.x - 1 - blockIdx.x);
+    const Span &span = at.span(P);
+    const Walk<V> w(threadIdx.x, span, shift_of<T, V>(P, at.sample, at.place0), at.places, P.channels, at.place0, at.channel0);
     if (w.count == 0) return;
     Channels<V> ch;
-    fill_channels<V>(P, at, w, ch);
+    int group[V];
+    fill_channels<V>(P, at, w, ch, group);
     const long long sample0 = at.sample * P.places * P.channels;
-    const T *x = static_cast<const T *>(P.x);
-    constexpr int N = 4;
-    for (int j = 0; j < w.count; j += N) {
-        Pack<T, V> v[N];
+    const T *x = static_cast<const T *>(P.x), *residual = static_cast<const T *>(P.residual);
+    T *y = static_cast<T *>(P.y);
+    batches<V>(w, std::integral_constant<int, 4>(), [&](auto whole, auto n, int j) {
+        constexpr int N = decltype(n)::value;
+        const long long from = sample0 + w.at + j * w.step;
+        Pack<T, V> v[N], r[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) load(x + sample0, w, j + k, v[k], x, P.values());
+        for (int k = 0; k < N; ++k) {
+            load<decltype(whole)::value>(x + from + k * w.step, w, j + k, v[k], x, P.values());
+            if (P.residual) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, r[k], residual, P.values());
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) finish<T, V>(P, ch, w, j + k, v[k], sample0);
-    }
+        for (int k = 0; k < N; ++k) {
+            Two z[kPairs<V>];
+            output_of<T, V>(P, ch, v[k], r[k], z);
+            store<decltype(whole)::value>(y + from + k * w.step, w, j + k, z, y, P.values());
+        }
+    });
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormArgs P)
 {
     after_previous();
-    __shared__ float2 entries[kNormThreads * V];
-    const Share at = Share::of(P, blockIdx.x, std::integral_constant<int, V>());
+    __shared__ float2 entries[2 * kNormThreads * V];
+    const Share at(P, blockIdx.x);
+    const Span &span = at.span(P);
     const int shift = shift_of<T, V>(P, at.sample, at.place0);
-    const Walk<V> w(threadIdx.x, at.active, shift, at.places, at.span, P.channels, at.place0, at.channel0);
-    float sum[V], sum_off[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = sum_off[i] = 0.0f;
+    const Walk<V> w(threadIdx.x, span, shift, at.places, P.channels, at.place0, at.channel0);
+    Sums<V> sums;
     if (w.count > 0) {
         Channels<V> ch;
-        fill_channels<V>(P, at, w, ch);
+        int group[V];
+        fill_channels<V>(P, at, w, ch, group);
         const long long sample0 = at.sample * P.places * P.channels, values = P.values();
         const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
+        T *dresidual = static_cast<T *>(P.dresidual);
         const bool with = P.residual && P.activation != kActNone;
-        constexpr int N = 2;
-        for (int j = 0; j < w.count; j += N) {
+        batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
+            constexpr int N = decltype(n)::value;
+            const long long from = sample0 + w.at + j * w.step;
             Pack<T, V> vx[N], vd[N], vr[N];
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (j + k < w.count) {
-                    load(x + sample0, w, j + k, vx[k], x, values);
-                    load(dy + sample0, w, j + k, vd[k], dy, values);
-                    if (with) load(residual + sample0, w, j + k, vr[k], residual, values);
-                }
+            for (int k = 0; k < N; ++k) {
+                load<decltype(whole)::value>(x + from + k * w.step, w, j + k, vx[k], x, values);
+                load<decltype(whole)::value>(dy + from + k * w.step, w, j + k, vd[k], dy, values);
+                if (with) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
+            }
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (j + k < w.count) {
-                    float dz[V], off[V];
-                    slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-                    if (!w.whole(j + k)) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (!w.has(j + k, i)) dz[i] = off[i] = 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        sum[i] += dz[i];
-                        sum_off[i] = fmaf(dz[i], off[i], sum_off[i]);
-                    }
-                    if (P.dresidual) store(static_cast<T *>(P.dresidual) + sample0, w, j + k, dz, static_cast<T *>(P.dresidual), values);
-                }
-        }
+            for (int k = 0; k < N; ++k) {
+                Two dz[kPairs<V>], off[kPairs<V>];
+                slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
+                sums.template add<decltype(whole)::value>(w, j + k, dz, off);
+                if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
+            }
+        });
     }
-    if (int(threadIdx.x) < at.active) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) entries[threadIdx.x * V + i] = make_float2(sum[i], sum_off[i]);
-    }
+    if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return sums.of(i); });
     __syncthreads();
-    const Entries E(at.active, V, at.span, shift, w.total);
+    const Entries E(span, shift, w.total);
     const long long to = (at.sample * P.shares + at.share) * P.channels + at.channel0;
     join_sums(entries, E, [&](int l, float a, float b) {
         if (AXC_GLOBAL_OK(to + l, P.samples * P.shares * P.channels, 515u)) P.part[to + l] = make_float2(a, b);
@@ -791,8 +1062,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_sums_kernel(const Norm
             a += P.part[from].x;
             b += P.part[from].y;
         }
-        a = over_lanes(a, 32);
-        b = over_lanes(b, 32) * r;
+        a = over_lanes(a, 5);
+        b = over_lanes(b, 5) * r;
         if (lane == 0) {
             if (P.sums) P.sums[sample * P.channels + c] = make_float2(a, b);
             const float scale = P.scale ? load_as_float(P.scale, c, P.scale_type) : 1.0f;
@@ -807,45 +1078,40 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_sums_kernel(const Norm
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_gradient_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 2) norm_gradient_kernel(const NormArgs P)
 {
     after_previous();
-    const Share at = Share::of(P, (long long)gridDim.x - 1 - blockIdx.x, std::integral_constant<int, V>());
-    const Walk<V> w(threadIdx.x, at.active, shift_of<T, V>(P, at.sample, at.place0), at.places, at.span, P.channels, at.place0, at.channel0);
+    const Share at(P, gridDim.x - 1 - blockIdx.x);
+    const Span &span = at.span(P);
+    const Walk<V> w(threadIdx.x, span, shift_of<T, V>(P, at.sample, at.place0), at.places, P.channels, at.place0, at.channel0);
     if (w.count == 0) return;
     Channels<V> ch;
-    fill_channels<V>(P, at, w, ch);
-    float first[V], second[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const long long from = at.sample * P.groups + (at.channel0 + local_channel<V>(w, at.span, i)) / P.each;
-        const float2 f = AXC_GLOBAL_OK(from, P.samples * P.groups, 517u) ? P.group_sums[from] : make_float2(0.0f, 0.0f);
-        first[i] = f.x;
-        second[i] = f.y;
-    }
+    int group[V];
+    fill_channels<V>(P, at, w, ch, group);
+    Gradient<V> gradient;
+    gradient.fill(group, false, [&](int g) { return AXC_GLOBAL_OK(g, P.groups, 517u) ? P.group_sums[at.sample * P.groups + g] : make_float2(0.0f, 0.0f); });
     const long long sample0 = at.sample * P.places * P.channels, values = P.values();
     const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
+    T *dx = static_cast<T *>(P.dx);
     const bool with = P.residual && P.activation != kActNone;
-    constexpr int N = 2;
-    for (int j = 0; j < w.count; j += N) {
+    batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
+        constexpr int N = decltype(n)::value;
+        const long long from = sample0 + w.at + j * w.step;
         Pack<T, V> vx[N], vd[N], vr[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) {
-                load(x + sample0, w, j + k, vx[k], x, values);
-                load(dy + sample0, w, j + k, vd[k], dy, values);
-                if (with) load(residual + sample0, w, j + k, vr[k], residual, values);
-            }
+        for (int k = 0; k < N; ++k) {
+            load<decltype(whole)::value>(x + from + k * w.step, w, j + k, vx[k], x, values);
+            load<decltype(whole)::value>(dy + from + k * w.step, w, j + k, vd[k], dy, values);
+            if (with) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (j + k < w.count) {
-                float dz[V], off[V];
-                slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-#pragma unroll
-                for (int i = 0; i < V; ++i) dz[i] = fmaf(-second[i], off[i], fmaf(dz[i], ch.factor[i], -first[i]));
-                store(static_cast<T *>(P.dx) + sample0, w, j + k, dz, static_cast<T *>(P.dx), values);
-            }
-    }
+        for (int k = 0; k < N; ++k) {
+            Two dz[kPairs<V>], off[kPairs<V>];
+            slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
+            gradient.of(ch, off, dz);
+            store<decltype(whole)::value>(dx + from + k * w.step, w, j + k, dz, dx, values);
+        }
+    });
 }
 
 // The channels' sums over the samples: 32 channels a block, its warps share the samples
@@ -945,7 +1211,7 @@ int check_desc(const axc_norm_desc *d)
 
 NormShape shape_of(const axc_norm_desc &d, bool aligned) { return {d.samples, d.places, d.channels, d.groups, d.type == kFloat32 ? 4 : 2, aligned}; }
 
-// The plan of a call.  Searching for one takes some 20 us of the host's time, so plans are remembered: they are functions of the shape alone.
+// The plan of a call; `residual`: whether its values take part.  Searching for one takes some 20 us of the host's time, so plans are remembered: they are functions of the shape alone.
 NormPlan plan_of(const NormShape &s, bool backward, bool residual, int sms)
 {
     struct Known {
@@ -959,7 +1225,8 @@ NormPlan plan_of(const NormShape &s, bool backward, bool residual, int sms)
     for (const long long v : {s.places, s.channels, s.groups, (long long)(key * 8 + s.size)}) hash = (hash ^ (unsigned long long)v) * 0x9E3779B97F4A7C15ull, hash ^= hash >> 29;
     Known &k = known[hash % known.size()];
     if (k.key != key || k.shape.samples != s.samples || k.shape.places != s.places || k.shape.channels != s.channels || k.shape.groups != s.groups || k.shape.size != s.size)
-        k = {s, key, backward ? norm_plan(s, s.size + 4, s.size * (residual ? 5 : 3), 1, sms) : norm_plan(s, s.size, s.size * (residual ? 3 : 2), 0, sms)};
+        k = {s, key, backward ? norm_plan(s, 2 * s.size, s.size * (residual ? 5 : 3), 1, sms)
+                              : norm_plan(s, s.size, s.size * (residual ? 3 : 2), 0, sms)};
     return k.plan;
 }
 
@@ -975,10 +1242,20 @@ NormArgs args_of(const axc_norm_desc &d, const NormPlan &plan)
     P.channels = d.channels;
     P.groups = int(d.groups);
     P.each = int(d.channels / d.groups);
-    P.span = plan.span;
+    P.by_group = divider(unsigned(P.each));
     P.spans = int((d.channels + plan.span - 1) / plan.span);
+    P.span = span_of(plan.span, norm_active(plan.threads, plan.span, plan.vec), plan.vec);
+    const int rest = int(d.channels - (long long)(P.spans - 1) * plan.span);
+    P.last = span_of(rest, norm_active(plan.threads, rest, plan.vec), plan.vec);
     P.blocks = plan.blocks;
-    P.active = norm_active(plan.threads, plan.span, plan.vec);
+    const long long parts = plan.resident ? plan.blocks : plan.shares;
+    P.per = (d.places + parts - 1) / parts;
+    if (plan.resident) {
+        P.steps = int(norm_steps(P.per, plan.span, plan.vec, P.span.active));
+        P.span_groups = plan.span / P.each;
+        P.whole_vectors = P.each % plan.vec == 0;
+        if (P.whole_vectors) P.vectors = span_of(plan.span / plan.vec, P.span.active, 1);
+    }
     P.shares = plan.shares;
     return P;
 }
@@ -1087,7 +1364,7 @@ extern "C" int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy
     rc = sm_count(device, &sms);
     if (rc) return rc;
     const NormShape s = shape_of(d, on_16(dy, x, residual, dx, dresidual));
-    const NormPlan plan = plan_of(s, true, residual != nullptr, sms);
+    const NormPlan plan = plan_of(s, true, residual && d.activation != kActNone, sms);
     NormArgs P = args_of(d, plan);
     if (too_many(P, plan)) return AXC_INVALID_ARGUMENT;
     if (some && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < workspace_of(s, plan, true))) return AXC_INTERNAL;

@@ -64,7 +64,7 @@ AXC_BOTH size_t norm_up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 // (a pair for the cluster's blocks to read, a pair of results).
 inline long long norm_smem(long long places, int span, int vec, int active, int kept, long long groups, int sums)
 {
-    return norm_steps(places, span, vec, active) * active * vec * kept + 32 + (long long)active * vec * 8 + (long long)span * 8 * sums + groups * 16;
+    return norm_steps(places, span, vec, active) * active * vec * kept + 48 + ((long long)active * vec + active * vec / span) * 8 + (long long)span * 8 * sums + groups * 16;
 }
 
 // Channels at a time where the tensors are read twice
@@ -102,6 +102,7 @@ inline NormPlan norm_plan(const NormShape &s, int kept, int moved, int sums, int
                 if (!active) continue;
                 for (int blocks = 1; blocks <= kNormCluster && blocks <= s.places; ++blocks) {
                     const long long places = (s.places + blocks - 1) / blocks;
+                    if ((blocks - 1) * places >= s.places) continue;           // the last one has none
                     if (places * span > (1ll << 20)) continue;
                     const long long smem = norm_smem(places, int(span), vec, active, kept, k, sums);
                     if (smem > kNormSmem) continue;
@@ -131,14 +132,16 @@ inline NormPlan norm_plan(const NormShape &s, int kept, int moved, int sums, int
     best.vec = vec;
     best.threads = kNormThreads;
     best.span = span;
-    // six blocks for every SM, of 32 KiB at least
+    // six blocks for every SM, of 32 KiB at least and a million values at most
     const long long across = s.samples * ((s.channels + span - 1) / span), most = s.places * span * s.size / (32 * 1024) + 1;
     long long shares = ((long long)sms * 6 + across - 1) / (across ? across : 1);
     if (shares > most) shares = most;
     if (shares > s.places) shares = s.places;
+    const long long fewest = (s.places * span >> 20) + 1;
+    if (shares < fewest) shares = fewest;
     if (shares < 1) shares = 1;
-    const long long fewest = (s.places * span >> 30) + 1;     // a block counts its values in 32 bits
-    best.shares = shares < fewest ? fewest : shares;
+    const long long per = s.places > 0 ? (s.places + shares - 1) / shares : 1;
+    best.shares = s.places > 0 ? (s.places + per - 1) / per : 1;
     return best;
 }
 
@@ -151,26 +154,56 @@ inline size_t norm_part_bytes(const NormShape &s, const NormPlan &p)
 inline size_t norm_sums_bytes(const NormShape &s) { return norm_pad(size_t(s.samples) * size_t(s.channels) * 8); }
 inline size_t norm_group_bytes(const NormShape &s) { return norm_pad(size_t(s.samples) * size_t(s.groups) * 8); }
 
+// n / by for n by < 2^32, by one multiplication
+struct Divider {
+    unsigned by, magic;
+    AXC_BOTH unsigned of(unsigned n) const
+    {
+#ifdef __CUDA_ARCH__
+        return magic ? __umulhi(n, magic) : n;
+#else
+        return magic ? unsigned((unsigned long long)n * magic >> 32) : n;
+#endif
+    }
+};
+inline Divider divider(unsigned by) { return {by, by > 1 ? unsigned(((1ull << 32) + by - 1) / by) : 0u}; }
+
+// A span as the kernels have it: its channels and groups, the threads that take part, the values that they take in a step, lines of a step, sets of
+// entries (see Entries)
+struct Span {
+    int channels, active, each, lines, copies;
+    Divider by_channels, by_each;
+};
+inline Span span_of(int channels, int active, int vec)
+{
+    const int each = active * vec;
+    return {channels, active, each, each / channels, each / channels, divider(unsigned(channels)), divider(unsigned(each))};
+}
+
 // ---- in the kernels ------------------------------------------------------------------------------------------------------------
 // A thread's way through the places and channels of its block: `count` vectors, the j-th with the values o + j * each .. of the block's own
-// (place by place, `total` of them), at at + j * step from the sample's start.
+// (place by place, `total` of them), at at + j * step from the sample's start.  Those from `first` to `end` are whole; one before and one
+// behind them may stick out of the block's values.
 template <int V>
 struct Walk {
-    int o, each, count, total;
+    int o, each, count, total, first, end;
     long long at, step;
-    AXC_BOTH Walk(int thread, int active, int shift, int places, int span, long long channels, long long place0, int channel0)
+    AXC_BOTH Walk(int thread, const Span &s, int shift, int places, long long channels, long long place0, int channel0)
     {
-        each = active * V;
+        each = s.each;
         o = thread * V - shift;
-        total = places * span;
-        count = thread < active && o < total ? (total - 1 - o) / each + 1 : 0;
-        if (span == channels) {
+        total = places * s.channels;
+        count = thread < s.active && o < total ? int(s.by_each.of(unsigned(total - 1 - o))) + 1 : 0;
+        if (s.channels == channels) {
             at = place0 * channels + o;
             step = each;
         } else {
-            at = (place0 + o / span) * channels + channel0 + o % span;
-            step = (each / span) * channels;
+            const int line = int(s.by_channels.of(unsigned(o)));
+            at = (place0 + line) * channels + channel0 + (o - line * s.channels);
+            step = s.lines * channels;
         }
+        first = V > 1 && count > 0 && !whole(0) ? 1 : 0;
+        end = V > 1 && count > first && !whole(count - 1) ? count - 1 : count;
     }
     AXC_BOTH bool whole(int j) const
     {
@@ -184,23 +217,26 @@ struct Walk {
         return s >= 0 && s < total;
     }
 };
-// Thread t's channel i is entry t * V + i; a span's channel l has the entries (l + shift) mod span + k * span.
+// Thread t's channel i is entry t * V + i; a span's channel l has the entries (l + shift) mod span + k * span, the k-th copy of it.  In shared
+// memory each copy is one place further on, or the copies of a channel would all be in the same banks.
 struct Entries {
     int span, shift, copies, each, rest, base;
-    AXC_BOTH Entries(int active, int vec, int span_, int shift_, int total)
+    AXC_BOTH Entries(const Span &s, int shift_, int total)
     {
-        span = span_;
+        span = s.channels;
         shift = shift_;
-        each = active * vec;
-        copies = each / span;
-        base = total / each;
+        each = s.each;
+        copies = s.copies;
+        base = int(s.by_each.of(unsigned(total)));
         rest = total - base * each;
     }
-    AXC_BOTH int entry(int l, int copy) const
+    AXC_BOTH int first_entry(int l) const
     {
-        const int e = l + shift;
-        return (e < span ? e : e % span) + copy * span;
+        int e = l + shift;
+        while (e >= span) e -= span;
+        return e;
     }
+    AXC_BOTH int place(int entry, int copy) const { return entry + copy; }
     // values that were added up in it
     AXC_BOTH float values(int entry) const
     {
@@ -209,13 +245,24 @@ struct Entries {
         return float(base + (o < rest ? 1 : 0));
     }
 };
+AXC_BOTH int entry_places(const Span &s) { return s.each + s.copies; }
 
-// local channel of a thread's value i
+// The channels of a thread's values, counted from the span's first, and their groups (of `by_group` channels) counted the same way
 template <int V>
-AXC_BOTH int local_channel(const Walk<V> &w, int span, int i)
+AXC_BOTH void local_channels(const Walk<V> &w, const Span &s, const Divider &by_group, int (&local)[V], int (&group)[V])
 {
-    const int o = w.o + i;
-    return o < 0 ? (o + (V + span - 1) / span * span) % span : o % span;
+    int l = w.o;
+    if (V > 1)
+        while (l < 0) l += s.channels;
+    l -= int(s.by_channels.of(unsigned(l))) * s.channels;
+    int g = int(by_group.of(unsigned(l))), d = l - g * int(by_group.by);
+    for (int i = 0; i < V; ++i) {
+        local[i] = l;
+        group[i] = g;
+        ++l;
+        if (++d == int(by_group.by)) d = 0, ++g;
+        if (l == s.channels) l = g = d = 0;
+    }
 }
 
 }  // namespace axc
