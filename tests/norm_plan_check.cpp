@@ -76,7 +76,7 @@ static void block(const NormShape &s, const NormPlan &p, const Span &sp, long lo
 }
 
 template <int V>
-static void whole(const NormShape &s, const NormPlan &p, int sums)
+static void whole(const NormShape &s, const NormPlan &p, bool residual, int sums)
 {
     std::vector<unsigned char> seen(size_t(s.values()));
     const int spans = int((s.channels + p.span - 1) / p.span);
@@ -90,8 +90,11 @@ static void whole(const NormShape &s, const NormPlan &p, int sums)
                 const long long steps = norm_steps((s.places + p.blocks - 1) / p.blocks, p.span, p.vec, active);
                 const size_t slots = size_t(steps) * active * p.vec;
                 // as the kernels lay it out
-                const size_t data = (sums ? 2 : 1) * norm_up16(slots * s.size);
-                CHECK(data + size_t(entry_places(sp)) * 8 + size_t(p.span) * 8 * sums + size_t(groups) * 16 <= p.smem && p.smem <= kNormSmem);
+                const size_t data = (sums ? residual ? 3 : 2 : 1) * norm_up16(slots * s.size);
+                if (sums && norm_lanes(p.span, p.vec, p.threads)) CHECK(active == p.threads && s.channels % p.vec == 0);
+                else if (!sums && V > 1 && s.each() % V == 0) CHECK(entry_places(span_of(p.span / V, active, 1)) == norm_entries(p.span, p.vec, p.threads, active, s.each(), false));
+                else CHECK(entry_places(sp) == norm_entries(p.span, p.vec, p.threads, active, s.each(), sums));
+                CHECK(data + size_t(norm_entries(p.span, p.vec, p.threads, active, s.each(), sums)) * 8 + size_t(p.span) * 8 * sums + size_t(groups) * 16 <= p.smem && p.smem <= kNormSmem);
                 const long long per = (s.places + p.blocks - 1) / p.blocks;
                 CHECK(per * (p.blocks - 1) < s.places);
                 for (int r = 0; r < p.blocks; ++r) {
@@ -128,13 +131,13 @@ int main(int argc, char **argv)
         s.aligned = pick(0, 4) != 0;
         for (int backward = 0; backward < 2; ++backward) {
             const bool residual = pick(0, 1);
-            const NormPlan p = norm_plan(s, (1 + backward) * s.size, (backward ? residual ? 5 : 3 : residual ? 3 : 2) * s.size, backward, 148);
+            const NormPlan p = norm_plan(s, (backward ? residual ? 3 : 2 : 1) * s.size, (backward ? residual ? 5 : 3 : residual ? 3 : 2) * s.size, backward, 148);
             ++(p.resident ? resident : twice);
             if (p.vec == 1) ++single;
             else if (s.channels % p.vec) ++loose;
-            if (p.vec == 8) whole<8>(s, p, backward);
-            else if (p.vec == 4) whole<4>(s, p, backward);
-            else whole<1>(s, p, backward);
+            if (p.vec == 8) whole<8>(s, p, residual, backward);
+            else if (p.vec == 4) whole<4>(s, p, residual, backward);
+            else whole<1>(s, p, residual, backward);
         }
     }
     std::printf("resident %d, twice %d, single values %d, loose lines %d\n", resident, twice, single, loose);

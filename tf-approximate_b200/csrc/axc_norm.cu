@@ -48,6 +48,7 @@ struct NormArgs {
     bool whole_vectors;                        // a thread's channels are neighbours, and of one group
     Span vectors;                              // then: the span's vectors in place of its channels
     Divider by_group;                          // channels of a group
+    int entries, lanes;                        // norm_entries, norm_lanes
     long long shares;
     float2 *part;                              // [samples][shares][channels] sums of a share of the places
     float2 *sums;                              // [samples][channels] {sum of dz, sum of dz xhat}; may be NULL
@@ -631,6 +632,20 @@ struct Sums {
             off[i] = fma2(d[i], o[i], off[i]);
         }
     }
+    // of all lanes of the warp whose number is this one's modulo `period`
+    __device__ __forceinline__ void over_lanes(int period)
+    {
+        for (int o = 16; o >= period; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                Two a, b;
+                a.v = __shfl_xor_sync(0xffffffffu, dz[i].v, o);
+                b.v = __shfl_xor_sync(0xffffffffu, off[i].v, o);
+                dz[i] = add2(dz[i], a);
+                off[i] = add2(off[i], b);
+            }
+        }
+    }
     __device__ __forceinline__ float2 of(int i) const
     {
         const float2 a = dz[i / 2].both(), b = off[i / 2].both();
@@ -673,7 +688,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_forward_kernel(const Nor
     const size_t room = norm_up16(size_t(P.steps) * P.span.active * V * sizeof(T));
     Word *kept = reinterpret_cast<Word *>(raw) + thread;
     float2 *entries = reinterpret_cast<float2 *>(raw + room);
-    float2 *mine = entries + entry_places(P.span), *result = mine + groups;
+    float2 *mine = entries + P.entries, *result = mine + groups;
     const T *x = static_cast<const T *>(P.x), *residual = static_cast<const T *>(P.residual);
     fetch<T, V>(x + at.sample0, w, kept, stride, x, P.values());
     wait_copies();
@@ -755,7 +770,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_forward_kernel(const Nor
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_backward_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const NormArgs P)
 {
     after_previous();
     extern __shared__ __align__(16) char raw[];
@@ -766,12 +781,14 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_backward_kernel(const No
     const bool with = P.residual && P.activation != kActNone;
     const size_t room = norm_up16(size_t(P.steps) * P.span.active * V * sizeof(T));
     Word *kept = reinterpret_cast<Word *>(raw) + thread, *kept_dz = reinterpret_cast<Word *>(raw + room) + thread;      // dy's, first
-    float2 *entries = reinterpret_cast<float2 *>(raw + 2 * room);
-    float2 *channels = entries + entry_places(P.span), *mine = channels + P.span.channels, *result = mine + groups;
+    Word *kept_residual = reinterpret_cast<Word *>(raw + 2 * room) + thread;
+    float2 *entries = reinterpret_cast<float2 *>(raw + (with ? 3 : 2) * room);
+    float2 *channels = entries + P.entries, *mine = channels + P.span.channels, *result = mine + groups;
     const long long values = P.values();
     const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
     fetch<T, V>(x + at.sample0, w, kept, stride, x, values);
     fetch<T, V>(dy + at.sample0, w, kept_dz, stride, dy, values);
+    if (with) fetch<T, V>(residual + at.sample0, w, kept_residual, stride, residual, values);
     const float2 *statistics = P.statistics + at.sample * P.groups + at.span * groups;
     [[maybe_unused]] const long long in_statistics = P.samples * P.groups - (at.sample * P.groups + at.span * groups);
     auto stats = [&](int g) { return AXC_GLOBAL_OK(g, in_statistics, 508u) ? statistics[g] : make_float2(0.0f, 0.0f); };
@@ -782,29 +799,34 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_backward_kernel(const No
     Sums<V> sums;
     T *dresidual = static_cast<T *>(P.dresidual);
     wait_copies();
-    batches<V>(w, std::integral_constant<int, 4>(), [&](auto whole, auto n, int j) {
+    batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
         constexpr int N = decltype(n)::value;
         const long long from = at.sample0 + w.at + j * w.step;
-        Pack<T, V> vr[N];
-        if (with) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
-        }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            Pack<T, V> vx, vd;
+            Pack<T, V> vx, vd, vr;
             vx.w = kept[(j + k) * stride];
             vd.w = kept_dz[(j + k) * stride];
+            if (with) vr.w = kept_residual[(j + k) * stride];
             Two dz[kPairs<V>], off[kPairs<V>];
-            slope_at<T, V>(P, ch, vx, vd, vr[k], dz, off);
+            slope_at<T, V>(P, ch, vx, vd, vr, dz, off);
             sums.template add<decltype(whole)::value>(w, j + k, dz, off);
             if (P.activation != kActNone) kept_dz[(j + k) * stride] = narrow_pairs<T, V>(dz).w;
             if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
         }
     });
-    if (thread < P.span.active) give_entries<V>(entries, P.span, [&](int i) { return sums.of(i); });
+    Entries E(P.span, shift, w.total);
+    if (P.lanes) {
+        // (every thread takes part, and no line starts inside 16 bytes)
+        sums.over_lanes(P.lanes);
+        E.copies = int(blockDim.x) / 32;
+        if ((thread & 31) < P.lanes) {
+            float2 *to = entries + (thread >> 5) * (P.span.channels + 1) + (thread & 31) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) to[i] = sums.of(i);
+        }
+    } else if (thread < P.span.active) give_entries<V>(entries, P.span, [&](int i) { return sums.of(i); });
     __syncthreads();
-    const Entries E(P.span, shift, w.total);
     join_sums(entries, E, [&](int l, float a, float b) { channels[l] = make_float2(a, b); });
     __syncthreads();
     {
@@ -1225,12 +1247,12 @@ NormPlan plan_of(const NormShape &s, bool backward, bool residual, int sms)
     for (const long long v : {s.places, s.channels, s.groups, (long long)(key * 8 + s.size)}) hash = (hash ^ (unsigned long long)v) * 0x9E3779B97F4A7C15ull, hash ^= hash >> 29;
     Known &k = known[hash % known.size()];
     if (k.key != key || k.shape.samples != s.samples || k.shape.places != s.places || k.shape.channels != s.channels || k.shape.groups != s.groups || k.shape.size != s.size)
-        k = {s, key, backward ? norm_plan(s, 2 * s.size, s.size * (residual ? 5 : 3), 1, sms)
-                              : norm_plan(s, s.size, s.size * (residual ? 3 : 2), 0, sms)};
+        k = {s, key, backward ? norm_plan(s, (residual ? 3 : 2) * s.size, s.size * (residual ? 5 : 3), true, sms)
+                              : norm_plan(s, s.size, s.size * (residual ? 3 : 2), false, sms)};
     return k.plan;
 }
 
-NormArgs args_of(const axc_norm_desc &d, const NormPlan &plan)
+NormArgs args_of(const axc_norm_desc &d, const NormPlan &plan, bool backward)
 {
     NormArgs P = {};
     P.scale_type = d.scale_type;
@@ -1253,7 +1275,9 @@ NormArgs args_of(const axc_norm_desc &d, const NormPlan &plan)
     if (plan.resident) {
         P.steps = int(norm_steps(P.per, plan.span, plan.vec, P.span.active));
         P.span_groups = plan.span / P.each;
-        P.whole_vectors = P.each % plan.vec == 0;
+        P.whole_vectors = plan.vec > 1 && P.each % plan.vec == 0;
+        P.entries = int(norm_entries(plan.span, plan.vec, plan.threads, P.span.active, P.each, backward));
+        P.lanes = norm_lanes(plan.span, plan.vec, plan.threads);
         if (P.whole_vectors) P.vectors = span_of(plan.span / plan.vec, P.span.active, 1);
     }
     P.shares = plan.shares;
@@ -1327,7 +1351,7 @@ extern "C" int axc_group_norm_forward(const axc_norm_desc *desc, const void *x, 
     if (rc) return rc;
     const NormShape s = shape_of(d, on_16(x, residual, y));
     const NormPlan plan = plan_of(s, false, residual != nullptr, sms);
-    NormArgs P = args_of(d, plan);
+    NormArgs P = args_of(d, plan, false);
     if (too_many(P, plan)) return AXC_INVALID_ARGUMENT;
     const size_t need = workspace_of(s, plan, false);
     if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < need)) return AXC_INTERNAL;
@@ -1365,7 +1389,7 @@ extern "C" int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy
     if (rc) return rc;
     const NormShape s = shape_of(d, on_16(dy, x, residual, dx, dresidual));
     const NormPlan plan = plan_of(s, true, residual && d.activation != kActNone, sms);
-    NormArgs P = args_of(d, plan);
+    NormArgs P = args_of(d, plan, true);
     if (too_many(P, plan)) return AXC_INVALID_ARGUMENT;
     if (some && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < workspace_of(s, plan, true))) return AXC_INTERNAL;
     P.dy = dy;

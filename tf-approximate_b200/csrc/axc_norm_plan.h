@@ -60,11 +60,28 @@ inline long long norm_steps(long long places, int span, int vec, int active)
 
 AXC_BOTH size_t norm_up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// Shared memory of a resident block: `kept` bytes for each value, a pair of sums for each of the threads' channels, four floats for each group
-// (a pair for the cluster's blocks to read, a pair of results).
-inline long long norm_smem(long long places, int span, int vec, int active, int kept, long long groups, int sums)
+// Vectors of a line where the lanes of a warp can add up what they have of the same channels, else 0: a power of two, with two lines in a warp at least
+inline int norm_lanes(int span, int vec, int threads)
 {
-    return norm_steps(places, span, vec, active) * active * vec * kept + 48 + ((long long)active * vec + active * vec / span) * 8 + (long long)span * 8 * sums + groups * 16;
+    const int period = span % vec ? 0 : span / vec;
+    return vec > 1 && period > 0 && period <= 16 && (period & (period - 1)) == 0 && threads % 32 == 0 ? period : 0;
+}
+
+// Pairs of sums that a resident block's threads leave each other: one for each thread where its channels are of one group (forward), for each
+// channel and warp where the lanes add up theirs (backward), else for each channel of each thread; a place more for every copy of the span.
+inline long long norm_entries(int span, int vec, int threads, int active, long long each, bool backward)
+{
+    if (!backward && vec > 1 && each % vec == 0) return active + (long long)active * vec / span;
+    if (backward && norm_lanes(span, vec, threads)) return (long long)threads / 32 * (span + 1);
+    return (long long)active * vec + (long long)active * vec / span;
+}
+
+// Shared memory of a resident block: `kept` bytes for each value, the entries, pairs of sums of single channels (backward), four floats for each
+// group (a pair for the cluster's blocks to read, a pair of results).
+inline long long norm_smem(long long places, int span, int vec, int threads, int active, int kept, long long each, bool backward)
+{
+    return norm_steps(places, span, vec, active) * active * vec * kept + 48 + norm_entries(span, vec, threads, active, each, backward) * 8 + (long long)span * 8 * backward +
+           span / each * 16;
 }
 
 // Channels at a time where the tensors are read twice
@@ -77,13 +94,12 @@ inline int norm_columns(const NormShape &s, int *vec)
     return int(s.channels < most ? s.channels : most);
 }
 
-// `kept`: bytes that stay in shared memory for each value; `moved`: bytes read and written for each; `sums`: 1 where sums of single channels are kept,
-// too (the backward pass).
+// `kept`: bytes that stay in shared memory for each value; `moved`: bytes read and written for each.
 //
 // The estimate, in us: all bytes at memory's rate, or the blocks' own times in as many rounds as the SMs take them, whichever is more, and one block's
 // time.  A block takes 3 us for its start, its two exchanges and its end, 1 more in a cluster, and its bytes at what an SM moves with the blocks that
 // fit on it (20 bytes a ns for each, 44 at most).  Pieces of a line below 64 bytes are charged for the rest of what memory moves.
-inline NormPlan norm_plan(const NormShape &s, int kept, int moved, int sums, int sms)
+inline NormPlan norm_plan(const NormShape &s, int kept, int moved, bool backward, int sms)
 {
     NormPlan best = {};
     double least = 1e300;
@@ -104,11 +120,11 @@ inline NormPlan norm_plan(const NormShape &s, int kept, int moved, int sums, int
                     const long long places = (s.places + blocks - 1) / blocks;
                     if ((blocks - 1) * places >= s.places) continue;           // the last one has none
                     if (places * span > (1ll << 20)) continue;
-                    const long long smem = norm_smem(places, int(span), vec, active, kept, k, sums);
+                    const long long smem = norm_smem(places, int(span), vec, threads, active, kept, each, backward);
                     if (smem > kNormSmem) continue;
                     const double line = double(span) * s.size, waste = span == s.channels || line >= 64 ? 1.0 : line >= 32 ? 1.15 : 32 / line;
                     long long fit = kNormSmem / (smem + 1024);
-                    if (fit > 768 / threads) fit = 768 / threads;
+                    if (fit > (backward ? 512 : 768) / threads) fit = (backward ? 512 : 768) / threads;       // registers
                     const double units = double(s.samples) * double(s.groups / k) * blocks;
                     // a thread has four accesses on their way
                     double rate = double(fit) * threads * vec * s.size * 4 / 800.0;
