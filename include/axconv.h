@@ -444,6 +444,29 @@ int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy, const voi
                             const void *residual, void *dx, void *dscale, void *doffset, void *dresidual, void *workspace, size_t workspace_bytes, int device,
                             void *stream);
 
+/* Values in e4m3 codes with one fp32 scale for each block: codes[r, k] = e4m3(x[r, k] / scale), rounded to the nearest, scale the least power of two,
+ * 2^-126 at least, with which the block's largest magnitude is a code (448 at most); a block that has an infinity or a NaN has the scale NaN.
+ * block_rows 1: blocks of 128 neighbours in a row; AXC_SCALE_BLOCK: of 128 rows x 128.  x [rows, inputs] with unit stride along a row; codes
+ * [rows, inputs] contiguous; scales [ceil(rows / block_rows), ceil(inputs / 128)]. */
+enum { AXC_SCALE_BLOCK = 128 };
+int axc_quantize_blocks(const void *x, int64_t rows, int64_t inputs, int64_t row_stride, int32_t type, int32_t block_rows, uint8_t *codes, float *scales, int device,
+                        void *stream);
+/* The dense layer on 8-bit operands:  y = act(x kernel^T + bias + residual),  x [rows, inputs] quantised on the way as axc_quantize_blocks has it for
+ * blocks of one row, kernel [units, inputs] in e4m3 codes with scales [ceil(units / 128), ceil(inputs / 128)], any finite ones.  x, kernel and
+ * residual have unit stride along a row; y [rows, units] contiguous; x, residual and y are of one type, bias [units] of its own.  Sums are fp32 and y is
+ * rounded once.  An infinity or a NaN in a row makes that row of y NaN.
+ * Workspace: axc_dense8_workspace_bytes for the kernel's address (NULL: enough for any), 256-byte aligned, nothing kept in it; axc_matrix_status
+ * reads its status word.  Calls only enqueue kernels: capturable.  Addresses must be multiples of their type's size; a kernel that starts on 16
+ * bytes, with rows of a multiple of 16, is read where it is, any other is copied by every call. */
+typedef struct {
+    int64_t rows, inputs, units;
+    int32_t type, bias_type, activation, reserved;
+    int64_t x_row_stride, kernel_row_stride, residual_row_stride;
+} axc_dense8_desc;
+int axc_dense8_workspace_bytes(const axc_dense8_desc *desc, const void *kernel, int device, size_t *bytes);
+int axc_dense8_forward(const axc_dense8_desc *desc, const void *x, const void *kernel, const float *kernel_scales, const void *bias, const void *residual, void *y,
+                       void *workspace, size_t workspace_bytes, int device, void *stream);
+
 /* Dropout whose mask is computed, and computed again for the gradient, instead of stored:
  *   y[i] = (bits[i] >= share ? x[i] * factor : 0) + residual[i],  share = rate 2^16 rounded, factor = 2^16 / (2^16 - share)  (0 for share 2^16)
  * bits: 16 of the random generator Philox 4x32 with 10 rounds (Salmon, Moraes, Dror, Shaw 2011) under the key `seed` (low word first); values 8 j to
@@ -480,7 +503,7 @@ int axc_debug_bounds_record(int device, uint32_t out4[4]);
  * tables in global memory, and the convolution); negative: the built-in limit of about a second.  With 0 every wait runs
  * out at once: the kernels finish, the outputs are not valid, and axc_conv2d_plan_info reports status 3. */
 int axc_debug_wait_polls(int device, int32_t expand, int32_t convolution);
-/* The same for the waits of the matrix kernels (dense layer, cross entropy), whose status axc_matrix_status reads. */
+/* The same for the waits of the matrix kernels (dense layers, cross entropy), whose status axc_matrix_status reads. */
 int axc_debug_matrix_wait_polls(int device, int32_t polls);
 
 /* Measures what one SM sustains in conflict-free 16-bit shared-memory loads - the operation a table MAC of the

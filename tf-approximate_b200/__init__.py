@@ -15,7 +15,8 @@ from .tables import (exact_table, truncated_table, noisy_table, write_table, rea
 from .ops import (approx_conv2d_with_min_max_vars, approx_depthwise_conv2d_with_min_max_vars,  # noqa: F401
                   ax_conv2d, approx_conv2d,
                   conv2d_output_shape, launch_count, measure_lookup_peak, Table)
-from .layers import Dense, Dropout, FakeApproxConv2D, GroupNorm, fake_quant_with_min_max_vars  # noqa: F401
+from .layers import Dense, Dense8bit, Dropout, FakeApproxConv2D, GroupNorm, fake_quant_with_min_max_vars  # noqa: F401
 from .optimizers import AdamW  # noqa: F401
-from .dense_ops import dense, dense_forward, dense_backward, dense_cross_entropy, dense_cross_entropy_gradients  # noqa: F401
+from .dense_ops import (dense, dense_8bit, dense_backward, dense_cross_entropy, dense_cross_entropy_gradients, dense_forward,  # noqa: F401
+                        quantize_blocks)
 from .norm_ops import dropout, group_norm, group_norm_backward, group_norm_forward  # noqa: F401

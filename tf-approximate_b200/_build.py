@@ -16,7 +16,7 @@ LIB_CHECK = os.path.join(HERE, "libaxconv_check.so")
 OBJDIR = os.path.join(HERE, "build")
 SOURCES = ["axc_api.cu", "axc_conv.cu", "axc_sched.cu", "axc_xtab.cu", "axc_depthwise.cu", "axc_probe.cu", "axc_qconv.cu", "axc_prologue.cu",
            "axc_adamw.cu", "axc_gemm.cu", "axc_dense.cu", "axc_rows.cu", "axc_entropy.cu",
-           "axc_norm.cu", "axc_dropout.cu"]
+           "axc_norm.cu", "axc_dropout.cu", "axc_dense8.cu"]
 
 
 BINDING = os.path.join(HERE, "_axc_torch.so")

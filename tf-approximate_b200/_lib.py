@@ -19,6 +19,7 @@ SYMBOLS = [
     "axc_adamw_state_blocks", "axc_adamw_step",
     "axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes", "axc_entropy", "axc_scale",
     "axc_group_norm_workspace_bytes", "axc_group_norm_forward", "axc_group_norm_backward", "axc_dropout",
+    "axc_quantize_blocks", "axc_dense8_workspace_bytes", "axc_dense8_forward",
 ]
 
 
@@ -137,7 +138,7 @@ def binding():
 
         names = ("axc_dense_workspace_bytes", "axc_dense_forward", "axc_dense_backward", "axc_matrix_status", "axc_entropy_workspace_bytes",
                  "axc_entropy", "axc_adamw_step", "axc_scale", "axc_group_norm_workspace_bytes", "axc_group_norm_forward", "axc_group_norm_backward",
-                 "axc_dropout")
+                 "axc_dropout", "axc_quantize_blocks", "axc_dense8_workspace_bytes", "axc_dense8_forward")
         module.init(tuple(C.cast(getattr(L, n), C.c_void_p).value for n in names), errors.InvalidArgumentError, errors.InternalError, raise_for_status)
         _binding = module
     return _binding

@@ -738,7 +738,7 @@ int axc_debug_bounds_record(int device, uint32_t out4[4])
     cudaError_t e = cudaDeviceSynchronize();
     int (*const readers[])(unsigned[4]) = {axc::bounds_record_sched, axc::bounds_record_conv, axc::bounds_record_depthwise, axc::bounds_record_xtab,
                                            axc::bounds_record_adamw, axc::bounds_record_gemm, axc::bounds_record_dense, axc::bounds_record_rows,
-                                           axc::bounds_record_entropy, axc::bounds_record_norm, axc::bounds_record_dropout};
+                                           axc::bounds_record_entropy, axc::bounds_record_norm, axc::bounds_record_dropout, axc::bounds_record_dense8};
     constexpr int kParts = int(sizeof(readers) / sizeof(readers[0]));
     unsigned parts[kParts][4] = {};
     int rc = e == cudaSuccess ? AXC_OK : axc::cuda_failed(e);
@@ -779,7 +779,8 @@ int axc_debug_matrix_wait_polls(int device, int32_t polls)
     AXC_CUDA(cudaGetDevice(&prev));
     if (prev != device) AXC_CUDA(cudaSetDevice(device));
     cudaError_t e = cudaDeviceSynchronize();
-    const int rc = e == cudaSuccess ? axc::set_matrix_wait_polls(polls) : axc::cuda_failed(e);
+    int rc = e == cudaSuccess ? axc::set_matrix_wait_polls(polls) : axc::cuda_failed(e);
+    if (!rc) rc = axc::set_dense8_wait_polls(polls);
     if (prev != device) cudaSetDevice(prev);
     return rc;
 #endif

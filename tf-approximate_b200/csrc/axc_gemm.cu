@@ -23,11 +23,10 @@
 //
 // Products whose tiles are too few have k split over CTAs; the partial sums are added in a fixed order by a second
 // kernel, which also applies what follows the product.
-#include <cudaTypedefs.h>
-
 #include <atomic>
 
 #include "axc_gemm.h"
+#include "axc_lines.cuh"
 #include "axc_mma.cuh"
 
 namespace axc {
@@ -72,230 +71,6 @@ struct Header {                                // in shared memory
     uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2];
     unsigned tmem;
 };
-
-// ---- lines of 32 rows between a warp's registers and memory --------------------------------------------------------------
-// A lane has a row of the sums, memory wants neighbouring lanes to have neighbouring values: 16 bytes stored by every lane to its own
-// row took 11 300 clocks for a tile of 128 x 256, three times what 512 k of the matrix instructions take.  So the warp turns the
-// rows over in shared memory, 16-byte units exchanged by row so that neither side has bank conflicts, and moves N units of a row
-// (128 bytes, or 32 where the stages leave no more room) at a time.
-struct Lines {
-    unsigned stage;                            // the warp's shared memory
-    int lane, rows;                            // rows of the 32 that exist
-};
-// What the lines are a part of (debug flavour)
-struct Whole {
-    const char *base;
-    long long bytes;
-};
-
-template <int N>
-__device__ __forceinline__ unsigned unit_at(unsigned stage, int row, int unit) { return stage + unsigned(row * N + (unit ^ (row & (N - 1)))) * 16u; }
-
-// Lines that do not start on 16 bytes: value by value, neighbouring lanes neighbouring ones, several on their way at a time.
-template <int N, typename Pointer, typename Move>
-__device__ __forceinline__ void single_values(const Lines &L, Pointer lines, long long line, int left, int size, const Whole &all, Move move)
-{
-    const int in_row = N * 16 / size;          // a power of two, 8 to 64
-#pragma unroll 8
-    for (int i = 0; i < in_row; ++i) {
-        const int at = i * 32 + L.lane, r = at / in_row, b = (at & (in_row - 1)) * size;
-        if (r < L.rows && b < left && AXC_VALUES_OK(lines + r * line + b, size, all.base, all.bytes, 431u) &&
-            AXC_SHARED_OK(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), unsigned(size), L.stage, L.stage + N * 512u, 432u))
-            move(unit_at<N>(L.stage, r, b >> 4) + unsigned(b & 15), lines + r * line + b, size);
-    }
-}
-
-// `bytes`: how many of a row exist; aligned: all rows start on 16 bytes
-template <int M, int N>
-__device__ __forceinline__ void store_lines(const Lines &L, const uint4 (&q)[M], char *out, long long line, int bytes, int size, bool aligned, const Whole &all)
-{
-#pragma unroll
-    for (int part = 0; part < M; part += N) {
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            if (!AXC_SHARED_OK(unit_at<N>(L.stage, L.lane, u), 16u, L.stage, L.stage + N * 512u, 433u)) continue;
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, L.lane, u)), "r"(q[part + u].x), "r"(q[part + u].y),
-                         "r"(q[part + u].z), "r"(q[part + u].w) : "memory");
-        }
-        __syncwarp();
-        char *to = out + part * 16;
-        const int left = bytes - part * 16;
-        if (aligned && left >= N * 16) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int r = (i * 32 + L.lane) / N, u = L.lane % N;
-                uint4 w;
-                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(unit_at<N>(L.stage, r, u)));
-                if (r < L.rows && AXC_VALUES_OK(to + r * line + u * 16, 16, all.base, all.bytes, 434u)) *reinterpret_cast<uint4 *>(to + r * line + u * 16) = w;
-            }
-        } else {
-            single_values<N>(L, to, line, left, size, all, [](unsigned from, char *at, int size) {
-                if (size == 2) {
-                    unsigned short h;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from));
-                    *reinterpret_cast<unsigned short *>(at) = h;
-                } else {
-                    unsigned w;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from));
-                    *reinterpret_cast<unsigned *>(at) = w;
-                }
-            });
-        }
-    }
-}
-
-// The other way: M units of the lane's row, zeros where there is nothing.
-template <int M, int N>
-__device__ __forceinline__ void load_lines(const Lines &L, uint4 (&q)[M], const char *in, long long line, int bytes, int size, bool aligned, const Whole &all)
-{
-#pragma unroll
-    for (int part = 0; part < M; part += N) {
-        __syncwarp();
-        const char *from = in + part * 16;
-        const int left = bytes - part * 16;
-        if (aligned && left >= N * 16) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int r = (i * 32 + L.lane) / N, u = L.lane % N;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (r < L.rows && AXC_VALUES_OK(from + r * line + u * 16, 16, all.base, all.bytes, 435u)) w = *reinterpret_cast<const uint4 *>(from + r * line + u * 16);
-                if (!AXC_SHARED_OK(unit_at<N>(L.stage, r, u), 16u, L.stage, L.stage + N * 512u, 436u)) continue;
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(unit_at<N>(L.stage, r, u)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
-            }
-        } else {
-            single_values<N>(L, from, line, left, size, all, [](unsigned to, const char *at, int size) {
-                if (size == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(*reinterpret_cast<const unsigned short *>(at)) : "memory");
-                else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<const unsigned *>(at)) : "memory");
-            });
-        }
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[part + u].x), "=r"(q[part + u].y), "=r"(q[part + u].z), "=r"(q[part + u].w)
-                         : "r"(unit_at<N>(L.stage, L.lane, u)));
-    }
-}
-
-__device__ __forceinline__ bool lines_aligned(const void *base, long long line_bytes) { return ((reinterpret_cast<uintptr_t>(base) | uintptr_t(line_bytes)) & 15u) == 0; }
-
-// W fp32 values of every lane's row, as `type`; columns n0 .. of n; values: all that there are from `base` on
-template <int W, int N>
-__device__ __forceinline__ void store_row(const Lines &L, const float (&v)[W], void *base, int type, long long line, int row0, int n0, int n, long long values)
-{
-    const int size = type == kFloat32 ? 4 : 2, left = n - n0;
-    char *out = static_cast<char *>(base) + (row0 * line + n0) * size;
-    const bool aligned = lines_aligned(base, line * size);
-    const int bytes = (left < W ? left : W) * size;
-    const Whole all = {static_cast<const char *>(base), values * size};
-    if (type == kFloat32) {
-        uint4 q[W / 4];
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i)
-            q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
-        store_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, out, line * 4, bytes, 4, aligned, all);
-    } else {
-        const bool bf16 = type == kBfloat16;
-        uint4 q[W / 8];
-#pragma unroll
-        for (int i = 0; i < W / 8; ++i)
-            q[i] = make_uint4(pack2(v[8 * i], v[8 * i + 1], bf16), pack2(v[8 * i + 2], v[8 * i + 3], bf16), pack2(v[8 * i + 4], v[8 * i + 5], bf16),
-                              pack2(v[8 * i + 6], v[8 * i + 7], bf16));
-        store_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, out, line * 2, bytes, 2, aligned, all);
-    }
-}
-
-// bias[n0 + i] of W columns, W / 32 in each lane; column() hands one to all lanes
-template <int W>
-struct ColumnValues {
-    float mine[W < 32 ? 1 : W / 32];
-    __device__ __forceinline__ ColumnValues(const void *values, int type, int n0, int n, int lane)
-    {
-#pragma unroll
-        for (int i = 0; i < (W < 32 ? 1 : W / 32); ++i) {
-            const int c = n0 + 32 * i + lane;
-            mine[i] = values && c < n && AXC_GLOBAL_OK(c, n, 437u) ? load_as_float(values, c, type) : 0.0f;
-        }
-    }
-    __device__ __forceinline__ float column(int i) const { return __shfl_sync(0xffffffffu, mine[i / 32], i & 31); }
-};
-
-// One row of W sums (columns n0 ..), W a multiple of 16; all lanes of the warp, whether their row exists or not
-template <int W, int N>
-__device__ __forceinline__ void finish_row(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0, float alpha)
-{
-    const Finish &f = P.fin;
-    if (n0 >= P.n) return;
-    const bool exact = f.out_type == kFloat32;
-    float v[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = alpha * __uint_as_float(x[i]);
-    if (f.bias) {
-        const ColumnValues<W> bias(f.bias, f.bias_type, n0, P.n, L.lane);
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] += bias.column(i);
-    }
-    if (f.addend) {
-        const int size = f.addend_type == kFloat32 ? 4 : 2, left = P.n - n0, bytes = (left < W ? left : W) * size;
-        const char *in = static_cast<const char *>(f.addend) + ((long long)row0 * f.addend_line + n0) * size;
-        const bool aligned = lines_aligned(f.addend, f.addend_line * size);
-        const Whole all = {static_cast<const char *>(f.addend), f.addend_values() * size};
-        if (size == 4) {
-            uint4 q[W / 4];
-            load_lines<W / 4, (W / 4 < N ? W / 4 : N)>(L, q, in, f.addend_line * 4, bytes, 4, aligned, all);
-#pragma unroll
-            for (int i = 0; i < W / 4; ++i) {
-                v[4 * i] += __uint_as_float(q[i].x);
-                v[4 * i + 1] += __uint_as_float(q[i].y);
-                v[4 * i + 2] += __uint_as_float(q[i].z);
-                v[4 * i + 3] += __uint_as_float(q[i].w);
-            }
-        } else {
-            uint4 q[W / 8];
-            load_lines<W / 8, (W / 8 < N ? W / 8 : N)>(L, q, in, f.addend_line * 2, bytes, 2, aligned, all);
-#pragma unroll
-            for (int i = 0; i < W / 8; ++i) {
-                const unsigned u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 t = f.addend_type == kBfloat16 ? __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 &>(u[j]))
-                                                                : __half22float2(reinterpret_cast<const __half2 &>(u[j]));
-                    v[8 * i + 2 * j] += t.x;
-                    v[8 * i + 2 * j + 1] += t.y;
-                }
-            }
-        }
-    }
-    if (f.pre) store_row<W, N>(L, v, f.pre, f.out_type, f.out_line, row0, n0, P.n, f.out_values());
-    if (f.activation == kActRelu) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActRelu, exact);
-    } else if (f.activation == kActGelu) {
-        if (exact) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActGelu, true);
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActGelu, false);
-        }
-    } else if (f.activation == kActSilu) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = exact ? activate(v[i], kActSilu, true) : activate(v[i], kActSilu, false);
-    }
-    store_row<W, N>(L, v, f.out, f.out_type, f.out_line, row0, n0, P.n, f.out_values());
-}
-
-// Partial sums in the order of the output's lines
-template <int W, int N>
-__device__ __forceinline__ void store_part(const GemmArgs &P, const Lines &L, unsigned (&x)[W], int row0, int n0, int split)
-{
-    if (n0 >= P.n) return;
-    float *part = P.part + (long long)split * P.part_stride;
-    float v[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = __uint_as_float(x[i]);
-    store_row<W, N>(L, v, part, kFloat32, P.part_line, row0, n0, P.n, (P.splits - split) * P.part_stride);
-}
 
 // One segment of 64 logits of a row: the exponentials relative to the largest, their sum, and the label's logit on the way.
 // A segment of -inf has the exponentials 0 (relative to 0, not to itself); one with a NaN has nothing else.  `label`: the row's.
@@ -522,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             const int of_lane = row0 + lane < P.m ? row0 + lane : P.m - 1;
             const long long label = MODE == kEntropy ? P.ent.labels[of_lane] : 0;
             auto take = [&](unsigned (&x)[W], int c) {
-                if constexpr (MODE == kStore) finish_row<W, kUnits>(P, L, x, row0, n0 + c, alpha);
-                else if constexpr (MODE == kPartial) store_part<W, kUnits>(P, L, x, row0, n0 + c, split);
+                if constexpr (MODE == kStore) finish_row<W, kUnits>(P.fin, P.n, L, x, row0, n0 + c, alpha);
+                else if constexpr (MODE == kPartial) store_part<W, kUnits>(P.part, P.part_line, P.part_stride, P.splits, P.n, L, x, row0, n0 + c, split);
                 else if constexpr (MODE == kGradient) gradient_columns<W, kUnits, PLANES == 3>(P, L, x, row0, n0 + c);
                 else entropy_segment<kUnits, PLANES == 3>(P, L, x, row0, n0 + c, label);
             };
@@ -626,6 +401,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const float *part, long lon
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
+}  // namespace
+
 PFN_cuTensorMapEncodeTiled_v12000 encoder()
 {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
@@ -636,6 +413,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder()
     }();
     return fn;
 }
+
+namespace {
 
 // Boxes of 64 k x `box` rows (k contiguous), or 64 rows x 64 k; what lies outside the matrix arrives as zeros.
 bool make_map(const Operand &o, long long rows, long long k, int planes, bool bf16, unsigned box, CUtensorMap *map)
@@ -651,12 +430,9 @@ bool make_map(const Operand &o, long long rows, long long k, int planes, bool bf
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a product is cut up: CTAs per tile, columns of a tile, splits of k.
-struct Plan {
-    int cg, bn, splits;
-};
-
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+}  // namespace
 
 // The cheapest of the tiles and splits by an estimate in clocks.  A stage takes what its matrix instructions take (2 for each column of
 // a tile, 390 at least) or what its bytes take (114 a clock and SM when all SMs have tiles, in proportion when few have), whichever is
@@ -694,6 +470,8 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
     }
     return best;
 }
+
+namespace {
 
 template <int CG, int BN, int MODE, int PLANES, bool CLOSE>
 int launch_gemm(GemmArgs &P, long long units, const DeviceInfo &di, Queue &q)

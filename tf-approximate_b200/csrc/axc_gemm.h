@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cudaTypedefs.h>
 #include <float.h>
 
 #include "axc_internal.h"
@@ -251,6 +252,14 @@ struct Gemm {
     bool bf16;
     Finish fin;
 };
+
+// How a product is cut up: CTAs per tile, columns of a tile, splits of k.
+struct Plan {
+    int cg, bn, splits;
+};
+// planes: terms of an operand; may_split: also tiles below 64 columns
+Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, int sms);
+PFN_cuTensorMapEncodeTiled_v12000 encoder();    // NULL where the driver has none
 
 // Scratch for the partial sums of a product whose k is split; 0 where it is not.
 size_t gemm_scratch(long long m, long long n, long long k, int planes, const DeviceInfo &di);

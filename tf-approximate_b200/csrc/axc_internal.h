@@ -79,8 +79,10 @@ int bounds_record_rows(unsigned out4[4]);
 int bounds_record_entropy(unsigned out4[4]);
 int bounds_record_norm(unsigned out4[4]);
 int bounds_record_dropout(unsigned out4[4]);
+int bounds_record_dense8(unsigned out4[4]);
 int set_wait_polls(int expand, int convolution);      // debug flavour only
 int set_matrix_wait_polls(int polls);                 // debug flavour only
+int set_dense8_wait_polls(int polls);                 // debug flavour only
 
 // Quantisation state of one call: what the reference keeps in
 // BaseTableApproxOpType_t::quantProps (tf2/src/approx_ops_types.h:84-96).

@@ -30,6 +30,9 @@ struct Entry {
     decltype(&axc_group_norm_forward) norm_forward;
     decltype(&axc_group_norm_backward) norm_backward;
     decltype(&axc_dropout) dropout;
+    decltype(&axc_quantize_blocks) quantize;
+    decltype(&axc_dense8_workspace_bytes) dense8_bytes;
+    decltype(&axc_dense8_forward) dense8_forward;
 };
 Entry g_entry = {};
 PyObject *g_invalid = nullptr, *g_internal = nullptr, *g_raise = nullptr;    // exception classes; raise_for_status(status, what)
@@ -554,6 +557,88 @@ PyObject *dropout(PyObject *, PyObject *const *a, Py_ssize_t count)
     AXC_TORCH_END
 }
 
+// rows of a matrix with unit stride along them, as they lie or copied
+at::Tensor in_lines(const at::Tensor &t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
+int64_t line_of(const at::Tensor &t) { return t.size(1) <= 1 ? (t.stride(0) > 0 ? t.stride(0) : 0) : t.stride(0); }
+
+// quantize_blocks(x, rows) -> (codes, scales)
+PyObject *quantize_blocks(PyObject *, PyObject *const *a, Py_ssize_t count)
+{
+    AXC_TORCH_BEGIN
+    if (count != 2) invalid("quantize_blocks takes 2 arguments");
+    c10::NoGradGuard no_grad;
+    const at::Tensor x = tensor_of(a[0], "x", false);
+    if (!x.is_cuda() || type_of(x) < 0) invalid("x must be a float32, bfloat16 or float16 CUDA tensor (this build has no CPU kernel)");
+    const int64_t rows = PyLong_AsLongLong(a[1]);
+    if (PyErr_Occurred()) throw Raised();
+    if (rows != 1 && rows != AXC_SCALE_BLOCK) invalid("a block has 1 row or 128");
+    if (x.dim() < 1 || (rows != 1 && x.dim() != 2)) invalid("x [..., inputs] expected, with two dimensions where a block has 128 rows; got " + text_of(x.sizes()));
+    const at::Tensor m = in_lines(as_rows(x));
+    const int64_t r = m.size(0), k = m.size(1), blocks = (k + AXC_SCALE_BLOCK - 1) / AXC_SCALE_BLOCK;
+    const at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = blocks;
+    if (rows != 1) shape[0] = (r + rows - 1) / rows;
+    const at::Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
+    check(g_entry.quantize(address(m), r, k, line_of(m), type_of(x), int32_t(rows), static_cast<uint8_t *>(out_address(codes)), static_cast<float *>(out_address(scales)),
+                           x.device().index(), stream_of(x)),
+          "quantize_blocks");
+    return Py_BuildValue("(NN)", wrap(codes), wrap(scales));
+    AXC_TORCH_END
+}
+
+// dense_8bit(x, kernel, kernel_scales, bias, residual, activation, check) -> y
+PyObject *dense_8bit(PyObject *, PyObject *const *a, Py_ssize_t count)
+{
+    AXC_TORCH_BEGIN
+    if (count != 7) invalid("dense_8bit takes 7 arguments");
+    c10::NoGradGuard no_grad;
+    const at::Tensor x = tensor_of(a[0], "x", false);
+    at::Tensor kernel = tensor_of(a[1], "kernel", false);
+    const at::Tensor scales = tensor_of(a[2], "kernel_scales", false), bias = tensor_of(a[3], "bias", true);
+    if (!x.is_cuda() || type_of(x) < 0) invalid("x must be a float32, bfloat16 or float16 CUDA tensor (this build has no CPU kernel)");
+    if (kernel.scalar_type() != at::kFloat8_e4m3fn || kernel.device() != x.device() || kernel.dim() != 2) invalid("kernel must be a float8_e4m3fn tensor [units, inputs] on x's device");
+    if (x.dim() < 1 || x.size(-1) != kernel.size(1) || kernel.size(1) < 1)
+        invalid("x [..., inputs] and kernel [units, inputs] expected, got " + text_of(x.sizes()) + " and " + text_of(kernel.sizes()));
+    const int64_t units = kernel.size(0), inputs = kernel.size(1), squares = (units + AXC_SCALE_BLOCK - 1) / AXC_SCALE_BLOCK, blocks = (inputs + AXC_SCALE_BLOCK - 1) / AXC_SCALE_BLOCK;
+    if (scales.scalar_type() != at::kFloat || scales.device() != x.device() || scales.dim() != 2 || scales.size(0) != squares || scales.size(1) != blocks)
+        invalid("kernel_scales must be a float32 tensor of shape (" + std::to_string(squares) + ", " + std::to_string(blocks) + ") on x's device");
+    if (bias.defined() && (type_of(bias) < 0 || bias.device() != x.device() || bias.dim() != 1 || bias.size(0) != units))
+        invalid("bias must be a float32, bfloat16 or float16 tensor of shape (" + std::to_string(units) + ",) on x's device");
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = units;
+    at::Tensor residual = tensor_of(a[4], "residual", true);
+    if (residual.defined()) {
+        if (residual.scalar_type() != x.scalar_type() || residual.device() != x.device() || residual.sizes() != at::IntArrayRef(shape))
+            invalid("residual must be a tensor of x's type, of shape " + text_of(shape) + " on x's device");
+        residual = in_lines(as_rows(residual));
+    }
+    const at::Tensor m = in_lines(as_rows(x)), s = scales.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+    kernel = in_lines(kernel);
+    const at::Tensor y = at::empty(shape, x.options());
+    axc_dense8_desc d = {};
+    d.rows = m.size(0);
+    d.inputs = inputs;
+    d.units = units;
+    d.type = type_of(x);
+    d.bias_type = b.defined() ? type_of(b) : AXC_TYPE_FLOAT32;
+    d.activation = int(PyLong_AsLong(a[5]));
+    d.x_row_stride = line_of(m);
+    d.kernel_row_stride = line_of(kernel);
+    d.residual_row_stride = residual.defined() ? line_of(residual) : 0;
+    const int device = x.device().index();
+    size_t bytes = 0;
+    check(g_entry.dense8_bytes(&d, address(kernel), device, &bytes), "dense_8bit");
+    const at::Tensor ws = scratch(x, bytes);
+    void *stream = stream_of(x);
+    check(g_entry.dense8_forward(&d, address(m), address(kernel), static_cast<const float *>(address(s)), address(b), address(residual), out_address(y), out_address(ws), bytes,
+                                 device, stream),
+          "dense_8bit");
+    if (a[6] == Py_True && y.numel()) check_waits(ws, device, stream);
+    return wrap(y);
+    AXC_TORCH_END
+}
+
 // init(addresses of the entry points, InvalidArgumentError, InternalError, raise_for_status)
 PyObject *init(PyObject *, PyObject *args)
 {
@@ -588,6 +673,8 @@ PyMethodDef g_methods[] = {{"init", init, METH_VARARGS, nullptr},
                            {"group_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_forward)), METH_FASTCALL, nullptr},
                            {"group_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_backward)), METH_FASTCALL, nullptr},
                            {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dropout)), METH_FASTCALL, nullptr},
+                           {"quantize_blocks", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_blocks)), METH_FASTCALL, nullptr},
+                           {"dense_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense_8bit)), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_axc_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -115,3 +115,26 @@ def dense_cross_entropy(x, kernel, labels, bias=None, ignore_index=-100, reducti
         return _EntropyFn.apply(x, kernel, bias, labels, ignore_index, reduction, scratch_limit)
     loss, rows, _, _, _ = _entropy(x, kernel, labels, bias, ignore_index, reduction, 1.0, scratch_limit, bool(row_losses), (False, False, False), False)
     return (loss, rows) if row_losses else loss
+
+
+def quantize_blocks(x, rows=1):
+    """(codes, scales): x in float8_e4m3fn codes with one fp32 scale for each block, so that codes * scale is x to within half a step of three bits.
+
+    rows=1: blocks of 128 neighbours along the last dimension, x [..., inputs], scales [..., ceil(inputs / 128)]; rows=128: blocks of 128 x 128,
+    x [units, inputs], scales [ceil(units / 128), ceil(inputs / 128)], as `dense_8bit` takes a kernel.  A scale is the least power of two, 2^-126 at
+    least, with which the block's largest magnitude is a code (448 at most); a block with an infinity or a NaN has the scale NaN."""
+    return _lib.binding().quantize_blocks(x, rows)
+
+
+def dense_8bit(x, kernel, kernel_scales, bias=None, residual=None, activation=None, check=False):
+    """activation(x kernel^T + bias + residual) on 8-bit operands: the dense layer of a network that answers.
+
+    kernel [units, inputs] and kernel_scales are what `quantize_blocks(..., rows=128)` makes of a trained kernel (of `Dense`: its transpose); x
+    [..., inputs] in float32, bfloat16 or float16 is quantised on the way, each row's blocks of 128 by themselves.  bias [units] may be of another of
+    these types; residual has y's shape, and y x's type.  Sums are fp32 and y is rounded once.  An infinity or a NaN in a row of x makes that row of y
+    NaN.  Up to 8 rows read the kernel once, at memory's rate.  A kernel whose rows do not start on 16 bytes is copied by every call.
+    There are no gradients: operands that are differentiated are refused.
+    check: wait for the call and raise InternalError if a wait inside the kernels ran out."""
+    if _differentiated(x, kernel_scales, bias, residual):
+        raise InvalidArgumentError("dense_8bit has no gradients: call it under torch.no_grad(), or on detached tensors")
+    return _lib.binding().dense_8bit(x, kernel, kernel_scales, bias, residual, _activation(activation), bool(check))

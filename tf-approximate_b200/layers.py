@@ -230,6 +230,34 @@ class Dense(torch.nn.Module):
         return dense_ops.dense_cross_entropy(inputs.to(self.kernel.dtype), self.kernel, labels, self.bias, ignore_index, reduction)
 
 
+class Dense8bit(torch.nn.Module):
+    """A trained `Dense` layer, ready to answer in 8-bit floating point: its kernel is quantised here, once, and kept as codes [units, in_features] with
+    their scales; inputs are quantised by the call.  It has buffers and no parameters."""
+
+    def __init__(self, dense):
+        super().__init__()
+        if not isinstance(dense, Dense):
+            raise ops.InvalidArgumentError("a Dense layer expected")
+        self.activation, self.units, self.in_features = dense.activation, dense.kernel.shape[1], dense.kernel.shape[0]
+        with torch.no_grad():
+            codes, scales = dense_ops.quantize_blocks(dense.kernel.detach().t().contiguous(), rows=128)
+            # rows of a multiple of 16 bytes, which the matrix kernels read where they are
+            lines = torch.zeros(self.units, -(-self.in_features // 16) * 16, dtype=torch.uint8, device=codes.device)
+            lines[:, :self.in_features] = codes.view(torch.uint8)
+        self.register_buffer("lines", lines)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", None if dense.bias is None else dense.bias.detach().clone())
+
+    @property
+    def kernel(self):
+        """The codes, [units, in_features]."""
+        return self.lines.view(torch.float8_e4m3fn)[:, :self.in_features]
+
+    @torch.no_grad()
+    def forward(self, inputs, residual=None):
+        return dense_ops.dense_8bit(inputs, self.kernel, self.scales, self.bias, residual, self.activation)
+
+
 class GroupNorm(torch.nn.Module):
     """Group norm of tensors with their channels last, in the manner of Keras' GroupNormalization, with the activation that follows it (and, where
     the call has one, the shortcut that is added before it): activation(normalised inputs * scale + offset + residual)."""
