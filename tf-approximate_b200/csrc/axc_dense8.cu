@@ -9,7 +9,7 @@
 //   many rows     tcgen05 matrix instructions on 8-bit operands, 128 k a stage, which is a block: its sums are taken out of tensor memory, times the two
 //                 scales, and added in registers, while the next block's are made in the other half of the tensor memory.  Tiles, splits of k and the
 //                 ring of stages are those of the 16-bit products (axc_gemm.cu): a stage has as many bytes, and as many clocks.
-//   up to 8 rows  bound by reading the kernel once.  Eight warps share a block's 16 units and have every eighth block of 128 inputs each; a lane reads 16
+//   up to 8 rows  bound by reading the kernel once.  Four warps share a block's 16 units and have every fourth block of 128 inputs each; a lane reads 16
 //                 bytes of two units at a time, turns them into fp16 (exact) and multiplies by mma with the rows as its columns: on plain
 //                 multiply-adds 8 rows would cost eight times what one does.  The order of k within a block is the lanes' own, the same for both operands.
 // Sums within a block are the matrix pipes', over blocks fp32 with rounding; y is rounded once.
@@ -169,7 +169,9 @@ __global__ void __launch_bounds__(256) lay_out_codes_kernel(const uint8_t *src, 
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------
-constexpr int kThreads = 320;                  // warps: 0 loads and holds the tensor memory, 1 multiplies, 2 to 9 take the sums out
+// Warps: 0 loads and holds the tensor memory, 1 multiplies, 4 to 11 take the sums out.  Those hold 128 sums a thread beside what is on its way, so
+// the first warpgroup leaves them its registers: 384 threads are launched with 168 each, 128 * 40 + 256 * 232 is as many.
+constexpr int kThreads = 384, kFewRegisters = 40, kManyRegisters = 232;
 constexpr unsigned kHeader = 1024, kSmem = 227 * 1024;
 constexpr int kMaxStages = 12, kUnits = 8;     // 16-byte units of a row that a warp turns over at a time
 
@@ -259,7 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
     asm volatile("griddepcontrol.wait;" ::: "memory");          // the codes of the rows come from the kernel before
     bool ok = true;
     const int polls = AXC_DENSE8_POLLS;
-
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
         const bool leader = mma::elect();
         const unsigned signal = CG == 2 ? mma::in_cta(full, 0) : full;
@@ -311,10 +314,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
                 if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
             }
         }
-    } else if (warp >= 2) {
-        // warps 2 to 5 take the first half of the columns, 6 to 9 the second; a half has one scale of the kernel at a time
-        constexpr int kHalves = BN >= 128 ? 2 : 1, kMine = BN / kHalves, W = kMine < 32 ? 16 : 32;
-        const int half = (warp - 2) >> 2, quarter = warp & 3;
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+        // warps 4 to 7 take the first half of the columns, 8 to 11 the second; a half has one scale of the kernel at a time
+        constexpr int kHalves = BN >= 128 ? 2 : 1, kMine = BN / kHalves, W = kMine < 32 ? 16 : 32, kChunks = kMine / W;
+        const int half = (warp - 4) >> 2, quarter = warp & 3;
         int buffer = 0;
         unsigned phase = 0;
         for (int u = worker; u < units && ok; u += workers) {
@@ -323,40 +328,41 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
             const int split = u % P.splits;
             const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + half * kMine;
             const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
-            const Lines L = {lines + unsigned(warp - 2) * kUnits * 512u, lane, min(32, P.m - row0)};
+            const Lines L = {lines + unsigned(warp - 4) * kUnits * 512u, lane, min(32, P.m - row0)};
             const int row = min(row0 + lane, P.m - 1), square = min(n0, P.n - 1) / kBlock;
             const float *sa = P.a_scales + row, *sb = P.b_scales + (long long)square * P.blocks;
             const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
             Two sum[kMine / 2];
 #pragma unroll
             for (int i = 0; i < kMine / 2; ++i) sum[i] = Two(0.0f);
-            auto scale_at = [&](int k) {
-                if (!AXC_GLOBAL_OK((long long)k * P.m + row, (long long)P.blocks * P.m, 612u)) return 0.0f;
-                return scales_product(sa[(long long)k * P.m], sb[k]);
-            };
-            float scale = scale_at(k0);
+            // two blocks' scales are on their way ahead of the sums that they belong to
+            auto a_scale = [&](int k) { return AXC_GLOBAL_OK((long long)k * P.m + row, (long long)P.blocks * P.m, 612u) ? __ldg(sa + (long long)k * P.m) : 0.0f; };
+            float a0 = a_scale(k0), b0 = __ldg(sb + k0), a1 = a_scale(min(k0 + 1, k1 - 1)), b1 = __ldg(sb + min(k0 + 1, k1 - 1));
             for (int k = k0; k < k1; ++k) {
-                const float next = scale_at(k + 1 < k1 ? k + 1 : k);
+                const float a2 = a_scale(min(k + 2, k1 - 1)), b2 = __ldg(sb + min(k + 2, k1 - 1));
                 if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase, polls))) break;
                 mma::fence_after();
                 __syncwarp();
                 if (half < kHalves) {
-                    const Two both(scale);
+                    const Two both(scales_product(a0, b0));
+                    const unsigned at = mine + unsigned(buffer) * kColumns;
+                    // the next columns are on their way while these are added
+                    unsigned x[2][W];
+                    mma::load_columns(at, x[0]);
 #pragma unroll
-                    for (int c = 0; c < kMine; c += W) {
-                        unsigned x[W];
-                        mma::load_columns(mine + unsigned(buffer) * kColumns + c, x);
-                        mma::load_wait(x);
+                    for (int c = 0; c < kChunks; ++c) {
+                        mma::load_wait(x[c & 1]);
+                        if (c + 1 < kChunks) mma::load_columns(at + (c + 1) * W, x[(c + 1) & 1]);
 #pragma unroll
                         for (int i = 0; i < W; i += 2)
-                            sum[(c + i) / 2] = fma2(Two(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), both, sum[(c + i) / 2]);
+                            sum[(c * W + i) / 2] = fma2(Two(__uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1])), both, sum[(c * W + i) / 2]);
                     }
                 }
                 mma::fence_before();
                 __syncwarp();
                 if (lane == 0) mma::barrier_arrive_cluster(mma::in_cta(sums_empty + 8 * buffer, 0));
                 if (++buffer == kBuffers) buffer = 0, phase ^= 1u;
-                scale = next;
+                a0 = a1, b0 = b1, a1 = a2, b1 = b2;
             }
             if (!ok) break;
             if (half < kHalves) {
@@ -392,16 +398,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
 
 // ---- up to 8 rows -----------------------------------------------------------------------------------------------------------------
 struct Few8Args {
-    const void *x;
-    int rows, type;
-    long long inputs, units, x_stride;
+    int rows;
+    long long inputs, units;
+    const uint8_t *codes;                      // of the rows, [rows][blocks * 128]
+    const float *a_scales;                     // [blocks][rows]
     const uint8_t *kernel;
     long long kernel_stride;
     const float *b_scales;
     Finish fin;
-    unsigned *status;
 };
-constexpr int kFewWarps = 8, kFewUnits = 16;
+constexpr int kFewWarps = 4, kFewUnits = 16;
 constexpr int kFewSmem = 64 * 1024;            // codes of the rows, at most
 
 // four codes as four fp16 values
@@ -418,19 +424,18 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], unsigned a0, unsigned a
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A block has 16 units.  Shared memory: the rows' codes, [8][line] with 16 bytes between the lines' banks, and their scales [blocks][8].
+// A block has 16 units.  Shared memory: the rows' codes, [rows][line] with 16 bytes between the lines' banks, and their scales [blocks][rows].
 template <bool VEC>
-__global__ void __launch_bounds__(kFewWarps * 32) few8_kernel(const Few8Args A)
+__global__ void __launch_bounds__(kFewWarps * 32, VEC ? 8 : 4) few8_kernel(const Few8Args A)
 {
     extern __shared__ __align__(16) char raw[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int blocks = int((A.inputs + kBlock - 1) / kBlock), line = blocks * kBlock + 16;
     uint8_t *codes = reinterpret_cast<uint8_t *>(raw);
     float *scales = reinterpret_cast<float *>(raw + A.rows * line);
-    float(*sums)[kFewUnits][kFewRows + 1] = reinterpret_cast<float(*)[kFewUnits][kFewRows + 1]>(scales + blocks * kFewRows);
+    float(*sums)[kFewUnits][kFewRows + 1] = reinterpret_cast<float(*)[kFewUnits][kFewRows + 1]>(scales + blocks * A.rows);
     const long long unit0 = (long long)blockIdx.x * kFewUnits;
-    after_previous();
-    if (blockIdx.x == 0 && threadIdx.x == 0) A.status[0] = A.status[1] = 0u;
     // the lane's two units, the last one again behind the last
     const long long u0 = unit0 + g < A.units ? unit0 + g : A.units - 1, u1 = unit0 + g + 8 < A.units ? unit0 + g + 8 : A.units - 1;
     const uint8_t *w0 = A.kernel + u0 * A.kernel_stride + t * 16, *w1 = A.kernel + u1 * A.kernel_stride + t * 16;
@@ -448,54 +453,32 @@ __global__ void __launch_bounds__(kFewWarps * 32) few8_kernel(const Few8Args A)
         }
         return v;
     };
-    // the first block's codes are on their way while the rows are quantised
-    uint4 a[2][2];
-    if (warp < blocks) {
+    auto read_block = [&](int b, uint4 (&a)[2][2]) {
+        if (b >= blocks) return;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const long long k = (long long)warp * kBlock + c * 64;
+            const long long k = (long long)b * kBlock + c * 64;
             a[c][0] = read(w0 + k, k + t * 16);
             a[c][1] = read(w1 + k, k + t * 16);
         }
+    };
+    // Two blocks' codes are on their way from here on.  (They do not come from the kernel before, which quantises the rows, and that one has started
+    // when all before it was over.)
+    uint4 a[2][2][2];
+    read_block(warp, a[0]);
+    read_block(warp + kFewWarps, a[1]);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = threadIdx.x; i < A.rows * blocks * (kBlock / 16); i += kFewWarps * 32) {
+        const int row = i / (blocks * (kBlock / 16)), at = i - row * (blocks * (kBlock / 16));
+        if (AXC_GLOBAL_OK((long long)i * 16 + 15, (long long)A.rows * blocks * kBlock, 615u))
+            *reinterpret_cast<uint4 *>(codes + row * line + at * 16) = reinterpret_cast<const uint4 *>(A.codes)[i];
     }
-    {
-        const int lane16 = threadIdx.x & 15, total = A.rows * blocks;
-        for (int first = 0; first < total; first += kFewWarps * 2) {
-            const int item = first + int(threadIdx.x >> 4), at = min(item, total - 1), row = at / blocks, block = at - row * blocks;
-            const long long k = (long long)block * kBlock + lane16 * 8;
-            float v[8], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const long long from = row * A.x_stride + k + i;
-                v[i] = k + i < A.inputs && AXC_GLOBAL_OK(from, (A.rows - 1) * A.x_stride + A.inputs, 615u) ? load_as_float(A.x, from, A.type) : 0.0f;
-                top = max_keep_nan(top, fabsf(v[i]));
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max_keep_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float inverse;
-            const float scale = scale_of(top, inverse);
-            if (item < total) {
-                *reinterpret_cast<uint2 *>(codes + row * line + block * kBlock + lane16 * 8) =
-                    make_uint2(codes_of(times(v[0], inverse), times(v[1], inverse)) | codes_of(times(v[2], inverse), times(v[3], inverse)) << 16,
-                               codes_of(times(v[4], inverse), times(v[5], inverse)) | codes_of(times(v[6], inverse), times(v[7], inverse)) << 16);
-                if (lane16 == 0) scales[block * kFewRows + row] = scale;
-            }
-        }
-    }
+    for (int i = threadIdx.x; i < A.rows * blocks; i += kFewWarps * 32) scales[i] = A.a_scales[i];
     __syncthreads();
     const int mine = min(g, A.rows - 1), column = 2 * t;      // rows that are not there: the last one again, not used
     const float *b_scales = A.b_scales + unit0 / kBlock * blocks;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = warp; b < blocks; b += kFewWarps) {
-        uint4 next[2][2];
-        if (b + kFewWarps < blocks) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const long long k = (long long)(b + kFewWarps) * kBlock + c * 64;
-                next[c][0] = read(w0 + k, k + t * 16);
-                next[c][1] = read(w1 + k, k + t * 16);
-            }
-        }
+    auto add_block = [&](int b, uint4 (&a)[2][2]) {
         float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -510,14 +493,20 @@ __global__ void __launch_bounds__(kFewWarps * 32) few8_kernel(const Few8Args A)
                 mma_16816(d, p0, q0, p1, q1, r0, r1);
             }
         }
-        const float sb = b_scales[b], t0 = scales_product(scales[b * kFewRows + min(column, A.rows - 1)], sb),
-                    t1 = scales_product(scales[b * kFewRows + min(column + 1, A.rows - 1)], sb);
+        const float sb = b_scales[b], t0 = scales_product(scales[b * A.rows + min(column, A.rows - 1)], sb),
+                    t1 = scales_product(scales[b * A.rows + min(column + 1, A.rows - 1)], sb);
         sum[0] = fmaf(d[0], t0, sum[0]);
         sum[1] = fmaf(d[1], t1, sum[1]);
         sum[2] = fmaf(d[2], t0, sum[2]);
         sum[3] = fmaf(d[3], t1, sum[3]);
+    };
+    for (int b = warp; b < blocks; b += 2 * kFewWarps) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) a[c][0] = next[c][0], a[c][1] = next[c][1];
+        for (int i = 0; i < 2; ++i)
+            if (b + i * kFewWarps < blocks) {
+                add_block(b + i * kFewWarps, a[i]);
+                read_block(b + (i + 2) * kFewWarps, a[i]);
+            }
     }
     sums[warp][g][column] = sum[0];
     sums[warp][g][column + 1] = sum[1];
@@ -542,7 +531,7 @@ size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t few_smem(long long rows, long long inputs)
 {
     const long long blocks = ceil_div(inputs, kBlock);
-    return size_t(rows * (blocks * kBlock + 16) + blocks * kFewRows * 4);
+    return size_t(rows * (blocks * kBlock + 16) + blocks * rows * 4);
 }
 constexpr size_t kFewSums = sizeof(float) * kFewWarps * kFewUnits * (kFewRows + 1);
 
@@ -557,10 +546,10 @@ struct Room8 {
 Room8 room_of(const axc_dense8_desc &d, const void *kernel, int sms)
 {
     Room8 r = {256, 256, 256, 256, 256};       // the status word comes first
-    if (few_rows8(d)) return r;
     const long long blocks = ceil_div(d.inputs, kBlock);
     r.scales = r.codes + up(size_t(d.rows) * size_t(blocks) * kBlock);
-    r.kernel = r.scales + up(size_t(d.rows) * size_t(blocks) * 4);
+    r.total = r.part = r.kernel = r.scales + up(size_t(d.rows) * size_t(blocks) * 4);
+    if (few_rows8(d)) return r;
     r.part = r.kernel + (in_place(d, kernel) ? 0 : up(size_t(d.units) * size_t(ceil_div(d.inputs, 16)) * 16));
     const Plan plan = choose_plan(d.rows, d.units, ceil_div(d.inputs, 2), 1, true, sms);
     r.total = r.part + (plan.splits > 1 ? up(size_t(plan.splits) * size_t(d.rows) * size_t(ceil_div(d.units, 4)) * 16) : 0);
@@ -653,19 +642,6 @@ int forward(const axc_dense8_desc &d, const void *x, const uint8_t *kernel, cons
 {
     unsigned *status = reinterpret_cast<unsigned *>(ws);
     const Finish fin = sized(finish_of(d, bias, residual, y), d.rows, d.units);
-    if (few_rows8(d)) {
-        const Few8Args A = {x, int(d.rows), d.type, d.inputs, d.units, d.x_row_stride, kernel, d.kernel_row_stride, kernel_scales, fin, status};
-        const unsigned smem = unsigned(few_smem(d.rows, d.inputs) + kFewSums);
-        const dim3 grid(unsigned(ceil_div(d.units, kFewUnits)));
-        if (in_place(d, kernel)) {
-            static std::atomic<unsigned long long> ready{0};
-            const int rc = allow_smem(few8_kernel<true>, unsigned(kFewSmem + kFewSums), ready);
-            return rc ? rc : launch(q, few8_kernel<true>, grid, kFewWarps * 32, smem, 1, A);
-        }
-        static std::atomic<unsigned long long> ready{0};
-        const int rc = allow_smem(few8_kernel<false>, unsigned(kFewSmem + kFewSums), ready);
-        return rc ? rc : launch(q, few8_kernel<false>, grid, kFewWarps * 32, smem, 1, A);
-    }
     const Room8 room = room_of(d, kernel, sms);
     const long long blocks = ceil_div(d.inputs, kBlock);
     QuantArgs A = {};
@@ -681,6 +657,19 @@ int forward(const axc_dense8_desc &d, const void *x, const uint8_t *kernel, cons
     A.status = status;
     int rc = quantize_rows(A, d.type, sms, q);
     if (rc) return rc;
+    if (few_rows8(d)) {
+        const Few8Args F = {int(d.rows), d.inputs, d.units, A.codes, A.scales, kernel, d.kernel_row_stride, kernel_scales, fin};
+        const unsigned smem = unsigned(few_smem(d.rows, d.inputs) + kFewSums);
+        const dim3 grid(unsigned(ceil_div(d.units, kFewUnits)));
+        if (in_place(d, kernel)) {
+            static std::atomic<unsigned long long> ready{0};
+            rc = allow_smem(few8_kernel<true>, unsigned(kFewSmem + kFewSums), ready);
+            return rc ? rc : launch(q, few8_kernel<true>, grid, kFewWarps * 32, smem, 1, F);
+        }
+        static std::atomic<unsigned long long> ready{0};
+        rc = allow_smem(few8_kernel<false>, unsigned(kFewSmem + kFewSums), ready);
+        return rc ? rc : launch(q, few8_kernel<false>, grid, kFewWarps * 32, smem, 1, F);
+    }
     const void *codes = kernel;
     long long line = d.kernel_row_stride;
     if (!in_place(d, kernel)) {
