@@ -212,6 +212,21 @@ __device__ __forceinline__ void multiply8(unsigned d, uint64_t a, uint64_t b, un
                      ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"(unsigned(add)) : "memory");
 }
 
+// As barrier_wait and barrier_arrive_cluster of axc_mma.cuh, for barriers that hand over nothing but tensor memory and what bulk copies bring, which the
+// matrix pipes' own fences order: without a scope that reaches the other CTA's generic memory.  With it each cost about a thousand clocks, once
+// for every block of inputs.
+__device__ __forceinline__ bool wait_here(unsigned bar, unsigned parity, int polls)
+{
+    for (int it = 0; it < polls; ++it) {
+        unsigned done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (__all_sync(0xffffffffu, done != 0)) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void arrive_at(unsigned bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
 // groups of 8 rows of tiles, so that the tiles in flight share lines of both operands
 __device__ __forceinline__ void place_of(const Gemm8Args &P, int tile, int &tm, int &tn)
 {
@@ -275,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
             const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
             const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
             for (int k = k0; k < k1; ++k) {
-                if (!(ok = mma::barrier_wait(empty + 8 * s, phase, polls))) break;
+                if (!(ok = wait_here(empty + 8 * s, phase, polls))) break;
                 if (leader) {
                     if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
                     const unsigned at = ring + unsigned(s) * stage_bytes;
@@ -297,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
             const int split = u % P.splits;
             const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
             for (int k = k0; k < k1; ++k) {
-                if (!(ok = mma::barrier_wait(sums_empty + 8 * buffer, sums_phase, polls))) break;
-                if (!(ok = mma::barrier_wait(full + 8 * s, phase, polls))) break;
+                if (!(ok = wait_here(sums_empty + 8 * buffer, sums_phase, polls))) break;
+                if (!(ok = wait_here(full + 8 * s, phase, polls))) break;
                 mma::fence_after();
                 const unsigned at = (ring + unsigned(s) * stage_bytes) >> 4, d = tmem + unsigned(buffer) * kColumns;
                 if (leader) {
@@ -340,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
             float a0 = a_scale(k0), b0 = __ldg(sb + k0), a1 = a_scale(min(k0 + 1, k1 - 1)), b1 = __ldg(sb + min(k0 + 1, k1 - 1));
             for (int k = k0; k < k1; ++k) {
                 const float a2 = a_scale(min(k + 2, k1 - 1)), b2 = __ldg(sb + min(k + 2, k1 - 1));
-                if (!(ok = mma::barrier_wait(sums_full + 8 * buffer, phase, polls))) break;
+                if (!(ok = wait_here(sums_full + 8 * buffer, phase, polls))) break;
                 mma::fence_after();
                 __syncwarp();
                 if (half < kHalves) {
@@ -360,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
                 }
                 mma::fence_before();
                 __syncwarp();
-                if (lane == 0) mma::barrier_arrive_cluster(mma::in_cta(sums_empty + 8 * buffer, 0));
+                if (lane == 0) arrive_at(mma::in_cta(sums_empty + 8 * buffer, 0));
                 if (++buffer == kBuffers) buffer = 0, phase ^= 1u;
                 a0 = a1, b0 = b1, a1 = a2, b1 = b2;
             }
