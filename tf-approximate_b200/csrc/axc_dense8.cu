@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
         // warps 4 to 7 take the first half of the columns, 8 to 11 the second; a half has one scale of the kernel at a time
-        constexpr int kHalves = BN >= 128 ? 2 : 1, kMine = BN / kHalves, W = kMine < 32 ? 16 : 32, kChunks = kMine / W;
+        constexpr int kHalves = BN >= 128 ? 2 : 1, kMine = BN / kHalves, F = kMine < 32 ? 16 : 32, W = kMine < 64 ? F : 64, kChunks = kMine / W;
         const int half = (warp - 4) >> 2, quarter = warp & 3;
         int buffer = 0;
         unsigned phase = 0;
@@ -358,40 +358,43 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
                 if (!(ok = wait_here(sums_full + 8 * buffer, phase, polls))) break;
                 mma::fence_after();
                 __syncwarp();
+                auto release = [&] {
+                    mma::fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(mma::in_cta(sums_empty + 8 * buffer, 0));
+                };
                 if (half < kHalves) {
                     const Two both(scales_product(a0, b0));
                     const unsigned at = mine + unsigned(buffer) * kColumns;
-                    // the next columns are on their way while these are added
-                    unsigned x[2][W];
-                    mma::load_columns(at, x[0]);
+                    unsigned x[W];
+                    mma::load_columns(at, x);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        mma::load_wait(x[c & 1]);
-                        if (c + 1 < kChunks) mma::load_columns(at + (c + 1) * W, x[(c + 1) & 1]);
+                        mma::load_wait(x);
+                        // the matrix instructions may write here again as soon as all has been read
+                        if (c + 1 == kChunks) release();
 #pragma unroll
                         for (int i = 0; i < W; i += 2)
-                            sum[(c * W + i) / 2] = fma2(Two(__uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1])), both, sum[(c * W + i) / 2]);
+                            sum[(c * W + i) / 2] = fma2(Two(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), both, sum[(c * W + i) / 2]);
+                        if (c + 1 < kChunks) mma::load_columns(at + (c + 1) * W, x);
                     }
-                }
-                mma::fence_before();
-                __syncwarp();
-                if (lane == 0) arrive_at(mma::in_cta(sums_empty + 8 * buffer, 0));
+                } else release();
                 if (++buffer == kBuffers) buffer = 0, phase ^= 1u;
                 a0 = a1, b0 = b1, a1 = a2, b1 = b2;
             }
             if (!ok) break;
             if (half < kHalves) {
 #pragma unroll
-                for (int c = 0; c < kMine; c += W) {
-                    unsigned x[W];
+                for (int c = 0; c < kMine; c += F) {
+                    unsigned x[F];
 #pragma unroll
-                    for (int i = 0; i < W; i += 2) {
+                    for (int i = 0; i < F; i += 2) {
                         const float2 f = sum[(c + i) / 2].both();
                         x[i] = __float_as_uint(f.x);
                         x[i + 1] = __float_as_uint(f.y);
                     }
-                    if constexpr (PARTIAL) store_part<W, kUnits>(P.part, P.part_line, P.part_stride, P.splits, P.n, L, x, row0, n0 + c, split);
-                    else finish_row<W, kUnits>(P.fin, P.n, L, x, row0, n0 + c, 1.0f);
+                    if constexpr (PARTIAL) store_part<F, kUnits>(P.part, P.part_line, P.part_stride, P.splits, P.n, L, x, row0, n0 + c, split);
+                    else finish_row<F, kUnits, true>(P.fin, P.n, L, x, row0, n0 + c, 1.0f);
                 }
             }
         }

@@ -7,6 +7,7 @@
 
 #include "axc_internal.h"
 #include "axc_pieces.h"
+#include "axc_two.cuh"
 
 namespace axc {
 
@@ -136,6 +137,36 @@ __device__ __forceinline__ float normal_below(float z, float &bell, bool exact)
 }
 // 1 / (1 + exp(-z))
 __device__ __forceinline__ float sigmoid(float z, bool exact) { return reciprocal(1.0f + (exact ? expf(-z) : __expf(-z))); }
+
+// The same for two values at a time, for 16-bit results.  exp(x) = 2^(x log2 e), values below the normal ones as 0.
+__device__ __forceinline__ Two power2(Two x)
+{
+    const float2 f = x.both();
+    float a, b;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(f.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(f.y));
+    return Two(a, b);
+}
+__device__ __forceinline__ Two reciprocal2(Two x)
+{
+    const float2 f = x.both();
+    return Two(reciprocal(f.x), reciprocal(f.y));
+}
+__device__ __forceinline__ Two sigmoid2(Two z) { return reciprocal2(add2(power2(mul2(z, Two(-1.44269504f))), Two(1.0f))); }
+__device__ __forceinline__ Two normal_below2(Two z, Two &bell)
+{
+    const float2 f = z.both();
+    const Two a(fabsf(f.x), fabsf(f.y)), t = reciprocal2(fma2(Two(0.30759144f), a, Two(1.0f)));
+    bell = power2(mul2(mul2(a, Two(-0.72134752f)), a));
+    Two poly = fma2(t, Two(-0.0758679435f), Two(0.191902518f));
+    poly = fma2(t, poly, Two(0.00506413169f));
+    poly = fma2(t, poly, Two(0.137423128f));
+    poly = fma2(t, poly, Two(0.118498363f));
+    poly = mul2(t, fma2(t, poly, Two(0.122977965f)));
+    const Two side = mul2(poly, bell);
+    const float2 low = side.both(), high = fma2(side, Two(-1.0f), Two(1.0f)).both();
+    return Two(f.x < 0.0f ? low.x : high.x, f.y < 0.0f ? low.y : high.y);
+}
 
 // The three bf16 terms of x and of y, x in the low half: the value rounded, the rest rounded again, and what is left then, which bf16
 // holds exactly.  A value beyond bf16's range has its largest finite term first.  An infinity is (1, 0, inf) with its sign: of the six products of terms

@@ -151,8 +151,9 @@ struct ColumnValues {
     __device__ __forceinline__ float column(int i) const { return __shfl_sync(0xffffffffu, mine[i / 32], i & 31); }
 };
 
-// One row of W sums (columns n0 ..), W a multiple of 16; all lanes of the warp, whether their row exists or not
-template <int W, int N>
+// One row of W sums (columns n0 ..), W a multiple of 16; all lanes of the warp, whether their row exists or not.  PAIRS: activations of 16-bit
+// results two at a time.
+template <int W, int N, bool PAIRS = false>
 __device__ __forceinline__ void finish_row(const Finish &f, int n, const Lines &L, unsigned (&x)[W], int row0, int n0, float alpha)
 {
     if (n0 >= n) return;
@@ -197,7 +198,16 @@ __device__ __forceinline__ void finish_row(const Finish &f, int n, const Lines &
         }
     }
     if (f.pre) store_row<W, N>(L, v, f.pre, f.out_type, f.out_line, row0, n0, n, f.out_values());
-    if (f.activation == kActRelu) {
+    if (PAIRS && !exact && f.activation >= kActGelu) {
+#pragma unroll
+        for (int i = 0; i < W; i += 2) {
+            const Two z(v[i], v[i + 1]);
+            Two bell;
+            const float2 y = mul2(z, f.activation == kActGelu ? normal_below2(z, bell) : sigmoid2(z)).both();
+            v[i] = y.x;
+            v[i + 1] = y.y;
+        }
+    } else if (f.activation == kActRelu) {
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = activate(v[i], kActRelu, exact);
     } else if (f.activation == kActGelu) {

@@ -200,16 +200,6 @@ __device__ __forceinline__ void fetch(const T *sample, const Walk<V> &w, Word *t
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// 1 / (1 + exp(-z)) for 16-bit results: 2^(-z log2 e), and both approximations good to 2^-22
-__device__ __forceinline__ Two sigmoid2(Two z)
-{
-    const float2 t = mul2(z, Two(-1.44269504f)).both();
-    float2 e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-    const float2 d = add2(Two(e.x, e.y), Two(1.0f)).both();
-    return Two(reciprocal(d.x), reciprocal(d.y));
-}
 template <int H, bool EXACT>
 __device__ __forceinline__ void activate_pairs(Two (&z)[H], int act)
 {
@@ -231,8 +221,13 @@ __device__ __forceinline__ void activate_pairs(Two (&z)[H], int act)
     } else {
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            const float2 f = z[i].both();
-            z[i] = Two(activate(f.x, kActGelu, EXACT), activate(f.y, kActGelu, EXACT));
+            if constexpr (EXACT) {
+                const float2 f = z[i].both();
+                z[i] = Two(activate(f.x, kActGelu, true), activate(f.y, kActGelu, true));
+            } else {
+                Two bell;
+                z[i] = mul2(z[i], normal_below2(z[i], bell));
+            }
         }
     }
 }
@@ -260,7 +255,14 @@ __device__ __forceinline__ void slopes(Two (&d)[H], const Two (&z)[H], int act)
         for (int i = 0; i < H; ++i) d[i] = mul2(d[i], slope2<kActRelu, EXACT>(z[i]));
     } else {
 #pragma unroll
-        for (int i = 0; i < H; ++i) d[i] = mul2(d[i], slope2<kActGelu, EXACT>(z[i]));
+        for (int i = 0; i < H; ++i) {
+            if constexpr (EXACT) d[i] = mul2(d[i], slope2<kActGelu, true>(z[i]));
+            else {
+                Two bell;
+                const Two below = normal_below2(z[i], bell);
+                d[i] = mul2(d[i], fma2(mul2(z[i], bell), Two(0.39894228f), below));
+            }
+        }
     }
 }
 
