@@ -1,5 +1,5 @@
 """CPU: the generator that the tests of dropout compare with, against the answers that its authors publish, and its two forms against each other;
-what the C entry point refuses before it touches a GPU."""
+what the C entry points of dropout, group norm and the 8-bit dense layer refuse before they touch a GPU."""
 import ctypes as C
 
 import numpy as np
@@ -64,11 +64,38 @@ def test_group_norm_descriptions(built):
     assert L.axc_group_norm_backward(C.byref(d), *[null] * 10, null, C.c_size_t(0), 0, null) == 0
 
 
+class Dense8(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "inputs", "units")] + [(n, C.c_int32) for n in ("type", "bias", "act", "reserved")] + [(n, C.c_int64) for n in ("xr", "kr", "rr")]
+
+
+def test_8bit_descriptions(built):
+    from tf_approximate_b200 import _lib
+    L, null, at = _lib.load(), C.c_void_p(), C.c_void_p
+    good = dict(rows=40, inputs=200, units=300, type=1, bias=0, act=1, reserved=0, xr=200, kr=208, rr=300)
+    for bad in (dict(rows=-1), dict(inputs=0), dict(units=-1), dict(units=1 << 40), dict(type=3), dict(bias=-1), dict(act=4), dict(xr=-1), dict(kr=-1), dict(rr=-1)):
+        d, size = Dense8(**{**good, **bad}), C.c_size_t()
+        assert L.axc_dense8_workspace_bytes(C.byref(d), null, 0, C.byref(size)) == 3, bad
+        assert L.axc_dense8_forward(C.byref(d), at(256), at(512), at(768), null, null, at(1024), at(2048), C.c_size_t(1 << 30), 0, null) == 3, bad
+    d = Dense8(**good)
+    call = lambda x=256, k=512, s=768, b=None, r=None, y=1024: L.axc_dense8_forward(  # noqa: E731
+        C.byref(d), at(x), at(k), at(s), at(b), at(r), at(y), null, C.c_size_t(0), 0, null)
+    for bad in (dict(x=None), dict(k=None), dict(s=None), dict(y=None), dict(x=257), dict(s=770), dict(b=258), dict(r=255), dict(y=1025)):
+        assert call(**bad) == 3, bad
+    d = Dense8(**{**good, "rows": 0})
+    assert call(x=None, y=None) == 0
+    quantize = lambda x=256, rows=4, inputs=200, stride=200, type=1, block=1, codes=512, scales=1024, device=0: L.axc_quantize_blocks(  # noqa: E731
+        at(x), C.c_int64(rows), C.c_int64(inputs), C.c_int64(stride), type, block, at(codes), at(scales), device, null)
+    for bad in (dict(x=None), dict(codes=None), dict(scales=None), dict(rows=-1), dict(inputs=-1), dict(stride=-1), dict(type=5), dict(block=2), dict(x=257), dict(scales=1026), dict(device=-1),
+                dict(rows=1 << 40)):
+        assert quantize(**bad) == 3, bad
+    assert quantize(rows=0, x=None) == 0
+
+
 def test_python_refusals_without_a_gpu(built):
     import torch
     import tf_approximate_b200 as ax
     x = torch.zeros(2, 8)
-    for call in (lambda: ax.dropout(x, 0.5, 1), lambda: ax.dropout(None, 0.5, 1), lambda: ax.group_norm(x, 2), lambda: ax.group_norm(None, 2), lambda: ax.GroupNorm(8, 3),
+    for call in (lambda: ax.dropout(x, 0.5, 1), lambda: ax.dropout(None, 0.5, 1), lambda: ax.group_norm(x, 2), lambda: ax.group_norm(None, 2), lambda: ax.quantize_blocks(x), lambda: ax.dense_8bit(x, x, x), lambda: ax.Dense8bit(None), lambda: ax.GroupNorm(8, 3),
                  lambda: ax.Dropout(1.5), lambda: ax.Dropout(-0.5), lambda: ax.GroupNorm(8, 0)):
         with pytest.raises(ax.InvalidArgumentError):
             call()

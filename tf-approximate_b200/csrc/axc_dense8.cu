@@ -9,8 +9,8 @@
 //   many rows     tcgen05 matrix instructions on 8-bit operands, 128 k a stage, which is a block: its sums are taken out of tensor memory, times the two
 //                 scales, and added in registers, while the next block's are made in the other half of the tensor memory.  Tiles, splits of k and the
 //                 ring of stages are those of the 16-bit products (axc_gemm.cu): a stage has as many bytes, and as many clocks.
-//   up to 8 rows  bound by reading the kernel once.  Four warps share a block's 16 units and have every fourth block of 128 inputs each; a lane reads 16
-//                 bytes of two units at a time, turns them into fp16 (exact) and multiplies by mma with the rows as its columns: on plain
+//   up to 8 rows  bound by reading the kernel once.  Four warps share 16 units and have every fourth block of 128 inputs each; a lane reads 16 bytes of two
+//                 units at a time, two blocks on their way, and multiplies them, as they are, by mma with the rows as its columns: with plain
 //                 multiply-adds 8 rows would cost eight times what one does.  The order of k within a block is the lanes' own, the same for both operands.
 // Sums within a block are the matrix pipes', over blocks fp32 with rounding; y is rounded once.
 #include <atomic>
@@ -426,51 +426,38 @@ struct Few8Args {
     Finish fin;
 };
 constexpr int kFewWarps = 4, kFewUnits = 16;
-constexpr int kFewSmem = 64 * 1024;            // codes of the rows, at most
 
-// four codes as four fp16 values
-__device__ __forceinline__ void to_halves(unsigned codes, unsigned &low, unsigned &high)
+// D += A B^T for 16 units, 8 rows and 32 inputs
+__device__ __forceinline__ void mma_16832(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
 {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes & 0xffffu), __NV_E4M3), b = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes >> 16), __NV_E4M3);
-    low = unsigned(a.x) | unsigned(a.y) << 16;
-    high = unsigned(b.x) | unsigned(b.y) << 16;
-}
-
-__device__ __forceinline__ void mma_16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A block has 16 units.  Shared memory: the rows' codes, [rows][line] with 16 bytes between the lines' banks, and their scales [blocks][rows].
+// A block has 16 units; its warps have every kFewWarps-th block of inputs each, and add up in shared memory what they have.
 template <bool VEC>
-__global__ void __launch_bounds__(kFewWarps * 32, VEC ? 8 : 4) few8_kernel(const Few8Args A)
+__global__ void __launch_bounds__(kFewWarps * 32, VEC ? 7 : 4) few8_kernel(const Few8Args A)
 {
-    extern __shared__ __align__(16) char raw[];
+    __shared__ float sums[kFewWarps][kFewUnits][kFewRows + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int blocks = int((A.inputs + kBlock - 1) / kBlock), line = blocks * kBlock + 16;
-    uint8_t *codes = reinterpret_cast<uint8_t *>(raw);
-    float *scales = reinterpret_cast<float *>(raw + A.rows * line);
-    float(*sums)[kFewUnits][kFewRows + 1] = reinterpret_cast<float(*)[kFewUnits][kFewRows + 1]>(scales + blocks * A.rows);
+    const int blocks = int((A.inputs + kBlock - 1) / kBlock);
     const long long unit0 = (long long)blockIdx.x * kFewUnits;
-    // the lane's two units, the last one again behind the last
+    // the lane's two units, the last one again behind the last; its row, the last one again (its sums are not used)
     const long long u0 = unit0 + g < A.units ? unit0 + g : A.units - 1, u1 = unit0 + g + 8 < A.units ? unit0 + g + 8 : A.units - 1;
+    const int row = min(g, A.rows - 1), column = 2 * t, row0 = min(column, A.rows - 1), row1 = min(column + 1, A.rows - 1);
     const uint8_t *w0 = A.kernel + u0 * A.kernel_stride + t * 16, *w1 = A.kernel + u1 * A.kernel_stride + t * 16;
-    [[maybe_unused]] const long long kernel_bytes = (A.units - 1) * A.kernel_stride + A.inputs;
+    const uint8_t *x = A.codes + (long long)row * blocks * kBlock + t * 16;
+    [[maybe_unused]] const long long kernel_bytes = (A.units - 1) * A.kernel_stride + A.inputs, code_bytes = (long long)A.rows * blocks * kBlock;
     auto read = [&](const uint8_t *from, long long k) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (VEC && k + 16 <= A.inputs) {
-            if (AXC_VALUES_OK(from, 16, A.kernel, kernel_bytes, 613u)) v = __ldcs(reinterpret_cast<const uint4 *>(from));
-        } else {
-            unsigned w[4] = {0u, 0u, 0u, 0u};
+        if (VEC && k + 16 <= A.inputs) return AXC_VALUES_OK(from, 16, A.kernel, kernel_bytes, 613u) ? __ldcs(reinterpret_cast<const uint4 *>(from)) : make_uint4(0u, 0u, 0u, 0u);
+        unsigned w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (k + i < A.inputs && AXC_VALUES_OK(from + i, 1, A.kernel, kernel_bytes, 614u)) w[i / 4] |= unsigned(from[i]) << (8 * (i & 3));
-            v = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        return v;
+        for (int i = 0; i < 16; ++i)
+            if (k + i < A.inputs && AXC_VALUES_OK(from + i, 1, A.kernel, kernel_bytes, 614u)) w[i / 4] |= unsigned(from[i]) << (8 * (i & 3));
+        return make_uint4(w[0], w[1], w[2], w[3]);
     };
+    // a block of 128 inputs of the lane's units, 64 at a time
     auto read_block = [&](int b, uint4 (&a)[2][2]) {
         if (b >= blocks) return;
 #pragma unroll
@@ -485,34 +472,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, VEC ? 8 : 4) few8_kernel(const
     uint4 a[2][2][2];
     read_block(warp, a[0]);
     read_block(warp + kFewWarps, a[1]);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = threadIdx.x; i < A.rows * blocks * (kBlock / 16); i += kFewWarps * 32) {
-        const int row = i / (blocks * (kBlock / 16)), at = i - row * (blocks * (kBlock / 16));
-        if (AXC_GLOBAL_OK((long long)i * 16 + 15, (long long)A.rows * blocks * kBlock, 615u))
-            *reinterpret_cast<uint4 *>(codes + row * line + at * 16) = reinterpret_cast<const uint4 *>(A.codes)[i];
-    }
-    for (int i = threadIdx.x; i < A.rows * blocks; i += kFewWarps * 32) scales[i] = A.a_scales[i];
-    __syncthreads();
-    const int mine = min(g, A.rows - 1), column = 2 * t;      // rows that are not there: the last one again, not used
     const float *b_scales = A.b_scales + unit0 / kBlock * blocks;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     auto add_block = [&](int b, uint4 (&a)[2][2]) {
+        const float sb = __ldg(b_scales + b);
+        const bool there = AXC_GLOBAL_OK((long long)b * A.rows + row1, (long long)blocks * A.rows, 616u);
+        const float s0 = there ? A.a_scales[b * A.rows + row0] : 0.0f, s1 = there ? A.a_scales[b * A.rows + row1] : 0.0f;
         float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(codes + mine * line + b * kBlock + c * 64 + t * 16);
-            const unsigned p[4] = {a[c][0].x, a[c][0].y, a[c][0].z, a[c][0].w}, q[4] = {a[c][1].x, a[c][1].y, a[c][1].z, a[c][1].w}, r[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                unsigned p0, p1, q0, q1, r0, r1;
-                to_halves(p[i], p0, p1);
-                to_halves(q[i], q0, q1);
-                to_halves(r[i], r0, r1);
-                mma_16816(d, p0, q0, p1, q1, r0, r1);
-            }
+            const uint8_t *from = x + b * kBlock + c * 64;
+            const uint4 r = AXC_VALUES_OK(from, 16, A.codes, code_bytes, 615u) ? *reinterpret_cast<const uint4 *>(from) : make_uint4(0u, 0u, 0u, 0u);
+            mma_16832(d, a[c][0].x, a[c][1].x, a[c][0].y, a[c][1].y, r.x, r.y);
+            mma_16832(d, a[c][0].z, a[c][1].z, a[c][0].w, a[c][1].w, r.z, r.w);
         }
-        const float sb = b_scales[b], t0 = scales_product(scales[b * A.rows + min(column, A.rows - 1)], sb),
-                    t1 = scales_product(scales[b * A.rows + min(column + 1, A.rows - 1)], sb);
+        const float t0 = scales_product(s0, sb), t1 = scales_product(s1, sb);
         sum[0] = fmaf(d[0], t0, sum[0]);
         sum[1] = fmaf(d[1], t1, sum[1]);
         sum[2] = fmaf(d[2], t0, sum[2]);
@@ -532,12 +507,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, VEC ? 8 : 4) few8_kernel(const
     sums[warp][g + 8][column + 1] = sum[3];
     __syncthreads();
     if (threadIdx.x < kFewUnits * kFewRows) {
-        const int unit = threadIdx.x & (kFewUnits - 1), row = threadIdx.x / kFewUnits;
-        if (row < A.rows && unit0 + unit < A.units) {
-            float z = sums[0][unit][row];
+        const int unit = threadIdx.x & (kFewUnits - 1), line = threadIdx.x / kFewUnits;
+        if (line < A.rows && unit0 + unit < A.units) {
+            float z = sums[0][unit][line];
 #pragma unroll
-            for (int i = 1; i < kFewWarps; ++i) z += sums[i][unit][row];
-            finish_value(A.fin, z, row, unit0 + unit);
+            for (int i = 1; i < kFewWarps; ++i) z += sums[i][unit][line];
+            finish_value(A.fin, z, line, unit0 + unit);
         }
     }
 }
@@ -546,15 +521,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, VEC ? 8 : 4) few8_kernel(const
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-size_t few_smem(long long rows, long long inputs)
-{
-    const long long blocks = ceil_div(inputs, kBlock);
-    return size_t(rows * (blocks * kBlock + 16) + blocks * rows * 4);
-}
-constexpr size_t kFewSums = sizeof(float) * kFewWarps * kFewUnits * (kFewRows + 1);
-
 // The calls that take the kernel for few rows
-bool few_rows8(const axc_dense8_desc &d) { return d.rows <= kFewRows && few_smem(d.rows, d.inputs) <= kFewSmem; }
+bool few_rows8(const axc_dense8_desc &d) { return d.rows <= kFewRows; }
 // Codes that TMA reads where they are
 bool in_place(const axc_dense8_desc &d, const void *kernel) { return (reinterpret_cast<uintptr_t>(kernel) & 15u) == 0 && d.kernel_row_stride % 16 == 0 && d.kernel_row_stride >= d.inputs; }
 
@@ -677,16 +645,8 @@ int forward(const axc_dense8_desc &d, const void *x, const uint8_t *kernel, cons
     if (rc) return rc;
     if (few_rows8(d)) {
         const Few8Args F = {int(d.rows), d.inputs, d.units, A.codes, A.scales, kernel, d.kernel_row_stride, kernel_scales, fin};
-        const unsigned smem = unsigned(few_smem(d.rows, d.inputs) + kFewSums);
         const dim3 grid(unsigned(ceil_div(d.units, kFewUnits)));
-        if (in_place(d, kernel)) {
-            static std::atomic<unsigned long long> ready{0};
-            rc = allow_smem(few8_kernel<true>, unsigned(kFewSmem + kFewSums), ready);
-            return rc ? rc : launch(q, few8_kernel<true>, grid, kFewWarps * 32, smem, 1, F);
-        }
-        static std::atomic<unsigned long long> ready{0};
-        rc = allow_smem(few8_kernel<false>, unsigned(kFewSmem + kFewSums), ready);
-        return rc ? rc : launch(q, few8_kernel<false>, grid, kFewWarps * 32, smem, 1, F);
+        return launch(q, in_place(d, kernel) ? few8_kernel<true> : few8_kernel<false>, grid, kFewWarps * 32, 0, 1, F);
     }
     const void *codes = kernel;
     long long line = d.kernel_row_stride;

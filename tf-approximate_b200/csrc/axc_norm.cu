@@ -616,6 +616,16 @@ template <int V>
 struct Sums {
     static constexpr int H = kPairs<V>;
     Two dz[H], off[H];
+    // of more than a run of values, which are added up by themselves first, so that no chain of additions is longer than one
+    __device__ __forceinline__ void take(Sums &run)
+    {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            dz[i] = add2(dz[i], run.dz[i]);
+            off[i] = add2(off[i], run.off[i]);
+            run.dz[i] = run.off[i] = Two(0.0f);
+        }
+    }
     __device__ __forceinline__ Sums()
     {
 #pragma unroll
@@ -917,7 +927,7 @@ struct Share {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_moments_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 4) norm_moments_kernel(const NormArgs P)
 {
     after_previous();
     __shared__ float2 entries[2 * kNormThreads * V];
@@ -928,7 +938,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_moments_kernel(const NormAr
     const T *x = static_cast<const T *>(P.x);
     Moments<V> mo;
     const T *sample = x + at.sample * P.places * P.channels;
-    take_moments<V == 1 ? 8 : 4, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto whole) { load<decltype(whole)::value>(sample + w.at + j * w.step, w, j, v, x, P.values()); });
+    take_moments<V == 1 ? 8 : 2, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto whole) { load<decltype(whole)::value>(sample + w.at + j * w.step, w, j, v, x, P.values()); });
     if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return mo.of(i); });
     __syncthreads();
     const Entries E(span, shift, w.total);
@@ -1031,7 +1041,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormAr
     const Span &span = at.span(P);
     const int shift = shift_of<T, V>(P, at.sample, at.place0);
     const Walk<V> w(threadIdx.x, span, shift, at.places, P.channels, at.place0, at.channel0);
-    Sums<V> sums;
+    Sums<V> sums, run;
     if (w.count > 0) {
         Channels<V> ch;
         int group[V];
@@ -1054,10 +1064,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormAr
             for (int k = 0; k < N; ++k) {
                 Two dz[kPairs<V>], off[kPairs<V>];
                 slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-                sums.template add<decltype(whole)::value>(w, j + k, dz, off);
+                run.template add<decltype(whole)::value>(w, j + k, dz, off);
                 if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
             }
+            if (((j - w.first) & (kRun - 1)) == 0) sums.take(run);
         });
+        sums.take(run);
     }
     if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return sums.of(i); });
     __syncthreads();
