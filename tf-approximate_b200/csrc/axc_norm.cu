@@ -927,7 +927,7 @@ struct Share {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_moments_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_moments_kernel(const NormArgs P)
 {
     after_previous();
     __shared__ float2 entries[2 * kNormThreads * V];
@@ -938,7 +938,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_moments_kernel(const Nor
     const T *x = static_cast<const T *>(P.x);
     Moments<V> mo;
     const T *sample = x + at.sample * P.places * P.channels;
-    take_moments<V == 1 ? 8 : 2, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto whole) { load<decltype(whole)::value>(sample + w.at + j * w.step, w, j, v, x, P.values()); });
+    take_moments<V == 1 ? 8 : 4, T, V>(w, mo, [&](int j, Pack<T, V> &v, auto whole) { load<decltype(whole)::value>(sample + w.at + j * w.step, w, j, v, x, P.values()); });
     if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return mo.of(i); });
     __syncthreads();
     const Entries E(span, shift, w.total);
@@ -988,6 +988,65 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
     if (threadIdx.x == 0) P.statistics[blockIdx.x] = make_float2(mean, __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(square, all) + P.epsilon)));
 }
 
+// body(whole, one, j, vectors of the tensors) for all vectors of a thread, from tensors at p[0] .. p[n - 1] (from the sample's start).  Where there
+// is an asynchronous copy of that size, the next D - 1 of them are on their way: a thread has D places in `ring` for each tensor, which it alone uses.
+// Else one after the other, N at a time.
+constexpr int ring_bytes(int depth, int tensors) { return depth * tensors * kNormThreads * 16; }
+template <int D, int NT, typename T, int V, typename Body>
+__device__ __forceinline__ void stream(const Walk<V> &w, const T *const (&p)[NT], int n, char *ring, [[maybe_unused]] const T *const (&base)[NT], [[maybe_unused]] long long count,
+                                       Body body)
+{
+    if constexpr (V * sizeof(T) == 16) {
+        const unsigned place = mma::smem_address(ring) + threadIdx.x * 16u;
+        auto at = [&](int slot, int t) { return unsigned((slot * NT + t) * kNormThreads * 16); };
+        long long ahead = w.at + w.first * w.step;
+        int slot_in = 0, slot = 0;
+        auto issue = [&](int j) {
+            if (j < w.end) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (t < n && AXC_VALUES_OK(p[t] + ahead, V, base[t], count, 520u))
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place + at(slot_in, t)), "l"(p[t] + ahead) : "memory");
+                ahead += w.step;
+                if (++slot_in == D) slot_in = 0;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int d = 0; d < D - 1; ++d) issue(w.first + d);
+        for (int j = w.first; j < w.end; ++j) {
+            issue(j + D - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+            Pack<T, V> v[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < n) v[t].w = *reinterpret_cast<const uint4 *>(ring + threadIdx.x * 16u + at(slot, t));
+            if (++slot == D) slot = 0;
+            body(std::true_type(), j, v);
+        }
+        wait_copies();
+    } else {
+        for (int j = w.first; j < w.end; ++j) {
+            Pack<T, V> v[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < n) load<true>(p[t] + w.at + j * w.step, w, j, v[t], base[t], count);
+            body(std::true_type(), j, v);
+        }
+    }
+    if constexpr (V > 1) {
+        for (int side = 0; side < 2; ++side) {
+            if (side == 0 ? w.first == 0 : w.end == w.count) continue;
+            const int j = side == 0 ? 0 : w.end;
+            Pack<T, V> v[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < n) load<false>(p[t] + w.at + j * w.step, w, j, v[t], base[t], count);
+            body(std::false_type(), j, v);
+        }
+    }
+}
+
 template <int V>
 __device__ __forceinline__ void fill_channels(const NormArgs &P, const Share &at, const Walk<V> &w, Channels<V> &ch, int (&group)[V])
 {
@@ -1001,9 +1060,10 @@ __device__ __forceinline__ void fill_channels(const NormArgs &P, const Share &at
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_apply_kernel(const NormArgs P)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(const NormArgs P)
 {
     after_previous();
+    extern __shared__ __align__(16) char ring[];
     const Share at(P, gridDim.x - 1 - blockIdx.x);
     const Span &span = at.span(P);
     const Walk<V> w(threadIdx.x, span, shift_of<T, V>(P, at.sample, at.place0), at.places, P.channels, at.place0, at.channel0);
@@ -1014,21 +1074,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_apply_kernel(const NormA
     const long long sample0 = at.sample * P.places * P.channels;
     const T *x = static_cast<const T *>(P.x), *residual = static_cast<const T *>(P.residual);
     T *y = static_cast<T *>(P.y);
-    batches<V>(w, std::integral_constant<int, 4>(), [&](auto whole, auto n, int j) {
-        constexpr int N = decltype(n)::value;
-        const long long from = sample0 + w.at + j * w.step;
-        Pack<T, V> v[N], r[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            load<decltype(whole)::value>(x + from + k * w.step, w, j + k, v[k], x, P.values());
-            if (P.residual) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, r[k], residual, P.values());
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            Two z[kPairs<V>];
-            output_of<T, V>(P, ch, v[k], r[k], z);
-            store<decltype(whole)::value>(y + from + k * w.step, w, j + k, z, y, P.values());
-        }
+    const T *const base[2] = {x, residual}, *const p[2] = {x + sample0, P.residual ? residual + sample0 : nullptr};
+    stream<6>(w, p, P.residual ? 2 : 1, ring, base, P.values(), [&](auto whole, int j, const Pack<T, V> (&v)[2]) {
+        Two z[kPairs<V>];
+        output_of<T, V>(P, ch, v[0], v[1], z);
+        store<decltype(whole)::value>(y + sample0 + w.at + j * w.step, w, j, z, y, P.values());
     });
 }
 
@@ -1036,7 +1086,8 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormArgs P)
 {
     after_previous();
-    __shared__ float2 entries[2 * kNormThreads * V];
+    extern __shared__ __align__(16) char ring[];
+    float2 *entries = reinterpret_cast<float2 *>(ring);        // once all has come through
     const Share at(P, blockIdx.x);
     const Span &span = at.span(P);
     const int shift = shift_of<T, V>(P, at.sample, at.place0);
@@ -1050,27 +1101,17 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormAr
         const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
         T *dresidual = static_cast<T *>(P.dresidual);
         const bool with = P.residual && P.activation != kActNone;
-        batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
-            constexpr int N = decltype(n)::value;
-            const long long from = sample0 + w.at + j * w.step;
-            Pack<T, V> vx[N], vd[N], vr[N];
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                load<decltype(whole)::value>(x + from + k * w.step, w, j + k, vx[k], x, values);
-                load<decltype(whole)::value>(dy + from + k * w.step, w, j + k, vd[k], dy, values);
-                if (with) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
-            }
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                Two dz[kPairs<V>], off[kPairs<V>];
-                slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-                run.template add<decltype(whole)::value>(w, j + k, dz, off);
-                if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
-            }
-            if (((j - w.first) & (kRun - 1)) == 0) sums.take(run);
+        const T *const base[3] = {x, dy, residual}, *const p[3] = {x + sample0, dy + sample0, with ? residual + sample0 : nullptr};
+        stream<4>(w, p, with ? 3 : 2, ring, base, values, [&](auto whole, int j, const Pack<T, V> (&v)[3]) {
+            Two dz[kPairs<V>], off[kPairs<V>];
+            slope_at<T, V>(P, ch, v[0], v[1], v[2], dz, off);
+            run.template add<decltype(whole)::value>(w, j, dz, off);
+            if (dresidual) store<decltype(whole)::value>(dresidual + sample0 + w.at + j * w.step, w, j, dz, dresidual, values);
+            if (((j - w.first) & (kRun - 1)) == kRun - 1) sums.take(run);
         });
         sums.take(run);
     }
+    __syncthreads();
     if (int(threadIdx.x) < span.active) give_entries<V>(entries, span, [&](int i) { return sums.of(i); });
     __syncthreads();
     const Entries E(span, shift, w.total);
@@ -1117,6 +1158,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_gradient_kernel(const NormArgs P)
 {
     after_previous();
+    extern __shared__ __align__(16) char ring[];
     const Share at(P, gridDim.x - 1 - blockIdx.x);
     const Span &span = at.span(P);
     const Walk<V> w(threadIdx.x, span, shift_of<T, V>(P, at.sample, at.place0), at.places, P.channels, at.place0, at.channel0);
@@ -1130,23 +1172,12 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_gradient_kernel(const No
     const T *x = static_cast<const T *>(P.x), *dy = static_cast<const T *>(P.dy), *residual = static_cast<const T *>(P.residual);
     T *dx = static_cast<T *>(P.dx);
     const bool with = P.residual && P.activation != kActNone;
-    batches<V>(w, std::integral_constant<int, 2>(), [&](auto whole, auto n, int j) {
-        constexpr int N = decltype(n)::value;
-        const long long from = sample0 + w.at + j * w.step;
-        Pack<T, V> vx[N], vd[N], vr[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            load<decltype(whole)::value>(x + from + k * w.step, w, j + k, vx[k], x, values);
-            load<decltype(whole)::value>(dy + from + k * w.step, w, j + k, vd[k], dy, values);
-            if (with) load<decltype(whole)::value>(residual + from + k * w.step, w, j + k, vr[k], residual, values);
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            Two dz[kPairs<V>], off[kPairs<V>];
-            slope_at<T, V>(P, ch, vx[k], vd[k], vr[k], dz, off);
-            gradient.of(ch, off, dz);
-            store<decltype(whole)::value>(dx + from + k * w.step, w, j + k, dz, dx, values);
-        }
+    const T *const base[3] = {x, dy, residual}, *const p[3] = {x + sample0, dy + sample0, with ? residual + sample0 : nullptr};
+    stream<4>(w, p, with ? 3 : 2, ring, base, values, [&](auto whole, int j, const Pack<T, V> (&v)[3]) {
+        Two dz[kPairs<V>], off[kPairs<V>];
+        slope_at<T, V>(P, ch, v[0], v[1], v[2], dz, off);
+        gradient.of(ch, off, dz);
+        store<decltype(whole)::value>(dx + sample0 + w.at + j * w.step, w, j, dz, dx, values);
     });
 }
 
@@ -1202,7 +1233,7 @@ int forward(NormArgs P, const NormPlan &plan, Queue &q)
     const dim3 grid(unsigned(P.samples * P.shares * P.spans));
     int rc = launch(q, norm_moments_kernel<T, V>, grid, kNormThreads, 0, 1, P);
     if (!rc) rc = launch(q, norm_join_kernel, dim3(unsigned(P.samples * P.groups)), kNormThreads, 0, 1, P);
-    if (!rc) rc = launch(q, norm_apply_kernel<T, V>, grid, kNormThreads, 0, 1, P);
+    if (!rc) rc = launch(q, norm_apply_kernel<T, V>, grid, kNormThreads, ring_bytes(6, 2), 1, P);
     return rc;
 }
 
@@ -1216,9 +1247,10 @@ int backward(NormArgs P, const NormPlan &plan, Queue &q)
         if (!rc) rc = launch(q, norm_backward_kernel<T, V>, dim3(unsigned(P.samples * P.spans * P.blocks)), unsigned(plan.threads), plan.smem, unsigned(plan.blocks), P);
     } else {
         const dim3 grid(unsigned(P.samples * P.shares * P.spans));
-        rc = launch(q, norm_sums_kernel<T, V>, grid, kNormThreads, 0, 1, P);
+        static_assert(ring_bytes(4, 3) >= int(sizeof(float2)) * 2 * kNormThreads * V, "the entries fit where the tensors came through");
+        rc = launch(q, norm_sums_kernel<T, V>, grid, kNormThreads, ring_bytes(4, 3), 1, P);
         if (!rc) rc = launch(q, norm_join_sums_kernel, dim3(unsigned(P.samples * P.groups)), kNormThreads, 0, 1, P);
-        if (!rc && P.dx) rc = launch(q, norm_gradient_kernel<T, V>, grid, kNormThreads, 0, 1, P);
+        if (!rc && P.dx) rc = launch(q, norm_gradient_kernel<T, V>, grid, kNormThreads, ring_bytes(4, 3), 1, P);
     }
     return rc;
 }
