@@ -526,6 +526,35 @@ bool few_rows8(const axc_dense8_desc &d) { return d.rows <= kFewRows; }
 // Codes that TMA reads where they are
 bool in_place(const axc_dense8_desc &d, const void *kernel) { return (reinterpret_cast<uintptr_t>(kernel) & 15u) == 0 && d.kernel_row_stride % 16 == 0 && d.kernel_row_stride >= d.inputs; }
 
+// The cheapest tiles and splits by an estimate in clocks, as choose_plan's, with what was measured here: taking a block's sums out bounds a stage, 1480
+// clocks for 256 columns, 930 for 128 (the matrix instructions alone 512 and 390), and what follows the sums is not hidden by the next tile's.
+Plan choose_plan8(long long m, long long n, long long blocks, int sms)
+{
+    Plan best = {1, 128, 1};
+    double least = 1e300;
+    const double memory = (double(m) + double(n)) * double(blocks) * kBlock / 3400;
+    for (int c = 0; c < 6; ++c) {
+        static const int kCg[6] = {2, 1, 1, 1, 1, 1}, kBn[6] = {256, 256, 128, 64, 32, 16};
+        const int cg = kCg[c], bn = kBn[c];
+        const double bytes = (double(m < 128 ? m : 128) + bn / cg) * kBlock;
+        const long long tiles = ceil_div(m, 128 * cg) * ceil_div(n, bn), workers = sms / cg;
+        for (int splits = 1; splits <= 16; splits *= 2) {
+            if (splits > 1 && blocks / splits < 2) break;
+            const long long units = tiles * splits;
+            const double copies = bytes / 114 * double(units < workers ? units : workers) / double(workers), taking = 400 + 4.2 * bn, stage = taking > copies ? taking : copies;
+            double clocks = double(ceil_div(units, workers)) * (double(ceil_div(blocks, splits)) * stage + 2500 + 12 * bn);
+            if (clocks < memory) clocks = memory;
+            clocks += 4500;
+            if (splits > 1) clocks += 7600 + double(m) * double(n) * splits * 8 / 7400;
+            if (clocks < least) {
+                least = clocks;
+                best = {cg, bn, splits};
+            }
+        }
+    }
+    return best;
+}
+
 struct Room8 {
     size_t codes, scales, kernel, part, total;
 };
@@ -537,7 +566,7 @@ Room8 room_of(const axc_dense8_desc &d, const void *kernel, int sms)
     r.total = r.part = r.kernel = r.scales + up(size_t(d.rows) * size_t(blocks) * 4);
     if (few_rows8(d)) return r;
     r.part = r.kernel + (in_place(d, kernel) ? 0 : up(size_t(d.units) * size_t(ceil_div(d.inputs, 16)) * 16));
-    const Plan plan = choose_plan(d.rows, d.units, ceil_div(d.inputs, 2), 1, true, sms);
+    const Plan plan = choose_plan8(d.rows, d.units, blocks, sms);
     r.total = r.part + (plan.splits > 1 ? up(size_t(plan.splits) * size_t(d.rows) * size_t(ceil_div(d.units, 4)) * 16) : 0);
     return r;
 }
@@ -658,7 +687,7 @@ int forward(const axc_dense8_desc &d, const void *x, const uint8_t *kernel, cons
                     reinterpret_cast<uint8_t *>(ws + room.kernel), line);
         if (rc) return rc;
     }
-    const Plan plan = choose_plan(d.rows, d.units, ceil_div(d.inputs, 2), 1, true, sms);
+    const Plan plan = choose_plan8(d.rows, d.units, blocks, sms);
     Gemm8Args P = {};
     P.m = int(d.rows);
     P.n = int(d.units);

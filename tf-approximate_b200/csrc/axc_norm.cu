@@ -23,7 +23,6 @@
 // see below).  It makes dx off by 0.0024 in all where its own rounding alone makes 0.0017 (bf16).
 #include <atomic>
 #include <type_traits>
-#include <vector>
 
 #include "axc_gemm.h"
 #include "axc_mma.cuh"
@@ -1287,11 +1286,12 @@ NormPlan plan_of(const NormShape &s, bool backward, bool residual, int sms)
         int key;
         NormPlan plan;
     };
-    thread_local std::vector<Known> known(512);
+    constexpr unsigned kKnown = 256;
+    thread_local Known known[kKnown];          // zeros at first: no call has the key 0
     const int key = 1 + (backward ? 1 : 0) + (residual ? 2 : 0) + (s.aligned ? 4 : 0) + 8 * sms;
     unsigned long long hash = (unsigned long long)s.samples;
     for (const long long v : {s.places, s.channels, s.groups, (long long)(key * 8 + s.size)}) hash = (hash ^ (unsigned long long)v) * 0x9E3779B97F4A7C15ull, hash ^= hash >> 29;
-    Known &k = known[hash % known.size()];
+    Known &k = known[hash % kKnown];
     if (k.key != key || k.shape.samples != s.samples || k.shape.places != s.places || k.shape.channels != s.channels || k.shape.groups != s.groups || k.shape.size != s.size)
         k = {s, key, backward ? norm_plan(s, (residual ? 3 : 2) * s.size, s.size * (residual ? 5 : 3), true, sms)
                               : norm_plan(s, s.size, s.size * (residual ? 3 : 2), false, sms)};
