@@ -169,11 +169,11 @@ __global__ void __launch_bounds__(256) lay_out_codes_kernel(const uint8_t *src, 
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------
-// Warps: 0 loads and holds the tensor memory, 1 multiplies, 4 to 11 take the sums out.  Those hold 128 sums a thread beside what is on its way, so
-// the first warpgroup leaves them its registers: 384 threads are launched with 168 each, 128 * 40 + 256 * 232 is as many.
-constexpr int kThreads = 384, kFewRegisters = 40, kManyRegisters = 232;
+// Warps: 0 loads and holds the tensor memory, 1 multiplies, 4 to 19 take the sums out.  Those hold 64 sums a thread beside what is on its way, so the
+// first warpgroup leaves them its registers: 640 threads are launched with 96 each, 128 * 32 + 512 * 112 is as many.
+constexpr int kThreads = 640, kFewRegisters = 32, kManyRegisters = 112, kTakers = 16;
 constexpr unsigned kHeader = 1024, kSmem = 227 * 1024;
-constexpr int kMaxStages = 12, kUnits = 8;     // 16-byte units of a row that a warp turns over at a time
+constexpr int kMaxStages = 12, kUnits = 4;     // 16-byte units of a row that a warp turns over at a time
 
 #ifdef AXC_BOUNDS_CHECK
 __device__ int g_wait_polls = mma::kWaitPolls;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
     extern __shared__ char raw[];
     const unsigned base = (mma::smem_address(raw) + 1023u) & ~1023u;
     Header8 *head = reinterpret_cast<Header8 *>(raw + (base - mma::smem_address(raw)));
-    const unsigned lines = base + kHeader, ring = lines + 8u * kUnits * 512u, stage_bytes = kABytes + P.b_bytes;
+    const unsigned lines = base + kHeader, ring = lines + unsigned(kTakers * kUnits) * 512u, stage_bytes = kABytes + P.b_bytes;
     const unsigned full = mma::smem_address(head->full), empty = mma::smem_address(head->empty);
     const unsigned sums_full = mma::smem_address(head->sums_full), sums_empty = mma::smem_address(head->sums_empty);
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
         }
         for (int i = 0; i < kBuffers; ++i) {
             mma::barrier_init(sums_full + 8 * i, 1);
-            mma::barrier_init(sums_empty + 8 * i, 8 * CG);
+            mma::barrier_init(sums_empty + 8 * i, kTakers * CG);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         mma::prefetch_map(&P.map_a);
@@ -332,21 +332,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
-        // warps 4 to 7 take the first half of the columns, 8 to 11 the second; a half has one scale of the kernel at a time
-        constexpr int kHalves = BN >= 128 ? 2 : 1, kMine = BN / kHalves, F = kMine < 32 ? 16 : 32, W = kMine < 64 ? F : 64, kChunks = kMine / W;
-        const int half = (warp - 4) >> 2, quarter = warp & 3;
+        // four warps take a part of the columns, which has one scale of the kernel at a time
+        constexpr int kParts = BN >= 128 ? 4 : BN >= 64 ? 2 : 1, kMine = BN / kParts, W = kMine < 32 ? 16 : 32, kChunks = kMine / W;
+        const int part = (warp - 4) >> 2, quarter = warp & 3;
         int buffer = 0;
         unsigned phase = 0;
         for (int u = worker; u < units && ok; u += workers) {
             int tm, tn;
             place_of(P, u / P.splits, tm, tn);
             const int split = u % P.splits;
-            const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + half * kMine;
+            const int row0 = tm * TM + int(rank) * 128 + quarter * 32, n0 = tn * BN + part * kMine;
             const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
             const Lines L = {lines + unsigned(warp - 4) * kUnits * 512u, lane, min(32, P.m - row0)};
             const int row = min(row0 + lane, P.m - 1), square = min(n0, P.n - 1) / kBlock;
             const float *sa = P.a_scales + row, *sb = P.b_scales + (long long)square * P.blocks;
-            const unsigned mine = tmem + unsigned(half * kMine) + (unsigned(quarter * 32) << 16);
+            const unsigned mine = tmem + unsigned(part * kMine) + (unsigned(quarter * 32) << 16);
             Two sum[kMine / 2];
 #pragma unroll
             for (int i = 0; i < kMine / 2; ++i) sum[i] = Two(0.0f);
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
                     __syncwarp();
                     if (lane == 0) arrive_at(mma::in_cta(sums_empty + 8 * buffer, 0));
                 };
-                if (half < kHalves) {
+                if (part < kParts) {
                     const Two both(scales_product(a0, b0));
                     const unsigned at = mine + unsigned(buffer) * kColumns;
                     unsigned x[W];
@@ -383,18 +383,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
                 a0 = a1, b0 = b1, a1 = a2, b1 = b2;
             }
             if (!ok) break;
-            if (half < kHalves) {
+            if (part < kParts) {
 #pragma unroll
-                for (int c = 0; c < kMine; c += F) {
-                    unsigned x[F];
+                for (int c = 0; c < kMine; c += W) {
+                    unsigned x[W];
 #pragma unroll
-                    for (int i = 0; i < F; i += 2) {
+                    for (int i = 0; i < W; i += 2) {
                         const float2 f = sum[(c + i) / 2].both();
                         x[i] = __float_as_uint(f.x);
                         x[i + 1] = __float_as_uint(f.y);
                     }
-                    if constexpr (PARTIAL) store_part<F, kUnits>(P.part, P.part_line, P.part_stride, P.splits, P.n, L, x, row0, n0 + c, split);
-                    else finish_row<F, kUnits, true>(P.fin, P.n, L, x, row0, n0 + c, 1.0f);
+                    if constexpr (PARTIAL) store_part<W, kUnits>(P.part, P.part_line, P.part_stride, P.splits, P.n, L, x, row0, n0 + c, split);
+                    else finish_row<W, kUnits, true>(P.fin, P.n, L, x, row0, n0 + c, 1.0f);
                 }
             }
         }
@@ -597,7 +597,7 @@ int allow_smem(Kernel kernel, unsigned bytes, std::atomic<unsigned long long> &r
 template <int CG, int BN, bool PARTIAL>
 int launch_gemm8(Gemm8Args &P, int sms, Queue &q)
 {
-    const unsigned stage = kABytes + P.b_bytes, lines = 8 * kUnits * 512;
+    const unsigned stage = kABytes + P.b_bytes, lines = kTakers * kUnits * 512;
     P.stages = int((kSmem - kHeader - 1024 - lines) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     static std::atomic<unsigned long long> ready{0};
