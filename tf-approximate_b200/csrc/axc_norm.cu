@@ -19,8 +19,12 @@
 // Sums are fp32.  Those of the variance are never of squares that nearly cancel: a thread adds the squares of up to 32 values less the first of them,
 // and means and squared distances are joined by their means (Chan, Golub and LeVeque).  Every sum has a fixed order.
 // Roundings to 16 bits: the outputs, and dz of resident spans, which dx is made of (the sums take it before), as the dense layer's dz is: fp32
-// would take half as much shared memory again, which is what bounds how many loads are on their way (256 x 56 x 56 x 256 with a shortcut:
-// see below).  It makes dx off by 0.0024 in all where its own rounding alone makes 0.0017 (bf16).
+// would take half as much shared memory again, which is what bounds how many loads are on their way.  It makes dx off by 0.0024 in all where its own
+// rounding alone makes 0.0017 (bf16).
+//
+// Measured (256 x 56 x 56 x 256 bf16, groups of 8, shortcut, silu; us, bytes at memory's rate in brackets): forward 274 to 283 (188), backward 556 to 562
+// (314), the latter bound by instructions and by the time between a block's phases: 39 a value, of which 10 are the block's own costs.  The same with the tensors read
+// twice: 307 to 382 and 638.  2 x 512 x 512 x 128 bf16, which no cluster holds: 90 (41) and 134 (61).
 #include <atomic>
 #include <type_traits>
 
