@@ -52,6 +52,7 @@ struct NormArgs {
     Span vectors;                              // then: the span's vectors in place of its channels
     Divider by_group;                          // channels of a group
     int entries, lanes;                        // norm_entries, norm_lanes
+    bool single;                               // resident, one sample: no launch for the parameters' gradients
     long long shares;
     float2 *part;                              // [samples][shares][channels] sums of a share of the places
     float2 *sums;                              // [samples][channels] {sum of dz, sum of dz xhat}; may be NULL
@@ -418,41 +419,26 @@ __device__ __forceinline__ void give_entries(float2 *entries, const Span &s, Get
 // {mean, squared distances} of `items` neighbouring sets of `each` channels, from the threads' entries, `of_entry` values each for every one that the
 // entry counts: give(item, mean, square) in one thread
 template <typename Give>
-__device__ __forceinline__ void join_moments(const float2 *entries, const Entries &E, int items, int each, float values, float of_entry, Give give)
+__device__ __forceinline__ void join_moments(const float2 *entries, const Entries &E, const Divider &by_copies, int items, int each, float values, float of_entry, Give give)
 {
-    const int log2 = lanes_for(items), q = 1 << log2, lane = threadIdx.x & (q - 1), step = int(blockDim.x) >> log2;
+    const int log2 = lanes_for(items), q = 1 << log2, lane = threadIdx.x & (q - 1), step = int(blockDim.x) >> log2, all = each * E.copies;
     const float share = __fdividef(1.0f, values);
     for (int first = 0; first < items; first += step) {
-        const int item = first + (int(threadIdx.x) >> log2);
-        const bool mine = item < items;
-        float sum = 0.0f;
-        if (mine) {
-            for (int d = 0; d < each; ++d) {
-                const int e0 = E.first_entry(item * each + d);
-                for (int k = lane; k < E.copies; k += q) {
-                    const int e = e0 + k * E.span;
-                    const float n = of_entry * E.values(e);
-                    if (n > 0.0f) sum = fmaf(n, entries[E.place(e, k)].x, sum);
-                }
+        const int item = first + (int(threadIdx.x) >> log2), end = item < items ? all : 0;
+        // f(values of it, the entry)
+        auto each_entry = [&](auto f) {
+            for (int i = lane; i < end; i += q) {
+                const int d = int(by_copies.of(unsigned(i))), k = i - d * E.copies, e = E.first_entry(item * each + d) + k * E.span;
+                const float n = of_entry * E.values(e);
+                if (n > 0.0f) f(n, entries[E.place(e, k)]);
             }
-        }
+        };
+        float sum = 0.0f, square = 0.0f;
+        each_entry([&](float n, float2 f) { sum = fmaf(n, f.x, sum); });
         const float mean = over_lanes(sum, log2) * share;
-        float square = 0.0f;
-        if (mine) {
-            for (int d = 0; d < each; ++d) {
-                const int e0 = E.first_entry(item * each + d);
-                for (int k = lane; k < E.copies; k += q) {
-                    const int e = e0 + k * E.span;
-                    const float n = of_entry * E.values(e);
-                    if (n > 0.0f) {
-                        const float2 f = entries[E.place(e, k)];
-                        square += fmaf(n * (f.x - mean), f.x - mean, f.y);
-                    }
-                }
-            }
-        }
+        each_entry([&](float n, float2 f) { square += fmaf(n * (f.x - mean), f.x - mean, f.y); });
         square = over_lanes(square, log2);
-        if (mine && lane == 0) give(item, mean, square);
+        if (item < items && lane == 0) give(item, mean, square);
     }
 }
 
@@ -725,12 +711,12 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_forward_kernel(const Nor
         }
         __syncthreads();
         const Entries E(P.vectors, 0, at.places * P.vectors.channels);
-        join_moments(entries, E, groups, P.each / V, part, float(V), [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
+        join_moments(entries, E, P.vectors.by_copies, groups, P.each / V, part, float(V), [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
     } else {
         if (thread < P.span.active) give_entries<V>(entries, P.span, [&](int i) { return mo.of(i); });
         __syncthreads();
         const Entries E(P.span, shift, w.total);
-        join_moments(entries, E, groups, P.each, part, 1.0f, [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
+        join_moments(entries, E, P.span.by_copies, groups, P.each, part, 1.0f, [&](int g, float mean, float square) { mine[g] = make_float2(mean, square); });
     }
     __syncwarp();
     if (P.blocks > 1) mma::cluster_sync();
@@ -872,12 +858,18 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const No
         // the sums are of dz and of dz (x - mean): r makes xhat of that
         result[g] = make_float2(f.x * share * r, f.y * share * r * r * r);
     }
-    // the sums of single channels, shared out among the cluster's blocks
-    if (P.sums) {
+    // the sums of single channels, shared out among the cluster's blocks; those of a single sample are the parameters' gradients
+    if (P.sums || P.single) {
         for (int l = at.rank + thread * P.blocks; l < P.span.channels; l += int(blockDim.x) * P.blocks) {
             const float2 f = P.blocks > 1 ? sum_of_all(channels + l, P.blocks) : channels[l];
             const long long to = at.sample * P.channels + at.channel0 + l;
-            if (AXC_GLOBAL_OK(to, P.samples * P.channels, 510u)) P.sums[to] = make_float2(f.x, f.y * stats(int(P.by_group.of(unsigned(l)))).y);
+            if (!AXC_GLOBAL_OK(to, P.samples * P.channels, 510u)) continue;
+            const float by_scale = f.y * stats(int(P.by_group.of(unsigned(l)))).y;
+            if (P.sums) P.sums[to] = make_float2(f.x, by_scale);
+            else {
+                if (P.doffset) store_from_float(P.doffset, to, P.offset_type, f.x);
+                if (P.dscale) store_from_float(P.dscale, to, P.scale_type, by_scale);
+            }
         }
     }
     __syncthreads();
@@ -946,7 +938,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_moments_kernel(const Nor
     __syncthreads();
     const Entries E(span, shift, w.total);
     const long long to = (at.sample * P.shares + at.share) * P.channels + at.channel0;
-    join_moments(entries, E, span.channels, 1, float(at.places), 1.0f, [&](int l, float mean, float square) {
+    join_moments(entries, E, span.by_copies, span.channels, 1, float(at.places), 1.0f, [&](int l, float mean, float square) {
         if (AXC_GLOBAL_OK(to + l, P.samples * P.shares * P.channels, 511u)) P.part[to + l] = make_float2(mean, square);
     });
 }
@@ -962,31 +954,39 @@ __device__ __forceinline__ float over_block(float x, float *room)
     return sum;
 }
 
+// f(channel of the group, share) for all that are a thread's: neighbouring lanes have neighbouring channels, as many as a warp holds, the other lanes and the
+// warps other shares
+template <typename Each>
+__device__ __forceinline__ void over_shares(const NormArgs &P, Each f)
+{
+    const int log2 = P.each >= 32 ? 5 : 32 - __clz(max(P.each, 2) - 1), width = 1 << log2, lane = threadIdx.x & 31;
+    const long long first = (long long)(threadIdx.x >> 5) * (32 >> log2) + (lane >> log2), step = (kNormThreads / 32) * (32 >> log2);
+    for (int d = lane & (width - 1); d < P.each; d += width)
+#pragma unroll 8
+        for (long long s = first; s < P.shares; s += step) f(d, s);
+}
+
 // A block joins the shares of one sample's group
 __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs P)
 {
     after_previous();
     __shared__ float room[kNormThreads / 32];
-    const long long sample = blockIdx.x / P.groups;
-    const int group = int(blockIdx.x - sample * P.groups);
-    const float2 *part = P.part + sample * P.shares * P.channels + group * P.each;
-    const long long entries = P.shares * P.each;
+    const unsigned sample = blockIdx.x / unsigned(P.groups);
+    const int group = int(blockIdx.x - sample * unsigned(P.groups));
+    const float2 *part = P.part + sample * P.shares * P.channels + (long long)group * P.each;
     const float all = float(P.places) * float(P.each);
     const float of_share = float(P.per), of_last = float(P.places - P.per * (P.shares - 1));
-    auto values = [&](long long s) { return s + 1 < P.shares ? of_share : of_last; };
-    [[maybe_unused]] const long long room_for = P.shares * P.channels - group * P.each;
+    [[maybe_unused]] const long long room_for = P.shares * P.channels - (long long)group * P.each;
     float sum = 0.0f, square = 0.0f;
-    for (long long e = threadIdx.x; e < entries; e += kNormThreads) {
-        const long long s = e / P.each, from = s * P.channels + (e - s * P.each);
-        if (AXC_GLOBAL_OK(from, room_for, 512u)) sum = fmaf(values(s), part[from].x, sum);
-    }
+    over_shares(P, [&](int d, long long s) {
+        if (AXC_GLOBAL_OK(s * P.channels + d, room_for, 512u)) sum = fmaf(s + 1 < P.shares ? of_share : of_last, part[s * P.channels + d].x, sum);
+    });
     const float mean = __fdiv_rn(over_block(sum, room), all);
-    for (long long e = threadIdx.x; e < entries; e += kNormThreads) {
-        const long long s = e / P.each, from = s * P.channels + (e - s * P.each);
-        if (!AXC_GLOBAL_OK(from, room_for, 513u)) continue;
-        const float2 f = part[from];
-        square += fmaf(values(s) * (f.x - mean), f.x - mean, f.y);
-    }
+    over_shares(P, [&](int d, long long s) {
+        if (!AXC_GLOBAL_OK(s * P.channels + d, room_for, 513u)) return;
+        const float2 f = part[s * P.channels + d];
+        square += fmaf((s + 1 < P.shares ? of_share : of_last) * (f.x - mean), f.x - mean, f.y);
+    });
     square = over_block(square, room);
     if (threadIdx.x == 0) P.statistics[blockIdx.x] = make_float2(mean, __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(square, all) + P.epsilon)));
 }
@@ -1124,36 +1124,54 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_sums_kernel(const NormAr
     });
 }
 
-// A block joins the shares of one sample's group: a warp has a channel, its lanes have shares
+// A block joins the shares of one sample's group, for up to 32 channels at a time
 __global__ void __launch_bounds__(kNormThreads) norm_join_sums_kernel(const NormArgs P)
 {
     after_previous();
-    __shared__ float room[kNormThreads / 32];
-    const long long sample = blockIdx.x / P.groups;
-    const int group = int(blockIdx.x - sample * P.groups), lane = threadIdx.x & 31;
+    __shared__ float2 room[kNormThreads / 32][32];
+    __shared__ float sums[kNormThreads / 32];
+    const unsigned sample = blockIdx.x / unsigned(P.groups);
+    const int group = int(blockIdx.x - sample * unsigned(P.groups)), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float r = P.statistics[blockIdx.x].y;
+    const int log2 = P.each >= 32 ? 5 : 32 - __clz(max(P.each, 2) - 1), width = 1 << log2;
     float first = 0.0f, second = 0.0f;
-    for (int d = threadIdx.x >> 5; d < P.each; d += kNormThreads / 32) {
-        const int c = group * P.each + d;
-        float a = 0.0f, b = 0.0f;
-        for (long long s = lane; s < P.shares; s += 32) {
-            const long long from = (sample * P.shares + s) * P.channels + c;
-            if (!AXC_GLOBAL_OK(from, P.samples * P.shares * P.channels, 516u)) continue;
-            a += P.part[from].x;
-            b += P.part[from].y;
+    for (int d0 = 0; d0 < P.each; d0 += width) {
+        const int d = d0 + (lane & (width - 1));
+        const long long c = (long long)group * P.each + d;
+        float2 f = make_float2(0.0f, 0.0f);
+        if (d < P.each) {
+            const long long step = (kNormThreads / 32) * (32 >> log2);
+#pragma unroll 8
+            for (long long s = (long long)warp * (32 >> log2) + (lane >> log2); s < P.shares; s += step) {
+                const long long from = (sample * P.shares + s) * P.channels + c;
+                if (!AXC_GLOBAL_OK(from, P.samples * P.shares * P.channels, 516u)) continue;
+                const float2 more = P.part[from];
+                f.x += more.x;
+                f.y += more.y;
+            }
         }
-        a = over_lanes(a, 5);
-        b = over_lanes(b, 5) * r;
-        if (lane == 0) {
-            if (P.sums) P.sums[sample * P.channels + c] = make_float2(a, b);
+        for (int o = 16; o >= width; o >>= 1) {
+            f.x += __shfl_xor_sync(0xffffffffu, f.x, o);
+            f.y += __shfl_xor_sync(0xffffffffu, f.y, o);
+        }
+        __syncthreads();
+        room[warp][lane] = f;
+        __syncthreads();
+        if (warp == 0 && lane < width && d < P.each) {
+            for (int i = 1; i < kNormThreads / 32; ++i) {
+                f.x += room[i][lane].x;
+                f.y += room[i][lane].y;
+            }
+            f.y *= r;
+            if (P.sums) P.sums[sample * P.channels + c] = f;
             const float scale = P.scale ? load_as_float(P.scale, c, P.scale_type) : 1.0f;
-            first = fmaf(scale, a, first);
-            second = fmaf(scale, b, second);
+            first = fmaf(scale, f.x, first);
+            second = fmaf(scale, f.y, second);
         }
     }
     const float all = float(P.places) * float(P.each);
-    first = over_block(first, room);
-    second = over_block(second, room);
+    first = over_block(first, sums);
+    second = over_block(second, sums);
     if (threadIdx.x == 0) P.group_sums[blockIdx.x] = make_float2(__fdiv_rn(first, all) * r, __fdiv_rn(second, all) * r * r);
 }
 
@@ -1454,7 +1472,8 @@ extern "C" int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy
     P.dresidual = dresidual;
     char *ws = static_cast<char *>(workspace);
     P.part = reinterpret_cast<float2 *>(ws);
-    P.sums = dscale || doffset ? reinterpret_cast<float2 *>(ws + norm_part_bytes(s, plan)) : nullptr;
+    P.single = plan.resident && d.samples == 1 && (dscale || doffset);
+    P.sums = (dscale || doffset) && !P.single ? reinterpret_cast<float2 *>(ws + norm_part_bytes(s, plan)) : nullptr;
     P.group_sums = reinterpret_cast<float2 *>(ws + norm_part_bytes(s, plan) + norm_sums_bytes(s));
     if (!some) P.samples = 0;
     Queue q = {cudaStream_t(stream)};
@@ -1465,7 +1484,7 @@ extern "C" int axc_group_norm_backward(const axc_norm_desc *desc, const void *dy
             else if (d.type == kBfloat16) rc = plan.vec > 1 ? backward<__nv_bfloat16, 8>(P, plan, q) : backward<__nv_bfloat16, 1>(P, plan, q);
             else rc = plan.vec > 1 ? backward<__half, 8>(P, plan, q) : backward<__half, 1>(P, plan, q);
         }
-        if (!rc && (dscale || doffset)) rc = launch(q, norm_parameters_kernel, dim3(unsigned((P.channels + 31) / 32)), 1024, 0, 1, P);
+        if (!rc && (dscale || doffset) && !(some && P.single)) rc = launch(q, norm_parameters_kernel, dim3(unsigned((P.channels + 31) / 32)), 1024, 0, 1, P);
         return rc;
     });
 }

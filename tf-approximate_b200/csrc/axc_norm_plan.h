@@ -142,12 +142,16 @@ inline NormPlan norm_plan(const NormShape &s, int kept, int moved, bool backward
             }
         }
     }
-    if (best.resident) return best;
+    // Read twice: all bytes and those that are read again at 70 % of memory's rate (single values at a fourth of that), and three launches.
     int vec = 1;
     const int span = norm_columns(s, &vec);
+    const int again = backward ? (moved / s.size == 5 ? 3 : 2) : 1;
+    const double twice = 14.0 + double(s.values()) * (moved + again * s.size) / (4.6e6 * (vec > 1 ? 1.0 : 0.25));
+    if (best.resident && least <= twice) return best;
+    best = {};
+    best.span = span;
     best.vec = vec;
     best.threads = kNormThreads;
-    best.span = span;
     // six blocks for every SM, of 32 KiB at least and a million values at most
     const long long across = s.samples * ((s.channels + span - 1) / span), most = s.places * span * s.size / (32 * 1024) + 1;
     long long shares = ((long long)sms * 6 + across - 1) / (across ? across : 1);
@@ -188,12 +192,12 @@ inline Divider divider(unsigned by) { return {by, by > 1 ? unsigned(((1ull << 32
 // entries (see Entries)
 struct Span {
     int channels, active, each, lines, copies;
-    Divider by_channels, by_each;
+    Divider by_channels, by_each, by_copies;
 };
 inline Span span_of(int channels, int active, int vec)
 {
     const int each = active * vec;
-    return {channels, active, each, each / channels, each / channels, divider(unsigned(channels)), divider(unsigned(each))};
+    return {channels, active, each, each / channels, each / channels, divider(unsigned(channels)), divider(unsigned(each)), divider(unsigned(each / channels))};
 }
 
 // ---- in the kernels ------------------------------------------------------------------------------------------------------------
