@@ -237,6 +237,38 @@ def test_captured_with_another_call_beside_it(built):
         assert torch.equal(out[0], first) and torch.equal(out[1], few)
 
 
+def test_a_kernel_of_more_bytes_than_31_bits_count(built):
+    """70016 units of 32768 inputs: the last units' answers, for few rows and for many."""
+    import torch
+    import tf_approximate_b200 as ax
+    g = torch.Generator(device="cuda").manual_seed(2)
+    units, inputs = 70016, 32768
+    codes = torch.randint(0, 0x7f, (units, inputs), dtype=torch.uint8, device="cuda", generator=g).view(torch.float8_e4m3fn)      # any code but NaN
+    scales = torch.full((units // 128, inputs // 128), 2.0 ** -12, device="cuda")
+    for r in (2, 40):
+        x = torch.randn(r, inputs, device="cuda", generator=g)
+        y = ax.dense_8bit(x, codes, scales, check=True)
+        a, w = spread(*exact_quantized(x, 1), 1), codes[-200:].double() * 2.0 ** -12
+        # as above: 9 2^-23 for the blocks' own sums, 2^-24 for each of 256 additions
+        assert bool(((y[:, -200:].double() - a @ w.t()).abs() <= (a.abs() @ w.abs().t()) * (9 * 2.0 ** -23 + 256 * 2.0 ** -24)).all())
+
+
+def test_two_streams_at_once(built):
+    import torch
+    import tf_approximate_b200 as ax
+    cases = [make(r, k, u, "bfloat16")[:3] for r, k, u in ((3, 4096, 3000), (200, 1030, 777), (1500, 512, 2000))]
+    operands = [(x, *ax.quantize_blocks(w, 128), b) for x, w, b in cases]
+    want = [ax.dense_8bit(*o) for o in operands]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in operands], []
+    for _ in range(5):
+        for i, (o, s) in enumerate(zip(operands, streams)):
+            with torch.cuda.stream(s):
+                got.append((i, ax.dense_8bit(*o)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+
+
 def test_refusals(built):
     import torch
     import tf_approximate_b200 as ax

@@ -242,6 +242,52 @@ def test_the_same_every_time_and_in_a_graph(built):
                 assert torch.equal(a, b) and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("shape,groups", [((2, 1100000, 1024), 2), ((70001, 8, 8, 512), 16)])
+def test_more_values_than_31_bits_count(built, shape, groups):
+    """Both forms beyond 2^31 values: the last sample against 64 bits (its last places, where it has many), and the statistics of all."""
+    import torch
+    import tf_approximate_b200 as ax
+    c = shape[-1]
+    x = torch.empty(shape, dtype=torch.float16, device="cuda").normal_()
+    scale, offset = torch.rand(c, device="cuda") + 0.5, torch.randn(c, device="cuda")
+    y, statistics = ax.group_norm_forward(x, groups, scale, offset, None, "relu")
+    last = x[-1].view(-1, groups, c // groups)
+    mean = torch.stack([part.double().sum((0, 2)) for part in last.split(1 << 18)]).sum(0) / (last.shape[0] * last.shape[2])
+    var = torch.stack([(part.double() - mean[:, None]).square().sum((0, 2)) for part in last.split(1 << 18)]).sum(0) / (last.shape[0] * last.shape[2])
+    r = 1 / torch.sqrt(var + 1e-3)
+    # means of normal values: K D times the largest, below 6, as for the other sizes
+    assert float((statistics[-1, :, 0].double() - mean).abs().max()) < 1024 * D * 6 and float((statistics[-1, :, 1].double() / r - 1).abs().max()) < 1024 * D
+    tail = last[-2000:].double()
+    want = torch.relu(((tail - mean[:, None]) * r[:, None]).reshape(-1, c) * scale.double() + offset.double())
+    got = y[-1].reshape(-1, c)[-2000:].double()
+    assert bool(((got - want).abs() <= 1024 * D * 8 + UNIT["float16"] * want.abs() + TINY["float16"]).all())
+    dx = ax.group_norm_backward(x, x, statistics, groups, scale, offset, None, "relu")[0]
+    # the group's gradient has no part along its mean: S1 takes it out
+    sums = torch.stack([part.double().sum((0, 2)) for part in dx[-1].view(-1, groups, c // groups).split(1 << 18)]).sum(0)
+    assert float(sums.abs().max()) / (last.shape[0] * last.shape[2]) < 4 * UNIT["float16"]
+
+
+def test_two_streams_at_once(built):
+    import torch
+    import tf_approximate_b200 as ax
+    cases = [make(s, "bfloat16", "float32") + (g,) for s, g in (((64, 28, 28, 64), 16), ((2, 160, 160, 128), 32), ((31, 27, 45, 120), 24))]
+    def run(x, scale, offset, residual, grad, groups):
+        y, st = ax.group_norm_forward(x, groups, scale, offset, residual, "silu")
+        return (y, *ax.group_norm_backward(grad, x, st, groups, scale, offset, residual, "silu"))
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for _ in range(4):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(run(*c))
+    torch.cuda.synchronize()
+    for w, all_ in zip(want, got):
+        for g in all_:
+            assert all(torch.equal(a, b) for a, b in zip(w, g))
+
+
 def test_refusals(built):
     import torch
     import tf_approximate_b200 as ax

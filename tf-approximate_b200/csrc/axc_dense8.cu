@@ -282,59 +282,59 @@ __global__ void __launch_bounds__(kThreads, 1) gemm8_kernel(const __grid_constan
     bool ok = true;
     const int polls = AXC_DENSE8_POLLS;
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
-    if (warp == 0) {
-        const bool leader = mma::elect();
-        const unsigned signal = CG == 2 ? mma::in_cta(full, 0) : full;
-        int s = 0;
-        unsigned phase = 1;
-        for (int u = worker; u < units && ok; u += workers) {
-            int tm, tn;
-            place_of(P, u / P.splits, tm, tn);
-            const int split = u % P.splits;
-            const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
-            const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
-            for (int k = k0; k < k1; ++k) {
-                if (!(ok = wait_here(empty + 8 * s, phase, polls))) break;
-                if (leader) {
-                    if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
-                    const unsigned at = ring + unsigned(s) * stage_bytes;
-                    // (a stage that is not loaded runs the waits out)
-                    if (AXC_SHARED_OK(at, 1024u, ring, ring + unsigned(P.stages) * stage_bytes, 611u)) {
-                        mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kBlock, row_a, 0);
-                        mma::load_box<CG>(at + kABytes, &P.map_b, signal + 8 * s, k * kBlock, row_b, 0);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+        if (warp == 0) {
+            const bool leader = mma::elect();
+            const unsigned signal = CG == 2 ? mma::in_cta(full, 0) : full;
+            int s = 0;
+            unsigned phase = 1;
+            for (int u = worker; u < units && ok; u += workers) {
+                int tm, tn;
+                place_of(P, u / P.splits, tm, tn);
+                const int split = u % P.splits;
+                const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
+                const int row_a = tm * TM + int(rank) * 128, row_b = tn * BN + int(rank) * (BN / CG);
+                for (int k = k0; k < k1; ++k) {
+                    if (!(ok = wait_here(empty + 8 * s, phase, polls))) break;
+                    if (leader) {
+                        if (CG == 1 || rank == 0) mma::barrier_expect(full + 8 * s, stage_bytes * CG);
+                        const unsigned at = ring + unsigned(s) * stage_bytes;
+                        // (a stage that is not loaded runs the waits out)
+                        if (AXC_SHARED_OK(at, 1024u, ring, ring + unsigned(P.stages) * stage_bytes, 611u)) {
+                            mma::load_box<CG>(at, &P.map_a, signal + 8 * s, k * kBlock, row_a, 0);
+                            mma::load_box<CG>(at + kABytes, &P.map_b, signal + 8 * s, k * kBlock, row_b, 0);
+                        }
                     }
+                    __syncwarp();
+                    if (++s == P.stages) s = 0, phase ^= 1u;
                 }
-                __syncwarp();
-                if (++s == P.stages) s = 0, phase ^= 1u;
+            }
+        } else if (warp == 1 && rank == 0) {
+            const bool leader = mma::elect();
+            int s = 0, buffer = 0;
+            unsigned phase = 0, sums_phase = 1;
+            for (int u = worker; u < units && ok; u += workers) {
+                const int split = u % P.splits;
+                const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
+                for (int k = k0; k < k1; ++k) {
+                    if (!(ok = wait_here(sums_empty + 8 * buffer, sums_phase, polls))) break;
+                    if (!(ok = wait_here(full + 8 * s, phase, polls))) break;
+                    mma::fence_after();
+                    const unsigned at = (ring + unsigned(s) * stage_bytes) >> 4, d = tmem + unsigned(buffer) * kColumns;
+                    if (leader) {
+                        // 32 inputs an instruction: 32 bytes of each line
+    #pragma unroll
+                        for (int j = 0; j < kBlock / 32; ++j)
+                            multiply8<CG>(d, mma::operand(at + 2 * j, 0), mma::operand(at + (kABytes >> 4) + 2 * j, 0), P.shape, j > 0);
+                        mma::commit<CG>(empty + 8 * s);
+                        mma::commit<CG>(sums_full + 8 * buffer);
+                    }
+                    __syncwarp();
+                    if (++s == P.stages) s = 0, phase ^= 1u;
+                    if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
+                }
             }
         }
-    } else if (warp == 1 && rank == 0) {
-        const bool leader = mma::elect();
-        int s = 0, buffer = 0;
-        unsigned phase = 0, sums_phase = 1;
-        for (int u = worker; u < units && ok; u += workers) {
-            const int split = u % P.splits;
-            const int k0 = int((long long)P.blocks * split / P.splits), k1 = int((long long)P.blocks * (split + 1) / P.splits);
-            for (int k = k0; k < k1; ++k) {
-                if (!(ok = wait_here(sums_empty + 8 * buffer, sums_phase, polls))) break;
-                if (!(ok = wait_here(full + 8 * s, phase, polls))) break;
-                mma::fence_after();
-                const unsigned at = (ring + unsigned(s) * stage_bytes) >> 4, d = tmem + unsigned(buffer) * kColumns;
-                if (leader) {
-                    // 32 inputs an instruction: 32 bytes of each line
-#pragma unroll
-                    for (int j = 0; j < kBlock / 32; ++j)
-                        multiply8<CG>(d, mma::operand(at + 2 * j, 0), mma::operand(at + (kABytes >> 4) + 2 * j, 0), P.shape, j > 0);
-                    mma::commit<CG>(empty + 8 * s);
-                    mma::commit<CG>(sums_full + 8 * buffer);
-                }
-                __syncwarp();
-                if (++s == P.stages) s = 0, phase ^= 1u;
-                if (++buffer == kBuffers) buffer = 0, sums_phase ^= 1u;
-            }
-        }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
         // four warps take a part of the columns, which has one scale of the kernel at a time

@@ -23,8 +23,8 @@
 // rounding alone makes 0.0017 (bf16).
 //
 // Measured (256 x 56 x 56 x 256 bf16, groups of 8, shortcut, silu; us, bytes at memory's rate in brackets): forward 274 to 283 (188), backward 556 to 562
-// (314), the latter bound by instructions and by the time between a block's phases: 39 a value, of which 10 are the block's own costs.  The same with the tensors read
-// twice: 307 to 382 and 638.  2 x 512 x 512 x 128 bf16, which no cluster holds: 90 (41) and 134 (61).
+// (314), the latter bound by instructions and by the time between a block's phases.  The same with the tensors read twice: 307 and 638.
+// 2 x 512 x 512 x 128 bf16, which no cluster holds: 88 (41) and 134 (61).
 #include <atomic>
 #include <type_traits>
 
@@ -993,7 +993,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const NormArgs 
 
 // body(whole, one, j, vectors of the tensors) for all vectors of a thread, from tensors at p[0] .. p[n - 1] (from the sample's start).  Where there
 // is an asynchronous copy of that size, the next D - 1 of them are on their way: a thread has D places in `ring` for each tensor, which it alone uses.
-// Else one after the other, N at a time.
+// Else one after the other.
 constexpr int ring_bytes(int depth, int tensors) { return depth * tensors * kNormThreads * 16; }
 template <int D, int NT, typename T, int V, typename Body>
 __device__ __forceinline__ void stream(const Walk<V> &w, const T *const (&p)[NT], int n, char *ring, [[maybe_unused]] const T *const (&base)[NT], [[maybe_unused]] long long count,
