@@ -18,12 +18,14 @@
 //
 // Sums are fp32.  Those of the variance are never of squares that nearly cancel: a thread adds the squares of up to 32 values less the first of them,
 // and means and squared distances are joined by their means (Chan, Golub and LeVeque).  Every sum has a fixed order.
-// Roundings to 16 bits: the outputs, and dz of resident spans, which dx is made of (the sums take it before), as the dense layer's dz is: fp32
-// would take half as much shared memory again, which is what bounds how many loads are on their way.  It makes dx off by 0.0024 in all where its own
-// rounding alone makes 0.0017 (bf16).
+// Roundings to 16 bits: the outputs alone.  dx is a difference: where dz is nearly the same all over a group, as behind a mean over the places, next to
+// nothing of it is left, and a dz rounded to bf16 on the way makes dx off by 43 % (dy = 1, silu, an offset of 6).  So a resident block holds dz in fp32, in
+// the places of dy and of the residual together, and without a residual keeps dy and computes the slope again: fp32 places of its own would take half
+// as much shared memory again, which is what bounds how many loads are on their way (256 x 56 x 56 x 256 bf16, silu: 499 us, the slope again 428, a rounded dz 376).
 //
-// Measured (256 x 56 x 56 x 256 bf16, groups of 8, shortcut, silu; us, bytes at memory's rate in brackets): forward 274 to 283 (188), backward 556 to 562
-// (314), the latter bound by instructions and by the time between a block's phases.  The same with the tensors read twice: 307 and 638.
+// Measured (256 x 56 x 56 x 256 bf16, groups of 8, shortcut, silu; us, bytes at memory's rate in brackets): forward 274 to 286 (188), backward 565 to 571
+// (314), the latter bound by instructions and by the time between a block's phases; without the shortcut 203 (126) and 428 (188).  The first two with the tensors
+// read twice: 307 and 638.
 // 2 x 512 x 512 x 128 bf16, which no cluster holds: 88 (41) and 134 (61).
 #include <atomic>
 #include <type_traits>
@@ -653,6 +655,32 @@ struct Sums {
         return i & 1 ? make_float2(a.y, b.y) : make_float2(a.x, b.x);
     }
 };
+// fp32 values of one vector in the places of two 16-bit ones
+template <int V, typename Word>
+__device__ __forceinline__ void split_pairs(const Two (&x)[kPairs<V>], Word &a, Word &b)
+{
+    if constexpr (V == 1) {
+        const unsigned w = __float_as_uint(x[0].both().x);
+        a = Word(w & 0xffffu);
+        b = Word(w >> 16);
+    } else {
+        static_assert(V == 8, "16 bytes are four of them");
+        const float2 f[4] = {x[0].both(), x[1].both(), x[2].both(), x[3].both()};
+        a = make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+        b = make_uint4(__float_as_uint(f[2].x), __float_as_uint(f[2].y), __float_as_uint(f[3].x), __float_as_uint(f[3].y));
+    }
+}
+template <int V, typename Word>
+__device__ __forceinline__ void join_pairs(const Word &a, const Word &b, Two (&x)[kPairs<V>])
+{
+    if constexpr (V == 1) x[0] = Two(__uint_as_float(unsigned(a) | unsigned(b) << 16), 0.0f);
+    else {
+        x[0] = Two(__uint_as_float(a.x), __uint_as_float(a.y));
+        x[1] = Two(__uint_as_float(a.z), __uint_as_float(a.w));
+        x[2] = Two(__uint_as_float(b.x), __uint_as_float(b.y));
+        x[3] = Two(__uint_as_float(b.z), __uint_as_float(b.w));
+    }
+}
 // dx = dz factor - first - (x - mean) second
 template <int V>
 struct Gradient {
@@ -770,7 +798,8 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_forward_kernel(const Nor
     if (P.blocks > 1) cluster_wait();          // what others read of this block's shared memory
 }
 
-template <typename T, int V>
+// AGAIN: the slope is computed a second time for dx (an activation, 16-bit types, no residual)
+template <typename T, int V, bool AGAIN>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const NormArgs P)
 {
     after_previous();
@@ -779,7 +808,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const No
     const int shift = shift_of<T, V>(P, at.sample, at.place0), thread = threadIdx.x, groups = P.span_groups, stride = P.span.active;
     const Walk<V> w(thread, P.span, shift, at.places, P.channels, at.place0, at.channel0);
     typedef typename Bits<V * sizeof(T)>::type Word;
-    const bool with = P.residual && P.activation != kActNone;
+    const bool with = !AGAIN && P.residual && P.activation != kActNone;
     const size_t room = norm_up16(size_t(P.steps) * P.span.active * V * sizeof(T));
     Word *kept = reinterpret_cast<Word *>(raw) + thread, *kept_dz = reinterpret_cast<Word *>(raw + room) + thread;      // dy's, first
     Word *kept_residual = reinterpret_cast<Word *>(raw + 2 * room) + thread;
@@ -812,7 +841,9 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const No
             Two dz[kPairs<V>], off[kPairs<V>];
             slope_at<T, V>(P, ch, vx, vd, vr, dz, off);
             sums.template add<decltype(whole)::value>(w, j + k, dz, off);
-            if (P.activation != kActNone) kept_dz[(j + k) * stride] = narrow_pairs<T, V>(dz).w;
+            if constexpr (sizeof(T) == 4) {
+                if (P.activation != kActNone) kept_dz[(j + k) * stride] = narrow_pairs<T, V>(dz).w;
+            } else if (with) split_pairs<V>(dz, kept_dz[(j + k) * stride], kept_residual[(j + k) * stride]);
             if (dresidual) store<decltype(whole)::value>(dresidual + from + k * w.step, w, j + k, dz, dresidual, values);
         }
     });
@@ -887,10 +918,15 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_backward_kernel(const No
                 v.w = kept[(j + k) * stride];
                 vd.w = kept_dz[(j + k) * stride];
                 Two d[kPairs<V>], off[kPairs<V>];
-                widen_pairs<T, V>(vd, d);
-                widen_pairs<T, V>(v, off);
+                if constexpr (AGAIN) slope_at<T, V>(P, ch, v, vd, vd, d, off);
+                else {
+                    if constexpr (sizeof(T) == 4) widen_pairs<T, V>(vd, d);
+                    else if (with) join_pairs<V>(vd.w, kept_residual[(j + k) * stride], d);
+                    else widen_pairs<T, V>(vd, d);
+                    widen_pairs<T, V>(v, off);
 #pragma unroll
-                for (int i = 0; i < kPairs<V>; ++i) off[i] = add2(off[i], ch.less[i]);
+                    for (int i = 0; i < kPairs<V>; ++i) off[i] = add2(off[i], ch.less[i]);
+                }
                 gradient.of(ch, off, d);
                 store<decltype(whole)::value>(dx + from + k * w.step, w, j + k, d, dx, values);
             }
@@ -1263,9 +1299,13 @@ int backward(NormArgs P, const NormPlan &plan, Queue &q)
 {
     int rc;
     if (plan.resident) {
-        static std::atomic<unsigned long long> ready{0};
-        rc = allow_smem(norm_backward_kernel<T, V>, ready);
-        if (!rc) rc = launch(q, norm_backward_kernel<T, V>, dim3(unsigned(P.samples * P.spans * P.blocks)), unsigned(plan.threads), plan.smem, unsigned(plan.blocks), P);
+        auto run = [&](auto kernel, std::atomic<unsigned long long> &ready) {
+            const int rc = allow_smem(kernel, ready);
+            return rc ? rc : launch(q, kernel, dim3(unsigned(P.samples * P.spans * P.blocks)), unsigned(plan.threads), plan.smem, unsigned(plan.blocks), P);
+        };
+        static std::atomic<unsigned long long> ready[2];
+        if (sizeof(T) == 2 && P.activation != kActNone && !P.residual) rc = run(norm_backward_kernel<T, V, sizeof(T) == 2>, ready[1]);
+        else rc = run(norm_backward_kernel<T, V, false>, ready[0]);
     } else {
         const dim3 grid(unsigned(P.samples * P.shares * P.spans));
         static_assert(ring_bytes(4, 3) >= int(sizeof(float2)) * 2 * kNormThreads * V, "the entries fit where the tensors came through");
