@@ -278,7 +278,13 @@ class GroupNorm(torch.nn.Module):
 class Dropout(torch.nn.Module):
     """Dropout without a stored mask, in the manner of the Keras layer; in evaluation the inputs pass.  `calls`, which picks the mask and counts up with
     every call in training, is an int, or with `capturable` one int64 on the inputs' device that the call itself counts up, so that a captured step
-    has another mask at every replay.  seed: None for one of torch's."""
+    has another mask at every replay.  seed: None for one of torch's.
+
+    A call that a backward pass makes is one made again (torch.utils.checkpoint) and has the mask of the first time, which it is known by: every call in
+    training draws a number from torch's generator of the CPU, whose state such a recomputation sets back.  Where it does not (preserve_rng_state=False),
+    or the last `REMEMBERED` calls of the layer do not have it, the call is refused."""
+
+    REMEMBERED = 4096
 
     def __init__(self, rate, seed=None, capturable=False):
         super().__init__()
@@ -287,18 +293,37 @@ class Dropout(torch.nn.Module):
         self.rate = float(rate)
         self.seed = int(torch.randint(1 << 62, ()).item()) if seed is None else seed
         self.capturable = capturable
+        self._recent = {}                                       # number drawn from torch's generator -> offset of that call
         if capturable:
             self.register_buffer("calls", torch.zeros((), dtype=torch.int64))
         else:
             self.calls = 0
 
-    def forward(self, inputs, residual=None):
-        if not self.training:
-            return inputs if residual is None else inputs + residual
+    def __getstate__(self):
+        return dict(super().__getstate__(), _recent={})
+
+    def __setstate__(self, state):
+        super().__setstate__(dict(state, _recent={}))
+
+    def _offset(self):
+        drawn = torch.randint(1 << 62, (), device="cpu").item()
+        if torch._C._current_graph_task_id() != -1:             # inside a backward pass
+            if drawn not in self._recent:
+                raise ops.InvalidArgumentError("dropout is run again in a backward pass that has not set torch's random state back to that of the first time")
+            return self._recent[drawn]
         if self.capturable:
             offset = self.calls.clone()                         # the backward pass reads this call's own
             self.calls.add_(1)
         else:
             offset = self.calls
             self.calls += 1
-        return norm_ops.dropout(inputs, self.rate, self.seed, offset, residual)
+        self._recent.pop(drawn, None)
+        self._recent[drawn] = offset
+        if len(self._recent) > self.REMEMBERED:
+            del self._recent[next(iter(self._recent))]
+        return offset
+
+    def forward(self, inputs, residual=None):
+        if not self.training:
+            return inputs if residual is None else inputs + residual
+        return norm_ops.dropout(inputs, self.rate, self.seed, self._offset(), residual)
