@@ -282,7 +282,9 @@ class Dropout(torch.nn.Module):
 
     A call that a backward pass makes is one made again (torch.utils.checkpoint) and has the mask of the first time, which it is known by: every call in
     training draws a number from torch's generator of the CPU, whose state such a recomputation sets back.  Where it does not (preserve_rng_state=False),
-    or the last `REMEMBERED` calls of the layer do not have it, the call is refused."""
+    or the last `REMEMBERED` calls of the layer do not have it, the call is refused.
+
+    The seed and `calls` are in the layer's state, so that a run that is taken up again has the masks that it would have had."""
 
     REMEMBERED = 4096
 
@@ -290,6 +292,8 @@ class Dropout(torch.nn.Module):
         super().__init__()
         if not 0.0 <= rate <= 1.0:
             raise ops.InvalidArgumentError("a rate must lie in [0, 1]")
+        if seed is not None and not (isinstance(seed, int) and 0 <= seed < 1 << 64):
+            raise ops.InvalidArgumentError("a seed must be an int in [0, 2^64)")
         self.rate = float(rate)
         self.seed = int(torch.randint(1 << 62, ()).item()) if seed is None else seed
         self.capturable = capturable
@@ -304,6 +308,25 @@ class Dropout(torch.nn.Module):
 
     def __setstate__(self, state):
         super().__setstate__(dict(state, _recent={}))
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "seed"] = torch.tensor(self.seed - (self.seed >> 63 << 64), dtype=torch.int64)        # its 64 bits
+        if not self.capturable:
+            destination[prefix + "calls"] = torch.tensor(self.calls, dtype=torch.int64)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        own, rest = {}, dict(state_dict)
+        for name in ("seed",) if self.capturable else ("seed", "calls"):
+            t = rest.pop(prefix + name, None)                   # (states from before there were any have none)
+            if t is None:
+                continue
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.dim() != 0:
+                error_msgs.append("%s%s must be one int64" % (prefix, name))
+                return
+            own[name] = int(t) % (1 << 64)
+        super()._load_from_state_dict(rest, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        self.__dict__.update(own)
 
     def _offset(self):
         drawn = torch.randint(1 << 62, (), device="cpu").item()
