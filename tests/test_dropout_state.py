@@ -54,3 +54,28 @@ def test_states_that_are_none():
             with pytest.raises(RuntimeError):
                 layer.load_state_dict({**layer.state_dict(), name: bad})
     assert layer.seed == 9 and layer.calls == 0
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_copies(capturable):
+    """A copy of a layer that was given no seed draws its own (blocks that are copied drop other places); one with a seed keeps it, and its count."""
+    import copy
+    import pickle
+    import torch
+    import tf_approximate_b200 as ax
+    x = torch.ones(1000)
+    block = torch.nn.Sequential(torch.nn.Linear(4, 4), ax.Dropout(0.5, capturable=capturable))
+    block[1](x)
+    blocks = [block] + [copy.deepcopy(block) for _ in range(3)]
+    assert len({b[1].seed for b in blocks}) == 4 and all(int(b[1].calls) == 1 for b in blocks)
+    masks = [b[1](x) for b in blocks]
+    assert not any(torch.equal(a, b) for i, a in enumerate(masks) for b in masks[:i])
+    # a copy is the same layer in every other respect, and a stored one in all
+    for other in (pickle.loads(pickle.dumps(block[1])), copy.copy(block[1])):
+        assert other.seed == block[1].seed and int(other.calls) == int(block[1].calls)
+    given = ax.Dropout(0.5, seed=7, capturable=capturable).eval()
+    again = copy.deepcopy(given)
+    assert again.seed == 7 and not again.training and again.rate == 0.5 and list(again.state_dict()) == list(given.state_dict())
+    if capturable:
+        again.calls.add_(1)
+        assert int(given.calls) == 0

@@ -2,6 +2,8 @@
 (tf2/python/keras/layers/fake_approx_convolutional.py): per-batch min/max, fake quantisation of
 input and kernel, the table convolution, then bias and activation; the backward pass is the exact
 convolution's (the reference registers `conv2d_backprop_input/filter` as the gradient, :264-302)."""
+import copy
+
 import torch
 
 from . import dense_ops, norm_ops, ops
@@ -284,7 +286,8 @@ class Dropout(torch.nn.Module):
     training draws a number from torch's generator of the CPU, whose state such a recomputation sets back.  Where it does not (preserve_rng_state=False),
     or the last `REMEMBERED` calls of the layer do not have it, the call is refused.
 
-    The seed and `calls` are in the layer's state, so that a run that is taken up again has the masks that it would have had."""
+    The seed and `calls` are in the layer's state, so that a run that is taken up again has the masks that it would have had.
+    copy.deepcopy makes a layer with a seed of its own where none was given: blocks that are copied drop other places."""
 
     REMEMBERED = 4096
 
@@ -295,7 +298,8 @@ class Dropout(torch.nn.Module):
         if seed is not None and not (isinstance(seed, int) and 0 <= seed < 1 << 64):
             raise ops.InvalidArgumentError("a seed must be an int in [0, 2^64)")
         self.rate = float(rate)
-        self.seed = int(torch.randint(1 << 62, ()).item()) if seed is None else seed
+        self._draws_seed = seed is None
+        self.seed = self._new_seed() if seed is None else seed
         self.capturable = capturable
         self._recent = {}                                       # number drawn from torch's generator -> offset of that call
         if capturable:
@@ -303,11 +307,23 @@ class Dropout(torch.nn.Module):
         else:
             self.calls = 0
 
+    @staticmethod
+    def _new_seed():
+        return torch.randint(1 << 62, (), device="cpu").item()
+
+    def __deepcopy__(self, memo):
+        other = type(self).__new__(type(self))
+        memo[id(self)] = other
+        other.__setstate__(copy.deepcopy(self.__getstate__(), memo))
+        if self._draws_seed:
+            other.seed = self._new_seed()
+        return other
+
     def __getstate__(self):
         return dict(super().__getstate__(), _recent={})
 
     def __setstate__(self, state):
-        super().__setstate__(dict(state, _recent={}))
+        super().__setstate__({"_draws_seed": False, **state, "_recent": {}})
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
