@@ -232,9 +232,21 @@ class Dense(torch.nn.Module):
         return dense_ops.dense_cross_entropy(inputs.to(self.kernel.dtype), self.kernel, labels, self.bias, ignore_index, reduction)
 
 
+class _AnswerFn(torch.autograd.Function):
+    """A result without gradients of something that has them."""
+
+    @staticmethod
+    def forward(ctx, layer, inputs, residual):
+        return layer._answer(inputs, residual)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise ops.InvalidArgumentError("Dense8bit has no gradients: train the Dense layer that it was made of")
+
+
 class Dense8bit(torch.nn.Module):
     """A trained `Dense` layer, ready to answer in 8-bit floating point: its kernel is quantised here, once, and kept as codes [units, in_features] with
-    their scales; inputs are quantised by the call.  It has buffers and no parameters."""
+    their scales; inputs are quantised by the call.  It has buffers and no parameters, and no gradients: a backward pass through it is refused."""
 
     def __init__(self, dense):
         super().__init__()
@@ -255,9 +267,13 @@ class Dense8bit(torch.nn.Module):
         """The codes, [units, in_features]."""
         return self.lines.view(torch.float8_e4m3fn)[:, :self.in_features]
 
-    @torch.no_grad()
-    def forward(self, inputs, residual=None):
+    def _answer(self, inputs, residual):
         return dense_ops.dense_8bit(inputs, self.kernel, self.scales, self.bias, residual, self.activation)
+
+    def forward(self, inputs, residual=None):
+        if dense_ops._differentiated(inputs, residual):
+            return _AnswerFn.apply(self, inputs, residual)
+        return self._answer(inputs, residual)
 
 
 class GroupNorm(torch.nn.Module):
