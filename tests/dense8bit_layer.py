@@ -36,3 +36,29 @@ def gradients_are_refused(device):
     y = layer(leaf.detach()) * leaf[:, :72]
     y.sum().backward()
     assert torch.equal(leaf.grad[:, :72], want)
+
+
+def casts_of_a_network_leave_the_operands(device):
+    """.half(), .bfloat16(), .to(...) and .float() are for the network around the layer: its codes and scales are what they were."""
+    import copy
+    import tf_approximate_b200 as ax
+    layer = ax.Dense8bit(make(device, bias=False))
+    # a scale that float16 flushes to 0, and one that it takes for an infinity
+    layer.scales[0, 0], layer.scales[0, 1] = 2.0 ** -30, 3.0 * 2.0 ** 17
+    bits, lines = layer.scales.view(torch.int32).clone(), layer.lines.clone()
+    x = torch.randn(3, 200, device=device)
+    net = torch.nn.Sequential(torch.nn.Linear(200, 200).to(device), layer)
+    steps = (lambda n: n.half(), lambda n: n.bfloat16(), lambda n: n.to(torch.float16), lambda n: n.to(device, torch.bfloat16), lambda n: n.double(), lambda n: n.type(torch.float16),
+             lambda n: n.float())
+    want = layer(x)
+    for step in steps:
+        step(net)
+        for which in (layer, copy.deepcopy(layer)):
+            assert which.scales.dtype == torch.float32 and torch.equal(which.scales.view(torch.int32), bits)
+            assert which.lines.dtype == torch.uint8 and torch.equal(which.lines, lines) and which.kernel.dtype == torch.float8_e4m3fn
+    assert torch.equal(layer(x), want) and list(layer.state_dict()) == ["lines", "scales"] and layer.state_dict()["scales"].dtype == torch.float32
+    moved = copy.deepcopy(layer).to("meta")
+    assert moved.scales.is_meta and moved.lines.is_meta and moved.scales.dtype == torch.float32
+    again = moved.to_empty(device=device)
+    again.load_state_dict(layer.state_dict())
+    assert torch.equal(again(x), want)

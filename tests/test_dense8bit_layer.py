@@ -12,3 +12,7 @@ def stand_in(built, monkeypatch):
 
 def test_gradients_are_refused():
     D.gradients_are_refused("cpu")
+
+
+def test_casts_of_a_network():
+    D.casts_of_a_network_leave_the_operands("cpu")

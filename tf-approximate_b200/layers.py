@@ -262,6 +262,21 @@ class Dense8bit(torch.nn.Module):
         self.register_buffer("scales", scales)
         self.register_buffer("bias", None if dense.bias is None else dense.bias.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        # A cast of the network is not one of the codes and scales: fn has them as whole numbers, and what it makes of those but a cast is taken.
+        kept = {name: self._buffers[name] for name in ("lines", "scales")}
+        moved = dict(kept)
+        self._buffers.update(dict.fromkeys(kept))
+        try:
+            super()._apply(fn, recurse)
+            for name, t in kept.items():
+                bits = t if name == "lines" else t.view(torch.int32)
+                to = fn(bits)
+                moved[name] = (to if to.dtype == bits.dtype else bits.to(to.device)).view(t.dtype)
+        finally:
+            self._buffers.update(moved)
+        return self
+
     @property
     def kernel(self):
         """The codes, [units, in_features]."""
