@@ -62,3 +62,20 @@ def casts_of_a_network_leave_the_operands(device):
     again = moved.to_empty(device=device)
     again.load_state_dict(layer.state_dict())
     assert torch.equal(again(x), want)
+
+
+def answers_have_the_types_that_the_dense_layers_have(device):
+    import tf_approximate_b200 as ax
+    types = (torch.float32, torch.bfloat16, torch.float16)
+    for dtype in types:
+        dense = make(device, dtype)
+        layer, x = ax.Dense8bit(dense), torch.randn(4, 200, device=device)
+        for given in types + (torch.float64,):
+            y = layer(x.to(given))
+            # as Dense does: inputs are cast to its type
+            assert y.dtype == dtype and torch.equal(y, ax.dense_8bit(x.to(given).to(dtype), layer.kernel, layer.scales, layer.bias, activation="silu"))
+            assert layer(x.to(given), torch.zeros(4, 72, device=device, dtype=dtype)).dtype == dtype
+        # and it follows a network's casts
+        for cast in types:
+            assert layer.to(cast)(x).dtype == cast and ax.Dense8bit(dense).to(dtype=cast)(x).dtype == cast
+        assert list(layer.state_dict()) == ["lines", "scales", "bias"]

@@ -16,3 +16,7 @@ def test_gradients_are_refused():
 
 def test_casts_of_a_network():
     D.casts_of_a_network_leave_the_operands("cpu")
+
+
+def test_types():
+    D.answers_have_the_types_that_the_dense_layers_have("cpu")

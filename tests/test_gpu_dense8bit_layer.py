@@ -12,3 +12,7 @@ def test_gradients_are_refused(built):
 
 def test_casts_of_a_network(built):
     D.casts_of_a_network_leave_the_operands("cuda")
+
+
+def test_types(built):
+    D.answers_have_the_types_that_the_dense_layers_have("cuda")

@@ -246,7 +246,8 @@ class _AnswerFn(torch.autograd.Function):
 
 class Dense8bit(torch.nn.Module):
     """A trained `Dense` layer, ready to answer in 8-bit floating point: its kernel is quantised here, once, and kept as codes [units, in_features] with
-    their scales; inputs are quantised by the call.  It has buffers and no parameters, and no gradients: a backward pass through it is refused."""
+    their scales; inputs are cast to the layer's type, as `Dense` does, and quantised by the call.  It has buffers and no parameters, and no gradients: a
+    backward pass through it is refused.  Casts of a network change the type of its inputs and of its bias, not what it holds in 8 bits."""
 
     def __init__(self, dense):
         super().__init__()
@@ -261,6 +262,7 @@ class Dense8bit(torch.nn.Module):
         self.register_buffer("lines", lines)
         self.register_buffer("scales", scales)
         self.register_buffer("bias", None if dense.bias is None else dense.bias.detach().clone())
+        self.register_buffer("_like", torch.empty(0, dtype=dense.kernel.dtype, device=codes.device), persistent=False)       # the inputs' type
 
     def _apply(self, fn, recurse=True):
         # A cast of the network is not one of the codes and scales: fn has them as whole numbers, and what it makes of those but a cast is taken.
@@ -283,7 +285,7 @@ class Dense8bit(torch.nn.Module):
         return self.lines.view(torch.float8_e4m3fn)[:, :self.in_features]
 
     def _answer(self, inputs, residual):
-        return dense_ops.dense_8bit(inputs, self.kernel, self.scales, self.bias, residual, self.activation)
+        return dense_ops.dense_8bit(inputs.to(self._like.dtype), self.kernel, self.scales, self.bias, residual, self.activation)
 
     def forward(self, inputs, residual=None):
         if dense_ops._differentiated(inputs, residual):
