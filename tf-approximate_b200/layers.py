@@ -397,5 +397,9 @@ class Dropout(torch.nn.Module):
 
     def forward(self, inputs, residual=None):
         if not self.training:
-            return inputs if residual is None else inputs + residual
+            if residual is None:
+                return inputs
+            if not isinstance(residual, torch.Tensor) or (residual.dtype, residual.device, residual.shape) != (inputs.dtype, inputs.device, inputs.shape):
+                raise ops.InvalidArgumentError("residual must be a tensor of the inputs' type, shape and device")
+            return inputs + residual
         return norm_ops.dropout(inputs, self.rate, self.seed, self._offset(), residual)
