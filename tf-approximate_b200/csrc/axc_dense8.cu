@@ -18,8 +18,6 @@
 //                 1 row of 4096 x 16384: 15.6 us, 8 rows 16.3, 2.5 of it the rows' quantisation (reading the codes once: 10.2); with codes turned into fp16
 //                 first 22.8 and 33.5.
 // Sums within a block are the matrix pipes', over blocks fp32 with rounding; y is rounded once.
-#include <atomic>
-
 #include <cuda_fp8.h>
 
 #include "axc_gemm.h"
@@ -587,19 +585,6 @@ bool make_map8(const void *data, long long rows, long long inputs, long long lin
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename Kernel>
-int allow_smem(Kernel kernel, unsigned bytes, std::atomic<unsigned long long> &ready)
-{
-    int device = 0;
-    AXC_CUDA(cudaGetDevice(&device));
-    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
-    if (!(ready.load(std::memory_order_acquire) & bit) || !bit) {
-        AXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-        ready.fetch_or(bit, std::memory_order_release);
-    }
-    return AXC_OK;
-}
-
 template <int CG, int BN, bool PARTIAL>
 int launch_gemm8(Gemm8Args &P, int sms, Queue &q)
 {
@@ -727,26 +712,6 @@ int check_desc(const axc_dense8_desc *d)
     if (d->type < kFloat32 || d->type > kFloat16 || d->bias_type < kFloat32 || d->bias_type > kFloat16) return AXC_INVALID_ARGUMENT;
     if (d->activation < kActNone || d->activation > kActSilu || d->x_row_stride < 0 || d->kernel_row_stride < 0 || d->residual_row_stride < 0) return AXC_INVALID_ARGUMENT;
     return AXC_OK;
-}
-
-int sm_count(int device, int *sms)
-{
-    if (device < 0) return AXC_INVALID_ARGUMENT;
-    AXC_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
-    return AXC_OK;
-}
-
-template <typename Call>
-int on_device(int device, Call call)
-{
-    int prev = 0;
-    AXC_CUDA(cudaGetDevice(&prev));
-    if (prev != device) AXC_CUDA(cudaSetDevice(device));
-    int rc = call();
-    const cudaError_t e = cudaGetLastError();
-    if (!rc && e != cudaSuccess) rc = cuda_failed(e);
-    if (prev != device) cudaSetDevice(prev);
-    return rc;
 }
 
 }  // namespace

@@ -167,14 +167,9 @@ extern "C" int axc_dropout(const axc_dropout_desc *desc, const void *x, const vo
     P.offset[0] = unsigned(d.offset);
     P.offset[1] = unsigned(d.offset >> 32);
     P.offset_device = reinterpret_cast<const long long *>(offset_device);
-    int prev = 0;
-    AXC_CUDA(cudaGetDevice(&prev));
-    if (prev != device) AXC_CUDA(cudaSetDevice(device));
     Queue q = {cudaStream_t(stream)};
     const bool vec = aligned_to(16, x, residual, y);
-    int rc = d.type == kFloat32 ? run_dropout<float>(P, vec, q) : d.type == kBfloat16 ? run_dropout<__nv_bfloat16>(P, vec, q) : run_dropout<__half>(P, vec, q);
-    const cudaError_t e = cudaGetLastError();
-    if (!rc && e != cudaSuccess) rc = cuda_failed(e);
-    if (prev != device) cudaSetDevice(prev);
-    return rc;
+    return on_device(device, [&] {
+        return d.type == kFloat32 ? run_dropout<float>(P, vec, q) : d.type == kBfloat16 ? run_dropout<__nv_bfloat16>(P, vec, q) : run_dropout<__half>(P, vec, q);
+    });
 }

@@ -432,8 +432,6 @@ bool make_map(const Operand &o, long long rows, long long k, int planes, bool bf
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-}  // namespace
-
 // The cheapest of the tiles and splits by an estimate in clocks.  A stage takes what its matrix instructions take (2 for each column of
 // a tile, 390 at least) or what its bytes take (114 a clock and SM when all SMs have tiles, in proportion when few have), whichever is
 // more; a wave of tiles 3400 more until its sums are out, the product another 4500 for its first bytes and its last tile; a split one 7600
@@ -470,8 +468,6 @@ Plan choose_plan(long long m, long long n, long long k, int planes, bool may_spl
     }
     return best;
 }
-
-namespace {
 
 template <int CG, int BN, int MODE, int PLANES, bool CLOSE>
 int launch_gemm(GemmArgs &P, long long units, const DeviceInfo &di, Queue &q)

@@ -5,6 +5,8 @@
 #include <cudaTypedefs.h>
 #include <float.h>
 
+#include <atomic>
+
 #include "axc_internal.h"
 #include "axc_pieces.h"
 #include "axc_two.cuh"
@@ -45,6 +47,38 @@ inline int launch(Queue &q, void (*kernel)(Params...), dim3 grid, unsigned threa
     AXC_CUDA(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
     count_launch();
     return AXC_OK;
+}
+// Lets a kernel have up to `bytes` of shared memory, once on each device; `ready`: the kernel's own, zero at first
+template <typename Kernel>
+inline int allow_smem(Kernel kernel, unsigned bytes, std::atomic<unsigned long long> &ready)
+{
+    int device = 0;
+    AXC_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (!(ready.load(std::memory_order_acquire) & bit) || !bit) {
+        AXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+        ready.fetch_or(bit, std::memory_order_release);
+    }
+    return AXC_OK;
+}
+inline int sm_count(int device, int *sms)
+{
+    if (device < 0) return AXC_INVALID_ARGUMENT;
+    AXC_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+    return AXC_OK;
+}
+// call() with `device` as the current one
+template <typename Call>
+inline int on_device(int device, Call call)
+{
+    int prev = 0;
+    AXC_CUDA(cudaGetDevice(&prev));
+    if (prev != device) AXC_CUDA(cudaSetDevice(device));
+    int rc = call();
+    const cudaError_t e = cudaGetLastError();
+    if (!rc && e != cudaSuccess) rc = cuda_failed(e);
+    if (prev != device) cudaSetDevice(prev);
+    return rc;
 }
 // First in every kernel that `launch` starts: the next kernel may come, the one before is over.
 __device__ __forceinline__ void after_previous()
@@ -288,8 +322,6 @@ struct Gemm {
 struct Plan {
     int cg, bn, splits;
 };
-// planes: terms of an operand; may_split: also tiles below 64 columns
-Plan choose_plan(long long m, long long n, long long k, int planes, bool may_split, int sms);
 PFN_cuTensorMapEncodeTiled_v12000 encoder();    // NULL where the driver has none
 
 // Scratch for the partial sums of a product whose k is split; 0 where it is not.

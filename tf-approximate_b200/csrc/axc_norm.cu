@@ -27,7 +27,6 @@
 // (314), the latter bound by instructions and by the time between a block's phases; without the shortcut 203 (126) and 428 (188).  The first two with the tensors
 // read twice: 307 and 638.
 // 2 x 512 x 512 x 128 bf16, which no cluster holds: 88 (41) and 134 (61).
-#include <atomic>
 #include <type_traits>
 
 #include "axc_gemm.h"
@@ -1265,25 +1264,12 @@ __global__ void __launch_bounds__(1024) norm_parameters_kernel(const NormArgs P)
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
-template <typename Kernel>
-int allow_smem(Kernel kernel, std::atomic<unsigned long long> &ready)
-{
-    int device = 0;
-    AXC_CUDA(cudaGetDevice(&device));
-    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
-    if (!(ready.load(std::memory_order_acquire) & bit) || !bit) {
-        AXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kNormSmem)));
-        ready.fetch_or(bit, std::memory_order_release);
-    }
-    return AXC_OK;
-}
-
 template <typename T, int V>
 int forward(NormArgs P, const NormPlan &plan, Queue &q)
 {
     if (plan.resident) {
         static std::atomic<unsigned long long> ready{0};
-        const int rc = allow_smem(norm_forward_kernel<T, V>, ready);
+        const int rc = allow_smem(norm_forward_kernel<T, V>, kNormSmem, ready);
         if (rc) return rc;
         return launch(q, norm_forward_kernel<T, V>, dim3(unsigned(P.samples * P.spans * P.blocks)), unsigned(plan.threads), plan.smem, unsigned(plan.blocks), P);
     }
@@ -1300,7 +1286,7 @@ int backward(NormArgs P, const NormPlan &plan, Queue &q)
     int rc;
     if (plan.resident) {
         auto run = [&](auto kernel, std::atomic<unsigned long long> &ready) {
-            const int rc = allow_smem(kernel, ready);
+            const int rc = allow_smem(kernel, kNormSmem, ready);
             return rc ? rc : launch(q, kernel, dim3(unsigned(P.samples * P.spans * P.blocks)), unsigned(plan.threads), plan.smem, unsigned(plan.blocks), P);
         };
         static std::atomic<unsigned long long> ready[2];
@@ -1317,13 +1303,6 @@ int backward(NormArgs P, const NormPlan &plan, Queue &q)
 }
 
 constexpr long long kMostBlocks = 0x7fffffffll;
-
-int sm_count(int device, int *sms)
-{
-    if (device < 0) return AXC_INVALID_ARGUMENT;
-    AXC_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
-    return AXC_OK;
-}
 
 int check_desc(const axc_norm_desc *d)
 {
@@ -1404,19 +1383,6 @@ size_t workspace_of(const NormShape &s, const NormPlan &plan, bool backward)
 
 template <typename... P>
 bool on_16(P... p) { return aligned_to(16, p...); }
-
-template <typename Call>
-int on_device(int device, Call call)
-{
-    int prev = 0;
-    AXC_CUDA(cudaGetDevice(&prev));
-    if (prev != device) AXC_CUDA(cudaSetDevice(device));
-    int rc = call();
-    const cudaError_t e = cudaGetLastError();
-    if (!rc && e != cudaSuccess) rc = cuda_failed(e);
-    if (prev != device) cudaSetDevice(prev);
-    return rc;
-}
 
 }  // namespace
 
