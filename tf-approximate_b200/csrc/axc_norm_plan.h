@@ -142,27 +142,27 @@ inline NormPlan norm_plan(const NormShape &s, int kept, int moved, bool backward
             }
         }
     }
-    // Read twice: all bytes and those that are read again at 70 % of memory's rate (single values at a fourth of that), and three launches.
-    int vec = 1;
-    const int span = norm_columns(s, &vec);
-    const int again = backward ? (moved / s.size == 5 ? 3 : 2) : 1;
-    const double twice = 14.0 + double(s.values()) * (moved + again * s.size) / (4.6e6 * (vec > 1 ? 1.0 : 0.25));
-    if (best.resident && least <= twice) return best;
-    best = {};
-    best.span = span;
-    best.vec = vec;
-    best.threads = kNormThreads;
+    NormPlan swept = {};
+    swept.span = norm_columns(s, &swept.vec);
+    swept.threads = kNormThreads;
     // six blocks for every SM, of 32 KiB at least and a million values at most
-    const long long across = s.samples * ((s.channels + span - 1) / span), most = s.places * span * s.size / (32 * 1024) + 1;
+    const long long across = s.samples * ((s.channels + swept.span - 1) / swept.span), most = s.places * swept.span * s.size / (32 * 1024) + 1;
     long long shares = ((long long)sms * 6 + across - 1) / (across ? across : 1);
     if (shares > most) shares = most;
     if (shares > s.places) shares = s.places;
-    const long long fewest = (s.places * span >> 20) + 1;
+    const long long fewest = (s.places * swept.span >> 20) + 1;
     if (shares < fewest) shares = fewest;
     if (shares < 1) shares = 1;
     const long long per = s.places > 0 ? (s.places + shares - 1) / shares : 1;
-    best.shares = s.places > 0 ? (s.places + per - 1) / per : 1;
-    return best;
+    swept.shares = s.places > 0 ? (s.places + per - 1) / per : 1;
+    // Read twice: all bytes and those that are read again at 70 % of memory's rate (single values at a fourth of that), or 3 us for each of the two
+    // passes' blocks, 3 of which (backward 2) an SM takes at a time, whichever is more; between the passes 4.1 us for each sample's groups, a block each, 8 an SM; and
+    // three launches.  (Without the blocks' times 200704 x 1 x 256 bf16 in 32 groups took 23.5 ms instead of 0.5, 16384 x 16 x 64 in 8 groups 629 us instead of 50.)
+    const int again = backward ? (moved / s.size == 5 ? 3 : 2) : 1;
+    const double bytes = double(s.values()) * (moved + again * s.size) / (4.6e6 * (swept.vec > 1 ? 1.0 : 0.25));
+    const double blocks = 2 * 3.0 * double(across) * double(swept.shares) / (double(sms) * (backward ? 2 : 3)), join = 4.1 * double(s.samples) * double(s.groups) / (8.0 * sms);
+    if (best.resident && least <= 14.0 + (bytes > blocks ? bytes : blocks) + join) return best;
+    return swept;
 }
 
 // Bytes of scratch: pairs of fp32 sums for every sample and channel, and share; group sums behind them
