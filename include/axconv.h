@@ -457,7 +457,9 @@ int axc_quantize_blocks(const void *x, int64_t rows, int64_t inputs, int64_t row
  * rounded once.  An infinity or a NaN in a row makes that row of y NaN.
  * Workspace: axc_dense8_workspace_bytes for the kernel's address (NULL: enough for any), 256-byte aligned, nothing kept in it; axc_matrix_status
  * reads its status word.  Calls only enqueue kernels: capturable.  Addresses must be multiples of their type's size; a kernel that starts on 16
- * bytes, with rows of a multiple of 16, is read where it is, any other is copied by every call. */
+ * bytes, with rows of a multiple of 16, is read where it is; any other is copied by every call of more than 8 rows, and read byte by byte, at about a
+ * fourth of the speed, by calls of up to 8.  A product of a row's and a kernel's scale beyond fp32's largest value counts as that value, and one below 2^-126
+ * has fewer bits. */
 typedef struct {
     int64_t rows, inputs, units;
     int32_t type, bias_type, activation, reserved;

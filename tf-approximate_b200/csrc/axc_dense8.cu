@@ -11,12 +11,14 @@
 //                 of the 16-bit products (axc_gemm.cu).  Bound by taking the sums out: a stage of a tile of 64, 128, 256 columns takes 740, 990, 1430
 //                 clocks, its matrix instructions alone 390 to 512, and with sums taken out every eighth block only 977 (at the clocks that the power limit
 //                 then leaves); four buffers of 128 columns instead of two of 256 change nothing, so it is the tensor memory's reading, not the waits.
-//                 8192 x 4096 x 16384, bf16: 665 us without an activation (1650 TFLOP/s; the same product in 16 bits 680), with gelu 757.
+//                 8192 x 4096 x 16384, bf16: 665 to 700 us without an activation (1650 to 1570 TFLOP/s; the same product in 16 bits 680), with gelu 757 to 867, by the
+//                 values and the card: the power limit is what differs.
 //   up to 8 rows  bound by reading the kernel once.  Four warps share 16 units and have every fourth block of 128 inputs each; a lane reads 16 bytes of two
 //                 units at a time, two blocks on their way, and multiplies them, as they are, by mma with the rows as its columns: with plain
 //                 multiply-adds 8 rows would cost eight times what one does.  The order of k within a block is the lanes' own, the same for both operands.
 //                 1 row of 4096 x 16384: 15.6 us, 8 rows 16.3, 2.5 of it the rows' quantisation (reading the codes once: 10.2); with codes turned into fp16
-//                 first 22.8 and 33.5.
+//                 first 22.8 and 33.5.  Lines that do not start on 16 bytes are read a byte at a time: 1 and 8 rows of 4094 x 16384 take 69 us, 19 with lines
+//                 of 4096 bytes.
 // Sums within a block are the matrix pipes', over blocks fp32 with rounding; y is rounded once.
 #include <cuda_fp8.h>
 
@@ -46,7 +48,7 @@ __device__ __forceinline__ float scale_of(float top, float &inverse)
     inverse = __uint_as_float(unsigned(127 - power) << 23);
     return __uint_as_float(unsigned(127 + power) << 23);
 }
-// The product of two scales: finite where it would leave fp32's range, so that a sum of zeros stays one; NaN stays NaN
+// The product of two scales: fp32's largest value where it would leave that range, so that a sum of zeros stays one; NaN stays NaN
 __device__ __forceinline__ float scales_product(float a, float b)
 {
     const float s = a * b;
@@ -119,7 +121,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs A)
     }
 }
 
-// A block of threads has a block of 128 x 128 values: a thread 8 neighbours of every sixteenth row
+// A block of threads has a block of 128 x 128 values: a thread 8 neighbours of every sixteenth row.  It reads them twice, one by one: a kernel is quantised once.
+// 16384 x 4096: bf16 108 us (31 at memory's rate), fp32 160 (51).
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_squares_kernel(const QuantArgs A)
 {

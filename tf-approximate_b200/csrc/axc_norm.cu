@@ -14,7 +14,9 @@
 // Threads: values are taken 16 bytes at a time, neighbouring threads neighbouring ones.  The number of threads that take part is such
 // that a thread's channels repeat with every step, so that it keeps their mean, factor, offset and sums in registers; that holds for lines that
 // start anywhere, too (20 channels of fp16: 5 vectors hold two lines), as a whole tensor has no gaps.  A vector that sticks out of what a block
-// has, at its start or its end, is moved value by value.
+// has, at its start or its end, is moved value by value.  Where the order of the channels repeats after more vectors than a block has threads (channels / gcd(channels,
+// values of a vector) > 256: 777 channels of fp16), or a tensor does not start on 16 bytes, all values are moved one by one: 64 x 56 x 56 x 777 fp16, silu, takes 931 us forward and
+// 1740 backward, with 776 channels 240 and 389.
 //
 // Sums are fp32.  Those of the variance are never of squares that nearly cancel: a thread adds the squares of up to 32 values less the first of them,
 // and means and squared distances are joined by their means (Chan, Golub and LeVeque).  Every sum has a fixed order.
@@ -1319,7 +1321,8 @@ int check_desc(const axc_norm_desc *d)
 
 NormShape shape_of(const axc_norm_desc &d, bool aligned) { return {d.samples, d.places, d.channels, d.groups, d.type == kFloat32 ? 4 : 2, aligned}; }
 
-// The plan of a call; `residual`: whether its values take part.  Searching for one takes some 20 us of the host's time, so plans are remembered: they are functions of the shape alone.
+// The plan of a call; `residual`: whether its values take part.  Searching for one takes 1 to 8 us of the host's time, so plans are remembered: they are functions of the shape alone.
+// (Shapes whose hashes collide, and every new thread, search again.)
 NormPlan plan_of(const NormShape &s, bool backward, bool residual, int sms)
 {
     struct Known {

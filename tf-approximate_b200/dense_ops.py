@@ -43,7 +43,7 @@ def dense_forward(x, kernel, bias=None, residual=None, activation=None, check=Fa
 def dense_backward(grad, x, kernel, kept=None, activation=None, bias=None, residual=None, need_x=True, need_kernel=True, check=False):
     """(dx, dkernel, dbias, dresidual) of `dense_forward` for the gradient of its output; `kept` is what it returned.  dbias and
     dresidual are there for the bias and the residual that are given (of which only type and shape count), dx and dkernel where
-    needed.  dkernel lies in memory as the kernel does."""
+    needed.  dkernel lies in memory as the kernel does.  Without an activation dresidual is `grad` itself: one tensor, not a copy."""
     return _lib.binding().dense_backward(grad, x, kernel, kept, _activation(activation), bias, residual, bool(need_x), bool(need_kernel), bool(check))
 
 
@@ -122,7 +122,8 @@ def quantize_blocks(x, rows=1):
 
     rows=1: blocks of 128 neighbours along the last dimension, x [..., inputs], scales [..., ceil(inputs / 128)]; rows=128: blocks of 128 x 128,
     x [units, inputs], scales [ceil(units / 128), ceil(inputs / 128)], as `dense_8bit` takes a kernel.  A scale is the least power of two, 2^-126 at
-    least, with which the block's largest magnitude is a code (448 at most); a block with an infinity or a NaN has the scale NaN."""
+    least, with which the block's largest magnitude is a code (448 at most); a block with an infinity or a NaN has the scale NaN.  The codes' rows are
+    `inputs` bytes apart; `dense_8bit` is fastest on rows of a multiple of 16 bytes, which `Dense8bit` pads them to."""
     return _lib.binding().quantize_blocks(x, rows)
 
 
@@ -132,7 +133,8 @@ def dense_8bit(x, kernel, kernel_scales, bias=None, residual=None, activation=No
     kernel [units, inputs] and kernel_scales are what `quantize_blocks(..., rows=128)` makes of a trained kernel (of `Dense`: its transpose); x
     [..., inputs] in float32, bfloat16 or float16 is quantised on the way, each row's blocks of 128 by themselves.  bias [units] may be of another of
     these types; residual has y's shape, and y x's type.  Sums are fp32 and y is rounded once.  An infinity or a NaN in a row of x makes that row of y
-    NaN.  Up to 8 rows read the kernel once, at memory's rate.  A kernel whose rows do not start on 16 bytes is copied by every call.
+    NaN; a product of two scales beyond fp32's largest value counts as that value.  Up to 8 rows read the kernel once.  A kernel whose rows do not start on
+    16 bytes is copied by every call of more than 8 rows, and read byte by byte, at about a fourth of the speed, by calls of up to 8.
     There are no gradients: operands that are differentiated are refused.
     check: wait for the call and raise InternalError if a wait inside the kernels ran out."""
     if _differentiated(x, kernel_scales, bias, residual):

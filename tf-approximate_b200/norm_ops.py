@@ -20,7 +20,8 @@ def group_norm_forward(x, groups, scale=None, offset=None, residual=None, activa
 
 def group_norm_backward(grad, x, statistics, groups, scale=None, offset=None, residual=None, activation=None, need_x=True):
     """(dx, dscale, doffset, dresidual) of `group_norm_forward` for the gradient of its output; `statistics` is what it returned, the rest what it
-    was given.  dscale, doffset and dresidual are there for what is given, dx where needed."""
+    was given.  dscale, doffset and dresidual are there for what is given, dx where needed.  Without an activation dresidual is `grad` itself: one
+    tensor, not a copy."""
     return _lib.binding().group_norm_backward(grad, x, statistics, groups, scale, offset, residual, _activation(activation), bool(need_x), True, True, True)
 
 
